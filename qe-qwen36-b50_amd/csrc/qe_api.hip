@@ -14,6 +14,7 @@
 
 #include "../../include/qe_moe.h"
 #include "qe_kernels.h"
+#include "qe_mixer.h"
 
 static thread_local std::string g_err;
 
@@ -26,6 +27,15 @@ static int fail(int code, const char *fmt, ...) {
     va_end(ap);
     g_err = buf;
     return code;
+}
+// the same for the other files of the library
+int qe_fail(int code, const char *fmt, ...) {
+    char buf[512];
+    va_list ap;
+    va_start(ap, fmt);
+    vsnprintf(buf, sizeof buf, fmt, ap);
+    va_end(ap);
+    return fail(code, "%s", buf);
 }
 #define HIP_TRY(expr)                                                                             \
     do {                                                                                          \

@@ -1,0 +1,335 @@
+// Rotary positions with the cache write, and attention of single tokens over a paged cache.
+#include "qe_mixer_device.h"
+
+// ---------------------------------------------------------------------------
+// Rotary positions and cache write, a workgroup per token.
+// Pair (i, i + rotary/2) turns by pos * theta^(-2 i / rotary).  The angle is taken in turns
+// in 64 bits (a position of 2^18 times a pair's 24-bit rate would leave 2^-6 of a turn in
+// 32) and only the fraction goes to the 32-bit sine and cosine; they are made once per token
+// and pair, in LDS, for all of its heads.  A work item is 16 elements of a head: 8 pairs,
+// or 16 elements behind the rotated ones.  Bound by memory: q read and written, k and v
+// read and written.
+// ---------------------------------------------------------------------------
+template <typename IN>
+__device__ __forceinline__ void load8(const IN *p, float *x) {
+    if constexpr (sizeof(IN) == 4) {
+        const qe_f4 a = *(const qe_f4 *)p, b = *(const qe_f4 *)(p + 4);
+        for (int i = 0; i < 4; ++i) x[i] = a[i], x[4 + i] = b[i];
+    } else {
+        const auto a = *(const __attribute__((ext_vector_type(8))) IN *)p;
+        for (int i = 0; i < 8; ++i) x[i] = (float)a[i];
+    }
+}
+template <typename OUT>
+__device__ __forceinline__ void store8(OUT *p, const float *x) {
+    __attribute__((ext_vector_type(8))) OUT a;
+    for (int i = 0; i < 8; ++i) a[i] = (OUT)x[i];
+    *(__attribute__((ext_vector_type(8))) OUT *)p = a;
+}
+
+template <typename IN, typename OUT>
+__global__ __launch_bounds__(256) void k_append(const QeAppendArgs a) {
+    __shared__ float2 cs[128];
+    __shared__ long row_s;
+    __shared__ int seq_s[2];
+    const int t = blockIdx.x, tid = threadIdx.x, half = a.rotary / 2;
+    if (tid < 64) { // the token's sequence: the last whose first row is not behind t (64 at a time)
+        int seq = -1;
+        if (!a.cu) {
+            seq = t;
+        } else {
+            int lo = 0, hi = a.n_seqs; // cu[lo] <= t < cu[hi], as far as cu rises
+            while (hi - lo > 1) {
+                const int mid = (lo + hi) >> 1;
+                if (a.cu[mid] <= t) lo = mid;
+                else hi = mid;
+            }
+            if (a.cu[lo] <= t && t < a.cu[lo + 1]) seq = lo;
+        }
+        long row = -1;
+        int place = 0;
+        if (seq >= 0) {
+            unsigned bad = 0;
+            const int most = a.max_pages << a.page_log2;
+            const int len = qe_checked(a.kv_len[seq], 0, most, -1, &bad);
+            const int end = a.cu ? qe_checked(a.cu[seq + 1], 0, a.n_tokens, -1, &bad) : t + 1;
+            unsigned what = QE_BAD_LENGTH;
+            if (!bad) {
+                place = len - end + t;
+                if (place >= 0) {
+                    const unsigned p = (unsigned)a.table[(size_t)seq * a.table_stride + (place >> a.page_log2)];
+                    if (p >= a.n_pages) bad = 1, what = QE_BAD_PAGE;
+                    else row = ((long)p * a.kv_heads << a.page_log2) + (place & ((1 << a.page_log2) - 1));
+                }
+            }
+            if (bad) {
+                if (tid == 0) report(a.err, what);
+                seq = -1;
+            }
+        }
+        if (tid == 0) row_s = row, seq_s[0] = seq, seq_s[1] = place;
+    }
+    __syncthreads();
+    if (seq_s[0] < 0) return;
+    if (tid < half) {
+        const int pos = a.pos ? a.pos[(size_t)(a.n_axes > 1 ? a.axis[tid] : 0) * a.n_tokens + t] : seq_s[1];
+        const double turn = (double)pos * a.turns[tid];
+        float s, c;
+        sincospif((float)(2.0 * (turn - rint(turn))), &s, &c);
+        cs[tid] = make_float2(c, s);
+    }
+    __syncthreads();
+    const int per = a.head_dim / 16; // items of a head
+    const int n_q = a.q ? a.q_heads * per : 0, n_k = a.kv_heads * per;
+    const long row = row_s;
+    for (int it = tid; it < n_q + 2 * n_k; it += 256) {
+        const int kind = it < n_q ? 0 : it < n_q + n_k ? 1 : 2, j = it - (kind == 0 ? 0 : kind == 1 ? n_q : n_q + n_k);
+        if (kind && row < 0) break; // a token before the sequence's first position
+        const int head = j / per, c = j - head * per;
+        const bool turned = kind < 2 && c * 16 < a.rotary;
+        const int e0 = turned ? c * 8 : c * 16, e1 = turned ? half + c * 8 : c * 16 + 8;
+        const IN *src = kind == 0   ? (const IN *)a.q + (size_t)t * a.q_stride
+                        : kind == 1 ? (const IN *)a.k + (size_t)t * a.k_stride
+                                    : (const IN *)a.v + (size_t)t * a.v_stride;
+        src += (size_t)head * a.head_dim;
+        float x[8], y[8];
+        load8(src + e0, x);
+        load8(src + e1, y);
+        if (turned)
+            for (int i = 0; i < 8; ++i) {
+                const float2 r = cs[e0 + i];
+                const float u = x[i], w = y[i];
+                x[i] = fmaf(u, r.x, -(w * r.y));
+                y[i] = fmaf(w, r.x, u * r.y);
+            }
+        OUT *dst = kind == 0 ? (OUT *)a.q_out + (size_t)t * a.q_out_stride + (size_t)head * a.head_dim
+                             : (OUT *)(kind == 1 ? a.kc : a.vc) + (row + ((long)head << a.page_log2)) * a.head_dim;
+        store8(dst + e0, x);
+        store8(dst + e1, y);
+    }
+}
+
+hipError_t qe_launch_append(const QeAppendArgs &a, int in_type, int type, hipStream_t st) {
+    if (a.n_tokens == 0) return hipSuccess;
+    const dim3 g(a.n_tokens), b(256);
+    if (type == QE_BF16) {
+        if (in_type == QE_F32) k_append<float, __bf16><<<g, b, 0, st>>>(a);
+        else k_append<__bf16, __bf16><<<g, b, 0, st>>>(a);
+    } else {
+        if (in_type == QE_F32) k_append<float, _Float16><<<g, b, 0, st>>>(a);
+        else k_append<_Float16, _Float16><<<g, b, 0, st>>>(a);
+    }
+    return hipGetLastError();
+}
+
+// ---------------------------------------------------------------------------
+// Decode: a workgroup per (sequence, key-value head, split of its length), its four waves
+// each over their own 32-key steps, no barrier before the end.
+//
+// The heads that share a key-value head are the columns of both products, so every key and
+// value is read once: S^T = K Q^T (16 keys x 16 heads per matrix product, K rows straight
+// from memory to the operand registers) and O^T += V^T P^T.  S^T leaves 4 consecutive keys of
+// a lane's column in its registers; two such groups are the 8 k of the second product's
+// operand, and V^T is read from LDS with the transposing read in that same order of keys, so
+// probabilities never cross lanes.  V reaches LDS by direct loads, its 64-byte units
+// permuted by row so that the four rows of a transposing read hit different banks.
+// Running maximum and sum in 32 bits per head; O is rescaled only when a maximum grew.
+// ---------------------------------------------------------------------------
+template <int DH>
+__device__ __forceinline__ int v_swizzle(int row) { // of the 16-byte chunk index
+    return DH == 64 ? ((row >> 1) & 1) << 2 : (row & 3) << 2;
+}
+
+template <bool BF, int DH>
+__global__ __launch_bounds__(256, 2) void k_attn_decode(const QeAttnArgs a) {
+    constexpr int CH = DH / 8;       // 16-byte chunks of a row
+    constexpr int ROWS = 64 / CH;    // rows of one direct load
+    constexpr int KS = DH / 32, DB = DH / 16;
+    __shared__ __align__(16) short v_lds[4][QE_ATTN_TILE * DH];
+    __shared__ float2 ml[4][16];
+    const int tid = threadIdx.x, wave = tid >> 6, lane = tid & 63, col = lane & 15, c = lane >> 4;
+    const int split = blockIdx.x % a.splits, item = blockIdx.x / a.splits, seq = item / a.kv_heads, kvh = item % a.kv_heads;
+    unsigned bad_len = 0, bad = 0;
+    const int len = qe_checked(a.kv_len[seq], 0, a.max_pages << a.page_log2, 0, &bad_len);
+    const int32_t *table = a.table + (size_t)seq * a.table_stride;
+    const size_t G = a.group;
+
+    qe_s8 qf[KS];
+    const short *q = (const short *)a.q + (size_t)seq * a.q_stride + ((size_t)kvh * G + col) * DH + c * 8;
+    for (int s = 0; s < KS; ++s) qf[s] = col < a.group ? *(const qe_s8 *)(q + s * 32) : qe_s8{};
+
+    int lo, hi;
+    qe_split_range((len + QE_ATTN_TILE - 1) / QE_ATTN_TILE, a.splits, split, &lo, &hi);
+    qe_f4 acc[DB];
+    for (int d = 0; d < DB; ++d) acc[d] = qe_f4{0, 0, 0, 0};
+    float m = -INFINITY, l = 0;
+    short *vb = v_lds[wave];
+    const int tr_row = col >> 2, tr_el = (col & 3) * 4; // of a transposing read
+    for (int t = lo + wave; t < hi; t += 4) {
+        const int k0 = t * QE_ATTN_TILE;
+        // the 16 positions from k0 + 16 on may be behind the end: any page of the sequence does
+        const size_t r0 = sub_row(a, table, kvh, k0, &bad);
+        const size_t r1 = k0 + 16 < len ? sub_row(a, table, kvh, k0 + 16, &bad) : r0;
+        qe_s8 kf[2][KS];
+        const short *kp0 = (const short *)a.kc + (r0 + col) * DH + c * 8, *kp1 = (const short *)a.kc + (r1 + col) * DH + c * 8;
+#pragma unroll
+        for (int s = 0; s < KS; ++s) kf[0][s] = *(const qe_s8 *)(kp0 + s * 32);
+#pragma unroll
+        for (int s = 0; s < KS; ++s) kf[1][s] = *(const qe_s8 *)(kp1 + s * 32);
+#pragma unroll
+        for (int i = 0; i < QE_ATTN_TILE / ROWS; ++i) {
+            const int row = i * ROWS + lane / CH, ch = (lane % CH) ^ v_swizzle<DH>(row);
+            const size_t base = (i * ROWS < 16 ? r0 : r1) + (row & 15);
+            load_lds16((const short *)a.vc + base * DH + ch * 8, vb + i * 512);
+        }
+        qe_f4 s[2] = {qe_f4{0, 0, 0, 0}, qe_f4{0, 0, 0, 0}};
+#pragma unroll
+        for (int st = 0; st < KS; ++st) {
+            s[0] = mfma16<BF>(kf[0][st], qf[st], s[0]);
+            s[1] = mfma16<BF>(kf[1][st], qf[st], s[1]);
+        }
+        if (k0 + QE_ATTN_TILE > len) {
+            for (int i = 0; i < 4; ++i) {
+                if (k0 + 4 * c + i >= len) s[0][i] = -INFINITY;
+                if (k0 + 16 + 4 * c + i >= len) s[1][i] = -INFINITY;
+            }
+        }
+        float top = fmaxf(fmaxf(fmaxf(s[0][0], s[0][1]), fmaxf(s[0][2], s[0][3])),
+                          fmaxf(fmaxf(s[1][0], s[1][1]), fmaxf(s[1][2], s[1][3])));
+        top = fmaxf(top, __shfl_xor(top, 16));
+        top = fmaxf(top, __shfl_xor(top, 32));
+        if (__any(top > m)) {
+            const float mn = fmaxf(m, top), f = m == -INFINITY ? 0.f : exp2f((m - mn) * a.scale_log2);
+            for (int d = 0; d < DB; ++d) acc[d] *= f;
+            l *= f;
+            m = mn;
+        }
+        const float base = m == -INFINITY ? 0.f : -m * a.scale_log2;
+        float p[8];
+        for (int i = 0; i < 4; ++i) {
+            p[i] = __builtin_amdgcn_exp2f(fmaf(s[0][i], a.scale_log2, base));
+            p[4 + i] = __builtin_amdgcn_exp2f(fmaf(s[1][i], a.scale_log2, base));
+        }
+        l += ((p[0] + p[1]) + (p[2] + p[3])) + ((p[4] + p[5]) + (p[6] + p[7]));
+        union {
+            unsigned u[4];
+            qe_s8 v;
+        } pf;
+        for (int i = 0; i < 4; ++i) pf.u[i] = pack2<BF>(p[2 * i], p[2 * i + 1]);
+        __builtin_amdgcn_s_waitcnt(0x0f70); // the direct loads have landed (vmcnt 0)
+        if (k0 + QE_ATTN_TILE > len) {       // rows behind the end hold anything: a probability of 0 times NaN is NaN
+            for (int i = lane; i < QE_ATTN_TILE * CH; i += 64)
+                if (k0 + i / CH >= len) *(qe_s8 *)(vb + i * 8) = qe_s8{};
+        }
+#pragma unroll
+        for (int d = 0; d < DB; ++d) {
+            const int ra = 4 * c + tr_row, rb = ra + 16;
+            const int el = d * 16 + tr_el;
+            const qe_s4 x = lds_tr(vb + ra * DH + (((el >> 3) ^ v_swizzle<DH>(ra)) << 3) + (el & 7));
+            const qe_s4 y = lds_tr(vb + rb * DH + (((el >> 3) ^ v_swizzle<DH>(rb)) << 3) + (el & 7));
+            acc[d] = mfma16<BF>(qe_s8{x[0], x[1], x[2], x[3], y[0], y[1], y[2], y[3]}, pf.v, acc[d]);
+        }
+    }
+    l += __shfl_xor(l, 16);
+    l += __shfl_xor(l, 32);
+    if (lane < 16) ml[wave][lane] = make_float2(m, l);
+    // the waves' results through LDS (a wave's own V buffer holds 16 heads x DH floats)
+    float *o = (float *)vb;
+    for (int d = 0; d < DB; ++d) *(qe_f4 *)(o + col * DH + d * 16 + c * 4) = acc[d];
+    bad = __syncthreads_or(bad) ? 1 : 0;
+    if (tid == 0 && (bad | bad_len)) report(a.err, bad ? QE_BAD_PAGE : QE_BAD_LENGTH);
+    for (int i = tid; i < a.group * (DH / 4); i += 256) {
+        const int h = i / (DH / 4), d = i % (DH / 4) * 4;
+        float top = ml[0][h].x;
+        for (int w = 1; w < 4; ++w) top = fmaxf(top, ml[w][h].x);
+        float sum = 0;
+        qe_f4 r = {0, 0, 0, 0};
+        for (int w = 0; w < 4; ++w) {
+            const float mw = ml[w][h].x, f = mw == -INFINITY ? 0.f : exp2f((mw - top) * a.scale_log2);
+            if (ml[w][h].y == 0.f) continue; // a wave without keys
+            sum += f * ml[w][h].y;
+            r += f * *(const qe_f4 *)((const float *)v_lds[w] + h * DH + d);
+        }
+        if (a.splits == 1) {
+            const float inv = sum == 0.f ? 0.f : 1.f / sum;
+            r *= inv;
+            if (bad) r = qe_f4{0, 0, 0, 0};
+            uint2 w;
+            w.x = pack2<BF>(r[0], r[1]);
+            w.y = pack2<BF>(r[2], r[3]);
+            *(uint2 *)((short *)a.out + (size_t)seq * a.out_stride + ((size_t)kvh * G + h) * DH + d) = w;
+        } else {
+            const size_t row = ((size_t)item * a.splits + split) * G + h;
+            *(qe_f4 *)(a.part_o + row * DH + d) = r;
+            if (d == 0) a.part_ml[row] = make_float2(top, bad ? -1.f : sum);
+        }
+    }
+}
+
+// ---------------------------------------------------------------------------
+// The splits' results of a row joined: o = sum 2^(m_s - m) o_s / sum 2^(m_s - m) l_s.  A
+// workgroup per row of a decode call.
+// ---------------------------------------------------------------------------
+template <bool BF, int DH>
+__global__ __launch_bounds__(256) void k_attn_join(const QeAttnArgs a) {
+    constexpr int TD = DH / 4, GR = 256 / TD; // threads of a row's elements, groups of splits
+    __shared__ float w_s[QE_ATTN_WGS];
+    __shared__ float red[256];
+    __shared__ __align__(16) qe_f4 o_s[256];
+    const int tid = threadIdx.x, head = blockIdx.x % a.q_heads, seq = blockIdx.x / a.q_heads;
+    const int kvh = head / a.group, h = head % a.group;
+    const size_t row0 = ((size_t)seq * a.kv_heads + kvh) * a.splits * a.group + h;
+    float m = -INFINITY;
+    int bad = 0;
+    for (int s = tid; s < a.splits; s += 256) {
+        const float2 x = a.part_ml[row0 + (size_t)s * a.group];
+        bad |= x.y < 0.f;
+        m = fmaxf(m, x.x);
+    }
+    for (int k = 32; k; k >>= 1) m = fmaxf(m, __shfl_xor(m, k));
+    if ((tid & 63) == 0) red[tid >> 6] = m;
+    bad = __syncthreads_or(bad);
+    m = fmaxf(fmaxf(red[0], red[1]), fmaxf(red[2], red[3]));
+    __syncthreads();
+    float sum = 0;
+    for (int s = tid; s < a.splits; s += 256) {
+        const float2 x = a.part_ml[row0 + (size_t)s * a.group];
+        const float f = x.y == 0.f || x.x == -INFINITY ? 0.f : exp2f((x.x - m) * a.scale_log2);
+        w_s[s] = x.y == 0.f ? -1.f : f; // -1: nothing of that split is used
+        sum += x.y == 0.f ? 0.f : f * x.y;
+    }
+    for (int k = 32; k; k >>= 1) sum += __shfl_xor(sum, k);
+    if ((tid & 63) == 0) red[tid >> 6] = sum;
+    __syncthreads();
+    sum = (red[0] + red[1]) + (red[2] + red[3]);
+    const int d = tid % TD * 4;
+    qe_f4 r = {0, 0, 0, 0};
+    for (int s = tid / TD; s < a.splits; s += GR) {
+        const float f = w_s[s];
+        if (f >= 0.f || f != f) r += f * *(const qe_f4 *)(a.part_o + (row0 + (size_t)s * a.group) * DH + d);
+    }
+    o_s[tid] = r;
+    __syncthreads();
+    if (tid < TD) {
+        for (int g = 1; g < GR; ++g) r += o_s[g * TD + tid];
+        r *= sum == 0.f ? 0.f : 1.f / sum;
+        if (bad) r = qe_f4{0, 0, 0, 0};
+        uint2 w;
+        w.x = pack2<BF>(r[0], r[1]);
+        w.y = pack2<BF>(r[2], r[3]);
+        *(uint2 *)((short *)a.out + (size_t)seq * a.out_stride + (size_t)head * DH + d) = w;
+    }
+}
+
+template <bool BF, int DH>
+static hipError_t launch_decode(const QeAttnArgs &a, hipStream_t st) {
+    k_attn_decode<BF, DH><<<dim3((unsigned)(a.n_seqs * a.kv_heads * a.splits)), dim3(256), 0, st>>>(a);
+    if (a.splits > 1) k_attn_join<BF, DH><<<dim3((unsigned)(a.n_seqs * a.q_heads)), dim3(256), 0, st>>>(a);
+    return hipGetLastError();
+}
+
+hipError_t qe_launch_attn_decode(const QeAttnArgs &a, int head_dim, int type, hipStream_t st) {
+    if (type == QE_BF16)
+        return head_dim == 64 ? launch_decode<true, 64>(a, st) : head_dim == 128 ? launch_decode<true, 128>(a, st) : launch_decode<true, 256>(a, st);
+    return head_dim == 64 ? launch_decode<false, 64>(a, st) : head_dim == 128 ? launch_decode<false, 128>(a, st) : launch_decode<false, 256>(a, st);
+}

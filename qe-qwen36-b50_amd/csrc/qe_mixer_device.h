@@ -1,0 +1,73 @@
+// Device helpers of the token mixers: 16-bit types on the matrix cores, page lookups.
+#pragma once
+#include "qe_mixer.h"
+
+typedef float qe_f2 __attribute__((ext_vector_type(2)));
+typedef float qe_f4 __attribute__((ext_vector_type(4)));
+typedef float qe_f16v __attribute__((ext_vector_type(16)));
+typedef short qe_s4 __attribute__((ext_vector_type(4)));
+typedef short qe_s8 __attribute__((ext_vector_type(8)));
+typedef __bf16 qe_b8 __attribute__((ext_vector_type(8)));
+typedef _Float16 qe_h8 __attribute__((ext_vector_type(8)));
+typedef __bf16 qe_b2 __attribute__((ext_vector_type(2)));
+typedef _Float16 qe_h2 __attribute__((ext_vector_type(2)));
+
+#define QE_LDS(T, p) ((__attribute__((address_space(3))) T *)(p))
+#define QE_GLOBAL(T, p) ((const __attribute__((address_space(1))) T *)(p))
+
+// v_mfma_f32_16x16x32: A lane l supplies row l % 16, k = 8 (l / 16) .. + 7; B the same of
+// column l % 16; D has column l % 16, rows 4 (l / 16) .. + 3.
+// v_mfma_f32_32x32x16: A row l % 32, k = 8 (l / 32) .. + 7; D column l % 32, register i holds
+// row 8 (i / 4) + 4 (l / 32) + i % 4.
+template <bool BF>
+__device__ __forceinline__ qe_f4 mfma16(qe_s8 a, qe_s8 b, qe_f4 c) {
+    if constexpr (BF)
+        return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(qe_b8, a), __builtin_bit_cast(qe_b8, b), c, 0, 0, 0);
+    else
+        return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(qe_h8, a), __builtin_bit_cast(qe_h8, b), c, 0, 0, 0);
+}
+template <bool BF>
+__device__ __forceinline__ qe_f16v mfma32(qe_s8 a, qe_s8 b, qe_f16v c) {
+    if constexpr (BF)
+        return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(qe_b8, a), __builtin_bit_cast(qe_b8, b), c, 0, 0, 0);
+    else
+        return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(qe_h8, a), __builtin_bit_cast(qe_h8, b), c, 0, 0, 0);
+}
+
+// two floats to the 16-bit type, to nearest even
+template <bool BF>
+__device__ __forceinline__ unsigned pack2(float a, float b) {
+    if constexpr (BF)
+        return __builtin_bit_cast(unsigned, qe_b2{(__bf16)a, (__bf16)b});
+    else
+        return __builtin_bit_cast(unsigned, qe_h2{(_Float16)a, (_Float16)b});
+}
+template <bool BF>
+__device__ __forceinline__ float from16(short x) {
+    if constexpr (BF)
+        return __uint_as_float((unsigned)(unsigned short)x << 16);
+    else
+        return (float)__builtin_bit_cast(_Float16, x);
+}
+
+// Transposing LDS read: of each 16 lanes, lane l addresses 4 elements of row l / 4 (columns
+// 4 (l % 4) .. + 3) and gets column l of the four rows.
+__device__ __forceinline__ qe_s4 lds_tr(const short *p) {
+    return __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) qe_s4 *)p);
+}
+// 64 lanes x 16 bytes from global memory straight to LDS: lane l's land at dst + 16 l
+__device__ __forceinline__ void load_lds16(const void *src, void *dst) {
+    __builtin_amdgcn_global_load_lds(QE_GLOBAL(void, src), QE_LDS(void, dst), 16, 0, 0);
+}
+
+__device__ __forceinline__ void report(unsigned *err, unsigned what) {
+    __hip_atomic_store(err, what, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_SYSTEM);
+}
+
+// First row of the 16 positions from pos16 (a multiple of 16) on, of one key-value head: they
+// stand in one page.  A page id outside the cache becomes page 0 and sets *bad.  Wave-uniform.
+__device__ __forceinline__ size_t sub_row(const QeAttnArgs &a, const int32_t *table, int kvh, int pos16, unsigned *bad) {
+    unsigned p = (unsigned)__builtin_amdgcn_readfirstlane(table[pos16 >> a.page_log2]);
+    if (p >= a.n_pages) *bad = 1, p = 0;
+    return (((size_t)p * a.kv_heads + kvh) << a.page_log2) + (pos16 & ((1 << a.page_log2) - 1));
+}

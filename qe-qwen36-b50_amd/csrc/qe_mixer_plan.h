@@ -1,0 +1,83 @@
+// How a call of the token mixers is cut into workgroups, and which values from device
+// memory are used.  Plain C++ that the launchers, the kernels and the CPU tests share.
+#pragma once
+#include <stdint.h>
+
+#ifdef __HIPCC__
+#define QE_MIX_HD __host__ __device__ __forceinline__
+#else
+#define QE_MIX_HD static inline
+#endif
+
+// ---- attention ----------------------------------------------------------------
+#define QE_ATTN_SUB 16     /* keys that share one page lookup: the smallest page */
+#define QE_ATTN_TILE 32    /* keys of a decode wave's step */
+#define QE_ATTN_WGS 512    /* workgroups a call is split up to: two for each of the 256 CUs */
+#define QE_ATTN_BN 64      /* keys of a prompt workgroup's step */
+#define QE_ATTN_PART_WGS 1024 /* partial results a decode call can need (see qe_attn_decode_splits) */
+
+// Splits of every sequence's length in a decode call: as many as make QE_ATTN_WGS workgroups,
+// but no more than one per 128 positions (four waves' steps).  units = n_seqs * kv_heads;
+// with more than one split units < QE_ATTN_WGS and units * splits < QE_ATTN_WGS + units.
+QE_MIX_HD int qe_attn_decode_splits(int64_t units, int64_t max_len) {
+    const int64_t most = (max_len + 127) / 128, want = (QE_ATTN_WGS + units - 1) / units;
+    const int64_t s = want < most ? want : most;
+    return s < 1 ? 1 : (int)s;
+}
+
+// Query rows of a prompt call are its tokens times the heads that share a key-value head,
+// and a workgroup takes `bm` of one sequence.  Tile numbers are handed out so that the
+// launch needs no lengths from the device: sequence i's tiles start at first(i) =
+// cu[i] * group / bm + i, and since floor(a + b) + 1 >= floor(a) + ceil(b) they end before
+// first(i + 1).  Numbers between are of no sequence and do nothing.
+QE_MIX_HD int qe_attn_first_tile(int cu, int i, int group, int bm) { return (int)((int64_t)cu * group / bm) + i; }
+QE_MIX_HD int qe_attn_max_tiles(int n_tokens, int n_seqs, int group, int bm) {
+    return (int)((int64_t)n_tokens * group / bm) + n_seqs;
+}
+
+// Splits of a prompt call's keys: none if its tiles fill half the CUs.
+QE_MIX_HD int qe_attn_prompt_splits(int64_t tiles, int64_t max_len) {
+    if (tiles > 128) return 1;
+    const int64_t most = (max_len + 255) / 256, want = QE_ATTN_WGS / tiles;
+    const int64_t s = want < most ? want : most;
+    return s < 1 ? 1 : (int)s;
+}
+
+// The part [*lo, *hi) of n steps that split s of `splits` takes.
+QE_MIX_HD void qe_split_range(int n, int splits, int s, int *lo, int *hi) {
+    const int per = (n + splits - 1) / splits;
+    const int64_t a = (int64_t)s * per, b = a + per;
+    *lo = a < n ? (int)a : n;
+    *hi = b < n ? (int)b : n;
+}
+
+// A length or offset from device memory that is outside lo .. hi becomes `other`, and *bad is set.
+QE_MIX_HD int qe_checked(int v, int lo, int hi, int other, unsigned *bad) {
+    if (v < lo || v > hi) {
+        *bad = 1;
+        return other;
+    }
+    return v;
+}
+
+// ---- gated delta rule ------------------------------------------------------------
+#define QE_DELTA_C 64                     /* tokens of a chunk */
+#define QE_DELTA_WS (2 * 64 * 64 + 4 * 64) /* floats kept per chunk and value head */
+
+// Chunk numbers are handed out as a prompt's tiles are: sequence i's start at first(i).
+QE_MIX_HD int qe_delta_first_chunk(int cu, int i) { return cu / QE_DELTA_C + i; }
+QE_MIX_HD int qe_delta_max_chunks(int n_tokens, int n_seqs) { return n_tokens / QE_DELTA_C + n_seqs; }
+
+// Whether sequence i of a call may be computed: its slots are in the pool (or -1), and nobody
+// else reads the slot it writes, and no earlier one writes it.  0, or what is wrong: the two
+// values below.  Of the sequences that are computed no two touch a slot that one of them
+// writes: a later writer of the same slot is refused, and so is the writer of a slot that
+// any other sequence reads.
+#define QE_SLOT_OUTSIDE 1
+#define QE_SLOT_SHARED 2
+QE_MIX_HD int qe_slot_pair(int64_t n_slots, int in_i, int out_i) {
+    return in_i < -1 || in_i >= n_slots || out_i < -1 || out_i >= n_slots ? QE_SLOT_OUTSIDE : 0;
+}
+QE_MIX_HD int qe_slot_conflict(int i, int out_i, int j, int in_j, int out_j) {
+    return out_i >= 0 && j != i && (in_j == out_i || (j < i && out_j == out_i)) ? QE_SLOT_SHARED : 0;
+}
