@@ -14,7 +14,13 @@
 // k_delta_scan then walks a sequence's chunks with the state in registers, a workgroup per
 // (sequence, value head, 16 columns of the state).
 //
-// State, sums and products are in 32 bits, b in 64 (a difference of two long sums).
+// State and sums are in 32 bits, b in 64 (a difference of two long sums).  Products run on the bf16
+// matrix cores at 32-bit precision: an operand is cut into planes of 8 significant bits, x = x0 + x1
+// + x2 (bf16 inputs are one plane, fp16 two, fp32 three), and of the planes' products, each exact
+// and summed in 32 bits, those down to 2^-16 of the largest are taken; what is left out is
+// a rounding of 32 bits.  Six such products of 16x16x32 take 96 cycles where v_mfma_f32_16x16x4
+// takes 256 (bf16 inputs: three products, 48).  Results in 16 bits need two planes less
+// exactly: see NO below.
 #include "qe_mixer_device.h"
 
 template <typename T>
@@ -37,6 +43,45 @@ __device__ __forceinline__ qe_f4 mma4(qe_f4 a, qe_f4 b, qe_f4 c) {
 }
 
 __device__ __forceinline__ float log_decay(float g) { return g < -1e4f ? -1e4f : g; } // e^-1e4 is 0; a NaN stays
+
+// Planes of a type's values, and planes that the product for the outputs takes of S, M and U.
+template <typename T>
+constexpr int planes_of() { return sizeof(T) == 4 ? 3 : __is_same(T, __bf16) ? 1 : 2; }
+
+__device__ __forceinline__ short bf16_bits(float x) { return __builtin_bit_cast(short, (__bf16)x); }
+// the next plane of x, which is taken off it
+__device__ __forceinline__ short next_plane(float &x) {
+    const __bf16 h = (__bf16)x;
+    x -= (float)h;
+    return __builtin_bit_cast(short, h);
+}
+// 4 values to N planes, `apart` elements from each other.  Planes are cut off here, not rounded
+// (8 bits of 24 each): half the instructions, in the chain that bounds a prompt.  The matrices
+// that they meet are rounded, so what is left out of a product has no sign of its own.
+template <int N>
+__device__ __forceinline__ void put4(short *p, int apart, qe_f4 x) {
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+        unsigned u[4];
+        for (int j = 0; j < 4; ++j) u[j] = __float_as_uint(x[j]);
+        uint2 h;
+        h.x = __builtin_amdgcn_perm(u[1], u[0], 0x07060302);
+        h.y = __builtin_amdgcn_perm(u[3], u[2], 0x07060302);
+        *(uint2 *)(p + i * apart) = h;
+        if (i + 1 < N)
+            for (int j = 0; j < 4; ++j) x[j] -= __uint_as_float(u[j] & 0xffff0000u);
+    }
+}
+// Products of planes i of a and j of b with i + j <= LIM, summed apart by size: the sums of many
+// small ones are then as exact as the large one's, and the chains overlap.
+template <int NA, int NB, int LIM>
+__device__ __forceinline__ void mul_planes(const qe_s8 *a, const qe_s8 *b, qe_f4 *acc) {
+#pragma unroll
+    for (int i = 0; i < NA; ++i)
+#pragma unroll
+        for (int j = 0; j < NB; ++j)
+            if (i + j <= LIM) acc[i + j] = mfma16<true>(a[i], b[j], acc[i + j]);
+}
 
 // ---------------------------------------------------------------------------
 // Which sequences of a call are computed (rules in qe_mixer_plan.h).
@@ -133,15 +178,41 @@ __global__ __launch_bounds__(256) void k_delta_decode(const QeDeltaArgs a) {
 // ---------------------------------------------------------------------------
 // T and M of every chunk, a workgroup per (chunk, key head).  K K^T and Q K^T are shared by the
 // key head's value heads.  Wave w has rows 16 w .. + 15.  The inverse of I + A by blocks of
-// 16: the diagonal ones by substitution, a lane per column; then by distance from the
-// diagonal T_ij = -T_ii sum_k A_ik T_kj.
-// Workspace of a chunk and value head: T [64][64], M [64][64] (blocks above the diagonal are not
-// written), then per token e^b / |k|, scale e^b / |q|, e^(b_last - b) / |k|, and e^(b_last).
+// 16, in 32 bits: the diagonal ones by substitution, a lane per column; then by distance
+// from the diagonal T_ij = -T_ii sum_k A_ik T_kj.
+// Workspace of a chunk and value head, as k_delta_scan's waves load it: T's planes and M's, each
+// [wave][32 columns][plane][lane][8] (columns that lie above the diagonal for all of a wave's rows
+// are not written), then per token e^b / |k|, scale e^b / |q|, e^(b_last - b) / |k|, and
+// e^(b_last).  fp16 and fp32 keys and queries are cut into planes here too, for a chunk and key
+// head: K [plane][64][DK] as it lies in LDS, Q [wave][32 of DK][plane][lane][8].
 // ---------------------------------------------------------------------------
+template <int DK>
+__device__ __forceinline__ int key_swz(int row) { // of the 16-byte chunk index: 8 rows' pairs of chunks in different banks
+    return DK == 64 ? ((row >> 1) & 3) << 1 : (row & 7) << 1;
+}
+
+template <typename IN>
+__device__ __forceinline__ void load8_planes(const IN *p, bool there, qe_s8 *h, float &square) {
+    constexpr int NP = planes_of<IN>();
+    float x[8];
+    if constexpr (sizeof(IN) == 4) {
+        const qe_f4 a = there ? *(const qe_f4 *)p : qe_f4{0, 0, 0, 0}, b = there ? *(const qe_f4 *)(p + 4) : qe_f4{0, 0, 0, 0};
+        for (int i = 0; i < 4; ++i) x[i] = a[i], x[4 + i] = b[i];
+    } else {
+        const qe_s8 a = there ? *(const qe_s8 *)p : qe_s8{};
+        for (int i = 0; i < 8; ++i) x[i] = from16<__is_same(IN, __bf16)>(a[i]);
+        if constexpr (NP == 1) h[0] = a;
+    }
+    for (int i = 0; i < 8; ++i) square += x[i] * x[i];
+    if constexpr (NP > 1)
+        for (int n = 0; n < NP; ++n)
+            for (int i = 0; i < 8; ++i) h[n][i] = next_plane(x[i]);
+}
+
 template <typename IN, int DK>
 __global__ __launch_bounds__(256) void k_delta_chunks(const QeDeltaArgs a) {
-    constexpr int LD = 68, KS = DK / 16;
-    __shared__ __align__(16) float A[64 * LD], T[64 * LD];
+    constexpr int LD = 68, KS = DK / 32, NP = planes_of<IN>(), NO = sizeof(IN) == 4 ? 3 : 2;
+    __shared__ __align__(16) float A[64 * LD], T[64 * LD], M[64 * LD];
     __shared__ double b_s[64];
     __shared__ float kk_s[64], rk_s[64], rq_s[64], beta_s[64];
     const int tid = threadIdx.x, wave = tid >> 6, lane = tid & 63, r = lane & 15, c = lane >> 4;
@@ -158,44 +229,58 @@ __global__ __launch_bounds__(256) void k_delta_chunks(const QeDeltaArgs a) {
     if (bad || a.skip[seq] || local < 0 || local * QE_DELTA_C >= end - begin) return; // uniform
     const int t0 = begin + (int)local * QE_DELTA_C, n = end - t0 < QE_DELTA_C ? end - t0 : QE_DELTA_C;
 
-    const IN *q = (const IN *)a.q + (size_t)kh * DK + 4 * c, *k = (const IN *)a.k + (size_t)kh * DK + 4 * c;
+    const IN *q = (const IN *)a.q + (size_t)kh * DK + 8 * c, *k = (const IN *)a.k + (size_t)kh * DK + 8 * c;
     const int row = 16 * wave + r;
-    qe_f4 kr[KS], qr[KS];
-    float kk = 0, qq = 0;
-    for (int s = 0; s < KS; ++s) {
-        kr[s] = row < n ? load4(k + (size_t)(t0 + row) * a.k_stride + 16 * s) : qe_f4{0, 0, 0, 0};
-        qr[s] = row < n ? load4(q + (size_t)(t0 + row) * a.q_stride + 16 * s) : qe_f4{0, 0, 0, 0};
-        for (int j = 0; j < 4; ++j) kk += kr[s][j] * kr[s][j], qq += qr[s][j] * qr[s][j];
-    }
-    kk += __shfl_xor(kk, 16), qq += __shfl_xor(qq, 16);
-    kk += __shfl_xor(kk, 32), qq += __shfl_xor(qq, 32);
-    if (lane < 16) {
-        kk_s[row] = kk;
-        rk_s[row] = a.l2norm ? 1.f / sqrtf(kk + 1e-6f) : 1.f;
-        rq_s[row] = (a.l2norm ? 1.f / sqrtf(qq + 1e-6f) : 1.f) * a.scale;
-    }
     qe_f4 gk[4], gq[4]; // K K^T and Q K^T, blocks 0 .. wave of the wave's rows
+    {
+        qe_s8 kr[KS][NP], qr[KS][NP];
+        float kk = 0, qq = 0;
 #pragma unroll
-    for (int cb = 0; cb < 4; ++cb) {
-        gk[cb] = gq[cb] = qe_f4{0, 0, 0, 0};
-        if (cb > wave) continue;
-        const int col = 16 * cb + r;
         for (int s = 0; s < KS; ++s) {
-            const qe_f4 kb = col < n ? load4(k + (size_t)(t0 + col) * a.k_stride + 16 * s) : qe_f4{0, 0, 0, 0};
-            gk[cb] = mma4(kr[s], kb, gk[cb]);
-            gq[cb] = mma4(qr[s], kb, gq[cb]);
+            load8_planes(k + (size_t)(t0 + row) * a.k_stride + 32 * s, row < n, kr[s], kk);
+            load8_planes(q + (size_t)(t0 + row) * a.q_stride + 32 * s, row < n, qr[s], qq);
+            if constexpr (NP > 1) {
+                short *ws = a.ws_kq + ((size_t)chunk * a.k_heads + kh) * 2 * NP * 64 * DK;
+                for (int i = 0; i < NP; ++i) {
+                    *(qe_s8 *)(ws + (i * 64 + row) * DK + (((4 * s + c) ^ key_swz<DK>(row)) << 3)) = kr[s][i];
+                    *(qe_s8 *)(ws + NP * 64 * DK + ((wave * KS + s) * NP + i) * 512 + lane * 8) = qr[s][i];
+                }
+            }
+        }
+        kk += __shfl_xor(kk, 16), qq += __shfl_xor(qq, 16);
+        kk += __shfl_xor(kk, 32), qq += __shfl_xor(qq, 32);
+        if (lane < 16) {
+            kk_s[row] = kk;
+            rk_s[row] = a.l2norm ? 1.f / sqrtf(kk + 1e-6f) : 1.f;
+            rq_s[row] = (a.l2norm ? 1.f / sqrtf(qq + 1e-6f) : 1.f) * a.scale;
+        }
+#pragma unroll
+        for (int cb = 0; cb < 4; ++cb) {
+            if (cb > wave) continue;
+            const int col = 16 * cb + r;
+            qe_f4 k3[3] = {}, q3[3] = {};
+#pragma unroll
+            for (int s = 0; s < KS; ++s) {
+                qe_s8 kb[NP];
+                float unused = 0;
+                load8_planes(k + (size_t)(t0 + col) * a.k_stride + 32 * s, col < n, kb, unused);
+                mul_planes<NP, NP, 2>(kr[s], kb, k3);
+                mul_planes<NP, NP, 2>(qr[s], kb, q3);
+            }
+            gk[cb] = k3[0] + (k3[1] + k3[2]);
+            gq[cb] = q3[0] + (q3[1] + q3[2]);
         }
     }
     for (int gi = 0; gi < a.group; ++gi) {
         const int head = kh * a.group + gi;
-        float *ws = a.ws + ((size_t)chunk * a.v_heads + head) * QE_DELTA_WS;
+        float *ws = a.ws + ((size_t)chunk * a.v_heads + head) * QE_DELTA_WS, *factors = ws + QE_DELTA_WS - 256;
         double b = lane < n ? (double)log_decay(a.g[(size_t)(t0 + lane) * a.v_heads + head]) : 0.0;
         for (int d = 1; d < 64; d <<= 1) {
             const double up = __shfl_up(b, d);
             if (lane >= d) b += up;
         }
         float beta = lane < n ? a.beta[(size_t)(t0 + lane) * a.v_heads + head] : 0.f;
-        __syncthreads(); // rk_s and rq_s are written, the last head's b_s, beta_s, A and T are read
+        __syncthreads(); // rk_s and rq_s are written, the last head's b_s, beta_s, T and M are read
         // A product of 0 and an infinity or NaN is NaN, and in a block above the diagonal's zeros it would
         // reach tokens before its own.  So from the first token whose key, gate or decay is not finite on
         // (what comes after it is not finite either) the matrices are zeros and the factors NaN.
@@ -210,21 +295,22 @@ __global__ __launch_bounds__(256) void k_delta_chunks(const QeDeltaArgs a) {
         if (wave == 1) {
             const double last = __shfl(b, 63);
             const float e = expf((float)b), none = lane < fine ? 0.f : NAN;
-            ws[2 * 4096 + lane] = e * rk_s[lane] + none;
-            ws[2 * 4096 + 64 + lane] = e * rq_s[lane] + none;
-            ws[2 * 4096 + 128 + lane] = expf((float)(last - b)) * rk_s[lane] + (fine < 64 ? NAN : 0.f);
-            if (lane == 0) ws[2 * 4096 + 192] = expf((float)last) + (fine < 64 ? NAN : 0.f);
+            factors[lane] = e * rk_s[lane] + none;
+            factors[64 + lane] = e * rq_s[lane] + none;
+            factors[128 + lane] = expf((float)(last - b)) * rk_s[lane] + (fine < 64 ? NAN : 0.f);
+            if (lane == 0) factors[192] = expf((float)last) + (fine < 64 ? NAN : 0.f);
         }
         __syncthreads();
 #pragma unroll
         for (int cb = 0; cb < 4; ++cb) {
-            if (cb > wave) continue;
+            if (cb > (wave | 1)) continue; // and zeros to the right of the diagonal in its 32 columns
             for (int i = 0; i < 4; ++i) {
                 const int ri = 16 * wave + 4 * c + i, cj = 16 * cb + r;
-                const bool in = cj <= ri && ri < fine;
+                const bool in = cb <= wave && cj <= ri && ri < fine;
                 const float fade = in ? expf((float)(b_s[ri] - b_s[cj])) * rk_s[cj] : 0.f;
-                ws[4096 + ri * 64 + cj] = in ? gq[cb][i] * fade * rq_s[ri] : 0.f;
+                M[ri * LD + cj] = in ? gq[cb][i] * fade * rq_s[ri] : 0.f;
                 A[ri * LD + cj] = in && cj < ri ? gk[cb][i] * fade * (rk_s[ri] * beta_s[ri]) : 0.f;
+                if (cb > wave) T[ri * LD + cj] = 0.f;
             }
         }
         __syncthreads();
@@ -256,125 +342,257 @@ __global__ __launch_bounds__(256) void k_delta_chunks(const QeDeltaArgs a) {
             }
         }
         __syncthreads();
-        for (int i = 0; i < 4; ++i) {
-            const int ri = 16 * wave + 4 * i + c, cj = 4 * r;
-            if (cj / 16 > wave) continue;
-            qe_f4 t = *(const qe_f4 *)(T + ri * LD + cj);
-            for (int j = 0; j < 4; ++j) t[j] *= beta_s[cj + j];
-            *(qe_f4 *)(ws + ri * 64 + cj) = t;
+        // 8 columns of a row at a time to the planes: wave w has rows 16 w .. + 15, in steps of 8
+        for (int i = 0; i < 2; ++i) {
+            const int ri = 16 * wave + 8 * i + (lane >> 3), cj = (lane & 7) * 8;
+            if (cj / 32 > wave / 2) continue;
+            float t[8], m[8];
+            for (int j = 0; j < 8; ++j) {
+                t[j] = T[ri * LD + cj + j] * beta_s[cj + j];
+                m[j] = M[ri * LD + cj + j];
+            }
+            // the lane (cj % 32) / 8 * 16 + ri % 16 of the wave's operand for columns 32 (cj / 32) .. + 31
+            short *to = (short *)ws + (wave * 2 + cj / 32) * 1536 + ((cj % 32) / 8 * 16 + ri % 16) * 8;
+            for (int p = 0; p < 3; ++p) {
+                qe_s8 h;
+                for (int j = 0; j < 8; ++j) h[j] = next_plane(t[j]);
+                *(qe_s8 *)(to + p * 512) = h;
+            }
+            for (int p = 0; p < NO; ++p) {
+                qe_s8 h;
+                for (int j = 0; j < 8; ++j) h[j] = next_plane(m[j]);
+                *(qe_s8 *)(to + 12288 + p * 512) = h;
+            }
         }
     }
 }
 
 // ---------------------------------------------------------------------------
-// The walk over a sequence's chunks, 16 columns of a value head's state.  Wave w computes
-// rows 16 w .. + 15 of K S, Q S, U and O, and keeps rows DK / 4 w .. of the state.  What the
-// waves exchange (S, V - .. K S, U) goes through LDS transposed, [column][row], so that the
-// registers of a result are written, and an operand's read, 4 floats at a time.
+// The walk over a sequence's chunks, 16 columns of a value head's state: a workgroup of eight
+// waves.  The state's next value hangs on three products one after the other (K S, T times
+// what is left of V, K^T U), so waves 0 .. 3 do little else, 16 rows of the chunk and DK / 4
+// of the state each, and waves 4 .. 7 make the outputs of 16 rows each beside them.
+// What waves exchange (S, V - .. K S, U) goes through LDS as planes, transposed [column][row]: a
+// result's registers are 4 consecutive rows of its column, an operand's 8.  K lies in LDS in
+// two buffers, the next chunk's loaded directly while this one's is used: its rows are
+// the first product's operand, and transposing reads give the third's.
+// What bounds it: the chain of products, exchanges and barriers of a chunk, on 256 of the
+// GPU's 1024 SIMDs for each sequence (32 heads, 8 slices).  A load stalls the wave that issues it
+// while the CU's 64 bytes a cycle are taken (some 65 KiB a chunk), so the loads are few and
+// wide, and spread over the waves and over the chunk.
 // ---------------------------------------------------------------------------
 template <typename IN, int DK, int DV>
-__global__ __launch_bounds__(256) void k_delta_scan(const QeDeltaArgs a) {
-    constexpr int KS = DK / 16, SB = DK / 64, LK = DK + 4, LT = 68;
-    __shared__ __align__(16) float k_s[2][64 * LK], s_t[16 * LK], r_t[16 * LT], u_t[16 * LT];
+__global__ __launch_bounds__(512) void k_delta_scan(const QeDeltaArgs a) {
+    constexpr int KS = DK / 32, SB = DK / 64, LS = DK + 8, LT = 72, NP = planes_of<IN>(), NO = sizeof(IN) == 4 ? 3 : 2;
+    constexpr int SL = DV / 16, VL = 16 / sizeof(IN); // elements of V in 16 bytes
+    // what is loaded ahead has two buffers, variables of their own: else the compiler has every LDS read wait for
+    // the direct loads in flight
+    __shared__ __align__(16) short k_even[NP * 64 * DK], k_odd[NP * 64 * DK];
+    __shared__ __align__(16) IN v_even[64 * 16], v_odd[64 * 16];
+    __shared__ __align__(16) float f_even[256], f_odd[256];
+    __shared__ __align__(16) short s_p[3 * 16 * LS], r_p[3 * 16 * LT], u_p[NO * 16 * LT], w_p[3 * 16 * LT];
     __shared__ int odd_s[2][16]; // of each column: the chunk's first token with a value that is not finite, or 64
-    const int tid = threadIdx.x, wave = tid >> 6, lane = tid & 63, r = lane & 15, c = lane >> 4;
-    const int slice = blockIdx.x % (DV / 16), head = blockIdx.x / (DV / 16) % a.v_heads, seq = blockIdx.x / (DV / 16) / a.v_heads;
+    const int tid = threadIdx.x, wave = (tid >> 6) & 3, lane = tid & 63, r = lane & 15, c = lane >> 4;
+    const bool chain = tid < 256;
+    const int seq = blockIdx.x / (SL * a.v_heads), at = blockIdx.x - seq * SL * a.v_heads;
+    // Workgroups go to the eight XCDs in turn: a head's slices, which read the same K, Q, T and M, to one L2.
+    const bool eights = a.v_heads % 8 == 0;
+    const int slice = eights ? at / 8 % SL : at % SL, head = eights ? at / (8 * SL) * 8 + at % 8 : at / SL;
     const int kh = head / a.group, col = slice * 16 + r;
     unsigned bad = 0;
     const int begin = qe_checked(a.cu[seq], 0, a.n_tokens, 0, &bad), end = qe_checked(a.cu[seq + 1], begin, a.n_tokens, begin, &bad);
     if (bad && tid == 0) report(a.err, QE_BAD_LENGTH);
     if (bad | a.skip[seq]) {
-        for (int t = begin + (tid >> 4); t < end; t += 16) ((IN *)a.out)[(size_t)t * a.out_stride + (size_t)head * DV + slice * 16 + (tid & 15)] = (IN)0.f;
+        for (int t = begin + (tid >> 4); t < end; t += 32) ((IN *)a.out)[(size_t)t * a.out_stride + (size_t)head * DV + slice * 16 + (tid & 15)] = (IN)0.f;
         return;
     }
     const int in_i = a.slots_in[seq], out_i = a.slots_out[seq];
-    qe_f4 S[SB];
-    for (int i = 0; i < SB; ++i)
-        for (int j = 0; j < 4; ++j)
-            S[i][j] = in_i < 0 ? 0.f : a.pool[(((size_t)in_i * a.v_heads + head) * DK + 16 * (wave * SB + i) + 4 * c + j) * DV + col];
-
-    const IN *q = (const IN *)a.q + (size_t)kh * DK + 4 * c, *k = (const IN *)a.k + (size_t)kh * DK + 4 * c;
-    const float *ws = a.ws + ((size_t)qe_delta_first_chunk(a.cu[seq], seq) * a.v_heads + head) * QE_DELTA_WS;
-    int par = 0;
+    const int chunk0 = qe_delta_first_chunk(begin, seq), row = 16 * wave + r, kb = wave / 2; // kb: the last 32 columns that the wave's rows reach
+    const short *ws = (const short *)(a.ws + ((size_t)chunk0 * a.v_heads + head) * QE_DELTA_WS);
+    const size_t ws_step = (size_t)a.v_heads * QE_DELTA_WS * 2;
+    const short *kq = NP == 1 ? nullptr : a.ws_kq + ((size_t)chunk0 * a.k_heads + kh) * 2 * NP * 64 * DK;
+    const size_t kq_step = (size_t)a.k_heads * 2 * NP * 64 * DK;
     if (tid < 32) odd_s[tid >> 4][tid & 15] = 64;
-    // As in k_delta_chunks, what is not finite must not meet the zeros above the diagonal: it becomes
-    // 0, and its column's outputs from that token on, and its state, NaN.
-    auto cleared = [&](qe_f4 x, int p) {
-        bool odd = false;
-        for (int j = 0; j < 4; ++j) odd |= !__builtin_isfinite(x[j]);
-        if (__any(odd)) {
-            for (int j = 0; j < 4; ++j)
-                if (!__builtin_isfinite(x[j])) {
-                    x[j] = 0.f;
-                    atomicMin(&odd_s[p][r], 16 * wave + 4 * c + j);
-                }
-        }
-        return x;
-    };
-    for (int t0 = begin; t0 < end; t0 += QE_DELTA_C, ws += (size_t)a.v_heads * QE_DELTA_WS, par ^= 1) {
-        const int n = end - t0 < QE_DELTA_C ? end - t0 : QE_DELTA_C, row = 16 * wave + r;
-        qe_f4 kr[KS], qr[KS], tr[4], mr[4], v;
-        for (int s = 0; s < KS; ++s) {
-            kr[s] = row < n ? load4(k + (size_t)(t0 + row) * a.k_stride + 16 * s) : qe_f4{0, 0, 0, 0};
-            qr[s] = row < n ? load4(q + (size_t)(t0 + row) * a.q_stride + 16 * s) : qe_f4{0, 0, 0, 0};
-        }
-#pragma unroll
-        for (int s = 0; s < 4; ++s) {
-            if (s > wave) continue;
-            tr[s] = *(const qe_f4 *)(ws + row * 64 + 16 * s + 4 * c);
-            mr[s] = *(const qe_f4 *)(ws + 4096 + row * 64 + 16 * s + 4 * c);
-        }
-        for (int j = 0; j < 4; ++j) {
-            const int t = 16 * wave + 4 * c + j;
-            v[j] = t < n ? (float)((const IN *)a.v)[(size_t)(t0 + t) * a.v_stride + (size_t)head * DV + col] : 0.f;
-        }
-        const qe_f4 cx = *(const qe_f4 *)(ws + 2 * 4096 + 16 * wave + 4 * c), cq = *(const qe_f4 *)(ws + 2 * 4096 + 64 + 16 * wave + 4 * c);
-        const float last = ws[2 * 4096 + 192];
-        for (int i = 0; i < SB; ++i) *(qe_f4 *)(s_t + r * LK + 16 * (wave * SB + i) + 4 * c) = S[i];
-        for (int s = 0; s < KS; ++s) *(qe_f4 *)(k_s[par] + row * LK + 16 * s + 4 * c) = kr[s];
-        __syncthreads();
-        qe_f4 ks = {0, 0, 0, 0}, qs = {0, 0, 0, 0};
-#pragma unroll
-        for (int s = 0; s < KS; ++s) {
-            const qe_f4 b = *(const qe_f4 *)(s_t + r * LK + 16 * s + 4 * c);
-            ks = mma4(kr[s], b, ks);
-            qs = mma4(qr[s], b, qs);
-        }
-        *(qe_f4 *)(r_t + r * LT + 16 * wave + 4 * c) = cleared(v - cx * ks, par);
-        __syncthreads();
-        qe_f4 u = {0, 0, 0, 0};
-#pragma unroll
-        for (int s = 0; s < 4; ++s)
-            if (s <= wave) u = mma4(tr[s], *(const qe_f4 *)(r_t + r * LT + 16 * s + 4 * c), u);
-        *(qe_f4 *)(u_t + r * LT + 16 * wave + 4 * c) = cleared(u, par);
-        __syncthreads();
-        const int odd = odd_s[par][r];
-        if (tid < 16) odd_s[par ^ 1][tid] = 64; // last read a chunk ago, next written in the next
-        qe_f4 o = cq * qs, us[4];
-#pragma unroll
-        for (int s = 0; s < 4; ++s) {
-            us[s] = *(const qe_f4 *)(u_t + r * LT + 16 * s + 4 * c);
-            if (s <= wave) o = mma4(mr[s], us[s], o);
-            us[s] *= *(const qe_f4 *)(ws + 2 * 4096 + 128 + 16 * s + 4 * c);
-        }
-        for (int j = 0; j < 4; ++j) {
-            const int t = 16 * wave + 4 * c + j;
-            if (t < n) ((IN *)a.out)[(size_t)(t0 + t) * a.out_stride + (size_t)head * DV + col] = (IN)(t < odd ? o[j] : NAN);
-        }
-#pragma unroll
-        for (int i = 0; i < SB; ++i) {
-            S[i] *= odd < 64 ? NAN : last;
-#pragma unroll
-            for (int s = 0; s < 4; ++s) {
-                qe_f4 kt;
-                for (int j = 0; j < 4; ++j) kt[j] = k_s[par][(16 * s + 4 * c + j) * LK + 16 * (wave * SB + i) + r];
-                S[i] = mma4(kt, us[s], S[i]);
+    // Loads run one chunk ahead; behind the last chunk they take it again, for a branch around them would have the
+    // compiler wait for all of them.  Rows behind the sequence's end are its last one's: T's columns and rows are
+    // zeros there.
+    if (chain) {
+        // As in k_delta_chunks, what is not finite must not meet the zeros above the diagonal: it becomes
+        // 0, and its column's outputs from that token on, and its state, NaN.
+        auto cleared = [&](qe_f4 x, int p) {
+            bool odd = false;
+            for (int j = 0; j < 4; ++j) odd |= !__builtin_isfinite(x[j]);
+            if (__any(odd)) {
+                for (int j = 0; j < 4; ++j)
+                    if (!__builtin_isfinite(x[j])) {
+                        x[j] = 0.f;
+                        atomicMin(&odd_s[p][r], 16 * wave + 4 * c + j);
+                    }
             }
+            return x;
+        };
+        qe_f4 S[SB];
+        for (int i = 0; i < SB; ++i)
+            for (int j = 0; j < 4; ++j)
+                S[i][j] = in_i < 0 ? 0.f : a.pool[(((size_t)in_i * a.v_heads + head) * DK + 16 * (wave * SB + i) + 4 * c + j) * DV + col];
+        qe_s8 tf[2][3];
+        // waves 0 and 1, whose rows of T are short, also load V and the factors
+        auto load = [&](int t0, const short *w, IN *v_to, float *f_to) {
+            if (wave == 0) {
+                constexpr int PER = 16 / VL; // lanes of a row
+                for (int i = 0; i < PER; ++i) {
+                    const int t = t0 + i * (64 / PER) + lane / PER;
+                    load_lds16((const IN *)a.v + (size_t)(t < end ? t : end - 1) * a.v_stride + (size_t)head * DV + slice * 16 + lane % PER * VL, v_to + i * 64 * VL);
+                }
+            }
+            if (wave == 1) load_lds16((const float *)w + QE_DELTA_WS - 256 + lane * 4, f_to);
+            for (int p = 0; p < 3; ++p) {
+                tf[0][p] = *(const qe_s8 *)(w + wave * 3072 + p * 512 + lane * 8);
+                if (kb) tf[1][p] = *(const qe_s8 *)(w + wave * 3072 + 1536 + p * 512 + lane * 8);
+            }
+        };
+        auto step = [&](const int par, const short *k_s, const IN *v_s, const float *f_s, IN *v_next, float *f_next, int t0) {
+            for (int i = 0; i < SB; ++i) put4<3>(s_p + r * LS + 16 * (wave * SB + i) + 4 * c, 16 * LS, S[i]);
+            __builtin_amdgcn_s_waitcnt(0x0f70); // V and the factors have landed
+            lds_barrier();
+            qe_f4 x[3] = {};
+#pragma unroll
+            for (int s = 0; s < KS; ++s) {
+                qe_s8 kf[NP], sf[3];
+                for (int p = 0; p < NP; ++p) kf[p] = *(const qe_s8 *)(k_s + (p * 64 + row) * DK + (((4 * s + c) ^ key_swz<DK>(row)) << 3));
+                for (int p = 0; p < 3; ++p) sf[p] = *(const qe_s8 *)(s_p + (p * 16 + r) * LS + 32 * s + 8 * c);
+                mul_planes<NP, 3, 2>(kf, sf, x);
+            }
+            qe_f4 v;
+            if constexpr (sizeof(IN) == 2) {
+                const qe_s4 h = lds_tr((const short *)v_s + (16 * wave + 4 * c + (r >> 2)) * 16 + (r & 3) * 4);
+                for (int j = 0; j < 4; ++j) v[j] = from16<__is_same(IN, __bf16)>(h[j]);
+            } else {
+                for (int j = 0; j < 4; ++j) v[j] = v_s[(16 * wave + 4 * c + j) * 16 + r];
+            }
+            const qe_f4 cx = *(const qe_f4 *)(f_s + 16 * wave + 4 * c), cu = *(const qe_f4 *)(f_s + 128 + 16 * wave + 4 * c);
+            const float last = f_s[192];
+            put4<3>(r_p + r * LT + 16 * wave + 4 * c, 16 * LT, cleared(v - cx * (x[0] + (x[1] + x[2])), par));
+            lds_barrier();
+            qe_f4 u3[3] = {};
+#pragma unroll
+            for (int s = 0; s < 2; ++s) {
+                if (s > kb) continue;
+                qe_s8 rf[3];
+                for (int p = 0; p < 3; ++p) rf[p] = *(const qe_s8 *)(r_p + (p * 16 + r) * LT + 32 * s + 8 * c);
+                mul_planes<3, 3, 2>(tf[s], rf, u3);
+            }
+            const qe_f4 u = cleared(u3[0] + (u3[1] + u3[2]), par);
+            put4<3>(w_p + r * LT + 16 * wave + 4 * c, 16 * LT, u * cu);
+            put4<NO>(u_p + r * LT + 16 * wave + 4 * c, 16 * LT, u);
+            const int ahead = t0 + QE_DELTA_C < end;
+            ws += ahead * ws_step;
+            load(t0 + ahead * QE_DELTA_C, ws, v_next, f_next);
+            lds_barrier();
+            const int spoilt = odd_s[par][r];
+            if (tid < 16) odd_s[par ^ 1][tid] = 64; // last read a chunk ago, next written in the next
+            qe_s8 wf[2][3];
+#pragma unroll
+            for (int s = 0; s < 2; ++s)
+                for (int p = 0; p < 3; ++p) {
+                    const short *at = w_p + (p * 16 + r) * LT + 32 * s + 4 * c;
+                    const qe_s4 lo = *(const qe_s4 *)at, hi = *(const qe_s4 *)(at + 16);
+                    wf[s][p] = qe_s8{lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]};
+                }
+#pragma unroll
+            for (int i = 0; i < SB; ++i) {
+                qe_f4 d[3] = {};
+#pragma unroll
+                for (int s = 0; s < 2; ++s) {
+                    qe_s8 kt[NP];
+                    const int ra = 32 * s + 4 * c + (r >> 2), el = 16 * (wave * SB + i) + (r & 3) * 4;
+                    for (int p = 0; p < NP; ++p) {
+                        const short *at = k_s + (p * 64 + ra) * DK + (((el >> 3) ^ key_swz<DK>(ra)) << 3) + (el & 7);
+                        const qe_s4 lo = lds_tr(at), hi = lds_tr(at + 16 * DK); // 16 rows on the permutation is the same
+                        kt[p] = qe_s8{lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]};
+                    }
+                    mul_planes<NP, 3, 2>(kt, wf[s], d);
+                }
+                S[i] = S[i] * (spoilt < 64 ? NAN : last) + (d[0] + (d[1] + d[2]));
+            }
+        };
+        if (begin < end) load(begin, ws, v_even, f_even);
+        for (int t0 = begin; t0 < end; t0 += 2 * QE_DELTA_C) {
+            step(0, k_even, v_even, f_even, v_odd, f_odd, t0);
+            if (t0 + QE_DELTA_C < end) step(1, k_odd, v_odd, f_odd, v_even, f_even, t0 + QE_DELTA_C);
+        }
+        if (out_i >= 0)
+            for (int i = 0; i < SB; ++i)
+                for (int j = 0; j < 4; ++j) a.pool[(((size_t)out_i * a.v_heads + head) * DK + 16 * (wave * SB + i) + 4 * c + j) * DV + col] = S[i][j];
+    } else {
+        qe_s8 qf[KS][NP], mf[2][NO];
+        auto load_k = [&](int t0, const short *from, short *to) {
+            constexpr int ROWS = 512 / DK; // of one direct load
+#pragma unroll
+            for (int i = 0; i < NP * 16 / ROWS; ++i) {
+                const int p = i / (16 / ROWS), rr = wave * 16 + i % (16 / ROWS) * ROWS, mine = rr + lane / (DK / 8), ch = (lane % (DK / 8)) ^ key_swz<DK>(mine);
+                const short *src = NP == 1 ? (const short *)a.k + (size_t)(t0 + mine < end ? t0 + mine : end - 1) * a.k_stride + (size_t)kh * DK + ch * 8
+                                           : from + (p * 64 + rr) * DK + lane * 8;
+                load_lds16(src, to + (p * 64 + rr) * DK);
+            }
+        };
+        auto load_q = [&](int t0, const short *from) {
+            const short *q = (const short *)a.q + (size_t)(t0 + row < end ? t0 + row : end - 1) * a.q_stride + (size_t)kh * DK + 8 * c;
+            for (int s = 0; s < KS; ++s)
+                for (int p = 0; p < NP; ++p)
+                    qf[s][p] = *(const qe_s8 *)(NP == 1 ? q + 32 * s : from + NP * 64 * DK + ((wave * KS + s) * NP + p) * 512 + lane * 8);
+        };
+        auto load_m = [&](const short *w) {
+            for (int p = 0; p < NO; ++p) {
+                mf[0][p] = *(const qe_s8 *)(w + 12288 + wave * 3072 + p * 512 + lane * 8);
+                if (kb) mf[1][p] = *(const qe_s8 *)(w + 12288 + wave * 3072 + 1536 + p * 512 + lane * 8);
+            }
+        };
+        auto step = [&](const int par, const float *f_s, short *k_next, int t0) {
+            const int ahead = t0 + QE_DELTA_C < end;
+            // K has landed: younger than its direct loads are at least four loads of Q and M, and the last chunk's stores
+            __builtin_amdgcn_s_waitcnt(0x0f74);
+            lds_barrier();
+            qe_f4 x[3] = {};
+#pragma unroll
+            for (int s = 0; s < KS; ++s) {
+                qe_s8 sf[NO];
+                for (int p = 0; p < NO; ++p) sf[p] = *(const qe_s8 *)(s_p + (p * 16 + r) * LS + 32 * s + 8 * c);
+                mul_planes<NP, NO, NO - 1>(qf[s], sf, x);
+            }
+            qe_f4 o = *(const qe_f4 *)(f_s + 64 + 16 * wave + 4 * c) * (x[0] + (x[1] + x[2]));
+            kq += ahead * kq_step, ws += ahead * ws_step;
+            load_k(t0 + ahead * QE_DELTA_C, kq, k_next);
+            lds_barrier();
+            load_q(t0 + ahead * QE_DELTA_C, kq);
+            lds_barrier();
+            const int spoilt = odd_s[par][r];
+            qe_f4 y[3] = {};
+#pragma unroll
+            for (int s = 0; s < 2; ++s) {
+                if (s > kb) continue;
+                qe_s8 uf[NO];
+                for (int p = 0; p < NO; ++p) uf[p] = *(const qe_s8 *)(u_p + (p * 16 + r) * LT + 32 * s + 8 * c);
+                mul_planes<NO, NO, NO - 1>(mf[s], uf, y);
+            }
+            o += y[0] + (y[1] + y[2]);
+            load_m(ws);
+            for (int j = 0; j < 4; ++j) {
+                const int t = 16 * wave + 4 * c + j;
+                if (t0 + t < end) ((IN *)a.out)[(size_t)(t0 + t) * a.out_stride + (size_t)head * DV + col] = (IN)(t < spoilt ? o[j] : NAN);
+            }
+        };
+        if (begin < end) {
+            load_k(begin, kq, k_even);
+            load_q(begin, kq);
+            load_m(ws);
+            __builtin_amdgcn_s_waitcnt(0x0f70); // in whatever order they were issued here
+        }
+        for (int t0 = begin; t0 < end; t0 += 2 * QE_DELTA_C) {
+            step(0, f_even, k_odd, t0);
+            if (t0 + QE_DELTA_C < end) step(1, f_odd, k_even, t0 + QE_DELTA_C);
         }
     }
-    if (out_i >= 0)
-        for (int i = 0; i < SB; ++i)
-            for (int j = 0; j < 4; ++j) a.pool[(((size_t)out_i * a.v_heads + head) * DK + 16 * (wave * SB + i) + 4 * c + j) * DV + col] = S[i][j];
 }
 
 template <typename IN, int DK, int DV>
@@ -382,7 +600,7 @@ static hipError_t prompt(const QeDeltaArgs &a, hipStream_t st) {
     const unsigned chunks = (unsigned)qe_delta_max_chunks(a.n_tokens, a.n_seqs);
     k_delta_slots<<<dim3((unsigned)a.n_seqs), dim3(256), 0, st>>>(a);
     k_delta_chunks<IN, DK><<<dim3(chunks * a.k_heads), dim3(256), 0, st>>>(a);
-    k_delta_scan<IN, DK, DV><<<dim3((unsigned)a.n_seqs * a.v_heads * (DV / 16)), dim3(256), 0, st>>>(a);
+    k_delta_scan<IN, DK, DV><<<dim3((unsigned)a.n_seqs * a.v_heads * (DV / 16)), dim3(512), 0, st>>>(a);
     return hipGetLastError();
 }
 template <typename IN, int DK, int DV>

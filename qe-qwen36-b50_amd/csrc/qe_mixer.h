@@ -54,6 +54,7 @@ struct QeDeltaArgs {
     int l2norm;
     float scale;
     float *ws;           // [chunk][v_head][QE_DELTA_WS]: see qe_delta.hip
+    short *ws_kq;        // [chunk][k_head][K, Q][plane][64][dim_k], for types of more than one plane
     unsigned char *skip; // [n_seqs]: a sequence whose slots are bad
     unsigned *err;
 };

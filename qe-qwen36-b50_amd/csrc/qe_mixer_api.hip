@@ -298,11 +298,13 @@ struct qe_delta_ctx {
     float scale;
     ErrorWord err;
     float *ws = nullptr;
+    short *ws_kq = nullptr;
     unsigned char *skip = nullptr;
 };
 
 static void release(qe_delta_ctx *c) {
     (void)hipFree(c->ws);
+    (void)hipFree(c->ws_kq);
     (void)hipFree(c->skip);
     c->err.free();
     delete c;
@@ -331,7 +333,7 @@ static int delta_args(qe_delta_ctx *c, const qe_delta_args *x, const char *where
     a->n_seqs = x->n_seqs; a->n_tokens = x->n_tokens;
     a->k_heads = c->d.k_heads; a->v_heads = c->d.v_heads; a->group = c->d.v_heads / c->d.k_heads;
     a->l2norm = c->d.l2norm; a->scale = c->scale;
-    a->ws = c->ws; a->skip = c->skip; a->err = c->err.dev;
+    a->ws = c->ws; a->ws_kq = c->ws_kq; a->skip = c->skip; a->err = c->err.dev;
     return QE_OK;
 }
 
@@ -358,6 +360,8 @@ int qe_delta_create(int device, const qe_delta_desc *d, qe_delta_ctx **out) {
     hipError_t e = c->err.make();
     const size_t chunks = (size_t)qe_delta_max_chunks(d->t_max, d->seqs_max);
     if (e == hipSuccess) e = hipMalloc((void **)&c->ws, chunks * d->v_heads * QE_DELTA_WS * 4);
+    const size_t kept = (size_t)qe_delta_kept_planes((int)size_of(d->type), d->type == QE_BF16) * 2 * QE_DELTA_C * d->dim_k * 2;
+    if (e == hipSuccess && kept) e = hipMalloc((void **)&c->ws_kq, chunks * d->k_heads * kept);
     if (e == hipSuccess) e = hipMalloc((void **)&c->skip, (size_t)d->seqs_max);
     if (e != hipSuccess) {
         release(c);

@@ -60,6 +60,10 @@ __device__ __forceinline__ void load_lds16(const void *src, void *dst) {
     __builtin_amdgcn_global_load_lds(QE_GLOBAL(void, src), QE_LDS(void, dst), 16, 0, 0);
 }
 
+// A workgroup's barrier for what it exchanges through LDS.  __syncthreads() would also wait for
+// all global loads and direct loads in flight, which here are meant for later.
+__device__ __forceinline__ void lds_barrier() { asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory"); }
+
 __device__ __forceinline__ void report(unsigned *err, unsigned what) {
     __hip_atomic_store(err, what, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_SYSTEM);
 }

@@ -62,10 +62,12 @@ QE_MIX_HD int qe_checked(int v, int lo, int hi, int other, unsigned *bad) {
 
 // ---- gated delta rule ------------------------------------------------------------
 #define QE_DELTA_C 64                     /* tokens of a chunk */
-#define QE_DELTA_WS (2 * 64 * 64 + 4 * 64) /* floats kept per chunk and value head */
+#define QE_DELTA_WS (6 * 64 * 64 / 2 + 4 * 64) /* floats kept per chunk and value head: six planes of 16 bits, four vectors */
 
 // Chunk numbers are handed out as a prompt's tiles are: sequence i's start at first(i).
 QE_MIX_HD int qe_delta_first_chunk(int cu, int i) { return cu / QE_DELTA_C + i; }
+// 16-bit planes that keys and queries are cut into and kept as; bf16 ones are one as they stand.
+QE_MIX_HD int qe_delta_kept_planes(int bytes, int is_bf16) { return is_bf16 ? 0 : bytes == 4 ? 3 : 2; }
 QE_MIX_HD int qe_delta_max_chunks(int n_tokens, int n_seqs) { return n_tokens / QE_DELTA_C + n_seqs; }
 
 // Whether sequence i of a call may be computed: its slots are in the pool (or -1), and nobody
