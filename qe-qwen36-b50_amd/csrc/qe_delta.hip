@@ -388,11 +388,12 @@ __global__ __launch_bounds__(512) void k_delta_scan(const QeDeltaArgs a) {
     // what is loaded ahead has two buffers, variables of their own: else the compiler has every LDS read wait for
     // the direct loads in flight
     __shared__ __align__(16) short k_even[NP * 64 * DK], k_odd[NP * 64 * DK];
-    __shared__ __align__(16) IN v_even[64 * 16], v_odd[64 * 16];
-    __shared__ __align__(16) float f_even[256], f_odd[256];
+    constexpr int VW = 64 * VL; // elements of V that a wave loads: its 16 rows, in 16 bits twice
+    __shared__ __align__(16) IN v_even[4 * VW], v_odd[4 * VW];
+    __shared__ __align__(16) float f_even[4 * 256], f_odd[4 * 256]; // the factors, a copy for each wave
     __shared__ __align__(16) short s_p[3 * 16 * LS], r_p[3 * 16 * LT], u_p[NO * 16 * LT], w_p[3 * 16 * LT];
     __shared__ int odd_s[2][16]; // of each column: the chunk's first token with a value that is not finite, or 64
-    const int tid = threadIdx.x, wave = (tid >> 6) & 3, lane = tid & 63, r = lane & 15, c = lane >> 4;
+    const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane((tid >> 6) & 3), lane = tid & 63, r = lane & 15, c = lane >> 4;
     const bool chain = tid < 256;
     const int seq = blockIdx.x / (SL * a.v_heads), at = blockIdx.x - seq * SL * a.v_heads;
     // Workgroups go to the eight XCDs in turn: a head's slices, which read the same K, Q, T and M, to one L2.
@@ -413,9 +414,10 @@ __global__ __launch_bounds__(512) void k_delta_scan(const QeDeltaArgs a) {
     const short *kq = NP == 1 ? nullptr : a.ws_kq + ((size_t)chunk0 * a.k_heads + kh) * 2 * NP * 64 * DK;
     const size_t kq_step = (size_t)a.k_heads * 2 * NP * 64 * DK;
     if (tid < 32) odd_s[tid >> 4][tid & 15] = 64;
-    // Loads run one chunk ahead; behind the last chunk they take it again, for a branch around them would have the
-    // compiler wait for all of them.  Rows behind the sequence's end are its last one's: T's columns and rows are
-    // zeros there.
+    // Loads run one chunk ahead, without branches: what a wave may leave in flight is counted, and where a branch
+    // makes the count uncertain the compiler waits for loads just issued.  So behind the last chunk they take it
+    // again, and waves whose rows of T and M are short load their unwritten half as well.  Rows behind the
+    // sequence's end are its last one's: T's columns and rows are zeros there.
     if (chain) {
         // As in k_delta_chunks, what is not finite must not meet the zeros above the diagonal: it becomes
         // 0, and its column's outputs from that token on, and its state, NaN.
@@ -436,24 +438,13 @@ __global__ __launch_bounds__(512) void k_delta_scan(const QeDeltaArgs a) {
             for (int j = 0; j < 4; ++j)
                 S[i][j] = in_i < 0 ? 0.f : a.pool[(((size_t)in_i * a.v_heads + head) * DK + 16 * (wave * SB + i) + 4 * c + j) * DV + col];
         qe_s8 tf[2][3];
-        // waves 0 and 1, whose rows of T are short, also load V and the factors
-        auto load = [&](int t0, const short *w, IN *v_to, float *f_to) {
-            if (wave == 0) {
-                constexpr int PER = 16 / VL; // lanes of a row
-                for (int i = 0; i < PER; ++i) {
-                    const int t = t0 + i * (64 / PER) + lane / PER;
-                    load_lds16((const IN *)a.v + (size_t)(t < end ? t : end - 1) * a.v_stride + (size_t)head * DV + slice * 16 + lane % PER * VL, v_to + i * 64 * VL);
-                }
-            }
-            if (wave == 1) load_lds16((const float *)w + QE_DELTA_WS - 256 + lane * 4, f_to);
+        auto load = [&](const short *w) {
             for (int p = 0; p < 3; ++p) {
                 tf[0][p] = *(const qe_s8 *)(w + wave * 3072 + p * 512 + lane * 8);
-                if (kb) tf[1][p] = *(const qe_s8 *)(w + wave * 3072 + 1536 + p * 512 + lane * 8);
+                tf[1][p] = *(const qe_s8 *)(w + wave * 3072 + 1536 + p * 512 + lane * 8);
             }
         };
-        auto step = [&](const int par, const short *k_s, const IN *v_s, const float *f_s, IN *v_next, float *f_next, int t0) {
-            for (int i = 0; i < SB; ++i) put4<3>(s_p + r * LS + 16 * (wave * SB + i) + 4 * c, 16 * LS, S[i]);
-            __builtin_amdgcn_s_waitcnt(0x0f70); // V and the factors have landed
+        auto step = [&](const int par, const short *k_s, const IN *v_s, const float *f_s, int t0) {
             lds_barrier();
             qe_f4 x[3] = {};
 #pragma unroll
@@ -463,15 +454,26 @@ __global__ __launch_bounds__(512) void k_delta_scan(const QeDeltaArgs a) {
                 for (int p = 0; p < 3; ++p) sf[p] = *(const qe_s8 *)(s_p + (p * 16 + r) * LS + 32 * s + 8 * c);
                 mul_planes<NP, 3, 2>(kf, sf, x);
             }
+            qe_s8 kt[SB][2][NP]; // K^T for the last product
+#pragma unroll
+            for (int i = 0; i < SB; ++i)
+                for (int s = 0; s < 2; ++s)
+                    for (int p = 0; p < NP; ++p) {
+                        const int ra = 32 * s + 4 * c + (r >> 2), el = 16 * (wave * SB + i) + (r & 3) * 4;
+                        const short *at = k_s + (p * 64 + ra) * DK + (((el >> 3) ^ key_swz<DK>(ra)) << 3) + (el & 7);
+                        const qe_s4 lo = lds_tr(at), hi = lds_tr(at + 16 * DK); // 16 rows on the permutation is the same
+                        kt[i][s][p] = qe_s8{lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]};
+                    }
             qe_f4 v;
             if constexpr (sizeof(IN) == 2) {
-                const qe_s4 h = lds_tr((const short *)v_s + (16 * wave + 4 * c + (r >> 2)) * 16 + (r & 3) * 4);
+                const qe_s4 h = lds_tr((const short *)v_s + wave * VW + (4 * c + (r >> 2)) * 16 + (r & 3) * 4);
                 for (int j = 0; j < 4; ++j) v[j] = from16<__is_same(IN, __bf16)>(h[j]);
             } else {
-                for (int j = 0; j < 4; ++j) v[j] = v_s[(16 * wave + 4 * c + j) * 16 + r];
+                for (int j = 0; j < 4; ++j) v[j] = v_s[wave * VW + (4 * c + j) * 16 + r];
             }
-            const qe_f4 cx = *(const qe_f4 *)(f_s + 16 * wave + 4 * c), cu = *(const qe_f4 *)(f_s + 128 + 16 * wave + 4 * c);
-            const float last = f_s[192];
+            const float *f = f_s + 256 * wave;
+            const qe_f4 cx = *(const qe_f4 *)(f + 16 * wave + 4 * c), cu = *(const qe_f4 *)(f + 128 + 16 * wave + 4 * c);
+            const float last = f[192];
             put4<3>(r_p + r * LT + 16 * wave + 4 * c, 16 * LT, cleared(v - cx * (x[0] + (x[1] + x[2])), par));
             lds_barrier();
             qe_f4 u3[3] = {};
@@ -485,9 +487,8 @@ __global__ __launch_bounds__(512) void k_delta_scan(const QeDeltaArgs a) {
             const qe_f4 u = cleared(u3[0] + (u3[1] + u3[2]), par);
             put4<3>(w_p + r * LT + 16 * wave + 4 * c, 16 * LT, u * cu);
             put4<NO>(u_p + r * LT + 16 * wave + 4 * c, 16 * LT, u);
-            const int ahead = t0 + QE_DELTA_C < end;
-            ws += ahead * ws_step;
-            load(t0 + ahead * QE_DELTA_C, ws, v_next, f_next);
+            ws += (t0 + QE_DELTA_C < end) * ws_step;
+            load(ws);
             lds_barrier();
             const int spoilt = odd_s[par][r];
             if (tid < 16) odd_s[par ^ 1][tid] = 64; // last read a chunk ago, next written in the next
@@ -503,29 +504,22 @@ __global__ __launch_bounds__(512) void k_delta_scan(const QeDeltaArgs a) {
             for (int i = 0; i < SB; ++i) {
                 qe_f4 d[3] = {};
 #pragma unroll
-                for (int s = 0; s < 2; ++s) {
-                    qe_s8 kt[NP];
-                    const int ra = 32 * s + 4 * c + (r >> 2), el = 16 * (wave * SB + i) + (r & 3) * 4;
-                    for (int p = 0; p < NP; ++p) {
-                        const short *at = k_s + (p * 64 + ra) * DK + (((el >> 3) ^ key_swz<DK>(ra)) << 3) + (el & 7);
-                        const qe_s4 lo = lds_tr(at), hi = lds_tr(at + 16 * DK); // 16 rows on the permutation is the same
-                        kt[p] = qe_s8{lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]};
-                    }
-                    mul_planes<NP, 3, 2>(kt, wf[s], d);
-                }
+                for (int s = 0; s < 2; ++s) mul_planes<NP, 3, 2>(kt[i][s], wf[s], d);
                 S[i] = S[i] * (spoilt < 64 ? NAN : last) + (d[0] + (d[1] + d[2]));
+                put4<3>(s_p + r * LS + 16 * (wave * SB + i) + 4 * c, 16 * LS, S[i]);
             }
         };
-        if (begin < end) load(begin, ws, v_even, f_even);
+        for (int i = 0; i < SB; ++i) put4<3>(s_p + r * LS + 16 * (wave * SB + i) + 4 * c, 16 * LS, S[i]);
+        if (begin < end) load(ws);
         for (int t0 = begin; t0 < end; t0 += 2 * QE_DELTA_C) {
-            step(0, k_even, v_even, f_even, v_odd, f_odd, t0);
-            if (t0 + QE_DELTA_C < end) step(1, k_odd, v_odd, f_odd, v_even, f_even, t0 + QE_DELTA_C);
+            step(0, k_even, v_even, f_even, t0);
+            if (t0 + QE_DELTA_C < end) step(1, k_odd, v_odd, f_odd, t0 + QE_DELTA_C);
         }
         if (out_i >= 0)
             for (int i = 0; i < SB; ++i)
                 for (int j = 0; j < 4; ++j) a.pool[(((size_t)out_i * a.v_heads + head) * DK + 16 * (wave * SB + i) + 4 * c + j) * DV + col] = S[i][j];
     } else {
-        qe_s8 qf[KS][NP], mf[2][NO];
+        qe_s8 qf[KS][NP], m_even[2][NO], m_odd[2][NO];
         auto load_k = [&](int t0, const short *from, short *to) {
             constexpr int ROWS = 512 / DK; // of one direct load
 #pragma unroll
@@ -536,22 +530,37 @@ __global__ __launch_bounds__(512) void k_delta_scan(const QeDeltaArgs a) {
                 load_lds16(src, to + (p * 64 + rr) * DK);
             }
         };
+        auto load_v = [&](int t0, const short *w, IN *v_to, float *f_to) {
+            constexpr int PER = 16 / VL; // lanes of a row
+            const int t = t0 + 16 * wave + lane / PER % 16;
+            load_lds16((const IN *)a.v + (size_t)(t < end ? t : end - 1) * a.v_stride + (size_t)head * DV + slice * 16 + lane % PER * VL, v_to + wave * VW);
+            load_lds16((const float *)w + QE_DELTA_WS - 256 + lane * 4, f_to + wave * 256);
+        };
         auto load_q = [&](int t0, const short *from) {
             const short *q = (const short *)a.q + (size_t)(t0 + row < end ? t0 + row : end - 1) * a.q_stride + (size_t)kh * DK + 8 * c;
             for (int s = 0; s < KS; ++s)
                 for (int p = 0; p < NP; ++p)
                     qf[s][p] = *(const qe_s8 *)(NP == 1 ? q + 32 * s : from + NP * 64 * DK + ((wave * KS + s) * NP + p) * 512 + lane * 8);
         };
-        auto load_m = [&](const short *w) {
+        auto load_m = [&](const short *w, qe_s8 (*mf)[NO]) {
             for (int p = 0; p < NO; ++p) {
                 mf[0][p] = *(const qe_s8 *)(w + 12288 + wave * 3072 + p * 512 + lane * 8);
-                if (kb) mf[1][p] = *(const qe_s8 *)(w + 12288 + wave * 3072 + 1536 + p * 512 + lane * 8);
+                mf[1][p] = *(const qe_s8 *)(w + 12288 + wave * 3072 + 1536 + p * 512 + lane * 8);
             }
         };
-        auto step = [&](const int par, const float *f_s, short *k_next, int t0) {
+        IN *out[4]; // the lane's four rows
+        for (int j = 0; j < 4; ++j) out[j] = (IN *)a.out + (size_t)(begin + 16 * wave + 4 * c + j) * a.out_stride + (size_t)head * DV + col;
+        auto step = [&](const int par, const bool whole, const float *f_s, short *k_next, IN *v_next, float *f_next, const qe_s8 (*mf)[NO], qe_s8 (*m_next)[NO], int t0) {
             const int ahead = t0 + QE_DELTA_C < end;
-            // K has landed: younger than its direct loads are at least four loads of Q and M, and the last chunk's stores
+            kq += ahead * kq_step, ws += ahead * ws_step;
+            // K, V and the factors have landed: younger than their direct loads are at least four loads of Q and M, and the last chunk's stores
             __builtin_amdgcn_s_waitcnt(0x0f74);
+            lds_barrier();
+            // The chain's waves now read all of S, which takes the LDS's bandwidth; these issue loads meanwhile,
+            // and read S while the chain is at its next product.
+            load_v(t0 + ahead * QE_DELTA_C, ws, v_next, f_next);
+            load_k(t0 + ahead * QE_DELTA_C, kq, k_next);
+            load_m(ws, m_next);
             lds_barrier();
             qe_f4 x[3] = {};
 #pragma unroll
@@ -560,10 +569,7 @@ __global__ __launch_bounds__(512) void k_delta_scan(const QeDeltaArgs a) {
                 for (int p = 0; p < NO; ++p) sf[p] = *(const qe_s8 *)(s_p + (p * 16 + r) * LS + 32 * s + 8 * c);
                 mul_planes<NP, NO, NO - 1>(qf[s], sf, x);
             }
-            qe_f4 o = *(const qe_f4 *)(f_s + 64 + 16 * wave + 4 * c) * (x[0] + (x[1] + x[2]));
-            kq += ahead * kq_step, ws += ahead * ws_step;
-            load_k(t0 + ahead * QE_DELTA_C, kq, k_next);
-            lds_barrier();
+            qe_f4 o = *(const qe_f4 *)(f_s + 256 * wave + 64 + 16 * wave + 4 * c) * (x[0] + (x[1] + x[2]));
             load_q(t0 + ahead * QE_DELTA_C, kq);
             lds_barrier();
             const int spoilt = odd_s[par][r];
@@ -576,22 +582,26 @@ __global__ __launch_bounds__(512) void k_delta_scan(const QeDeltaArgs a) {
                 mul_planes<NO, NO, NO - 1>(mf[s], uf, y);
             }
             o += y[0] + (y[1] + y[2]);
-            load_m(ws);
             for (int j = 0; j < 4; ++j) {
                 const int t = 16 * wave + 4 * c + j;
-                if (t0 + t < end) ((IN *)a.out)[(size_t)(t0 + t) * a.out_stride + (size_t)head * DV + col] = (IN)(t < spoilt ? o[j] : NAN);
+                if (whole || t0 + t < end) *out[j] = (IN)(t < spoilt ? o[j] : NAN);
+                out[j] += QE_DELTA_C * a.out_stride;
             }
         };
         if (begin < end) {
+            load_v(begin, ws, v_even, f_even);
             load_k(begin, kq, k_even);
             load_q(begin, kq);
-            load_m(ws);
+            load_m(ws, m_even);
             __builtin_amdgcn_s_waitcnt(0x0f70); // in whatever order they were issued here
         }
-        for (int t0 = begin; t0 < end; t0 += 2 * QE_DELTA_C) {
-            step(0, f_even, k_odd, t0);
-            if (t0 + QE_DELTA_C < end) step(1, f_odd, k_even, t0 + QE_DELTA_C);
+        int t0 = begin;
+        for (; t0 + 2 * QE_DELTA_C <= end; t0 += 2 * QE_DELTA_C) {
+            step(0, true, f_even, k_odd, v_odd, f_odd, m_even, m_odd, t0);
+            step(1, true, f_odd, k_even, v_even, f_even, m_odd, m_even, t0 + QE_DELTA_C);
         }
+        if (t0 < end) step(0, false, f_even, k_odd, v_odd, f_odd, m_even, m_odd, t0);
+        if (t0 + QE_DELTA_C < end) step(1, false, f_odd, k_even, v_even, f_even, m_odd, m_even, t0 + QE_DELTA_C);
     }
 }
 
