@@ -553,8 +553,9 @@ __global__ __launch_bounds__(512) void k_delta_scan(const QeDeltaArgs a) {
         auto step = [&](const int par, const bool whole, const float *f_s, short *k_next, IN *v_next, float *f_next, const qe_s8 (*mf)[NO], qe_s8 (*m_next)[NO], int t0) {
             const int ahead = t0 + QE_DELTA_C < end;
             kq += ahead * kq_step, ws += ahead * ws_step;
-            // K, V and the factors have landed: younger than their direct loads are at least four loads of Q and M, and the last chunk's stores
-            __builtin_amdgcn_s_waitcnt(0x0f74);
+            // K, V and the factors have landed: younger than their direct loads are those of M and Q, and the last chunk's stores
+            constexpr int younger = 2 * NO + KS * NP;
+            __builtin_amdgcn_s_waitcnt(0x0f70 | (younger & 15) | (younger >> 4) << 14);
             lds_barrier();
             // The chain's waves now read all of S, which takes the LDS's bandwidth; these issue loads meanwhile,
             // and read S while the chain is at its next product.
