@@ -1,8 +1,8 @@
 // Causal attention of packed prompts over a paged cache.
 //
-// A workgroup takes BM = 128 NB query rows of one sequence and one key-value head (its tokens
-// times the heads that share the key-value head, so that no key is read for one head
-// alone), its four waves 32 NB rows each, and steps through the keys 64 at a time.  Per
+// A workgroup takes 32 query rows for each of its waves, of one sequence and one key-value head
+// (its tokens times the heads that share the key-value head, so that no key is read for one
+// head alone), and steps through the keys 64 at a time.  Per
 // step S^T = K Q^T and O^T += V^T P^T on v_mfma_f32_32x32x16: a lane's column is one query
 // row, so maximum, sum and rescaling are per lane (plus one exchange between the wave's
 // halves), and the registers that hold S^T's rows are, once rounded, the second product's
@@ -26,109 +26,113 @@ __device__ __forceinline__ int v_swz(int row) {
     return DH == 64 ? ((row >> 1) & 1) << 2 : (row & 3) << 2;
 }
 
-// a wave's part of a tile of BN keys from position k0 on: K and V to LDS
-template <int DH>
+// A wave's part of a tile of BN keys from position k0 on: K and V to LDS.  In one direct load's
+// rows, and in a wave's part, all rows lie in one page; rows behind the end may lie in none,
+// then any of the sequence's do (their probabilities are zero).
+template <int DH, int WAVES>
 __device__ __forceinline__ void load_tile(const QeAttnArgs &a, const int32_t *table, int kvh, int k0, int len, int wave, int lane,
                                           short *k_lds, short *v_lds, unsigned *bad) {
-    constexpr int CH = DH / 8, ROWS = 64 / CH; // chunks of a row, rows of one direct load
-    // a wave loads 16 consecutive rows, which lie in one page; rows behind the end may lie in
-    // none, then any of the sequence's do (their probabilities are zero)
-    const int sub = k0 + wave * 16;
-    const size_t r0 = sub_row(a, table, kvh, sub < len ? sub : (len - 1) & ~15, bad);
+    constexpr int CH = DH / 8, ROWS = 64 / CH, PART = BN / WAVES; // chunks of a row, rows of one direct load, rows of a wave
+    const int sub = k0 + wave * PART;
+    const size_t r0 = sub_row(a, table, kvh, sub < len ? sub & ~15 : (len - 1) & ~15, bad) + (wave * PART & 15);
     const short *kc = (const short *)a.kc + r0 * DH, *vc = (const short *)a.vc + r0 * DH;
 #pragma unroll
-    for (int i = 0; i < 16 / ROWS; ++i) {
-        const int row = i * ROWS + lane / CH, c = lane % CH;
-        load_lds16(kc + row * DH + ((c ^ k_swz<DH>(row)) << 3), k_lds + (wave * 16 + i * ROWS) * DH);
-        load_lds16(vc + row * DH + ((c ^ v_swz<DH>(row)) << 3), v_lds + (wave * 16 + i * ROWS) * DH);
+    for (int i = 0; i < PART / ROWS; ++i) {
+        const int row = wave * PART + i * ROWS + lane / CH, c = lane % CH;
+        load_lds16(kc + (i * ROWS + lane / CH) * DH + ((c ^ k_swz<DH>(row)) << 3), k_lds + (wave * PART + i * ROWS) * DH);
+        load_lds16(vc + (i * ROWS + lane / CH) * DH + ((c ^ v_swz<DH>(row)) << 3), v_lds + (wave * PART + i * ROWS) * DH);
     }
 }
 
-template <bool BF, int DH, int NB>
-struct Tile {
-    qe_f16v o[NB][DH / 32];
-    qe_s8 q[NB][DH / 16];
-    float m[NB], l[NB];
-    int place[NB]; // position of the lane's query, -1 where the lane has none
+__device__ __forceinline__ float max3(float a, float b, float c) { return fmaxf(fmaxf(a, b), c); }
+
+// A wave's 32 query rows.
+template <bool BF, int DH>
+struct Rows {
+    qe_f16v o[DH / 32]; // O^T: column = row of the wave
+    qe_s8 q[DH / 16];
+    float m, l; // running maximum of the scores (scaled, in powers of two) and sum
+    int place;  // position of the lane's query; below 0 where it attends to nothing
 
     __device__ __forceinline__ void step(const QeAttnArgs &a, const short *k_lds, const short *v_lds, int k0, bool masked, int lane) {
         const int r = lane & 31, h = lane >> 5;
-        qe_f16v s[NB][2];
-        for (int n = 0; n < NB; ++n)
-            for (int b = 0; b < 2; ++b)
-                for (int i = 0; i < 16; ++i) s[n][b][i] = 0;
+        // LDS addresses: four for K, whose chunk 2 st + h is permuted by the low bits of the row (chunks 8 apart are a
+        // constant apart), and for V, whose 64-byte unit d is permuted by the row in the transposing read's group
+        const char *ka[4], *va[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            ka[i] = (const char *)k_lds + r * DH * 2 + (((2 * i + h) ^ (r & 7)) << 4);
+            const int tr = (lane & 15) >> 2, el = ((lane >> 4) & 1) * 16 + (lane & 3) * 4;
+            va[i] = (const char *)v_lds + (4 * h + tr) * DH * 2 + ((((i << 2) + (el >> 3)) ^ v_swz<DH>(tr)) << 4) + (el & 7) * 2;
+        }
+        qe_f16v s[2];
 #pragma unroll
         for (int b = 0; b < 2; ++b) {
-            const short *kr = k_lds + (b * 32 + r) * DH;
+            for (int i = 0; i < 16; ++i) s[b][i] = 0;
 #pragma unroll
-            for (int st = 0; st < DH / 16; ++st) {
-                const qe_s8 kf = *(const qe_s8 *)(kr + (((2 * st + h) ^ (r & 7)) << 3));
-#pragma unroll
-                for (int n = 0; n < NB; ++n) s[n][b] = mfma32<BF>(kf, q[n][st], s[n][b]);
-            }
+            for (int st = 0; st < DH / 16; ++st)
+                s[b] = mfma32<BF>(*(const qe_s8 *)(ka[st & 3] + b * 64 * DH + (st >> 2) * 128), q[st], s[b]);
         }
-        union {
-            unsigned u[4];
-            qe_s8 v;
-        } p[NB][4];
-#pragma unroll
-        for (int n = 0; n < NB; ++n) {
-            if (masked) {
-                const int limit = place[n] - k0 - 4 * h; // the last key that the row attends to, counted from the lane's first
-#pragma unroll
-                for (int b = 0; b < 2; ++b)
-#pragma unroll
-                    for (int i = 0; i < 16; ++i)
-                        if (b * 32 + 8 * (i / 4) + i % 4 > limit) s[n][b][i] = -INFINITY;
-            }
-            float top = s[n][0][0];
-#pragma unroll
-            for (int i = 1; i < 16; ++i) top = fmaxf(top, s[n][0][i]);
-#pragma unroll
-            for (int i = 0; i < 16; ++i) top = fmaxf(top, s[n][1][i]);
-            top = fmaxf(top, __shfl_xor(top, 32));
-            if (__any(top > m[n])) {
-                const float mn = fmaxf(m[n], top), f = m[n] == -INFINITY ? 0.f : exp2f((m[n] - mn) * a.scale_log2);
-                for (int d = 0; d < DH / 32; ++d) o[n][d] *= f;
-                l[n] *= f;
-                m[n] = mn;
-            }
-            const float base = m[n] == -INFINITY ? 0.f : -m[n] * a.scale_log2;
-            float sum = 0;
+        if (masked) {
+            const int limit = place - k0 - 4 * h; // the last key that the row attends to, counted from the lane's first
 #pragma unroll
             for (int b = 0; b < 2; ++b)
 #pragma unroll
-                for (int i = 0; i < 16; i += 2) {
-                    const float x = __builtin_amdgcn_exp2f(fmaf(s[n][b][i], a.scale_log2, base));
-                    const float y = __builtin_amdgcn_exp2f(fmaf(s[n][b][i + 1], a.scale_log2, base));
-                    sum += x + y;
-                    p[n][b * 2 + i / 8].u[i % 8 / 2] = pack2<BF>(x, y);
-                }
-            l[n] += sum;
+                for (int i = 0; i < 16; ++i)
+                    if (b * 32 + 8 * (i / 4) + i % 4 > limit) s[b][i] = -INFINITY;
         }
-        const int tr = (lane & 15) >> 2, el = ((lane >> 4) & 1) * 16 + (lane & 3) * 4;
+        float top = s[0][0];
 #pragma unroll
-        for (int ks = 0; ks < 4; ++ks) {
-            const int ra = ks * 16 + 4 * h + tr;
+        for (int i = 1; i < 15; i += 2) top = max3(top, s[0][i], s[0][i + 1]);
+        top = max3(top, s[0][15], s[1][0]);
 #pragma unroll
-            for (int d = 0; d < DH / 32; ++d) {
-                const int e = d * 32 + el;
-                const short *vp = v_lds + ra * DH + (((e >> 3) ^ v_swz<DH>(ra)) << 3) + (e & 7);
-                const qe_s4 x = lds_tr(vp), y = lds_tr(vp + 8 * DH); // 8 rows on the permutation is the same
-                const qe_s8 vf = {x[0], x[1], x[2], x[3], y[0], y[1], y[2], y[3]};
+        for (int i = 1; i < 15; i += 2) top = max3(top, s[1][i], s[1][i + 1]);
+        top = fmaxf(top, s[1][15]);
+        top = fmaxf(top, __shfl_xor(top, 32)) * a.scale_log2;
+        // The maximum that is subtracted only has to keep the powers of two in range: it follows the true one
+        // when that has grown by more than 2^8, which after the first keys is rare.
+        if (__any(top > m + 8.f)) {
+            const float mn = fmaxf(m, top), f = m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m - mn);
+            for (int d = 0; d < DH / 32; ++d) o[d] *= f;
+            l *= f;
+            m = mn;
+        }
+        const float base = m == -INFINITY ? 0.f : -m;
 #pragma unroll
-                for (int n = 0; n < NB; ++n) o[n][d] = mfma32<BF>(vf, p[n][ks].v, o[n][d]);
+        for (int b = 0; b < 2; ++b) {
+            union {
+                unsigned u[4];
+                qe_s8 v;
+            } p[2];
+            float sum = 0;
+#pragma unroll
+            for (int i = 0; i < 16; i += 2) {
+                const float x = __builtin_amdgcn_exp2f(fmaf(s[b][i], a.scale_log2, base));
+                const float y = __builtin_amdgcn_exp2f(fmaf(s[b][i + 1], a.scale_log2, base));
+                sum += x + y;
+                p[i / 8].u[i % 8 / 2] = pack2<BF>(x, y);
             }
+            l += sum;
+#pragma unroll
+            for (int ks = 0; ks < 2; ++ks)
+#pragma unroll
+                for (int d = 0; d < DH / 32; ++d) {
+                    const char *vp = va[d & 3] + (b * 2 + ks) * 32 * DH + (d >> 2) * 256;
+                    const qe_s4 x = lds_tr((const short *)vp), y = lds_tr((const short *)(vp + 16 * DH)); // 8 rows on the permutation is the same
+                    o[d] = mfma32<BF>(qe_s8{x[0], x[1], x[2], x[3], y[0], y[1], y[2], y[3]}, p[ks].v, o[d]);
+                }
         }
     }
 };
 
-template <bool BF, int DH, int NB>
-__global__ __launch_bounds__(256) void k_attn_prompt(const QeAttnArgs a) {
-    constexpr int BM = 128 * NB;
+template <bool BF, int DH, int WAVES>
+__global__ __launch_bounds__(64 * WAVES, 2) void k_attn_prompt(const QeAttnArgs a) {
+    constexpr int BM = 32 * WAVES, THREADS = 64 * WAVES;
+    // two buffers, variables of their own: else the compiler has every LDS read wait for the direct loads in flight
     __shared__ __align__(16) short k_a[BN * DH], v_a[BN * DH], k_b[BN * DH], v_b[BN * DH];
-    __shared__ unsigned long long odd_rows; // rows of the tile whose V holds an infinity or a NaN
-    const int tid = threadIdx.x, wave = tid >> 6, lane = tid & 63, r = lane & 31, h = lane >> 5;
+    // rows with an infinity or a NaN in V, of the tiles that some rows attend to in part: from `clear` on, BM tokens at most
+    __shared__ unsigned long long odd_rows[BM / BN + 2];
+    const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63, r = lane & 31, h = lane >> 5;
     const int split = blockIdx.x % a.splits, kvh = blockIdx.x / a.splits % a.kv_heads;
     const int tile = a.tiles - 1 - blockIdx.x / a.splits / a.kv_heads; // late rows have more keys: first
     int seq = 0;
@@ -145,44 +149,41 @@ __global__ __launch_bounds__(256) void k_attn_prompt(const QeAttnArgs a) {
     if (bad_len && tid == 0) report(a.err, QE_BAD_LENGTH);
     const int n_rows = (end - begin) * a.group;
     if (local < 0 || (int64_t)local * BM >= n_rows) return; // uniform: no row of the sequence
-    const int row0 = local * BM;
+    const int row0 = local * BM, first = len - (end - begin); // first: position of the sequence's first row
     const int32_t *table = a.table + (size_t)seq * a.table_stride;
 
-    Tile<BF, DH, NB> w;
-    int tok[NB], head[NB];
-    for (int n = 0; n < NB; ++n) {
-        const int row = row0 + (wave * NB + n) * 32 + r;
-        tok[n] = row / a.group;
-        head[n] = kvh * a.group + row - tok[n] * a.group;
-        const bool there = row < n_rows;
-        w.place[n] = there ? len - (end - begin) + tok[n] : -1;
-        if (!there) tok[n] = -1;
-        const short *q = (const short *)a.q + (size_t)(begin + (there ? tok[n] : 0)) * a.q_stride + (size_t)head[n] * DH + h * 8;
-        for (int s = 0; s < DH / 16; ++s) w.q[n][s] = there ? *(const qe_s8 *)(q + s * 16) : qe_s8{};
-        w.m[n] = -INFINITY;
-        w.l[n] = 0;
-        for (int d = 0; d < DH / 32; ++d)
-            for (int i = 0; i < 16; ++i) w.o[n][d][i] = 0;
+    Rows<BF, DH> w;
+    const int row = row0 + wave * 32 + r;
+    const bool there = row < n_rows;
+    const int tok = there ? row / a.group : 0, head = kvh * a.group + (there ? row - tok * a.group : 0);
+    w.place = there ? first + tok : -1;
+    {
+        const short *q = (const short *)a.q + (size_t)(begin + tok) * a.q_stride + (size_t)head * DH + h * 8;
+        for (int s = 0; s < DH / 16; ++s) w.q[s] = there ? *(const qe_s8 *)(q + s * 16) : qe_s8{};
     }
+    w.m = -INFINITY;
+    w.l = 0;
+    for (int d = 0; d < DH / 32; ++d)
+        for (int i = 0; i < 16; ++i) w.o[d][i] = 0;
     // keys of the tile: up to its last row's place; below `clear` every row attends to every key
     const int last_tok = (row0 + BM < n_rows ? row0 + BM - 1 : n_rows - 1) / a.group;
-    const int keys = len - (end - begin) + last_tok + 1;
-    const int clear = len - (end - begin) + row0 / a.group + 1;
+    const int keys = first + last_tok + 1, clear = first + row0 / a.group + 1 > 0 ? first + row0 / a.group + 1 : 0;
+    // the same for the wave
+    const int wave_row = row0 + wave * 32, wave_keys = wave_row < n_rows ? first + (wave_row + 32 < n_rows ? wave_row + 31 : n_rows - 1) / a.group + 1 : 0;
+    const int wave_clear = first + wave_row / a.group + 1;
     int lo, hi;
     qe_split_range(keys > 0 ? (keys + BN - 1) / BN : 0, a.splits, split, &lo, &hi);
 
     auto work = [&](const short *k_lds, short *v_lds, short *k_next, short *v_next, int t) {
         __builtin_amdgcn_s_waitcnt(0x0f70); // this wave's direct loads have landed,
-        __syncthreads();                    // the others' too, and no wave reads the other buffers any more
+        lds_barrier();                      // the others' too, and no wave reads the other buffers any more
         const int k0 = t * BN;
-        if (t + 1 < hi) load_tile<DH>(a, table, kvh, k0 + BN, len, wave, lane, k_next, v_next, &bad);
+        if (t + 1 < hi) load_tile<DH, WAVES>(a, table, kvh, k0 + BN, len, wave, lane, k_next, v_next, &bad);
         const bool masked = k0 + BN > clear;
         if (masked) {
             // A probability of 0 times an infinity or NaN is NaN: rows behind the end become zeros, and
-            // so do elements that are not finite, which are added below for the rows that attend to them.
-            if (tid == 0) odd_rows = 0;
-            __syncthreads();
-            for (int i = tid; i < BN * (DH / 8); i += 256) {
+            // so do elements that are not finite, which are added in the end for the rows that attend to them.
+            for (int i = tid; i < BN * (DH / 8); i += THREADS) {
                 const int row = i / (DH / 8);
                 qe_s8 x = *(const qe_s8 *)(v_lds + i * 8);
                 if (k0 + row >= len) {
@@ -194,60 +195,61 @@ __global__ __launch_bounds__(256) void k_attn_prompt(const QeAttnArgs a) {
                         if ((x[j] & top) == top) x[j] = 0, odd = true;
                     if (odd) {
                         *(qe_s8 *)(v_lds + i * 8) = x;
-                        atomicOr(&odd_rows, 1ull << row);
+                        atomicOr(&odd_rows[t - clear / BN], 1ull << row);
                     }
                 }
             }
-            __syncthreads();
+            lds_barrier();
         }
-        w.step(a, k_lds, v_lds, k0, masked, lane);
-        if (masked) {
-            unsigned long long odd = odd_rows;
-            while (odd) { // uniform, and empty but for such values
-                const int row = __ffsll(odd) - 1;
-                odd &= odd - 1;
-                unsigned b2 = 0;
-                const size_t at = sub_row(a, table, kvh, (k0 + row) & ~15, &b2) + (row & 15);
-                const short *v = (const short *)a.vc + at * DH;
-                for (int n = 0; n < NB; ++n)
-                    if (k0 + row <= w.place[n])
-                        for (int d = 0; d < DH / 32; ++d)
-                            for (int i = 0; i < 16; ++i) {
-                                const float x = from16<BF>(v[d * 32 + 8 * (i / 4) + 4 * h + i % 4]);
-                                if (!__builtin_isfinite(x)) w.o[n][d][i] += x;
-                            }
-            }
-        }
+        if (k0 < wave_keys) w.step(a, k_lds, v_lds, k0, k0 + BN > wave_clear, lane);
     };
-    if (lo < hi) load_tile<DH>(a, table, kvh, lo * BN, len, wave, lane, k_a, v_a, &bad);
+    if (tid < BM / BN + 2) odd_rows[tid] = 0; // a barrier before the first tile's
+    if (lo < hi) load_tile<DH, WAVES>(a, table, kvh, lo * BN, len, wave, lane, k_a, v_a, &bad);
     for (int t = lo; t < hi; t += 2) {
         work(k_a, v_a, k_b, v_b, t);
         if (t + 1 < hi) work(k_b, v_b, k_a, v_a, t + 1);
     }
     if (bad && lane == 0) report(a.err, QE_BAD_PAGE);
     const bool void_rows = __syncthreads_or(bad);
-    for (int n = 0; n < NB; ++n) {
-        const float l = w.l[n] + __shfl_xor(w.l[n], 32);
-        if (a.splits == 1) {
-            if (tok[n] < 0) continue;
-            const float inv = l == 0.f ? 0.f : 1.f / l;
-            short *out = (short *)a.out + (size_t)(begin + tok[n]) * a.out_stride + (size_t)head[n] * DH;
-            for (int d = 0; d < DH / 32; ++d)
-                for (int i = 0; i < 16; i += 4) {
-                    uint2 x;
-                    x.x = pack2<BF>(w.o[n][d][i] * inv, w.o[n][d][i + 1] * inv);
-                    x.y = pack2<BF>(w.o[n][d][i + 2] * inv, w.o[n][d][i + 3] * inv);
-                    if (void_rows) x = make_uint2(0, 0);
-                    *(uint2 *)(out + d * 32 + 2 * i + 4 * h) = x;
-                }
-        } else {
-            const size_t row = (((size_t)tile * a.kv_heads + kvh) * a.splits + split) * BM + (wave * NB + n) * 32 + r;
-            for (int d = 0; d < DH / 32; ++d)
-                for (int i = 0; i < 16; i += 4)
-                    *(qe_f4 *)(a.part_o + row * DH + d * 32 + 2 * i + 4 * h) =
-                        qe_f4{w.o[n][d][i], w.o[n][d][i + 1], w.o[n][d][i + 2], w.o[n][d][i + 3]};
-            if (h == 0) a.part_ml[row] = make_float2(w.m[n], void_rows ? -1.f : l);
+    for (int t = clear / BN; t < hi; ++t) {
+        unsigned long long odd = t >= lo ? odd_rows[t - clear / BN] : 0;
+        while (odd) { // uniform, and empty but for values that are not finite
+            const int key = t * BN + __ffsll(odd) - 1;
+            odd &= odd - 1;
+            const size_t at = sub_row(a, table, kvh, key & ~15, &bad) + (key & 15);
+            const short *v = (const short *)a.vc + at * DH + 4 * h;
+            if (key <= w.place)
+#pragma unroll
+                for (int d = 0; d < DH / 32; ++d)
+#pragma unroll
+                    for (int i = 0; i < 16; i += 4) {
+                        const qe_s4 x = *(const qe_s4 *)(v + d * 32 + 2 * i);
+                        for (int j = 0; j < 4; ++j) {
+                            const float y = from16<BF>(x[j]);
+                            if (!__builtin_isfinite(y)) w.o[d][i + j] += y;
+                        }
+                        asm volatile("" ::: "memory"); // not all of the row in registers at once
+                    }
         }
+    }
+    const float l = w.l + __shfl_xor(w.l, 32);
+    if (a.splits == 1) {
+        if (!there) return;
+        const float inv = l == 0.f ? 0.f : 1.f / l;
+        short *out = (short *)a.out + (size_t)(begin + tok) * a.out_stride + (size_t)head * DH;
+        for (int d = 0; d < DH / 32; ++d)
+            for (int i = 0; i < 16; i += 4) {
+                uint2 x;
+                x.x = pack2<BF>(w.o[d][i] * inv, w.o[d][i + 1] * inv);
+                x.y = pack2<BF>(w.o[d][i + 2] * inv, w.o[d][i + 3] * inv);
+                if (void_rows) x = make_uint2(0, 0);
+                *(uint2 *)(out + d * 32 + 2 * i + 4 * h) = x;
+            }
+    } else {
+        const size_t at = (((size_t)tile * a.kv_heads + kvh) * a.splits + split) * BM + wave * 32 + r;
+        for (int d = 0; d < DH / 32; ++d)
+            for (int i = 0; i < 16; i += 4) *(qe_f4 *)(a.part_o + at * DH + d * 32 + 2 * i + 4 * h) = qe_f4{w.o[d][i], w.o[d][i + 1], w.o[d][i + 2], w.o[d][i + 3]};
+        if (h == 0) a.part_ml[at] = make_float2(w.m, void_rows ? -1.f : l);
     }
 }
 
@@ -281,7 +283,7 @@ __global__ __launch_bounds__(256) void k_attn_prompt_join(const QeAttnArgs a) {
     for (int s = 0; s < a.splits; ++s) {
         const float2 x = a.part_ml[at + (size_t)s * BM];
         if (x.y == 0.f) continue; // no key of that split
-        const float f = x.x == -INFINITY ? 0.f : exp2f((x.x - m) * a.scale_log2);
+        const float f = x.x == -INFINITY ? 0.f : exp2f(x.x - m);
         sum += f * x.y;
         for (int e = 0; e < E; ++e) o[e] += f * a.part_o[(at + (size_t)s * BM) * DH + e * 64 + lane];
     }
@@ -291,16 +293,18 @@ __global__ __launch_bounds__(256) void k_attn_prompt_join(const QeAttnArgs a) {
     for (int e = 0; e < E; ++e) out[e * 64 + lane] = (short)pack2<BF>(none ? 0.f : o[e] * inv, 0.f);
 }
 
-template <bool BF, int DH, int NB>
-static hipError_t launch_nb(const QeAttnArgs &a, hipStream_t st) {
-    k_attn_prompt<BF, DH, NB><<<dim3((unsigned)(a.tiles * a.kv_heads * a.splits)), dim3(256), 0, st>>>(a);
+template <bool BF, int DH, int WAVES>
+static hipError_t launch_waves(const QeAttnArgs &a, hipStream_t st) {
+    k_attn_prompt<BF, DH, WAVES><<<dim3((unsigned)(a.tiles * a.kv_heads * a.splits)), dim3(64 * WAVES), 0, st>>>(a);
     if (a.splits > 1)
-        k_attn_prompt_join<BF, DH, 128 * NB><<<dim3((unsigned)(a.tiles * a.kv_heads * (32 * NB))), dim3(256), 0, st>>>(a);
+        k_attn_prompt_join<BF, DH, 32 * WAVES><<<dim3((unsigned)(a.tiles * a.kv_heads * (8 * WAVES))), dim3(256), 0, st>>>(a);
     return hipGetLastError();
 }
 template <bool BF, int DH>
 static hipError_t launch_prompt(const QeAttnArgs &a, int bm, hipStream_t st) {
-    return bm == 128 ? launch_nb<BF, DH, 1>(a, st) : launch_nb<BF, DH, 2>(a, st);
+    if constexpr (DH == 256)
+        if (bm == 256) return launch_waves<BF, DH, 8>(a, st);
+    return launch_waves<BF, DH, 4>(a, st);
 }
 
 hipError_t qe_launch_attn_prompt(const QeAttnArgs &a, int head_dim, int type, int bm, hipStream_t st) {

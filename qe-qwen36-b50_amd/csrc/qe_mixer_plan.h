@@ -35,6 +35,12 @@ QE_MIX_HD int qe_attn_max_tiles(int n_tokens, int n_seqs, int group, int bm) {
     return (int)((int64_t)n_tokens * group / bm) + n_seqs;
 }
 
+// Rows of a prompt workgroup.  With heads of 256 its K and V tiles fill a CU's LDS, so eight
+// waves are the way to two waves a SIMD; with smaller heads several workgroups of four share a CU.
+QE_MIX_HD int qe_attn_prompt_rows(int n_tokens, int n_seqs, int group, int kv_heads, int head_dim) {
+    return head_dim == 256 && (int64_t)qe_attn_max_tiles(n_tokens, n_seqs, group, 256) * kv_heads >= 256 ? 256 : 128;
+}
+
 // Splits of a prompt call's keys: none if its tiles fill half the CUs.
 QE_MIX_HD int qe_attn_prompt_splits(int64_t tiles, int64_t max_len) {
     if (tiles > 128) return 1;
