@@ -35,12 +35,14 @@ __device__ __forceinline__ void load_tile(const QeAttnArgs &a, const int32_t *ta
     constexpr int CH = DH / 8, ROWS = 64 / CH, PART = BN / WAVES; // chunks of a row, rows of one direct load, rows of a wave
     const int sub = k0 + wave * PART;
     const size_t r0 = sub_row(a, table, kvh, sub < len ? sub & ~15 : (len - 1) & ~15, bad) + (wave * PART & 15);
-    const short *kc = (const short *)a.kc + r0 * DH, *vc = (const short *)a.vc + r0 * DH;
+    const char *kc = (const char *)a.kc + r0 * DH * 2, *vc = (const char *)a.vc + r0 * DH * 2;
+    // 32-bit offsets from the first row: a later row's permutation differs from the first load's by a constant
+    const int row = lane / CH, c = lane % CH;
+    const unsigned k_off = row * DH * 2 + ((c ^ k_swz<DH>(row)) << 4), v_off = row * DH * 2 + ((c ^ v_swz<DH>(row)) << 4);
 #pragma unroll
     for (int i = 0; i < PART / ROWS; ++i) {
-        const int row = wave * PART + i * ROWS + lane / CH, c = lane % CH;
-        load_lds16(kc + (i * ROWS + lane / CH) * DH + ((c ^ k_swz<DH>(row)) << 3), k_lds + (wave * PART + i * ROWS) * DH);
-        load_lds16(vc + (i * ROWS + lane / CH) * DH + ((c ^ v_swz<DH>(row)) << 3), v_lds + (wave * PART + i * ROWS) * DH);
+        load_lds16(kc + ((k_off ^ (k_swz<DH>(i * ROWS) << 4)) + i * 1024), k_lds + (wave * PART + i * ROWS) * DH);
+        load_lds16(vc + ((v_off ^ (v_swz<DH>(i * ROWS) << 4)) + i * 1024), v_lds + (wave * PART + i * ROWS) * DH);
     }
 }
 
@@ -56,71 +58,77 @@ struct Rows {
 
     __device__ __forceinline__ void step(const QeAttnArgs &a, const short *k_lds, const short *v_lds, int k0, bool masked, int lane) {
         const int r = lane & 31, h = lane >> 5;
-        // LDS addresses: four for K, whose chunk 2 st + h is permuted by the low bits of the row (chunks 8 apart are a
-        // constant apart), and for V, whose 64-byte unit d is permuted by the row in the transposing read's group
-        const char *ka[4], *va[4];
+        // Byte addresses in LDS.  K: chunk 2 st + h of row r is permuted by the row's low bits, so the four st of a
+        // 128-byte block are one address with constants exclusive-or'ed in.  V: so are the 64-byte units d of the
+        // row that a lane addresses in a transposing read.  The empty asm keeps them from being made ahead for both
+        // buffers, in registers that the loop needs.
+        const int tr = (lane & 15) >> 2, el = ((lane >> 4) & 1) * 16 + (lane & 3) * 4;
+        unsigned ka = (unsigned)(uintptr_t)QE_LDS(char, k_lds) + r * DH * 2 + ((h ^ k_swz<DH>(r)) << 4);
+        unsigned va = (unsigned)(uintptr_t)QE_LDS(char, v_lds) + (4 * h + tr) * DH * 2 + (((el >> 3) ^ v_swz<DH>(tr)) << 4) + (el & 7) * 2;
+        asm volatile("" : "+v"(ka), "+v"(va));
+        // Keys whose scores are held together: 64, or 32 where o and q leave no registers for more.
+        constexpr int NB = DH == 256 ? 1 : 2;
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            ka[i] = (const char *)k_lds + r * DH * 2 + (((2 * i + h) ^ (r & 7)) << 4);
-            const int tr = (lane & 15) >> 2, el = ((lane >> 4) & 1) * 16 + (lane & 3) * 4;
-            va[i] = (const char *)v_lds + (4 * h + tr) * DH * 2 + ((((i << 2) + (el >> 3)) ^ v_swz<DH>(tr)) << 4) + (el & 7) * 2;
-        }
-        qe_f16v s[2];
+        for (int b0 = 0; b0 < 2; b0 += NB) {
+            qe_f16v s[NB];
 #pragma unroll
-        for (int b = 0; b < 2; ++b) {
-            for (int i = 0; i < 16; ++i) s[b][i] = 0;
+            for (int b = 0; b < NB; ++b) {
+                for (int i = 0; i < 16; ++i) s[b][i] = 0;
 #pragma unroll
-            for (int st = 0; st < DH / 16; ++st)
-                s[b] = mfma32<BF>(*(const qe_s8 *)(ka[st & 3] + b * 64 * DH + (st >> 2) * 128), q[st], s[b]);
-        }
-        if (masked) {
-            const int limit = place - k0 - 4 * h; // the last key that the row attends to, counted from the lane's first
-#pragma unroll
-            for (int b = 0; b < 2; ++b)
-#pragma unroll
-                for (int i = 0; i < 16; ++i)
-                    if (b * 32 + 8 * (i / 4) + i % 4 > limit) s[b][i] = -INFINITY;
-        }
-        float top = s[0][0];
-#pragma unroll
-        for (int i = 1; i < 15; i += 2) top = max3(top, s[0][i], s[0][i + 1]);
-        top = max3(top, s[0][15], s[1][0]);
-#pragma unroll
-        for (int i = 1; i < 15; i += 2) top = max3(top, s[1][i], s[1][i + 1]);
-        top = fmaxf(top, s[1][15]);
-        top = fmaxf(top, __shfl_xor(top, 32)) * a.scale_log2;
-        // The maximum that is subtracted only has to keep the powers of two in range: it follows the true one
-        // when that has grown by more than 2^8, which after the first keys is rare.
-        if (__any(top > m + 8.f)) {
-            const float mn = fmaxf(m, top), f = m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m - mn);
-            for (int d = 0; d < DH / 32; ++d) o[d] *= f;
-            l *= f;
-            m = mn;
-        }
-        const float base = m == -INFINITY ? 0.f : -m;
-#pragma unroll
-        for (int b = 0; b < 2; ++b) {
-            union {
-                unsigned u[4];
-                qe_s8 v;
-            } p[2];
-            float sum = 0;
-#pragma unroll
-            for (int i = 0; i < 16; i += 2) {
-                const float x = __builtin_amdgcn_exp2f(fmaf(s[b][i], a.scale_log2, base));
-                const float y = __builtin_amdgcn_exp2f(fmaf(s[b][i + 1], a.scale_log2, base));
-                sum += x + y;
-                p[i / 8].u[i % 8 / 2] = pack2<BF>(x, y);
+                for (int st = 0; st < DH / 16; ++st)
+                    s[b] = mfma32<BF>(*(const __attribute__((address_space(3))) qe_s8 *)(uintptr_t)((ka ^ (st & 3) << 5) + (b0 + b) * 64 * DH + (st >> 2) * 128), q[st], s[b]);
             }
-            l += sum;
+            if (masked) {
+                const int limit = place - k0 - 4 * h - b0 * 32; // the last key that the row attends to, counted from the lane's first
 #pragma unroll
-            for (int ks = 0; ks < 2; ++ks)
+                for (int b = 0; b < NB; ++b)
 #pragma unroll
-                for (int d = 0; d < DH / 32; ++d) {
-                    const char *vp = va[d & 3] + (b * 2 + ks) * 32 * DH + (d >> 2) * 256;
-                    const qe_s4 x = lds_tr((const short *)vp), y = lds_tr((const short *)(vp + 16 * DH)); // 8 rows on the permutation is the same
-                    o[d] = mfma32<BF>(qe_s8{x[0], x[1], x[2], x[3], y[0], y[1], y[2], y[3]}, p[ks].v, o[d]);
+                    for (int i = 0; i < 16; ++i)
+                        if (b * 32 + 8 * (i / 4) + i % 4 > limit) s[b][i] = -INFINITY;
+            }
+            float top = s[0][0];
+#pragma unroll
+            for (int i = 1; i < 15; i += 2) top = max3(top, s[0][i], s[0][i + 1]);
+            top = max3(top, s[0][15], s[NB - 1][0]);
+            if constexpr (NB == 2) {
+#pragma unroll
+                for (int i = 1; i < 15; i += 2) top = max3(top, s[1][i], s[1][i + 1]);
+                top = fmaxf(top, s[1][15]);
+            }
+            top = fmaxf(top, __shfl_xor(top, 32)) * a.scale_log2;
+            // The maximum that is subtracted only has to keep the powers of two in range: it follows the true one
+            // when that has grown by more than 2^8, which after the first keys is rare.
+            if (__any(top > m + 8.f)) {
+                const float mn = fmaxf(m, top), f = m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m - mn);
+                for (int d = 0; d < DH / 32; ++d) o[d] *= f;
+                l *= f;
+                m = mn;
+            }
+            const float base = m == -INFINITY ? 0.f : -m;
+#pragma unroll
+            for (int b = 0; b < NB; ++b) {
+                union {
+                    unsigned u[4];
+                    qe_s8 v;
+                } p[2];
+                float sum = 0;
+#pragma unroll
+                for (int i = 0; i < 16; i += 2) {
+                    const float x = __builtin_amdgcn_exp2f(fmaf(s[b][i], a.scale_log2, base));
+                    const float y = __builtin_amdgcn_exp2f(fmaf(s[b][i + 1], a.scale_log2, base));
+                    sum += x + y;
+                    p[i / 8].u[i % 8 / 2] = pack2<BF>(x, y);
                 }
+                l += sum;
+#pragma unroll
+                for (int ks = 0; ks < 2; ++ks)
+#pragma unroll
+                    for (int d = 0; d < DH / 32; ++d) {
+                        const unsigned vp = (va ^ (d & 3) << 6) + ((b0 + b) * 2 + ks) * 32 * DH + (d >> 2) * 256;
+                        const qe_s4 x = lds_tr_at(vp), y = lds_tr_at(vp + 16 * DH); // 8 rows on the permutation is the same
+                        o[d] = mfma32<BF>(qe_s8{x[0], x[1], x[2], x[3], y[0], y[1], y[2], y[3]}, p[ks].v, o[d]);
+                    }
+            }
         }
     }
 };
