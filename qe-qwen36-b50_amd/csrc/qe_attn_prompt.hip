@@ -26,23 +26,32 @@ __device__ __forceinline__ int v_swz(int row) {
     return DH == 64 ? ((row >> 1) & 1) << 2 : (row & 3) << 2;
 }
 
-// A wave's part of a tile of BN keys from position k0 on: K and V to LDS.  In one direct load's
-// rows, and in a wave's part, all rows lie in one page; rows behind the end may lie in none,
-// then any of the sequence's do (their probabilities are zero).
+// The page of a wave's part of the tile of BN keys from position k0 on: all of the part's rows lie in one.
+// Rows behind the end may lie in none, then any of the sequence's do (their probabilities are zero).
+template <int WAVES>
+__device__ __forceinline__ int page_of(const QeAttnArgs &a, const int32_t *table, int k0, int len, int wave) {
+    const int sub = k0 + wave * (BN / WAVES);
+    return *(const __attribute__((address_space(4))) int32_t *)(uintptr_t)(table + ((sub < len ? sub : len - 1) >> a.page_log2));
+}
+// K and V of the part to LDS.
 template <int DH, int WAVES>
-__device__ __forceinline__ void load_tile(const QeAttnArgs &a, const int32_t *table, int kvh, int k0, int len, int wave, int lane,
-                                          short *k_lds, short *v_lds, unsigned *bad) {
+__device__ __forceinline__ void load_tile(const QeAttnArgs &a, int page, int kvh, int k0, int len, int wave, int lane, short *k_lds,
+                                          short *v_lds, unsigned *bad) {
     constexpr int CH = DH / 8, ROWS = 64 / CH, PART = BN / WAVES; // chunks of a row, rows of one direct load, rows of a wave
-    const int sub = k0 + wave * PART;
-    const size_t r0 = sub_row(a, table, kvh, sub < len ? sub & ~15 : (len - 1) & ~15, bad) + (wave * PART & 15);
+    const int sub = k0 + wave * PART, at = sub < len ? sub : (len - 1) & -PART;
+    unsigned p = (unsigned)page;
+    if (p >= a.n_pages) *bad = 1, p = 0;
+    const size_t r0 = (((size_t)p * a.kv_heads + kvh) << a.page_log2) + (at & ((1 << a.page_log2) - 1));
     const char *kc = (const char *)a.kc + r0 * DH * 2, *vc = (const char *)a.vc + r0 * DH * 2;
-    // 32-bit offsets from the first row: a later row's permutation differs from the first load's by a constant
+    // A uniform address and a 32-bit offset: a later row's permutation differs from the first load's by a constant.
+    // (The empty asm: made once for all tiles, the offsets would be spilled, and their reloads wait for the loads here.)
+    asm volatile("" : "+v"(lane));
     const int row = lane / CH, c = lane % CH;
     const unsigned k_off = row * DH * 2 + ((c ^ k_swz<DH>(row)) << 4), v_off = row * DH * 2 + ((c ^ v_swz<DH>(row)) << 4);
 #pragma unroll
     for (int i = 0; i < PART / ROWS; ++i) {
-        load_lds16(kc + ((k_off ^ (k_swz<DH>(i * ROWS) << 4)) + i * 1024), k_lds + (wave * PART + i * ROWS) * DH);
-        load_lds16(vc + ((v_off ^ (v_swz<DH>(i * ROWS) << 4)) + i * 1024), v_lds + (wave * PART + i * ROWS) * DH);
+        load_lds16(kc + i * 1024 + (k_off ^ (k_swz<DH>(i * ROWS) << 4)), k_lds + (wave * PART + i * ROWS) * DH);
+        load_lds16(vc + i * 1024 + (v_off ^ (v_swz<DH>(i * ROWS) << 4)), v_lds + (wave * PART + i * ROWS) * DH);
     }
 }
 
@@ -63,8 +72,8 @@ struct Rows {
         // row that a lane addresses in a transposing read.  The empty asm keeps them from being made ahead for both
         // buffers, in registers that the loop needs.
         const int tr = (lane & 15) >> 2, el = ((lane >> 4) & 1) * 16 + (lane & 3) * 4;
-        unsigned ka = (unsigned)(uintptr_t)QE_LDS(char, k_lds) + r * DH * 2 + ((h ^ k_swz<DH>(r)) << 4);
-        unsigned va = (unsigned)(uintptr_t)QE_LDS(char, v_lds) + (4 * h + tr) * DH * 2 + (((el >> 3) ^ v_swz<DH>(tr)) << 4) + (el & 7) * 2;
+        unsigned ka = r * DH * 2 + ((h ^ k_swz<DH>(r)) << 4);
+        unsigned va = (4 * h + tr) * DH * 2 + (((el >> 3) ^ v_swz<DH>(tr)) << 4) + (el & 7) * 2;
         asm volatile("" : "+v"(ka), "+v"(va));
         // Keys whose scores are held together: 64, or 32 where o and q leave no registers for more.
         constexpr int NB = DH == 256 ? 1 : 2;
@@ -76,7 +85,7 @@ struct Rows {
                 for (int i = 0; i < 16; ++i) s[b][i] = 0;
 #pragma unroll
                 for (int st = 0; st < DH / 16; ++st)
-                    s[b] = mfma32<BF>(*(const __attribute__((address_space(3))) qe_s8 *)(uintptr_t)((ka ^ (st & 3) << 5) + (b0 + b) * 64 * DH + (st >> 2) * 128), q[st], s[b]);
+                    s[b] = mfma32<BF>(*(const qe_s8 *)((const char *)k_lds + ((ka ^ (st & 3) << 5) + (b0 + b) * 64 * DH + (st >> 2) * 128)), q[st], s[b]);
             }
             if (masked) {
                 const int limit = place - k0 - 4 * h - b0 * 32; // the last key that the row attends to, counted from the lane's first
@@ -125,7 +134,7 @@ struct Rows {
 #pragma unroll
                     for (int d = 0; d < DH / 32; ++d) {
                         const unsigned vp = (va ^ (d & 3) << 6) + ((b0 + b) * 2 + ks) * 32 * DH + (d >> 2) * 256;
-                        const qe_s4 x = lds_tr_at(vp), y = lds_tr_at(vp + 16 * DH); // 8 rows on the permutation is the same
+                        const qe_s4 x = lds_tr((const short *)((const char *)v_lds + vp)), y = lds_tr((const short *)((const char *)v_lds + (vp + 16 * DH))); // 8 rows on the permutation is the same
                         o[d] = mfma32<BF>(qe_s8{x[0], x[1], x[2], x[3], y[0], y[1], y[2], y[3]}, p[ks].v, o[d]);
                     }
             }
@@ -182,11 +191,13 @@ __global__ __launch_bounds__(64 * WAVES, 2) void k_attn_prompt(const QeAttnArgs 
     int lo, hi;
     qe_split_range(keys > 0 ? (keys + BN - 1) / BN : 0, a.splits, split, &lo, &hi);
 
+    int page = 0; // of the wave's part of the next tile
     auto work = [&](const short *k_lds, short *v_lds, short *k_next, short *v_next, int t) {
         __builtin_amdgcn_s_waitcnt(0x0f70); // this wave's direct loads have landed,
         lds_barrier();                      // the others' too, and no wave reads the other buffers any more
         const int k0 = t * BN;
-        if (t + 1 < hi) load_tile<DH, WAVES>(a, table, kvh, k0 + BN, len, wave, lane, k_next, v_next, &bad);
+        if (t + 1 < hi) load_tile<DH, WAVES>(a, page, kvh, k0 + BN, len, wave, lane, k_next, v_next, &bad);
+        page = page_of<WAVES>(a, table, k0 + 2 * BN, len, wave); // looked up a step before it is needed
         const bool masked = k0 + BN > clear;
         if (masked) {
             // A probability of 0 times an infinity or NaN is NaN: rows behind the end become zeros, and
@@ -212,7 +223,10 @@ __global__ __launch_bounds__(64 * WAVES, 2) void k_attn_prompt(const QeAttnArgs 
         if (k0 < wave_keys) w.step(a, k_lds, v_lds, k0, k0 + BN > wave_clear, lane);
     };
     if (tid < BM / BN + 2) odd_rows[tid] = 0; // a barrier before the first tile's
-    if (lo < hi) load_tile<DH, WAVES>(a, table, kvh, lo * BN, len, wave, lane, k_a, v_a, &bad);
+    if (lo < hi) {
+        load_tile<DH, WAVES>(a, page_of<WAVES>(a, table, lo * BN, len, wave), kvh, lo * BN, len, wave, lane, k_a, v_a, &bad);
+        page = page_of<WAVES>(a, table, (lo + 1) * BN, len, wave);
+    }
     for (int t = lo; t < hi; t += 2) {
         work(k_a, v_a, k_b, v_b, t);
         if (t + 1 < hi) work(k_b, v_b, k_a, v_a, t + 1);
