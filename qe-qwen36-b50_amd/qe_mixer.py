@@ -88,36 +88,38 @@ def _type(dtype, allowed):
     return TYPES[dtype]
 
 
+# The checks are written for their cost: a single token's call is a few microseconds of GPU work, and a
+# tensor's shape, strides and device are fetched anew for every call.
 def _on(x, device, name):
-    if x.device.type != "cuda" or x.device.index != device:
+    if x.get_device() != device:
         _bad(f"{name} is on {x.device}, the context on cuda:{device}")
 
 
 def _ints(x, shape, device, name):
-    """A contiguous int32 tensor of the given shape (None = any) on the context's device."""
-    _on(x, device, name)
-    if x.dtype != torch.int32 or x.dim() != len(shape) or any(b is not None and a != b for a, b in zip(x.shape, shape)) \
-            or not x.is_contiguous():
+    """Pointer of a contiguous int32 tensor of the given shape on the context's device."""
+    if x.dtype is not torch.int32 or x.shape != shape or not x.is_contiguous() or x.get_device() != device:
+        _on(x, device, name)
         _bad(f"{name}: a contiguous int32 tensor of shape {shape} is wanted, got {x.dtype} {tuple(x.shape)}")
     return x.data_ptr()
 
 
 def _rows(x, heads, dim, dtype, device, name, tokens=None):
     """Pointer and token stride of [tokens, heads, dim], or [tokens, heads * dim], with contiguous tokens."""
+    shape = x.shape
+    if x.dtype is dtype and x.get_device() == device and (tokens is None or (shape and shape[0] == tokens)):
+        if len(shape) == 3 and shape[1] == heads and shape[2] == dim:
+            if x.is_contiguous():
+                return x.data_ptr(), heads * dim
+            stride = x.stride()
+            if stride[2] == 1 and (stride[1] == dim or heads == 1):
+                return x.data_ptr(), stride[0] if shape[0] > 1 else heads * dim
+        elif len(shape) == 2 and shape[1] == heads * dim and x.stride(1) == 1:
+            return x.data_ptr(), x.stride(0) if shape[0] > 1 else heads * dim
     _on(x, device, name)
     if x.dtype != dtype:
         _bad(f"{name} is {x.dtype}, {dtype} is wanted")
-    shape, stride = x.shape, x.stride()
-    if tokens is not None and (len(shape) == 0 or shape[0] != tokens):
-        _bad(f"{name} has shape {tuple(shape)}, {tokens} tokens are wanted")
-    if len(shape) == 3 and shape[1] == heads and shape[2] == dim:
-        fine = (stride[2] == 1 or dim == 1) and (stride[1] == dim or heads == 1)
-    else:
-        fine = len(shape) == 2 and shape[1] == heads * dim and stride[1] == 1
-    if not fine:
-        _bad(f"{name}: [{'tokens' if tokens is None else tokens}, {heads}, {dim}] with contiguous tokens is wanted, "
-             f"got {tuple(shape)} with strides {tuple(stride)}")
-    return x.data_ptr(), stride[0] if shape[0] > 1 else heads * dim
+    _bad(f"{name}: [{'tokens' if tokens is None else tokens}, {heads}, {dim}] with contiguous tokens is wanted, "
+         f"got {tuple(shape)} with strides {tuple(x.stride())}")
 
 
 class Batch:
@@ -138,13 +140,16 @@ class Batch:
         stride = table.stride(0) if n > 1 else table.shape[1]
         self.c = _Batch(n, n, None if cu_q is None else cu_q.data_ptr(), kv_len.data_ptr(), table.data_ptr(), stride,
                         table.shape[1], int(max_len))
+        self._ref = ctypes.byref(self.c)
 
-    def _with(self, rows):
-        n = rows.shape[0] if self.n_tokens is None else self.n_tokens
-        if n > rows.shape[0]:
-            _bad(f"the batch has {n} tokens, the tensors {rows.shape[0]}")
+    def _with(self, n):
+        """For tensors of n rows."""
+        if self.n_tokens is not None:
+            if self.n_tokens > n:
+                _bad(f"the batch has {self.n_tokens} tokens, the tensors {n}")
+            n = self.n_tokens
         self.c.n_tokens = n
-        return ctypes.byref(self.c)
+        return self._ref
 
 
 class Attention:
@@ -165,6 +170,9 @@ class Attention:
         self.h, self._lib = h, lib
         self.q_heads, self.kv_heads, self.head_dim, self.page, self.dtype, self.device = q_heads, kv_heads, head_dim, page, dtype, device
         self.n_axes = 3 if rotary and (s[1] or s[2]) else 1
+        self._pages = (kv_heads, page, head_dim)
+        self._c = _Cache()  # filled anew for every call
+        self._ref = ctypes.byref(self._c)
 
     def close(self):
         if self.h:
@@ -178,42 +186,51 @@ class Attention:
             pass
 
     def _cache(self, kc, vc):
-        want = (self.kv_heads, self.page, self.head_dim)
-        for x, name in ((kc, "k cache"), (vc, "v cache")):
-            _on(x, self.device, name)
-            if x.dtype != self.dtype or x.dim() != 4 or x.shape[1:] != want or not x.is_contiguous():
-                _bad(f"{name}: contiguous {self.dtype} [pages, {want[0]}, {want[1]}, {want[2]}] is wanted, got {x.dtype} {tuple(x.shape)}")
-        if kc.shape[0] != vc.shape[0]:
+        n = kc.shape
+        if not (n == vc.shape and len(n) == 4 and n[1:] == self._pages and kc.dtype is self.dtype and vc.dtype is self.dtype
+                and kc.is_contiguous() and vc.is_contiguous() and kc.get_device() == self.device and vc.get_device() == self.device):
+            for x, name in ((kc, "k cache"), (vc, "v cache")):
+                _on(x, self.device, name)
+                if x.dtype != self.dtype or x.dim() != 4 or x.shape[1:] != self._pages or not x.is_contiguous():
+                    _bad(f"{name}: contiguous {self.dtype} [pages, {', '.join(map(str, self._pages))}] is wanted, got {x.dtype} "
+                         f"{tuple(x.shape)}")
             _bad(f"k and v caches of {kc.shape[0]} and {vc.shape[0]} pages")
-        return ctypes.byref(_Cache(kc.data_ptr(), vc.data_ptr(), kc.shape[0]))
+        c = self._c
+        c.k, c.v, c.n_pages = kc.data_ptr(), vc.data_ptr(), n[0]
+        return self._ref
 
-    def _batch(self, batch, rows):
+    def _batch(self, batch, n):
         if batch.device != self.device:
             _bad(f"the batch is on cuda:{batch.device}, the context on cuda:{self.device}")
-        return batch._with(rows)
+        return batch._with(n)
 
     def append(self, batch, q, k, v, kc, vc, q_out, pos=None, stream=None):
         """Rotate q into q_out (both None: keys and values only), rotate k and write k and v to their pages."""
-        n = k.shape[0]
-        dt = k.dtype
-        _type(dt, (torch.float32, self.dtype))
-        kp, ks = _rows(k, self.kv_heads, self.head_dim, dt, self.device, "k")
-        vp, vs = _rows(v, self.kv_heads, self.head_dim, dt, self.device, "v", n)
-        qp = qs = op = os_ = None
+        n, dt, dev = k.shape[0], k.dtype, self.device
+        if dt is not self.dtype:
+            _type(dt, (torch.float32, self.dtype))
+        kp, ks = _rows(k, self.kv_heads, self.head_dim, dt, dev, "k")
+        vp, vs = _rows(v, self.kv_heads, self.head_dim, dt, dev, "v", n)
+        qp = op = None
+        qs = os_ = 0
         if (q is None) != (q_out is None):
             _bad("q and q_out go together")
         if q is not None:
-            qp, qs = _rows(q, self.q_heads, self.head_dim, dt, self.device, "q", n)
-            op, os_ = _rows(q_out, self.q_heads, self.head_dim, self.dtype, self.device, "q_out", n)
-        b = self._batch(batch, k)
-        pp = None if pos is None else _ints(pos, (self.n_axes, batch.c.n_tokens), self.device, "pos")
-        _check(self._lib.qe_attn_append(self.h, b, self._cache(kc, vc), TYPES[dt], qp, qs or 0, kp, ks, vp, vs, pp, op, os_ or 0,
-                                        _stream(stream)))
+            qp, qs = _rows(q, self.q_heads, self.head_dim, dt, dev, "q", n)
+            op, os_ = _rows(q_out, self.q_heads, self.head_dim, self.dtype, dev, "q_out", n)
+        b = self._batch(batch, n)
+        pp = None if pos is None else _ints(pos, (self.n_axes, batch.c.n_tokens), dev, "pos")
+        rc = self._lib.qe_attn_append(self.h, b, self._cache(kc, vc), TYPES[dt], qp, qs, kp, ks, vp, vs, pp, op, os_, _stream(stream))
+        if rc:
+            _check(rc)
 
     def _attend(self, entry, batch, q, kc, vc, out, stream):
         qp, qs = _rows(q, self.q_heads, self.head_dim, self.dtype, self.device, "q")
-        op, os_ = _rows(out, self.q_heads, self.head_dim, self.dtype, self.device, "out", q.shape[0])
-        _check(entry(self.h, self._batch(batch, q), self._cache(kc, vc), qp, qs, op, os_, _stream(stream)))
+        n = q.shape[0]
+        op, os_ = _rows(out, self.q_heads, self.head_dim, self.dtype, self.device, "out", n)
+        rc = entry(self.h, self._batch(batch, n), self._cache(kc, vc), qp, qs, op, os_, _stream(stream))
+        if rc:
+            _check(rc)
 
     def prompt(self, batch, q, kc, vc, out, stream=None):
         """Causal attention of the batch's new tokens, which are in the cache, over their sequences."""
@@ -240,6 +257,9 @@ class GatedDelta:
         _check(lib.qe_delta_create(device, ctypes.byref(desc), ctypes.byref(h)))
         self.h, self._lib = h, lib
         self.k_heads, self.v_heads, self.dim_k, self.dim_v, self.dtype, self.device = k_heads, v_heads, dim_k, dim_v, dtype, device
+        self._state = (v_heads, dim_k, dim_v)
+        self._a = _DeltaArgs()  # filled anew for every call
+        self._ref = ctypes.byref(self._a)
 
     def close(self):
         if self.h:
@@ -253,34 +273,39 @@ class GatedDelta:
             pass
 
     def _args(self, n_seqs, q, k, v, g, beta, pool, slots_in, slots_out, out):
-        n, dev = q.shape[0], self.device
-        qp, qs = _rows(q, self.k_heads, self.dim_k, self.dtype, dev, "q")
-        kp, ks = _rows(k, self.k_heads, self.dim_k, self.dtype, dev, "k", n)
-        vp, vs = _rows(v, self.v_heads, self.dim_v, self.dtype, dev, "v", n)
-        op, os_ = _rows(out, self.v_heads, self.dim_v, self.dtype, dev, "out", n)
+        n, dev, dt = q.shape[0], self.device, self.dtype
+        a = self._a
+        a.n_seqs, a.n_tokens = n_seqs, n
+        a.q, a.q_stride = _rows(q, self.k_heads, self.dim_k, dt, dev, "q")
+        a.k, a.k_stride = _rows(k, self.k_heads, self.dim_k, dt, dev, "k", n)
+        a.v, a.v_stride = _rows(v, self.v_heads, self.dim_v, dt, dev, "v", n)
+        a.out, a.out_stride = _rows(out, self.v_heads, self.dim_v, dt, dev, "out", n)
         for x, name in ((g, "g"), (beta, "beta")):
-            _on(x, dev, name)
-            if x.dtype != torch.float32 or tuple(x.shape) != (n, self.v_heads) or not x.is_contiguous():
+            if x.dtype is not torch.float32 or x.shape != (n, self.v_heads) or not x.is_contiguous() or x.get_device() != dev:
+                _on(x, dev, name)
                 _bad(f"{name}: contiguous float32 [{n}, {self.v_heads}] is wanted, got {x.dtype} {tuple(x.shape)}")
-        _on(pool, dev, "pool")
-        if pool.dtype != torch.float32 or pool.dim() != 4 or tuple(pool.shape[1:]) != (self.v_heads, self.dim_k, self.dim_v) \
-                or not pool.is_contiguous():
-            _bad(f"pool: contiguous float32 [slots, {self.v_heads}, {self.dim_k}, {self.dim_v}] is wanted, got {pool.dtype} "
-                 f"{tuple(pool.shape)}")
-        return _DeltaArgs(n_seqs, n, qp, kp, vp, qs, ks, vs, g.data_ptr(), beta.data_ptr(), pool.data_ptr(), pool.shape[0],
-                          _ints(slots_in, (n_seqs,), dev, "slots_in"), _ints(slots_out, (n_seqs,), dev, "slots_out"), op, os_)
+        p = pool.shape
+        if pool.dtype is not torch.float32 or len(p) != 4 or p[1:] != self._state or not pool.is_contiguous() or pool.get_device() != dev:
+            _on(pool, dev, "pool")
+            _bad(f"pool: contiguous float32 [slots, {', '.join(map(str, self._state))}] is wanted, got {pool.dtype} {tuple(p)}")
+        a.g, a.beta, a.pool, a.n_slots = g.data_ptr(), beta.data_ptr(), pool.data_ptr(), p[0]
+        a.slots_in, a.slots_out = _ints(slots_in, (n_seqs,), dev, "slots_in"), _ints(slots_out, (n_seqs,), dev, "slots_out")
+        return self._ref
 
     def prompt(self, q, k, v, g, beta, pool, slots_in, slots_out, cu, out, stream=None):
         """Packed prompts: sequence i is rows cu[i] .. cu[i + 1] - 1; its state comes from pool[slots_in[i]] (-1: zeros) and
         goes to pool[slots_out[i]] (-1: nowhere)."""
         n = slots_in.shape[0]
         a = self._args(n, q, k, v, g, beta, pool, slots_in, slots_out, out)
-        _check(self._lib.qe_delta_prompt(self.h, ctypes.byref(a), _ints(cu, (n + 1,), self.device, "cu"), _stream(stream)))
+        rc = self._lib.qe_delta_prompt(self.h, a, _ints(cu, (n + 1,), self.device, "cu"), _stream(stream))
+        if rc:
+            _check(rc)
 
     def decode(self, q, k, v, g, beta, pool, slots_in, slots_out, out, stream=None):
         """One token per sequence: row i is sequence i's."""
-        a = self._args(q.shape[0], q, k, v, g, beta, pool, slots_in, slots_out, out)
-        _check(self._lib.qe_delta_decode(self.h, ctypes.byref(a), _stream(stream)))
+        rc = self._lib.qe_delta_decode(self.h, self._args(q.shape[0], q, k, v, g, beta, pool, slots_in, slots_out, out), _stream(stream))
+        if rc:
+            _check(rc)
 
     def check(self, stream=None):
         """Synchronise `stream`; raise QeError if a kernel met a bad slot or token offset."""
