@@ -260,58 +260,110 @@ __global__ __launch_bounds__(256, 2) void k_attn_decode(const QeAttnArgs a) {
             *(uint2 *)((short *)a.out + (size_t)seq * a.out_stride + ((size_t)kvh * G + h) * DH + d) = w;
         } else {
             const size_t row = ((size_t)item * a.splits + split) * G + h;
-            *(qe_f4 *)(a.part_o + row * DH + d) = r;
-            if (d == 0) a.part_ml[row] = make_float2(top, bad ? -1.f : sum);
+            if (a.splits <= QE_ATTN_JOIN) {
+                store_through(a.part_o + row * DH + d, qe_f2{r[0], r[1]});
+                store_through(a.part_o + row * DH + d + 2, qe_f2{r[2], r[3]});
+                if (d == 0) store_through((float *)(a.part_ml + row), qe_f2{top, bad ? -1.f : sum});
+            } else {
+                *(qe_f4 *)(a.part_o + row * DH + d) = r;
+                if (d == 0) a.part_ml[row] = make_float2(top, bad ? -1.f : sum);
+            }
         }
+    }
+    if (a.splits == 1 || a.splits > QE_ATTN_JOIN) return;
+    // Few splits: the workgroup that is the last of its sequence and key-value head to arrive joins them.  Results
+    // are written through to, and read from, where all XCDs see the same; a workgroup counts itself when its own
+    // stores are acknowledged.  The last one sets the count back for the next call.
+    __shared__ unsigned before;
+    __builtin_amdgcn_s_waitcnt(0x0f70);
+    __syncthreads();
+    if (tid == 0) before = __hip_atomic_fetch_add(a.arrived + item, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    __syncthreads();
+    if (before != (unsigned)a.splits - 1) return;
+    if (tid == 0) __hip_atomic_store(a.arrived + item, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    for (int i = tid; i < a.group * (DH / 4); i += 256) {
+        const int h = i / (DH / 4), d = i % (DH / 4) * 4;
+        const size_t row = (size_t)item * a.splits * G + h;
+        qe_f2 x[QE_ATTN_JOIN], lo4[QE_ATTN_JOIN], hi4[QE_ATTN_JOIN];
+#pragma unroll
+        for (int s = 0; s < QE_ATTN_JOIN; ++s) {
+            const size_t at = row + (s < a.splits ? s : 0) * G; // behind the last split the first again, unused
+            x[s] = load_through((const float *)(a.part_ml + at));
+            lo4[s] = load_through(a.part_o + at * DH + d);
+            hi4[s] = load_through(a.part_o + at * DH + d + 2);
+        }
+        float top = -INFINITY, sum = 0;
+        bool none = false;
+#pragma unroll
+        for (int s = 0; s < QE_ATTN_JOIN; ++s)
+            if (s < a.splits) top = fmaxf(top, x[s][0]), none |= x[s][1] < 0.f;
+        qe_f4 r = {0, 0, 0, 0};
+#pragma unroll
+        for (int s = 0; s < QE_ATTN_JOIN; ++s) {
+            if (s >= a.splits || x[s][1] == 0.f) continue; // a split without keys
+            const float f = x[s][0] == -INFINITY ? 0.f : exp2f((x[s][0] - top) * a.scale_log2);
+            sum += f * x[s][1];
+            r += f * qe_f4{lo4[s][0], lo4[s][1], hi4[s][0], hi4[s][1]};
+        }
+        r *= sum == 0.f ? 0.f : 1.f / sum;
+        if (none) r = qe_f4{0, 0, 0, 0};
+        uint2 w;
+        w.x = pack2<BF>(r[0], r[1]);
+        w.y = pack2<BF>(r[2], r[3]);
+        *(uint2 *)((short *)a.out + (size_t)seq * a.out_stride + ((size_t)kvh * G + h) * DH + d) = w;
     }
 }
 
 // ---------------------------------------------------------------------------
-// The splits' results of a row joined: o = sum 2^(m_s - m) o_s / sum 2^(m_s - m) l_s.  A
-// workgroup per row of a decode call.
+// Many splits' results joined: o = sum 2^(m_s - m) o_s / sum 2^(m_s - m) l_s.  A workgroup for 64
+// elements of a row, 16 threads for them and 16 groups over the splits: 256 splits of 16 rows
+// of 256 are 4 MB, which 16 workgroups, one a row, took 27 us to read.
 // ---------------------------------------------------------------------------
 template <bool BF, int DH>
 __global__ __launch_bounds__(256) void k_attn_join(const QeAttnArgs a) {
-    constexpr int TD = DH / 4, GR = 256 / TD; // threads of a row's elements, groups of splits
     __shared__ float w_s[QE_ATTN_WGS];
-    __shared__ float red[256];
+    __shared__ float red[4], red2[4];
     __shared__ __align__(16) qe_f4 o_s[256];
-    const int tid = threadIdx.x, head = blockIdx.x % a.q_heads, seq = blockIdx.x / a.q_heads;
+    const int tid = threadIdx.x, part = blockIdx.x % (DH / 64), head = blockIdx.x / (DH / 64) % a.q_heads, seq = blockIdx.x / (DH / 64) / a.q_heads;
     const int kvh = head / a.group, h = head % a.group;
     const size_t row0 = ((size_t)seq * a.kv_heads + kvh) * a.splits * a.group + h;
+    const int d = part * 64 + tid % 16 * 4;
+    float2 x[QE_ATTN_WGS / 256];
     float m = -INFINITY;
     int bad = 0;
-    for (int s = tid; s < a.splits; s += 256) {
-        const float2 x = a.part_ml[row0 + (size_t)s * a.group];
-        bad |= x.y < 0.f;
-        m = fmaxf(m, x.x);
+#pragma unroll
+    for (int k = 0; k < QE_ATTN_WGS / 256; ++k) {
+        const int s = tid + k * 256;
+        x[k] = s < a.splits ? a.part_ml[row0 + (size_t)s * a.group] : make_float2(-INFINITY, 0.f);
+        bad |= x[k].y < 0.f;
+        m = fmaxf(m, x[k].x);
     }
     for (int k = 32; k; k >>= 1) m = fmaxf(m, __shfl_xor(m, k));
     if ((tid & 63) == 0) red[tid >> 6] = m;
     bad = __syncthreads_or(bad);
     m = fmaxf(fmaxf(red[0], red[1]), fmaxf(red[2], red[3]));
-    __syncthreads();
     float sum = 0;
-    for (int s = tid; s < a.splits; s += 256) {
-        const float2 x = a.part_ml[row0 + (size_t)s * a.group];
-        const float f = x.y == 0.f || x.x == -INFINITY ? 0.f : exp2f((x.x - m) * a.scale_log2);
-        w_s[s] = x.y == 0.f ? -1.f : f; // -1: nothing of that split is used
-        sum += x.y == 0.f ? 0.f : f * x.y;
+#pragma unroll
+    for (int k = 0; k < QE_ATTN_WGS / 256; ++k) {
+        const float f = x[k].y == 0.f || x[k].x == -INFINITY ? 0.f : exp2f((x[k].x - m) * a.scale_log2);
+        w_s[tid + k * 256] = x[k].y == 0.f ? -1.f : f; // -1: nothing of that split is used
+        sum += x[k].y == 0.f ? 0.f : f * x[k].y;
     }
     for (int k = 32; k; k >>= 1) sum += __shfl_xor(sum, k);
-    if ((tid & 63) == 0) red[tid >> 6] = sum;
+    if ((tid & 63) == 0) red2[tid >> 6] = sum;
     __syncthreads();
-    sum = (red[0] + red[1]) + (red[2] + red[3]);
-    const int d = tid % TD * 4;
+    sum = (red2[0] + red2[1]) + (red2[2] + red2[3]);
     qe_f4 r = {0, 0, 0, 0};
-    for (int s = tid / TD; s < a.splits; s += GR) {
+#pragma unroll 4
+    for (int s = tid / 16; s < a.splits; s += 16) {
         const float f = w_s[s];
-        if (f >= 0.f || f != f) r += f * *(const qe_f4 *)(a.part_o + (row0 + (size_t)s * a.group) * DH + d);
+        const qe_f4 o = *(const qe_f4 *)(a.part_o + (row0 + (size_t)s * a.group) * DH + d);
+        if (f >= 0.f || f != f) r += f * o;
     }
     o_s[tid] = r;
     __syncthreads();
-    if (tid < TD) {
-        for (int g = 1; g < GR; ++g) r += o_s[g * TD + tid];
+    if (tid < 16) {
+        for (int g = 1; g < 16; ++g) r += o_s[g * 16 + tid];
         r *= sum == 0.f ? 0.f : 1.f / sum;
         if (bad) r = qe_f4{0, 0, 0, 0};
         uint2 w;
@@ -324,7 +376,7 @@ __global__ __launch_bounds__(256) void k_attn_join(const QeAttnArgs a) {
 template <bool BF, int DH>
 static hipError_t launch_decode(const QeAttnArgs &a, hipStream_t st) {
     k_attn_decode<BF, DH><<<dim3((unsigned)(a.n_seqs * a.kv_heads * a.splits)), dim3(256), 0, st>>>(a);
-    if (a.splits > 1) k_attn_join<BF, DH><<<dim3((unsigned)(a.n_seqs * a.q_heads)), dim3(256), 0, st>>>(a);
+    if (a.splits > QE_ATTN_JOIN) k_attn_join<BF, DH><<<dim3((unsigned)(a.n_seqs * a.q_heads * (DH / 64))), dim3(256), 0, st>>>(a);
     return hipGetLastError();
 }
 

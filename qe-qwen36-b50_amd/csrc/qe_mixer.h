@@ -22,6 +22,7 @@ struct QeAttnArgs {
     int splits, tiles;
     float *part_o;   // partial results: [item][split][row][head_dim], unnormalised
     float2 *part_ml; // [item][split][row]: running maximum (raw scores) and sum; sum < 0: the split met a bad page
+    unsigned *arrived; // per sequence and key-value head, 0 between calls: decode's workgroups that are done
     unsigned *err;
 };
 

@@ -78,6 +78,7 @@ struct qe_attn_ctx {
     uint8_t *axis = nullptr;
     float *part_o = nullptr;
     float2 *part_ml = nullptr;
+    unsigned *arrived = nullptr;
 };
 
 namespace {
@@ -87,6 +88,7 @@ void release(qe_attn_ctx *c) {
     (void)hipFree(c->axis);
     (void)hipFree(c->part_o);
     (void)hipFree(c->part_ml);
+    (void)hipFree(c->arrived);
     c->err.free();
     delete c;
 }
@@ -134,7 +136,7 @@ QeAttnArgs attn_args(const qe_attn_ctx *c, const qe_attn_batch *b, const qe_kv_c
     a.page_log2 = log2_of(c->d.page);
     a.n_pages = (unsigned)kv->n_pages;
     a.scale_log2 = c->scale_log2;
-    a.part_o = c->part_o; a.part_ml = c->part_ml;
+    a.part_o = c->part_o; a.part_ml = c->part_ml; a.arrived = c->arrived;
     a.err = c->err.dev;
     return a;
 }
@@ -185,7 +187,10 @@ int qe_attn_create(int device, const qe_attn_desc *d, qe_attn_ctx **out) {
     if (e == hipSuccess) e = hipMalloc((void **)&c->axis, sizeof axis);
     if (e == hipSuccess) e = hipMalloc((void **)&c->part_o, rows * d->head_dim * 4);
     if (e == hipSuccess) e = hipMalloc((void **)&c->part_ml, rows * sizeof(float2));
+    if (e == hipSuccess) e = hipMalloc((void **)&c->arrived, QE_ATTN_WGS * sizeof(unsigned));
     const bool oom = e == hipErrorOutOfMemory;
+    if (e == hipSuccess) e = hipMemset(c->arrived, 0, QE_ATTN_WGS * sizeof(unsigned));
+    if (e == hipSuccess) e = hipDeviceSynchronize();
     if (e == hipSuccess && pairs) {
         e = hipMemcpy(c->turns, turns, pairs * sizeof(double), hipMemcpyHostToDevice);
         if (e == hipSuccess) e = hipMemcpy(c->axis, axis, pairs, hipMemcpyHostToDevice);

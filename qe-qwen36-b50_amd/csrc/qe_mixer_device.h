@@ -67,6 +67,14 @@ __device__ __forceinline__ void load_lds16(const void *src, void *dst) {
 // all global loads and direct loads in flight, which here are meant for later.
 __device__ __forceinline__ void lds_barrier() { asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory"); }
 
+// 8 bytes to and from where all XCDs see the same, past their L2s
+__device__ __forceinline__ void store_through(float *p, qe_f2 x) {
+    __hip_atomic_store((unsigned long long *)p, __builtin_bit_cast(unsigned long long, x), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+}
+__device__ __forceinline__ qe_f2 load_through(const float *p) {
+    return __builtin_bit_cast(qe_f2, __hip_atomic_load((const unsigned long long *)p, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT));
+}
+
 __device__ __forceinline__ void report(unsigned *err, unsigned what) {
     __hip_atomic_store(err, what, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_SYSTEM);
 }

@@ -14,6 +14,7 @@
 #define QE_ATTN_TILE 32    /* keys of a decode wave's step */
 #define QE_ATTN_WGS 512    /* workgroups a call is split up to: two for each of the 256 CUs */
 #define QE_ATTN_BN 64      /* keys of a prompt workgroup's step */
+#define QE_ATTN_JOIN 8     /* splits that the last workgroup of a decode call joins itself; more: a launch of its own */
 #define QE_ATTN_PART_WGS 1024 /* partial results a decode call can need (see qe_attn_decode_splits) */
 
 // Splits of every sequence's length in a decode call: as many as make QE_ATTN_WGS workgroups,
