@@ -147,19 +147,28 @@ __global__ __launch_bounds__(256, 2) void k_attn_decode(const QeAttnArgs a) {
     constexpr int KS = DH / 32, DB = DH / 16;
     __shared__ __align__(16) short v_lds[4][QE_ATTN_TILE * DH];
     __shared__ float2 ml[4][16];
-    const int tid = threadIdx.x, wave = tid >> 6, lane = tid & 63, col = lane & 15, c = lane >> 4;
-    const int split = blockIdx.x % a.splits, item = blockIdx.x / a.splits, seq = item / a.kv_heads, kvh = item % a.kv_heads;
+    const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63, col = lane & 15, c = lane >> 4;
+    // Workgroups go to the eight XCDs in turn.  Where the last one joins (below), a sequence's and head's all go to
+    // one, whose L2 then has their results; else any order does.
+    const bool near = a.splits > 1 && a.splits <= QE_ATTN_JOIN;
+    const int at = near ? blockIdx.x / 8 : blockIdx.x, split = at % a.splits, item = near ? at / a.splits * 8 + blockIdx.x % 8 : at / a.splits;
+    if (item >= a.n_seqs * a.kv_heads) return;
+    const int seq = item / a.kv_heads, kvh = item % a.kv_heads;
     unsigned bad_len = 0, bad = 0;
-    const int len = qe_checked(a.kv_len[seq], 0, a.max_pages << a.page_log2, 0, &bad_len);
+    // the wave's first page, looked up along with the length, as it is if the length is no longer than the host believed
+    const unsigned first = ((unsigned)split * a.steps + wave) * QE_ATTN_TILE, cap = a.max_pages - 1;
+    const unsigned guess0 = first >> a.page_log2 < cap ? first >> a.page_log2 : cap, guess1 = (first + 16) >> a.page_log2 < cap ? (first + 16) >> a.page_log2 : cap;
+    int page0 = scalar_load(a.table + (size_t)seq * a.table_stride + guess0), page1 = scalar_load(a.table + (size_t)seq * a.table_stride + guess1);
+    const short *q = (const short *)a.q + (size_t)seq * a.q_stride + ((size_t)kvh * a.group + col) * DH + c * 8;
+    qe_s8 qf[KS];
+    for (int s = 0; s < KS; ++s) qf[s] = col < a.group ? *(const qe_s8 *)(q + s * 32) : qe_s8{};
+    const int len = qe_checked(scalar_load(a.kv_len + seq), 0, a.max_pages << a.page_log2, 0, &bad_len);
     const int32_t *table = a.table + (size_t)seq * a.table_stride;
     const size_t G = a.group;
+    const int steps = qe_attn_decode_steps(len, a.steps, a.splits), active = qe_attn_decode_active(len, steps);
+    if (split >= (active > 1 ? active : 1)) return; // a sequence without keys is the first workgroup's, which writes zeros
 
-    qe_s8 qf[KS];
-    const short *q = (const short *)a.q + (size_t)seq * a.q_stride + ((size_t)kvh * G + col) * DH + c * 8;
-    for (int s = 0; s < KS; ++s) qf[s] = col < a.group ? *(const qe_s8 *)(q + s * 32) : qe_s8{};
-
-    int lo, hi;
-    qe_split_range((len + QE_ATTN_TILE - 1) / QE_ATTN_TILE, a.splits, split, &lo, &hi);
+    const int tiles = (len + QE_ATTN_TILE - 1) / QE_ATTN_TILE, lo = split * steps, hi = lo + steps < tiles ? lo + steps : tiles;
     qe_f4 acc[DB];
     for (int d = 0; d < DB; ++d) acc[d] = qe_f4{0, 0, 0, 0};
     float m = -INFINITY, l = 0;
@@ -168,8 +177,12 @@ __global__ __launch_bounds__(256, 2) void k_attn_decode(const QeAttnArgs a) {
     for (int t = lo + wave; t < hi; t += 4) {
         const int k0 = t * QE_ATTN_TILE;
         // the 16 positions from k0 + 16 on may be behind the end: any page of the sequence does
-        const size_t r0 = sub_row(a, table, kvh, k0, &bad);
-        const size_t r1 = k0 + 16 < len ? sub_row(a, table, kvh, k0 + 16, &bad) : r0;
+        if (t != lo + wave || steps != a.steps) {
+            page0 = scalar_load(table + (k0 >> a.page_log2));
+            if (k0 + 16 < len) page1 = scalar_load(table + ((k0 + 16) >> a.page_log2));
+        }
+        const size_t r0 = page_row(a, page0, kvh, k0, &bad);
+        const size_t r1 = k0 + 16 < len ? page_row(a, page1, kvh, k0 + 16, &bad) : r0;
         qe_s8 kf[2][KS];
         const short *kp0 = (const short *)a.kc + (r0 + col) * DH + c * 8, *kp1 = (const short *)a.kc + (r1 + col) * DH + c * 8;
 #pragma unroll
@@ -235,7 +248,7 @@ __global__ __launch_bounds__(256, 2) void k_attn_decode(const QeAttnArgs a) {
     if (lane < 16) ml[wave][lane] = make_float2(m, l);
     // the waves' results through LDS (a wave's own V buffer holds 16 heads x DH floats)
     float *o = (float *)vb;
-    for (int d = 0; d < DB; ++d) *(qe_f4 *)(o + col * DH + d * 16 + c * 4) = acc[d];
+    for (int d = 0; d < DB; ++d) *(qe_f4 *)(o + col * DH + ((d * 4 + c) ^ col) * 4) = acc[d]; // 16-byte units permuted by row: rows lie in the same banks
     bad = __syncthreads_or(bad) ? 1 : 0;
     if (tid == 0 && (bad | bad_len)) report(a.err, bad ? QE_BAD_PAGE : QE_BAD_LENGTH);
     for (int i = tid; i < a.group * (DH / 4); i += 256) {
@@ -245,12 +258,12 @@ __global__ __launch_bounds__(256, 2) void k_attn_decode(const QeAttnArgs a) {
         float sum = 0;
         qe_f4 r = {0, 0, 0, 0};
         for (int w = 0; w < 4; ++w) {
-            const float mw = ml[w][h].x, f = mw == -INFINITY ? 0.f : exp2f((mw - top) * a.scale_log2);
+            const float mw = ml[w][h].x, f = mw == -INFINITY ? 0.f : __builtin_amdgcn_exp2f((mw - top) * a.scale_log2);
             if (ml[w][h].y == 0.f) continue; // a wave without keys
             sum += f * ml[w][h].y;
-            r += f * *(const qe_f4 *)((const float *)v_lds[w] + h * DH + d);
+            r += f * *(const qe_f4 *)((const float *)v_lds[w] + h * DH + ((d / 4) ^ h) * 4);
         }
-        if (a.splits == 1) {
+        if (active <= 1) {
             const float inv = sum == 0.f ? 0.f : 1.f / sum;
             r *= inv;
             if (bad) r = qe_f4{0, 0, 0, 0};
@@ -270,43 +283,71 @@ __global__ __launch_bounds__(256, 2) void k_attn_decode(const QeAttnArgs a) {
             }
         }
     }
-    if (a.splits == 1 || a.splits > QE_ATTN_JOIN) return;
+    if (active <= 1 || a.splits > QE_ATTN_JOIN) return;
     // Few splits: the workgroup that is the last of its sequence and key-value head to arrive joins them.  Results
     // are written through to, and read from, where all XCDs see the same; a workgroup counts itself when its own
     // stores are acknowledged.  The last one sets the count back for the next call.
-    __shared__ unsigned before;
+    // The count's low 8 bits are all workgroups', then 7 for those of each XCD.
+    __shared__ unsigned long long count_s;
+    const unsigned xcd = xcd_id();
+    const unsigned long long one = 1ull + (1ull << (8 + 7 * xcd));
     __builtin_amdgcn_s_waitcnt(0x0f70);
     __syncthreads();
-    if (tid == 0) before = __hip_atomic_fetch_add(a.arrived + item, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    if (tid == 0) count_s = __hip_atomic_fetch_add(a.arrived + item, one, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) + one;
     __syncthreads();
-    if (before != (unsigned)a.splits - 1) return;
-    if (tid == 0) __hip_atomic_store(a.arrived + item, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-    for (int i = tid; i < a.group * (DH / 4); i += 256) {
-        const int h = i / (DH / 4), d = i % (DH / 4) * 4;
-        const size_t row = (size_t)item * a.splits * G + h;
-        qe_f2 x[QE_ATTN_JOIN], lo4[QE_ATTN_JOIN], hi4[QE_ATTN_JOIN];
-#pragma unroll
-        for (int s = 0; s < QE_ATTN_JOIN; ++s) {
-            const size_t at = row + (s < a.splits ? s : 0) * G; // behind the last split the first again, unused
-            x[s] = load_through((const float *)(a.part_ml + at));
-            lo4[s] = load_through(a.part_o + at * DH + d);
-            hi4[s] = load_through(a.part_o + at * DH + d + 2);
+    const unsigned long long count = count_s;
+    if ((count & 255) != (unsigned)active) return;
+    if (tid == 0) __hip_atomic_store(a.arrived + item, 0ull, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    const size_t row0 = (size_t)item * a.splits * G;
+    // All on this XCD, as the order of launch has it: their results are in its L2, and are read as usual (they were not
+    // before in this launch, so no older copy is nearer).  Else from behind the L2s.
+    const bool near_all = (count >> (8 + 7 * xcd) & 127) == (unsigned)active;
+    float2 *all_ml = (float2 *)v_lds[0]; // [split][16]
+    float *sums = (float *)(all_ml + QE_ATTN_JOIN * 16);
+    for (int i = tid; i < active * 16; i += 256)
+        if ((i & 15) < a.group) {
+            const float *p = (const float *)(a.part_ml + row0 + (i >> 4) * G + (i & 15));
+            const qe_f2 x = load_through(p); // rows of others, read in this launch by their last workgroups, share its line
+            all_ml[i] = make_float2(x[0], x[1]);
         }
+    __syncthreads();
+    if (tid < a.group) {
         float top = -INFINITY, sum = 0;
         bool none = false;
+        for (int s = 0; s < active; ++s) top = fmaxf(top, all_ml[s * 16 + tid].x), none |= all_ml[s * 16 + tid].y < 0.f;
+        for (int s = 0; s < active; ++s) {
+            const float2 x = all_ml[s * 16 + tid];
+            const float f = x.y == 0.f || x.x == -INFINITY ? 0.f : __builtin_amdgcn_exp2f((x.x - top) * a.scale_log2);
+            sum += x.y == 0.f ? 0.f : f * x.y;
+            all_ml[s * 16 + tid].x = f;
+        }
+        sums[tid] = none ? -1.f : sum;
+    }
+    __syncthreads();
+    // a thread's 16 bytes of a row, all splits' in flight
+    const int n = a.group * (DH / 4);
+    for (int i = tid; i < n; i += 256) {
+        const int h = i / (DH / 4), d = i % (DH / 4) * 4;
+        const float *p = a.part_o + (row0 + h) * DH + d;
+        qe_f4 o[QE_ATTN_JOIN];
+        if (near_all) {
 #pragma unroll
-        for (int s = 0; s < QE_ATTN_JOIN; ++s)
-            if (s < a.splits) top = fmaxf(top, x[s][0]), none |= x[s][1] < 0.f;
+            for (int s = 0; s < QE_ATTN_JOIN; ++s) o[s] = *(const qe_f4 *)(p + (s < active ? s : 0) * G * DH); // behind the last the first again, unused
+        } else {
+#pragma unroll
+            for (int s = 0; s < QE_ATTN_JOIN; ++s) {
+                const float *at = p + (s < active ? s : 0) * G * DH;
+                const qe_f2 x = load_through(at), y = load_through(at + 2);
+                o[s] = qe_f4{x[0], x[1], y[0], y[1]};
+            }
+        }
         qe_f4 r = {0, 0, 0, 0};
 #pragma unroll
-        for (int s = 0; s < QE_ATTN_JOIN; ++s) {
-            if (s >= a.splits || x[s][1] == 0.f) continue; // a split without keys
-            const float f = x[s][0] == -INFINITY ? 0.f : exp2f((x[s][0] - top) * a.scale_log2);
-            sum += f * x[s][1];
-            r += f * qe_f4{lo4[s][0], lo4[s][1], hi4[s][0], hi4[s][1]};
-        }
+        for (int s = 0; s < QE_ATTN_JOIN; ++s)
+            if (s < active && all_ml[s * 16 + h].y != 0.f) r += all_ml[s * 16 + h].x * o[s]; // else a split without sum
+        const float sum = sums[h];
         r *= sum == 0.f ? 0.f : 1.f / sum;
-        if (none) r = qe_f4{0, 0, 0, 0};
+        if (sum < 0.f) r = qe_f4{0, 0, 0, 0};
         uint2 w;
         w.x = pack2<BF>(r[0], r[1]);
         w.y = pack2<BF>(r[2], r[3]);
@@ -321,20 +362,24 @@ __global__ __launch_bounds__(256, 2) void k_attn_decode(const QeAttnArgs a) {
 // ---------------------------------------------------------------------------
 template <bool BF, int DH>
 __global__ __launch_bounds__(256) void k_attn_join(const QeAttnArgs a) {
-    __shared__ float w_s[QE_ATTN_WGS];
+    __shared__ float w_s[QE_ATTN_DECODE_SPLITS];
     __shared__ float red[4], red2[4];
     __shared__ __align__(16) qe_f4 o_s[256];
     const int tid = threadIdx.x, part = blockIdx.x % (DH / 64), head = blockIdx.x / (DH / 64) % a.q_heads, seq = blockIdx.x / (DH / 64) / a.q_heads;
     const int kvh = head / a.group, h = head % a.group;
+    unsigned bad_len = 0;
+    const int len = qe_checked(a.kv_len[seq], 0, a.max_pages << a.page_log2, 0, &bad_len);
+    const int active = qe_attn_decode_active(len, qe_attn_decode_steps(len, a.steps, a.splits));
+    if (active <= 1) return; // its one workgroup has written the row
     const size_t row0 = ((size_t)seq * a.kv_heads + kvh) * a.splits * a.group + h;
     const int d = part * 64 + tid % 16 * 4;
-    float2 x[QE_ATTN_WGS / 256];
+    float2 x[QE_ATTN_DECODE_SPLITS / 256];
     float m = -INFINITY;
     int bad = 0;
 #pragma unroll
-    for (int k = 0; k < QE_ATTN_WGS / 256; ++k) {
+    for (int k = 0; k < QE_ATTN_DECODE_SPLITS / 256; ++k) {
         const int s = tid + k * 256;
-        x[k] = s < a.splits ? a.part_ml[row0 + (size_t)s * a.group] : make_float2(-INFINITY, 0.f);
+        x[k] = s < active ? a.part_ml[row0 + (size_t)s * a.group] : make_float2(-INFINITY, 0.f);
         bad |= x[k].y < 0.f;
         m = fmaxf(m, x[k].x);
     }
@@ -344,7 +389,7 @@ __global__ __launch_bounds__(256) void k_attn_join(const QeAttnArgs a) {
     m = fmaxf(fmaxf(red[0], red[1]), fmaxf(red[2], red[3]));
     float sum = 0;
 #pragma unroll
-    for (int k = 0; k < QE_ATTN_WGS / 256; ++k) {
+    for (int k = 0; k < QE_ATTN_DECODE_SPLITS / 256; ++k) {
         const float f = x[k].y == 0.f || x[k].x == -INFINITY ? 0.f : exp2f((x[k].x - m) * a.scale_log2);
         w_s[tid + k * 256] = x[k].y == 0.f ? -1.f : f; // -1: nothing of that split is used
         sum += x[k].y == 0.f ? 0.f : f * x[k].y;
@@ -355,7 +400,7 @@ __global__ __launch_bounds__(256) void k_attn_join(const QeAttnArgs a) {
     sum = (red2[0] + red2[1]) + (red2[2] + red2[3]);
     qe_f4 r = {0, 0, 0, 0};
 #pragma unroll 4
-    for (int s = tid / 16; s < a.splits; s += 16) {
+    for (int s = tid / 16; s < active; s += 16) {
         const float f = w_s[s];
         const qe_f4 o = *(const qe_f4 *)(a.part_o + (row0 + (size_t)s * a.group) * DH + d);
         if (f >= 0.f || f != f) r += f * o;
@@ -375,7 +420,8 @@ __global__ __launch_bounds__(256) void k_attn_join(const QeAttnArgs a) {
 
 template <bool BF, int DH>
 static hipError_t launch_decode(const QeAttnArgs &a, hipStream_t st) {
-    k_attn_decode<BF, DH><<<dim3((unsigned)(a.n_seqs * a.kv_heads * a.splits)), dim3(256), 0, st>>>(a);
+    const unsigned units = (unsigned)(a.n_seqs * a.kv_heads), whole = a.splits > 1 && a.splits <= QE_ATTN_JOIN ? (units + 7) / 8 * 8 : units;
+    k_attn_decode<BF, DH><<<dim3(whole * a.splits), dim3(256), 0, st>>>(a);
     if (a.splits > QE_ATTN_JOIN) k_attn_join<BF, DH><<<dim3((unsigned)(a.n_seqs * a.q_heads * (DH / 64))), dim3(256), 0, st>>>(a);
     return hipGetLastError();
 }

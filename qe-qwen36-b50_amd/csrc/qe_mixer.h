@@ -19,10 +19,11 @@ struct QeAttnArgs {
     int q_heads, kv_heads, group, page_log2;
     unsigned n_pages;
     float scale_log2; // scale * log2(e)
-    int splits, tiles;
+    int splits, tiles; // workgroups for a sequence (decode) or tile of rows (prompt) and key-value head
+    int steps;         // decode: see qe_attn_decode_plan
     float *part_o;   // partial results: [item][split][row][head_dim], unnormalised
     float2 *part_ml; // [item][split][row]: running maximum (raw scores) and sum; sum < 0: the split met a bad page
-    unsigned *arrived; // per sequence and key-value head, 0 between calls: decode's workgroups that are done
+    unsigned long long *arrived; // per sequence and key-value head, 0 between calls: decode's workgroups that are done
     unsigned *err;
 };
 

@@ -78,7 +78,7 @@ struct qe_attn_ctx {
     uint8_t *axis = nullptr;
     float *part_o = nullptr;
     float2 *part_ml = nullptr;
-    unsigned *arrived = nullptr;
+    unsigned long long *arrived = nullptr;
 };
 
 namespace {
@@ -187,9 +187,9 @@ int qe_attn_create(int device, const qe_attn_desc *d, qe_attn_ctx **out) {
     if (e == hipSuccess) e = hipMalloc((void **)&c->axis, sizeof axis);
     if (e == hipSuccess) e = hipMalloc((void **)&c->part_o, rows * d->head_dim * 4);
     if (e == hipSuccess) e = hipMalloc((void **)&c->part_ml, rows * sizeof(float2));
-    if (e == hipSuccess) e = hipMalloc((void **)&c->arrived, QE_ATTN_WGS * sizeof(unsigned));
+    if (e == hipSuccess) e = hipMalloc((void **)&c->arrived, QE_ATTN_DECODE_WGS * sizeof(unsigned long long));
     const bool oom = e == hipErrorOutOfMemory;
-    if (e == hipSuccess) e = hipMemset(c->arrived, 0, QE_ATTN_WGS * sizeof(unsigned));
+    if (e == hipSuccess) e = hipMemset(c->arrived, 0, QE_ATTN_DECODE_WGS * sizeof(unsigned long long));
     if (e == hipSuccess) e = hipDeviceSynchronize();
     if (e == hipSuccess && pairs) {
         e = hipMemcpy(c->turns, turns, pairs * sizeof(double), hipMemcpyHostToDevice);
@@ -280,7 +280,7 @@ int qe_attn_decode(qe_attn_ctx *c, const qe_attn_batch *b, const qe_kv_cache *kv
     if (rc != QE_OK) return rc;
     QeAttnArgs a = attn_args(c, b, kv, q, q_stride, out, out_stride);
     const int64_t most = (int64_t)b->max_pages * c->d.page;
-    a.splits = qe_attn_decode_splits((int64_t)b->n_seqs * a.kv_heads, b->max_len && b->max_len < most ? b->max_len : most);
+    qe_attn_decode_plan(b->n_seqs, a.kv_heads, c->d.head_dim, b->max_len && b->max_len < most ? b->max_len : most, &a.steps, &a.splits);
     OnDevice on(c->device);
     HIP_TRY(on.e);
     HIP_TRY(qe_launch_attn_decode(a, c->d.head_dim, c->d.type, (hipStream_t)stream));

@@ -79,10 +79,18 @@ __device__ __forceinline__ void report(unsigned *err, unsigned what) {
     __hip_atomic_store(err, what, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_SYSTEM);
 }
 
-// First row of the 16 positions from pos16 (a multiple of 16) on, of one key-value head: they
-// stand in one page.  A page id outside the cache becomes page 0 and sets *bad.  Wave-uniform.
-__device__ __forceinline__ size_t sub_row(const QeAttnArgs &a, const int32_t *table, int kvh, int pos16, unsigned *bad) {
-    unsigned p = (unsigned)__builtin_amdgcn_readfirstlane(table[pos16 >> a.page_log2]);
+// a word of memory that no kernel in flight writes, at a wave-uniform address, through the scalar cache
+__device__ __forceinline__ int scalar_load(const int32_t *p) { return *(const __attribute__((address_space(4))) int32_t *)(uintptr_t)p; }
+__device__ __forceinline__ unsigned xcd_id() { return __builtin_amdgcn_s_getreg(20 | 3 << 11) & 7; } // HW_REG_XCC_ID, 4 bits
+
+// First row of the 16 positions from pos16 (a multiple of 16) on, of one key-value head, in their page.
+// A page id outside the cache becomes page 0 and sets *bad.
+__device__ __forceinline__ size_t page_row(const QeAttnArgs &a, int page, int kvh, int pos16, unsigned *bad) {
+    unsigned p = (unsigned)page;
     if (p >= a.n_pages) *bad = 1, p = 0;
     return (((size_t)p * a.kv_heads + kvh) << a.page_log2) + (pos16 & ((1 << a.page_log2) - 1));
+}
+// the same, with the page looked up
+__device__ __forceinline__ size_t sub_row(const QeAttnArgs &a, const int32_t *table, int kvh, int pos16, unsigned *bad) {
+    return page_row(a, scalar_load(table + (pos16 >> a.page_log2)), kvh, pos16, bad);
 }

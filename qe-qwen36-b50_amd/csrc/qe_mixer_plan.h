@@ -12,19 +12,45 @@
 // ---- attention ----------------------------------------------------------------
 #define QE_ATTN_SUB 16     /* keys that share one page lookup: the smallest page */
 #define QE_ATTN_TILE 32    /* keys of a decode wave's step */
-#define QE_ATTN_WGS 512    /* workgroups a call is split up to: two for each of the 256 CUs */
 #define QE_ATTN_BN 64      /* keys of a prompt workgroup's step */
-#define QE_ATTN_JOIN 8     /* splits that the last workgroup of a decode call joins itself; more: a launch of its own */
-#define QE_ATTN_PART_WGS 1024 /* partial results a decode call can need (see qe_attn_decode_splits) */
+#define QE_ATTN_WGS 512    /* workgroups a prompt call is split up to: two for each of the 256 CUs */
+#define QE_ATTN_DECODE_WGS 2048 /* and a decode call at most */
+#define QE_ATTN_DECODE_SPLITS 1024
+#define QE_ATTN_JOIN 16    /* splits that the last workgroup of a decode call joins itself; more: a launch of its own */
 
-// Splits of every sequence's length in a decode call: as many as make QE_ATTN_WGS workgroups,
-// but no more than one per 128 positions (four waves' steps).  units = n_seqs * kv_heads;
-// with more than one split units < QE_ATTN_WGS and units * splits < QE_ATTN_WGS + units.
-QE_MIX_HD int qe_attn_decode_splits(int64_t units, int64_t max_len) {
-    const int64_t most = (max_len + 127) / 128, want = (QE_ATTN_WGS + units - 1) / units;
-    const int64_t s = want < most ? want : most;
-    return s < 1 ? 1 : (int)s;
+// A decode call gives a workgroup `steps` steps of QE_ATTN_TILE keys of one sequence and key-value
+// head, the same for all sequences, so that a ragged batch is even: `splits` workgroups are
+// launched for each, enough for max_len, and those behind a sequence's end do nothing.
+// One sequence: as many workgroups as the GPU holds at once, two or three a CU (LDS; one round of
+// 512 took 35 us over 100,000 keys of two heads of 256, 695 took 41), of at least two steps.
+// Several, which may differ in length: up to 2048, but of at least eight steps where that
+// many fill the GPU.  units = n_seqs * kv_heads.
+QE_MIX_HD void qe_attn_decode_plan(int64_t n_seqs, int64_t kv_heads, int head_dim, int64_t max_len, int *steps, int *splits) {
+    const int64_t tiles = (max_len + QE_ATTN_TILE - 1) / QE_ATTN_TILE, units = n_seqs * kv_heads, total = tiles * units;
+    const int64_t round = head_dim == 256 ? 512 : 768, once = (total + round - 1) / round;
+    int64_t per = once;
+    if (n_seqs > 1) {
+        per = (total + QE_ATTN_DECODE_WGS - 1) / QE_ATTN_DECODE_WGS;
+        if (per < 8) per = once < 8 ? once : 8;
+    }
+    if (per > tiles) per = tiles; // one workgroup for each
+    if (per < 2) per = 2;
+    if (per < (tiles + QE_ATTN_DECODE_SPLITS - 1) / QE_ATTN_DECODE_SPLITS) per = (tiles + QE_ATTN_DECODE_SPLITS - 1) / QE_ATTN_DECODE_SPLITS;
+    int64_t s = (tiles + per - 1) / per;
+    if (s < 1 || units >= QE_ATTN_DECODE_WGS) s = 1;
+    *steps = (int)per;
+    *splits = (int)s;
 }
+// Steps of a sequence of `len` keys in each of its workgroups (more than planned where the host's max_len was short
+// of it), and how many of those have any.
+QE_MIX_HD int qe_attn_decode_steps(int len, int steps, int splits) {
+    const int tiles = (len + QE_ATTN_TILE - 1) / QE_ATTN_TILE, need = (tiles + splits - 1) / splits;
+    return need > steps ? need : steps;
+}
+QE_MIX_HD int qe_attn_decode_active(int len, int steps) { return ((len + QE_ATTN_TILE - 1) / QE_ATTN_TILE + steps - 1) / steps; }
+// Partial results that a decode call can need: with more than one split units < QE_ATTN_DECODE_WGS, and
+// units * splits < QE_ATTN_DECODE_WGS + units.
+#define QE_ATTN_PART_WGS (2 * QE_ATTN_DECODE_WGS)
 
 // Query rows of a prompt call are its tokens times the heads that share a key-value head,
 // and a workgroup takes `bm` of one sequence.  Tile numbers are handed out so that the

@@ -12,7 +12,9 @@ from conftest import PKG
 SHIM = """
 #include "qe_mixer_plan.h"
 extern "C" {
-int decode_splits(long units, long len) { return qe_attn_decode_splits(units, len); }
+void decode_plan(long seqs, long heads, int dim, long len, int *steps, int *splits) { qe_attn_decode_plan(seqs, heads, dim, len, steps, splits); }
+int decode_steps(int len, int steps, int splits) { return qe_attn_decode_steps(len, steps, splits); }
+int decode_active(int len, int steps) { return qe_attn_decode_active(len, steps); }
 int prompt_splits(long tiles, long len) { return qe_attn_prompt_splits(tiles, len); }
 int first_tile(int cu, int i, int g, int bm) { return qe_attn_first_tile(cu, i, g, bm); }
 int max_tiles(int n, int s, int g, int bm) { return qe_attn_max_tiles(n, s, g, bm); }
@@ -23,6 +25,8 @@ int checked(int v, int lo, int hi, int other, unsigned *bad) { return qe_checked
 int slot_pair(long n, int a, int b) { return qe_slot_pair(n, a, b); }
 int slot_conflict(int i, int oi, int j, int ij, int oj) { return qe_slot_conflict(i, oi, j, ij, oj); }
 int wgs() { return QE_ATTN_WGS; }
+int decode_wgs() { return QE_ATTN_DECODE_WGS; }
+int decode_splits() { return QE_ATTN_DECODE_SPLITS; }
 int part_wgs() { return QE_ATTN_PART_WGS; }
 }
 """
@@ -35,19 +39,39 @@ def plan(tmp_path_factory):
     subprocess.run(["g++", "-shared", "-fPIC", "-std=c++17", "-Wall", "-Wno-unused-function", "-I", os.path.join(PKG, "csrc"),
                     str(d / "shim.cpp"), "-o", str(d / "shim.so")], check=True)
     lib = ctypes.CDLL(str(d / "shim.so"))
-    for f in ("decode_splits", "prompt_splits"):
-        getattr(lib, f).argtypes = [ctypes.c_long, ctypes.c_long]
+    lib.prompt_splits.argtypes = [ctypes.c_long, ctypes.c_long]
+    lib.decode_plan.argtypes = [ctypes.c_long, ctypes.c_long, ctypes.c_int, ctypes.c_long, ctypes.c_void_p, ctypes.c_void_p]
     lib.slot_pair.argtypes = [ctypes.c_long, ctypes.c_int, ctypes.c_int]
     return lib
 
 
+def decode_plan(plan, seqs, heads, dim, n):
+    steps, splits = ctypes.c_int(), ctypes.c_int()
+    plan.decode_plan(seqs, heads, dim, n, ctypes.byref(steps), ctypes.byref(splits))
+    return steps.value, splits.value
+
+
+def test_decode_workgroups_cover_every_length(plan):
+    """Whatever the host believed the longest to be: all steps of 32 keys are some launched workgroup's, once."""
+    for seqs, heads, dim in itertools.product((1, 2, 7, 24, 300, 65535), (1, 2, 8, 12, 256), (64, 256)):
+        for told in (1, 31, 700, 8111, 100000, (1 << 31) - 1):
+            steps, splits = decode_plan(plan, seqs, heads, dim, told)
+            for n in (0, 1, 32, 33, 64, 65, 700, 8111, 100000, (1 << 31) - 32):
+                tiles = -(-n // 32)
+                mine = plan.decode_steps(n, steps, splits)
+                active = plan.decode_active(n, mine)
+                assert mine >= steps and active <= splits and active * mine >= tiles and (active - 1) * mine < max(tiles, 1)
+                if n <= told:
+                    assert mine == steps
+
+
 def test_partial_results_fit_their_scratch(plan):
     lens = [0, 1, 127, 128, 129, 1000, 65536, (1 << 31) - 1]
-    for units in list(range(1, 1200)) + [65535 * 256]:
+    for seqs, heads, dim in itertools.product([*range(1, 300), 2047, 2048, 65535], (1, 2, 3, 8, 256), (64, 256)):
         for n in lens:
-            s = plan.decode_splits(units, n)
-            assert 1 <= s <= plan.wgs()
-            assert s == 1 or units * s <= plan.part_wgs()
+            steps, s = decode_plan(plan, seqs, heads, dim, n)
+            assert 1 <= s <= plan.decode_splits() and steps >= 2
+            assert s == 1 or (seqs * heads < plan.decode_wgs() and seqs * heads * s <= plan.part_wgs())
     for tiles in list(range(1, 1200)) + [1 << 28]:
         for n in lens:
             s = plan.prompt_splits(tiles, n)
