@@ -356,56 +356,60 @@ __global__ __launch_bounds__(256, 2) void k_attn_decode(const QeAttnArgs a) {
 }
 
 // ---------------------------------------------------------------------------
-// Many splits' results joined: o = sum 2^(m_s - m) o_s / sum 2^(m_s - m) l_s.  A workgroup for 64
-// elements of a row, 16 threads for them and 16 groups over the splits: 256 splits of 16 rows
-// of 256 are 4 MB, which 16 workgroups, one a row, took 27 us to read.
+// Many splits' results joined: o = sum 2^(m_s - m) o_s / sum 2^(m_s - m) l_s.  A workgroup of
+// 1024 threads for 64 elements of a row, 16 threads for them and 64 groups over the splits: a
+// read of a few hundred partial rows is latency, so all of it is in flight at once.  (256 splits of
+// 16 rows of 256, 4 MB: 27 us by a workgroup of 256 threads a row, 10 by four a row.)
 // ---------------------------------------------------------------------------
 template <bool BF, int DH>
-__global__ __launch_bounds__(256) void k_attn_join(const QeAttnArgs a) {
-    __shared__ float w_s[QE_ATTN_DECODE_SPLITS];
-    __shared__ float red[4], red2[4];
+__global__ __launch_bounds__(1024) void k_attn_join(const QeAttnArgs a) {
+    static_assert(QE_ATTN_DECODE_SPLITS <= 1024, "a thread looks at one split's maximum");
+    __shared__ float w_s[1024], red[16], red2[16];
     __shared__ __align__(16) qe_f4 o_s[256];
     const int tid = threadIdx.x, part = blockIdx.x % (DH / 64), head = blockIdx.x / (DH / 64) % a.q_heads, seq = blockIdx.x / (DH / 64) / a.q_heads;
     const int kvh = head / a.group, h = head % a.group;
     unsigned bad_len = 0;
-    const int len = qe_checked(a.kv_len[seq], 0, a.max_pages << a.page_log2, 0, &bad_len);
+    const int len = qe_checked(scalar_load(a.kv_len + seq), 0, a.max_pages << a.page_log2, 0, &bad_len);
     const int active = qe_attn_decode_active(len, qe_attn_decode_steps(len, a.steps, a.splits));
     if (active <= 1) return; // its one workgroup has written the row
     const size_t row0 = ((size_t)seq * a.kv_heads + kvh) * a.splits * a.group + h;
     const int d = part * 64 + tid % 16 * 4;
-    float2 x[QE_ATTN_DECODE_SPLITS / 256];
-    float m = -INFINITY;
-    int bad = 0;
+    const float2 x = tid < active ? a.part_ml[row0 + (size_t)tid * a.group] : make_float2(-INFINITY, 0.f);
+    qe_f4 o[4];
 #pragma unroll
-    for (int k = 0; k < QE_ATTN_DECODE_SPLITS / 256; ++k) {
-        const int s = tid + k * 256;
-        x[k] = s < active ? a.part_ml[row0 + (size_t)s * a.group] : make_float2(-INFINITY, 0.f);
-        bad |= x[k].y < 0.f;
-        m = fmaxf(m, x[k].x);
+    for (int k = 0; k < 4; ++k) { // the first 256 splits; behind the last the first again, unused
+        const int s = tid / 16 + 64 * k;
+        o[k] = *(const qe_f4 *)(a.part_o + (row0 + (size_t)(s < active ? s : 0) * a.group) * DH + d);
     }
+    float m = x.x;
     for (int k = 32; k; k >>= 1) m = fmaxf(m, __shfl_xor(m, k));
     if ((tid & 63) == 0) red[tid >> 6] = m;
-    bad = __syncthreads_or(bad);
-    m = fmaxf(fmaxf(red[0], red[1]), fmaxf(red[2], red[3]));
-    float sum = 0;
-#pragma unroll
-    for (int k = 0; k < QE_ATTN_DECODE_SPLITS / 256; ++k) {
-        const float f = x[k].y == 0.f || x[k].x == -INFINITY ? 0.f : exp2f((x[k].x - m) * a.scale_log2);
-        w_s[tid + k * 256] = x[k].y == 0.f ? -1.f : f; // -1: nothing of that split is used
-        sum += x[k].y == 0.f ? 0.f : f * x[k].y;
-    }
+    const int bad = __syncthreads_or(x.y < 0.f);
+    m = red[0];
+    for (int k = 1; k < 16; ++k) m = fmaxf(m, red[k]);
+    const float f = x.y == 0.f || x.x == -INFINITY ? 0.f : __builtin_amdgcn_exp2f((x.x - m) * a.scale_log2);
+    w_s[tid] = x.y == 0.f ? -1.f : f; // -1: nothing of that split is used
+    float sum = x.y == 0.f ? 0.f : f * x.y;
     for (int k = 32; k; k >>= 1) sum += __shfl_xor(sum, k);
     if ((tid & 63) == 0) red2[tid >> 6] = sum;
     __syncthreads();
-    sum = (red2[0] + red2[1]) + (red2[2] + red2[3]);
+    sum = 0;
+    for (int k = 0; k < 16; ++k) sum += red2[k];
     qe_f4 r = {0, 0, 0, 0};
-#pragma unroll 4
-    for (int s = tid / 16; s < active; s += 16) {
-        const float f = w_s[s];
-        const qe_f4 o = *(const qe_f4 *)(a.part_o + (row0 + (size_t)s * a.group) * DH + d);
-        if (f >= 0.f || f != f) r += f * o;
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+        const int s = tid / 16 + 64 * k;
+        const float w = s < active ? w_s[s] : -1.f;
+        if (w >= 0.f || w != w) r += w * o[k];
     }
-    o_s[tid] = r;
+    for (int s = tid / 16 + 256; s < active; s += 64) {
+        const float w = w_s[s];
+        const qe_f4 y = *(const qe_f4 *)(a.part_o + (row0 + (size_t)s * a.group) * DH + d);
+        if (w >= 0.f || w != w) r += w * y;
+    }
+    for (int k = 16; k < 64; k <<= 1) // the wave's four groups
+        for (int j = 0; j < 4; ++j) r[j] += __shfl_xor(r[j], k);
+    if ((tid & 63) < 16) o_s[(tid >> 6) * 16 + tid % 16] = r;
     __syncthreads();
     if (tid < 16) {
         for (int g = 1; g < 16; ++g) r += o_s[g * 16 + tid];
@@ -422,7 +426,7 @@ template <bool BF, int DH>
 static hipError_t launch_decode(const QeAttnArgs &a, hipStream_t st) {
     const unsigned units = (unsigned)(a.n_seqs * a.kv_heads), whole = a.splits > 1 && a.splits <= QE_ATTN_JOIN ? (units + 7) / 8 * 8 : units;
     k_attn_decode<BF, DH><<<dim3(whole * a.splits), dim3(256), 0, st>>>(a);
-    if (a.splits > QE_ATTN_JOIN) k_attn_join<BF, DH><<<dim3((unsigned)(a.n_seqs * a.q_heads * (DH / 64))), dim3(256), 0, st>>>(a);
+    if (a.splits > QE_ATTN_JOIN) k_attn_join<BF, DH><<<dim3((unsigned)(a.n_seqs * a.q_heads * (DH / 64))), dim3(1024), 0, st>>>(a);
     return hipGetLastError();
 }
 

@@ -86,6 +86,19 @@ __device__ __forceinline__ void mul_planes(const qe_s8 *a, const qe_s8 *b, qe_f4
 // ---------------------------------------------------------------------------
 // Which sequences of a call are computed (rules in qe_mixer_plan.h).
 // ---------------------------------------------------------------------------
+// Up to 256 sequences: by every workgroup of its own sequence, else by a launch before.
+__device__ __forceinline__ int slots_of(const QeDeltaArgs &a, int seq, int in_i, int out_i) { // what is wrong; workgroup-uniform
+    if (a.skip) return a.skip[seq];
+    int what = qe_slot_pair(a.n_slots, in_i, out_i);
+    if (a.n_seqs > 1) {
+        const int j = threadIdx.x;
+        if (__syncthreads_or(j < a.n_seqs ? qe_slot_conflict(seq, out_i, j, a.slots_in[j], a.slots_out[j]) : 0) && !what) what = QE_SLOT_SHARED;
+    }
+    return what;
+}
+__device__ __forceinline__ void report_slots(const QeDeltaArgs &a, int what) {
+    if (threadIdx.x == 0 && what && !a.skip) report(a.err, what == QE_SLOT_OUTSIDE ? QE_BAD_SLOT : QE_BAD_SHARED_SLOT);
+}
 __global__ __launch_bounds__(256) void k_delta_slots(const QeDeltaArgs a) {
     const int i = blockIdx.x;
     const int in_i = a.slots_in[i], out_i = a.slots_out[i];
@@ -117,18 +130,10 @@ __global__ __launch_bounds__(256) void k_delta_decode(const QeDeltaArgs a) {
     const int kh = head / a.group, col = slice * 32 + (tid & 7) * 4, row = tid >> 3;
     IN *out = (IN *)a.out + (size_t)seq * a.out_stride + (size_t)head * DV;
     const int in_i = a.slots_in[seq], out_i = a.slots_out[seq];
-    int what = qe_slot_pair(a.n_slots, in_i, out_i);
-    if (a.n_seqs > 1) {
-        int shared = 0;
-        if (a.skip) what = a.skip[seq];
-        else {
-            if (tid < a.n_seqs) shared = qe_slot_conflict(seq, out_i, tid, a.slots_in[tid], a.slots_out[tid]);
-            if (__syncthreads_or(shared) && !what) what = QE_SLOT_SHARED;
-        }
-    }
+    const int what = slots_of(a, seq, in_i, out_i);
+    report_slots(a, what);
     if (what) {
         if (tid < 32) out[slice * 32 + tid] = (IN)0.f;
-        if (tid == 0 && !a.skip) report(a.err, what == QE_SLOT_OUTSIDE ? QE_BAD_SLOT : QE_BAD_SHARED_SLOT);
         return;
     }
     qe_f4 s[ROWS];
@@ -226,7 +231,7 @@ __global__ __launch_bounds__(256) void k_delta_chunks(const QeDeltaArgs a) {
     unsigned bad = 0;
     const int begin = qe_checked(a.cu[seq], 0, a.n_tokens, 0, &bad), end = qe_checked(a.cu[seq + 1], begin, a.n_tokens, begin, &bad);
     const int64_t local = chunk - qe_delta_first_chunk(a.cu[seq], seq);
-    if (bad || a.skip[seq] || local < 0 || local * QE_DELTA_C >= end - begin) return; // uniform
+    if (bad || local < 0 || local * QE_DELTA_C >= end - begin) return; // uniform
     const int t0 = begin + (int)local * QE_DELTA_C, n = end - t0 < QE_DELTA_C ? end - t0 : QE_DELTA_C;
 
     const IN *q = (const IN *)a.q + (size_t)kh * DK + 8 * c, *k = (const IN *)a.k + (size_t)kh * DK + 8 * c;
@@ -403,11 +408,12 @@ __global__ __launch_bounds__(512) void k_delta_scan(const QeDeltaArgs a) {
     unsigned bad = 0;
     const int begin = qe_checked(a.cu[seq], 0, a.n_tokens, 0, &bad), end = qe_checked(a.cu[seq + 1], begin, a.n_tokens, begin, &bad);
     if (bad && tid == 0) report(a.err, QE_BAD_LENGTH);
-    if (bad | a.skip[seq]) {
+    const int in_i = a.slots_in[seq], out_i = a.slots_out[seq], what = slots_of(a, seq, in_i, out_i);
+    report_slots(a, what);
+    if (bad || what) {
         for (int t = begin + (tid >> 4); t < end; t += 32) ((IN *)a.out)[(size_t)t * a.out_stride + (size_t)head * DV + slice * 16 + (tid & 15)] = (IN)0.f;
         return;
     }
-    const int in_i = a.slots_in[seq], out_i = a.slots_out[seq];
     const int chunk0 = qe_delta_first_chunk(begin, seq), row = 16 * wave + r, kb = wave / 2; // kb: the last 32 columns that the wave's rows reach
     const short *ws = (const short *)(a.ws + ((size_t)chunk0 * a.v_heads + head) * QE_DELTA_WS);
     const size_t ws_step = (size_t)a.v_heads * QE_DELTA_WS * 2;
@@ -607,16 +613,17 @@ __global__ __launch_bounds__(512) void k_delta_scan(const QeDeltaArgs a) {
 }
 
 template <typename IN, int DK, int DV>
-static hipError_t prompt(const QeDeltaArgs &a, hipStream_t st) {
+static hipError_t prompt(QeDeltaArgs a, hipStream_t st) {
     const unsigned chunks = (unsigned)qe_delta_max_chunks(a.n_tokens, a.n_seqs);
-    k_delta_slots<<<dim3((unsigned)a.n_seqs), dim3(256), 0, st>>>(a);
+    if (a.n_seqs <= 256) a.skip = nullptr;
+    else k_delta_slots<<<dim3((unsigned)a.n_seqs), dim3(256), 0, st>>>(a);
     k_delta_chunks<IN, DK><<<dim3(chunks * a.k_heads), dim3(256), 0, st>>>(a);
     k_delta_scan<IN, DK, DV><<<dim3((unsigned)a.n_seqs * a.v_heads * (DV / 16)), dim3(512), 0, st>>>(a);
     return hipGetLastError();
 }
 template <typename IN, int DK, int DV>
 static hipError_t decode(QeDeltaArgs a, hipStream_t st) {
-    if (a.n_seqs <= 256) a.skip = nullptr; // every workgroup looks at all slots itself
+    if (a.n_seqs <= 256) a.skip = nullptr;
     else k_delta_slots<<<dim3((unsigned)a.n_seqs), dim3(256), 0, st>>>(a);
     k_delta_decode<IN, DK, DV><<<dim3((unsigned)a.n_seqs * a.v_heads * (DV / 32)), dim3(256), 0, st>>>(a);
     return hipGetLastError();
