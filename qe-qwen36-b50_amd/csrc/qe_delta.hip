@@ -217,8 +217,12 @@ __device__ __forceinline__ void load8_planes(const IN *p, bool there, qe_s8 *h, 
 template <typename IN, int DK>
 __global__ __launch_bounds__(256) void k_delta_chunks(const QeDeltaArgs a) {
     constexpr int LD = 68, KS = DK / 32, NP = planes_of<IN>(), NO = sizeof(IN) == 4 ? 3 : 2;
-    __shared__ __align__(16) float A[64 * LD], T[64 * LD], M[64 * LD];
-    __shared__ double b_s[64];
+    // K's planes as they are in k_delta_scan's LDS, then the heads' matrices
+    constexpr int K_BYTES = NP * 64 * DK * 2, M_BYTES = 3 * 64 * LD * 4;
+    __shared__ __align__(16) char lds[K_BYTES > M_BYTES ? K_BYTES : M_BYTES];
+    short *k_s = (short *)lds;
+    float *A = (float *)lds, *T = A + 64 * LD, *M = T + 64 * LD;
+    __shared__ double b_s[64]; // in powers of two, as the hardware's exponential takes them
     __shared__ float kk_s[64], rk_s[64], rq_s[64], beta_s[64];
     const int tid = threadIdx.x, wave = tid >> 6, lane = tid & 63, r = lane & 15, c = lane >> 4;
     const int chunk = blockIdx.x / a.k_heads, kh = blockIdx.x % a.k_heads;
@@ -229,8 +233,9 @@ __global__ __launch_bounds__(256) void k_delta_chunks(const QeDeltaArgs a) {
         else hi = mid;
     }
     unsigned bad = 0;
-    const int begin = qe_checked(a.cu[seq], 0, a.n_tokens, 0, &bad), end = qe_checked(a.cu[seq + 1], begin, a.n_tokens, begin, &bad);
-    const int64_t local = chunk - qe_delta_first_chunk(a.cu[seq], seq);
+    const int cu0 = scalar_load(a.cu + seq), cu1 = scalar_load(a.cu + seq + 1);
+    const int begin = qe_checked(cu0, 0, a.n_tokens, 0, &bad), end = qe_checked(cu1, begin, a.n_tokens, begin, &bad);
+    const int64_t local = chunk - qe_delta_first_chunk(cu0, seq);
     if (bad || local < 0 || local * QE_DELTA_C >= end - begin) return; // uniform
     const int t0 = begin + (int)local * QE_DELTA_C, n = end - t0 < QE_DELTA_C ? end - t0 : QE_DELTA_C;
 
@@ -244,10 +249,12 @@ __global__ __launch_bounds__(256) void k_delta_chunks(const QeDeltaArgs a) {
         for (int s = 0; s < KS; ++s) {
             load8_planes(k + (size_t)(t0 + row) * a.k_stride + 32 * s, row < n, kr[s], kk);
             load8_planes(q + (size_t)(t0 + row) * a.q_stride + 32 * s, row < n, qr[s], qq);
-            if constexpr (NP > 1) {
-                short *ws = a.ws_kq + ((size_t)chunk * a.k_heads + kh) * 2 * NP * 64 * DK;
-                for (int i = 0; i < NP; ++i) {
-                    *(qe_s8 *)(ws + (i * 64 + row) * DK + (((4 * s + c) ^ key_swz<DK>(row)) << 3)) = kr[s][i];
+            for (int i = 0; i < NP; ++i) {
+                const int at = (i * 64 + row) * DK + (((4 * s + c) ^ key_swz<DK>(row)) << 3);
+                *(qe_s8 *)(k_s + at) = kr[s][i];
+                if constexpr (NP > 1) {
+                    short *ws = a.ws_kq + ((size_t)chunk * a.k_heads + kh) * 2 * NP * 64 * DK;
+                    *(qe_s8 *)(ws + at) = kr[s][i];
                     *(qe_s8 *)(ws + NP * 64 * DK + ((wave * KS + s) * NP + i) * 512 + lane * 8) = qr[s][i];
                 }
             }
@@ -259,6 +266,7 @@ __global__ __launch_bounds__(256) void k_delta_chunks(const QeDeltaArgs a) {
             rk_s[row] = a.l2norm ? 1.f / sqrtf(kk + 1e-6f) : 1.f;
             rq_s[row] = (a.l2norm ? 1.f / sqrtf(qq + 1e-6f) : 1.f) * a.scale;
         }
+        __syncthreads();
 #pragma unroll
         for (int cb = 0; cb < 4; ++cb) {
             if (cb > wave) continue;
@@ -267,8 +275,7 @@ __global__ __launch_bounds__(256) void k_delta_chunks(const QeDeltaArgs a) {
 #pragma unroll
             for (int s = 0; s < KS; ++s) {
                 qe_s8 kb[NP];
-                float unused = 0;
-                load8_planes(k + (size_t)(t0 + col) * a.k_stride + 32 * s, col < n, kb, unused);
+                for (int i = 0; i < NP; ++i) kb[i] = *(const qe_s8 *)(k_s + (i * 64 + col) * DK + (((4 * s + c) ^ key_swz<DK>(col)) << 3));
                 mul_planes<NP, NP, 2>(kr[s], kb, k3);
                 mul_planes<NP, NP, 2>(qr[s], kb, q3);
             }
@@ -279,13 +286,13 @@ __global__ __launch_bounds__(256) void k_delta_chunks(const QeDeltaArgs a) {
     for (int gi = 0; gi < a.group; ++gi) {
         const int head = kh * a.group + gi;
         float *ws = a.ws + ((size_t)chunk * a.v_heads + head) * QE_DELTA_WS, *factors = ws + QE_DELTA_WS - 256;
-        double b = lane < n ? (double)log_decay(a.g[(size_t)(t0 + lane) * a.v_heads + head]) : 0.0;
+        double b = lane < n ? (double)log_decay(a.g[(size_t)(t0 + lane) * a.v_heads + head]) * 1.4426950408889634 : 0.0;
         for (int d = 1; d < 64; d <<= 1) {
             const double up = __shfl_up(b, d);
             if (lane >= d) b += up;
         }
         float beta = lane < n ? a.beta[(size_t)(t0 + lane) * a.v_heads + head] : 0.f;
-        __syncthreads(); // rk_s and rq_s are written, the last head's b_s, beta_s, T and M are read
+        __syncthreads(); // rk_s and rq_s are written, K is read; the last head's b_s, beta_s, T and M are read
         // A product of 0 and an infinity or NaN is NaN, and in a block above the diagonal's zeros it would
         // reach tokens before its own.  So from the first token whose key, gate or decay is not finite on
         // (what comes after it is not finite either) the matrices are zeros and the factors NaN.
@@ -299,11 +306,11 @@ __global__ __launch_bounds__(256) void k_delta_chunks(const QeDeltaArgs a) {
         }
         if (wave == 1) {
             const double last = __shfl(b, 63);
-            const float e = expf((float)b), none = lane < fine ? 0.f : NAN;
+            const float e = __builtin_amdgcn_exp2f((float)b), none = lane < fine ? 0.f : NAN;
             factors[lane] = e * rk_s[lane] + none;
             factors[64 + lane] = e * rq_s[lane] + none;
-            factors[128 + lane] = expf((float)(last - b)) * rk_s[lane] + (fine < 64 ? NAN : 0.f);
-            if (lane == 0) factors[192] = expf((float)last) + (fine < 64 ? NAN : 0.f);
+            factors[128 + lane] = __builtin_amdgcn_exp2f((float)(last - b)) * rk_s[lane] + (fine < 64 ? NAN : 0.f);
+            if (lane == 0) factors[192] = __builtin_amdgcn_exp2f((float)last) + (fine < 64 ? NAN : 0.f);
         }
         __syncthreads();
 #pragma unroll
@@ -312,7 +319,7 @@ __global__ __launch_bounds__(256) void k_delta_chunks(const QeDeltaArgs a) {
             for (int i = 0; i < 4; ++i) {
                 const int ri = 16 * wave + 4 * c + i, cj = 16 * cb + r;
                 const bool in = cb <= wave && cj <= ri && ri < fine;
-                const float fade = in ? expf((float)(b_s[ri] - b_s[cj])) * rk_s[cj] : 0.f;
+                const float fade = in ? __builtin_amdgcn_exp2f((float)(b_s[ri] - b_s[cj])) * rk_s[cj] : 0.f;
                 M[ri * LD + cj] = in ? gq[cb][i] * fade * rq_s[ri] : 0.f;
                 A[ri * LD + cj] = in && cj < ri ? gk[cb][i] * fade * (rk_s[ri] * beta_s[ri]) : 0.f;
                 if (cb > wave) T[ri * LD + cj] = 0.f;
