@@ -39,145 +39,151 @@ __device__ __forceinline__ int lane_now() {
 template <int WAVES>
 __device__ __forceinline__ int page_of(const QeAttnArgs &a, const int32_t *table, int k0, int len, int wave) {
     const int sub = k0 + wave * (BN / WAVES);
-    return *(const __attribute__((address_space(4))) int32_t *)(uintptr_t)(table + ((sub < len ? sub : len - 1) >> a.page_log2));
+    return scalar_load(table + ((sub < len ? sub : len - 1) >> a.page_log2));
 }
-// K and V of the part to LDS.
-template <int DH, int WAVES>
-__device__ __forceinline__ void load_tile(const QeAttnArgs &a, int page, int kvh, int k0, int len, int wave, short *k_lds,
-                                          short *v_lds, unsigned *bad) {
+// The part's rows of K or V to LDS.
+template <int DH, int WAVES, bool IS_K>
+__device__ __forceinline__ void load_part(const QeAttnArgs &a, int page, int kvh, int k0, int len, int wave, short *lds, unsigned *bad) {
     constexpr int CH = DH / 8, ROWS = 64 / CH, PART = BN / WAVES; // chunks of a row, rows of one direct load, rows of a wave
     const int sub = k0 + wave * PART, at = sub < len ? sub : (len - 1) & -PART;
-    unsigned p = (unsigned)page;
-    if (p >= a.n_pages) *bad = 1, p = 0;
-    const size_t r0 = (((size_t)p * a.kv_heads + kvh) << a.page_log2) + (at & ((1 << a.page_log2) - 1));
-    const char *kc = (const char *)a.kc + r0 * DH * 2, *vc = (const char *)a.vc + r0 * DH * 2;
+    const size_t r0 = page_row(a, page, kvh, at, bad);
+    const char *from = (const char *)(IS_K ? a.kc : a.vc) + r0 * DH * 2;
     // A uniform address and a 32-bit offset: a later row's permutation differs from the first load's by a constant.
     const int lane = lane_now(), row = lane / CH, c = lane % CH;
-    const unsigned k_off = row * DH * 2 + ((c ^ k_swz<DH>(row)) << 4), v_off = row * DH * 2 + ((c ^ v_swz<DH>(row)) << 4);
+    const unsigned off = row * DH * 2 + ((c ^ (IS_K ? k_swz<DH>(row) : v_swz<DH>(row))) << 4);
 #pragma unroll
-    for (int i = 0; i < PART / ROWS; ++i) {
-        load_lds16(kc + i * 1024 + (k_off ^ (k_swz<DH>(i * ROWS) << 4)), k_lds + (wave * PART + i * ROWS) * DH);
-        load_lds16(vc + i * 1024 + (v_off ^ (v_swz<DH>(i * ROWS) << 4)), v_lds + (wave * PART + i * ROWS) * DH);
-    }
+    for (int i = 0; i < PART / ROWS; ++i)
+        load_lds16(from + i * 1024 + (off ^ ((IS_K ? k_swz<DH>(i * ROWS) : v_swz<DH>(i * ROWS)) << 4)), lds + (wave * PART + i * ROWS) * DH);
 }
 
 __device__ __forceinline__ float max3(float a, float b, float c) { return fmaxf(fmaxf(a, b), c); }
+// the larger of the values of lanes l and l ^ 32
+__device__ __forceinline__ float max_halves(float x) {
+    const auto y = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+    return fmaxf(__uint_as_float(y[0]), __uint_as_float(y[1]));
+}
 
-// Order of a block's `n` operands of `reads` LDS reads and `products` matrix products each: `ahead` operands read first.
-template <int AHEAD, int N, int READS, int PRODUCTS>
+// The order of N matrix products that take READS LDS reads each: the reads of AHEAD of them first, then those of one for
+// each product.  Left alone, the scheduler reads, waits and multiplies in turn.
+template <int AHEAD, int N, int READS>
 __device__ __forceinline__ void schedule() {
     __builtin_amdgcn_sched_group_barrier(0x100, AHEAD * READS, 0);
 #pragma unroll
     for (int i = 0; i < N - AHEAD; ++i) {
-        __builtin_amdgcn_sched_group_barrier(0x008, PRODUCTS, 0);
+        __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
         __builtin_amdgcn_sched_group_barrier(0x100, READS, 0);
     }
-    __builtin_amdgcn_sched_group_barrier(0x008, AHEAD * PRODUCTS, 0);
+    __builtin_amdgcn_sched_group_barrier(0x008, AHEAD, 0);
 }
 
-// A wave's query rows, 32 NB of them: column r of block n is row 32 n + r.
-template <bool BF, int DH, int NB>
-struct Rows {
-    qe_f16v o[NB][DH / 32]; // O^T
-    qe_s8 q[NB][DH / 16];
-    float m[NB], l[NB]; // running maximum of the scores (scaled, in powers of two) and sum
-    int place[NB];      // position of the lane's query; below 0 where it attends to nothing
+// A wave's 32 query rows, lane r of either half row r, and their scores of KB blocks of 32 keys.
+template <int KB>
+struct Scores {
+    qe_f16v s[KB]; // S^T
 
-    __device__ __forceinline__ void step(const QeAttnArgs &a, const short *k_lds, const short *v_lds, int k0, bool masked) {
-        const int lane = lane_now(), r = lane & 31, h = lane >> 5;
-        // Byte addresses in LDS.  K: chunk 2 st + h of row r is permuted by the row's low bits, so the four st of a
-        // 128-byte block are one address with constants exclusive-or'ed in.  V: so are the 64-byte units d of the
-        // row that a lane addresses in a transposing read.
-        const int tr = (lane & 15) >> 2, el = ((lane >> 4) & 1) * 16 + (lane & 3) * 4;
-        const unsigned ka = r * DH * 2 + ((h ^ k_swz<DH>(r)) << 4);
-        const unsigned va = (4 * h + tr) * DH * 2 + (((el >> 3) ^ v_swz<DH>(tr)) << 4) + (el & 7) * 2;
-        // Key blocks of 32 whose scores are held together: two, or one where o and q leave no registers for more.
-        constexpr int KB = DH == 256 ? 1 : 2;
+    // keys behind `limit`, counted from the lane's first, are not attended to
+    __device__ __forceinline__ void mask(int limit) {
 #pragma unroll
-        for (int b0 = 0; b0 < 2; b0 += KB) {
-            qe_f16v s[NB][KB];
+        for (int b = 0; b < KB; ++b)
 #pragma unroll
-            for (int b = 0; b < KB; ++b) {
+            for (int i = 0; i < 16; ++i)
+                if (b * 32 + 8 * (i / 4) + i % 4 > limit) s[b][i] = -INFINITY;
+    }
+    __device__ __forceinline__ float top() const { // of the row
+        float t = s[0][0];
 #pragma unroll
-                for (int n = 0; n < NB; ++n)
+        for (int i = 1; i < 15; i += 2) t = max3(t, s[0][i], s[0][i + 1]);
+        t = max3(t, s[0][15], s[KB - 1][0]);
+        if constexpr (KB == 2) {
 #pragma unroll
-                    for (int i = 0; i < 16; ++i) s[n][b][i] = 0;
-#pragma unroll
-                for (int st = 0; st < DH / 16; ++st) {
-                    const qe_s8 kf = *(const qe_s8 *)((const char *)k_lds + ((ka ^ (st & 3) << 5) + (b0 + b) * 64 * DH + (st >> 2) * 128));
-#pragma unroll
-                    for (int n = 0; n < NB; ++n) s[n][b] = mfma32<BF>(kf, q[n][st], s[n][b]);
-                }
-            }
-            // The matrix products take the LDS reads as they come: four in flight (and in the second product three pairs),
-            // then one more for each product.  Left alone, the scheduler reads, waits and multiplies in turn.
-            schedule<4, KB * DH / 16, 1, NB>();
-            union {
-                unsigned u[4];
-                qe_s8 v;
-            } p[NB][KB][2];
-#pragma unroll
-            for (int n = 0; n < NB; ++n) {
-                if (masked) {
-                    const int limit = place[n] - k0 - 4 * h - b0 * 32; // the last key that the row attends to, counted from the lane's first
-#pragma unroll
-                    for (int b = 0; b < KB; ++b)
-#pragma unroll
-                        for (int i = 0; i < 16; ++i)
-                            if (b * 32 + 8 * (i / 4) + i % 4 > limit) s[n][b][i] = -INFINITY;
-                }
-                float top = s[n][0][0];
-#pragma unroll
-                for (int i = 1; i < 15; i += 2) top = max3(top, s[n][0][i], s[n][0][i + 1]);
-                top = max3(top, s[n][0][15], s[n][KB - 1][0]);
-                if constexpr (KB == 2) {
-#pragma unroll
-                    for (int i = 1; i < 15; i += 2) top = max3(top, s[n][1][i], s[n][1][i + 1]);
-                    top = fmaxf(top, s[n][1][15]);
-                }
-                top = fmaxf(top, __shfl_xor(top, 32)) * a.scale_log2;
-                // The maximum that is subtracted only has to keep the powers of two in range: it follows the true one
-                // when that has grown by more than 2^8, which after the first keys is rare.
-                if (__any(top > m[n] + 8.f)) {
-                    const float mn = fmaxf(m[n], top), f = m[n] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m[n] - mn);
-#pragma unroll
-                    for (int d = 0; d < DH / 32; ++d) o[n][d] *= f;
-                    l[n] *= f;
-                    m[n] = mn;
-                }
-                const float base = m[n] == -INFINITY ? 0.f : -m[n];
-                float sum = 0;
-#pragma unroll
-                for (int b = 0; b < KB; ++b)
-#pragma unroll
-                    for (int i = 0; i < 16; i += 2) {
-                        const float x = __builtin_amdgcn_exp2f(fmaf(s[n][b][i], a.scale_log2, base));
-                        const float y = __builtin_amdgcn_exp2f(fmaf(s[n][b][i + 1], a.scale_log2, base));
-                        sum += x + y;
-                        p[n][b][i / 8].u[i % 8 / 2] = pack2<BF>(x, y);
-                    }
-                l[n] += sum;
-            }
-#pragma unroll
-            for (int b = 0; b < KB; ++b)
-#pragma unroll
-                for (int ks = 0; ks < 2; ++ks)
-#pragma unroll
-                    for (int d = 0; d < DH / 32; ++d) {
-                        const unsigned vp = (va ^ (d & 3) << 6) + ((b0 + b) * 2 + ks) * 32 * DH + (d >> 2) * 256;
-                        const qe_s4 x = lds_tr((const short *)((const char *)v_lds + vp)), y = lds_tr((const short *)((const char *)v_lds + (vp + 16 * DH))); // 8 rows on the permutation is the same
-                        const qe_s8 vf = {x[0], x[1], x[2], x[3], y[0], y[1], y[2], y[3]};
-#pragma unroll
-                        for (int n = 0; n < NB; ++n) o[n][d] = mfma32<BF>(vf, p[n][b][ks].v, o[n][d]);
-                    }
-            schedule<3, KB * 2 * DH / 32, 2, NB>();
+            for (int i = 1; i < 15; i += 2) t = max3(t, s[1][i], s[1][i + 1]);
+            t = fmaxf(t, s[1][15]);
         }
+        return max_halves(t);
+    }
+};
+template <int KB>
+struct Probs {
+    union {
+        unsigned u[4];
+        qe_s8 v;
+    } p[KB][2]; // 16 keys each, as the second product's operand
+};
+
+template <bool BF, int DH>
+struct Rows {
+    qe_f16v o[DH / 32]; // O^T
+    qe_s8 q[DH / 16];
+    float m, l; // running maximum of the scores (scaled, in powers of two) and sum
+    int place;  // position of the lane's query; below 0 where it attends to nothing
+
+    // S^T = K Q^T of KB blocks from block b0 of the tile on.  Chunk 2 st + h of K's row r is permuted by the row's low
+    // bits, so the four st of a 128-byte block are one address with constants exclusive-or'ed in.
+    template <int KB>
+    __device__ __forceinline__ void scores(const short *k_lds, int b0, Scores<KB> &x) const {
+        const int lane = lane_now(), r = lane & 31, h = lane >> 5;
+        const unsigned ka = r * DH * 2 + ((h ^ k_swz<DH>(r)) << 4);
+#pragma unroll
+        for (int b = 0; b < KB; ++b) {
+#pragma unroll
+            for (int i = 0; i < 16; ++i) x.s[b][i] = 0;
+#pragma unroll
+            for (int st = 0; st < DH / 16; ++st)
+                x.s[b] = mfma32<BF>(*(const qe_s8 *)((const char *)k_lds + ((ka ^ (st & 3) << 5) + (b0 + b) * 64 * DH + (st >> 2) * 128)), q[st], x.s[b]);
+        }
+    }
+    // The maximum that is subtracted only has to keep the powers of two in range: it follows the true one
+    // when that has grown by more than 2^8, which after the first keys is rare.
+    __device__ __forceinline__ void raise(float top) {
+        if (__any(top > m + 8.f)) {
+            const float mn = fmaxf(m, top), f = m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m - mn);
+#pragma unroll
+            for (int d = 0; d < DH / 32; ++d) o[d] *= f;
+            l *= f;
+            m = mn;
+        }
+    }
+    template <int KB>
+    __device__ __forceinline__ void exponentials(float scale, const Scores<KB> &x, Probs<KB> &p) {
+        const float base = m == -INFINITY ? 0.f : -m;
+        float sum[2] = {0, 0};
+#pragma unroll
+        for (int b = 0; b < KB; ++b)
+#pragma unroll
+            for (int i = 0; i < 16; i += 2) {
+                const float y = __builtin_amdgcn_exp2f(fmaf(x.s[b][i], scale, base));
+                const float z = __builtin_amdgcn_exp2f(fmaf(x.s[b][i + 1], scale, base));
+                sum[0] += y;
+                sum[1] += z;
+                p.p[b][i / 8].u[i % 8 / 2] = pack2<BF>(y, z);
+            }
+        l += sum[0] + sum[1];
+    }
+    // O^T += V^T P^T.  The 64-byte units d of the row that a lane addresses in a transposing read are one address with
+    // constants, too.
+    template <int KB>
+    __device__ __forceinline__ void values(const short *v_lds, int b0, const Probs<KB> &p) {
+        const int lane = lane_now(), h = lane >> 5, tr = (lane & 15) >> 2, el = ((lane >> 4) & 1) * 16 + (lane & 3) * 4;
+        const unsigned va = (4 * h + tr) * DH * 2 + (((el >> 3) ^ v_swz<DH>(tr)) << 4) + (el & 7) * 2;
+#pragma unroll
+        for (int ks = 0; ks < 2 * KB; ++ks)
+#pragma unroll
+            for (int d = 0; d < DH / 32; ++d) {
+                const unsigned vp = (va ^ (d & 3) << 6) + (b0 * 2 + ks) * 32 * DH + (d >> 2) * 256;
+                const qe_s4 x = lds_tr((const short *)((const char *)v_lds + vp)), y = lds_tr((const short *)((const char *)v_lds + (vp + 16 * DH))); // 8 rows on the permutation is the same
+                o[d] = mfma32<BF>(qe_s8{x[0], x[1], x[2], x[3], y[0], y[1], y[2], y[3]}, p.p[ks / 2][ks % 2].v, o[d]);
+            }
     }
 };
 
-template <bool BF, int DH, int WAVES, int NB>
-__global__ __launch_bounds__(64 * WAVES, NB == 2 && DH == 256 ? 1 : 2) void k_attn_prompt(const QeAttnArgs a) {
-    constexpr int BM = 32 * WAVES * NB, THREADS = 64 * WAVES;
+// Four waves with heads of up to 128, and two or more workgroups on a CU.  With heads of 256 the tiles fill a CU's LDS, so
+// eight waves (unless the call is too small to need them) are the way to two waves a SIMD, and o and q leave
+// registers for 32 keys' scores at a time, not 64.  (Measured and not kept: the next tile's scores made among this
+// one's exponentials, 10 % slower over 4096 tokens of heads of 64 and 128; the second four waves half a tile behind the
+// first, 8 % slower over 8192 of 256; 64 rows a wave, whose 512 registers do not hold them.)
+template <bool BF, int DH, int WAVES>
+__global__ __launch_bounds__(64 * WAVES, 2) void k_attn_prompt(const QeAttnArgs a) {
+    constexpr int BM = 32 * WAVES, PART = BN / WAVES;
     // two buffers, variables of their own: else the compiler has every LDS read wait for the direct loads in flight
     __shared__ __align__(16) short k_a[BN * DH], v_a[BN * DH], k_b[BN * DH], v_b[BN * DH];
     // rows with an infinity or a NaN in V, of the tiles that some rows attend to in part: from `clear` on, BM tokens at most
@@ -188,63 +194,68 @@ __global__ __launch_bounds__(64 * WAVES, NB == 2 && DH == 256 ? 1 : 2) void k_at
     int seq = 0;
     for (int hi = a.n_seqs; hi - seq > 1;) { // the last sequence whose first tile is not behind this one
         const int mid = (seq + hi) >> 1;
-        if (qe_attn_first_tile(a.cu[mid], mid, a.group, BM) <= tile) seq = mid;
+        if (qe_attn_first_tile(scalar_load(a.cu + mid), mid, a.group, BM) <= tile) seq = mid;
         else hi = mid;
     }
-    const int local = tile - qe_attn_first_tile(a.cu[seq], seq, a.group, BM);
+    const int cu0 = scalar_load(a.cu + seq), cu1 = scalar_load(a.cu + seq + 1), kv = scalar_load(a.kv_len + seq);
+    const int local = tile - qe_attn_first_tile(cu0, seq, a.group, BM);
     unsigned bad_len = 0, bad = 0;
-    const int begin = qe_checked(a.cu[seq], 0, a.n_tokens, 0, &bad_len);
-    const int end = qe_checked(a.cu[seq + 1], begin, a.n_tokens, begin, &bad_len);
-    const int len = qe_checked(a.kv_len[seq], 0, a.max_pages << a.page_log2, 0, &bad_len);
+    const int begin = qe_checked(cu0, 0, a.n_tokens, 0, &bad_len);
+    const int end = qe_checked(cu1, begin, a.n_tokens, begin, &bad_len);
+    const int len = qe_checked(kv, 0, a.max_pages << a.page_log2, 0, &bad_len);
     if (bad_len && tid == 0) report(a.err, QE_BAD_LENGTH);
     const int n_rows = (end - begin) * a.group;
     if (local < 0 || (int64_t)local * BM >= n_rows) return; // uniform: no row of the sequence
     const int row0 = local * BM, first = len - (end - begin); // first: position of the sequence's first row
     const int32_t *table = a.table + (size_t)seq * a.table_stride;
 
-    Rows<BF, DH, NB> w;
-    const int wave_row = row0 + wave * 32 * NB;
-#pragma unroll
-    for (int n = 0; n < NB; ++n) {
-        const int row = wave_row + n * 32 + (tid & 31), h = tid >> 5 & 1;
-        const bool there = row < n_rows;
-        const int tok = there ? row / a.group : 0, head = kvh * a.group + (there ? row - tok * a.group : 0);
-        w.place[n] = there ? first + tok : -1;
-        const short *q = (const short *)a.q + (size_t)(begin + tok) * a.q_stride + (size_t)head * DH + h * 8;
-#pragma unroll
-        for (int s = 0; s < DH / 16; ++s) w.q[n][s] = there ? *(const qe_s8 *)(q + s * 16) : qe_s8{};
-        w.m[n] = -INFINITY;
-        w.l[n] = 0;
-#pragma unroll
-        for (int d = 0; d < DH / 32; ++d)
-#pragma unroll
-            for (int i = 0; i < 16; ++i) w.o[n][d][i] = 0;
-    }
     // keys of the tile: up to its last row's place; below `clear` every row attends to every key
     const int last_tok = (row0 + BM < n_rows ? row0 + BM - 1 : n_rows - 1) / a.group;
     const int keys = first + last_tok + 1, clear = first + row0 / a.group + 1 > 0 ? first + row0 / a.group + 1 : 0;
     // the same for the wave
-    const int wave_end = wave_row + 32 * NB < n_rows ? wave_row + 32 * NB : n_rows;
+    const int wave_row = row0 + wave * 32, wave_end = wave_row + 32 < n_rows ? wave_row + 32 : n_rows;
     const int wave_keys = wave_row < n_rows ? first + (wave_end - 1) / a.group + 1 : 0, wave_clear = first + wave_row / a.group + 1;
     int lo, hi;
     qe_split_range(keys > 0 ? (keys + BN - 1) / BN : 0, a.splits, split, &lo, &hi);
 
     int page = 0; // of the wave's part of the next tile
-    auto work = [&](const short *k_lds, short *v_lds, short *k_next, short *v_next, int t) {
-        __builtin_amdgcn_s_waitcnt(0x0f70); // this wave's direct loads have landed,
-        lds_barrier();                      // the others' too, and no wave reads the other buffers any more
+    if (lo < hi) {
+        page = page_of<WAVES>(a, table, lo * BN, len, wave);
+        load_part<DH, WAVES, true>(a, page, kvh, lo * BN, len, wave, k_a, &bad);
+        load_part<DH, WAVES, false>(a, page, kvh, lo * BN, len, wave, v_a, &bad);
+        page = page_of<WAVES>(a, table, (lo + 1) * BN, len, wave);
+    }
+    Rows<BF, DH> w;
+    {
+        const int row = wave_row + (tid & 31), h = tid >> 5 & 1;
+        const bool there = row < n_rows;
+        const int tok = there ? row / a.group : 0, head = kvh * a.group + (there ? row - tok * a.group : 0);
+        w.place = there ? first + tok : -1;
+        const short *q = (const short *)a.q + (size_t)(begin + tok) * a.q_stride + (size_t)head * DH + h * 8;
+#pragma unroll
+        for (int s = 0; s < DH / 16; ++s) w.q[s] = there ? *(const qe_s8 *)(q + s * 16) : qe_s8{};
+        w.m = -INFINITY;
+        w.l = 0;
+#pragma unroll
+        for (int d = 0; d < DH / 32; ++d)
+#pragma unroll
+            for (int i = 0; i < 16; ++i) w.o[d][i] = 0;
+    }
+    if (tid < BM / BN + 2) odd_rows[tid] = 0; // a barrier before the first tile's
+
+    // The wave's direct loads have landed.  A probability of 0 times an infinity or NaN is NaN: in its part of V's tile t rows
+    // behind the end become zeros, and so do elements that are not finite, which are added in the end for the rows
+    // that attend to them.
+    auto arrived = [&](int t, short *v_lds) {
+        __builtin_amdgcn_s_waitcnt(0x0f70);
         const int k0 = t * BN;
-        if (t + 1 < hi) load_tile<DH, WAVES>(a, page, kvh, k0 + BN, len, wave, k_next, v_next, &bad);
-        page = page_of<WAVES>(a, table, k0 + 2 * BN, len, wave); // looked up a step before it is needed
-        const bool masked = k0 + BN > clear;
-        if (masked) {
-            // A probability of 0 times an infinity or NaN is NaN: rows behind the end become zeros, and
-            // so do elements that are not finite, which are added in the end for the rows that attend to them.
-            for (int i = wave * 64 + lane_now(); i < BN * (DH / 8); i += THREADS) {
-                const int row = i / (DH / 8);
-                qe_s8 x = *(const qe_s8 *)(v_lds + i * 8);
+        if (k0 + BN > clear)
+            for (int i = lane_now(); i < PART * (DH / 8); i += 64) {
+                const int row = wave * PART + i / (DH / 8);
+                short *at = v_lds + wave * PART * DH + i * 8;
+                qe_s8 x = *(const qe_s8 *)at;
                 if (k0 + row >= len) {
-                    *(qe_s8 *)(v_lds + i * 8) = qe_s8{};
+                    *(qe_s8 *)at = qe_s8{};
                 } else {
                     constexpr int top = BF ? 0x7f80 : 0x7c00;
                     bool odd = false;
@@ -252,23 +263,39 @@ __global__ __launch_bounds__(64 * WAVES, NB == 2 && DH == 256 ? 1 : 2) void k_at
                     for (int j = 0; j < 8; ++j)
                         if ((x[j] & top) == top) x[j] = 0, odd = true;
                     if (odd) {
-                        *(qe_s8 *)(v_lds + i * 8) = x;
+                        *(qe_s8 *)at = x;
                         atomicOr(&odd_rows[t - clear / BN], 1ull << row);
                     }
                 }
             }
-            lds_barrier();
-        }
-        if (k0 < wave_keys) w.step(a, k_lds, v_lds, k0, k0 + BN > wave_clear);
     };
-    if (tid < BM / BN + 2) odd_rows[tid] = 0; // a barrier before the first tile's
-    if (lo < hi) {
-        load_tile<DH, WAVES>(a, page_of<WAVES>(a, table, lo * BN, len, wave), kvh, lo * BN, len, wave, k_a, v_a, &bad);
-        page = page_of<WAVES>(a, table, (lo + 1) * BN, len, wave);
-    }
+    auto work = [&](int t, const short *k_lds, short *v_lds, short *k_next, short *v_next) {
+        arrived(t, v_lds);
+        lds_barrier(); // the others' loads, too, and no wave reads the other buffers any more
+        const int k0 = t * BN;
+        if (t + 1 < hi) {
+            load_part<DH, WAVES, true>(a, page, kvh, k0 + BN, len, wave, k_next, &bad);
+            load_part<DH, WAVES, false>(a, page, kvh, k0 + BN, len, wave, v_next, &bad);
+        }
+        page = page_of<WAVES>(a, table, k0 + 2 * BN, len, wave); // looked up a step before it is needed
+        if (k0 >= wave_keys) return;
+        constexpr int KB = DH == 256 ? 1 : 2;
+#pragma unroll
+        for (int b = 0; b < 2; b += KB) {
+            Scores<KB> s;
+            w.scores(k_lds, b, s);
+            schedule<4, KB * DH / 16, 1>();
+            if (k0 + BN > wave_clear) s.mask(w.place - k0 - b * 32 - 4 * (lane_now() >> 5));
+            w.raise(s.top() * a.scale_log2);
+            Probs<KB> p;
+            w.exponentials(a.scale_log2, s, p);
+            w.values(v_lds, b, p);
+            schedule<3, KB * DH / 16, 2>();
+        }
+    };
     for (int t = lo; t < hi; t += 2) {
-        work(k_a, v_a, k_b, v_b, t);
-        if (t + 1 < hi) work(k_b, v_b, k_a, v_a, t + 1);
+        work(t, k_a, v_a, k_b, v_b);
+        if (t + 1 < hi) work(t + 1, k_b, v_b, k_a, v_a);
     }
     if (bad && (tid & 63) == 0) report(a.err, QE_BAD_PAGE);
     const bool void_rows = __syncthreads_or(bad);
@@ -278,54 +305,48 @@ __global__ __launch_bounds__(64 * WAVES, NB == 2 && DH == 256 ? 1 : 2) void k_at
         while (odd) { // uniform, and empty but for values that are not finite
             const int key = t * BN + __ffsll(odd) - 1;
             odd &= odd - 1;
-            const size_t at = sub_row(a, table, kvh, key & ~15, &bad) + (key & 15);
+            const size_t at = sub_row(a, table, kvh, __builtin_amdgcn_readfirstlane(key) & ~15, &bad) + (key & 15);
             const short *v = (const short *)a.vc + at * DH + 4 * h;
-#pragma unroll
-            for (int n = 0; n < NB; ++n)
-                if (key <= w.place[n])
-#pragma unroll
-                    for (int d = 0; d < DH / 32; ++d)
-#pragma unroll
-                        for (int i = 0; i < 16; i += 4) {
-                            const qe_s4 x = *(const qe_s4 *)(v + d * 32 + 2 * i);
-#pragma unroll
-                            for (int j = 0; j < 4; ++j) {
-                                const float y = from16<BF>(x[j]);
-                                if (!__builtin_isfinite(y)) w.o[n][d][i + j] += y;
-                            }
-                            asm volatile("" ::: "memory"); // not all of the row in registers at once
-                        }
-        }
-    }
-#pragma unroll
-    for (int n = 0; n < NB; ++n) {
-        const float l = w.l[n] + __shfl_xor(w.l[n], 32);
-        const int row = wave_row + n * 32 + r;
-        if (a.splits == 1) {
-            if (row < n_rows) {
-                const int tok = row / a.group, head = kvh * a.group + row - tok * a.group;
-                const float inv = l == 0.f ? 0.f : 1.f / l;
-                short *out = (short *)a.out + (size_t)(begin + tok) * a.out_stride + (size_t)head * DH;
+            if (key <= w.place)
 #pragma unroll
                 for (int d = 0; d < DH / 32; ++d)
 #pragma unroll
                     for (int i = 0; i < 16; i += 4) {
-                        uint2 x;
-                        x.x = pack2<BF>(w.o[n][d][i] * inv, w.o[n][d][i + 1] * inv);
-                        x.y = pack2<BF>(w.o[n][d][i + 2] * inv, w.o[n][d][i + 3] * inv);
-                        if (void_rows) x = make_uint2(0, 0);
-                        *(uint2 *)(out + d * 32 + 2 * i + 4 * h) = x;
+                        const qe_s4 x = *(const qe_s4 *)(v + d * 32 + 2 * i);
+#pragma unroll
+                        for (int j = 0; j < 4; ++j) {
+                            const float y = from16<BF>(x[j]);
+                            if (!__builtin_isfinite(y)) w.o[d][i + j] += y;
+                        }
+                        asm volatile("" ::: "memory"); // not all of the row in registers at once
                     }
-            }
-        } else {
-            const size_t at = (((size_t)tile * a.kv_heads + kvh) * a.splits + split) * BM + row - row0;
-#pragma unroll
-            for (int d = 0; d < DH / 32; ++d)
-#pragma unroll
-                for (int i = 0; i < 16; i += 4)
-                    *(qe_f4 *)(a.part_o + at * DH + d * 32 + 2 * i + 4 * h) = qe_f4{w.o[n][d][i], w.o[n][d][i + 1], w.o[n][d][i + 2], w.o[n][d][i + 3]};
-            if (h == 0) a.part_ml[at] = make_float2(w.m[n], void_rows ? -1.f : l);
         }
+    }
+    const float l = w.l + __shfl_xor(w.l, 32);
+    const int row = wave_row + r;
+    if (a.splits == 1) {
+        if (row >= n_rows) return;
+        const int tok = row / a.group, head = kvh * a.group + row - tok * a.group;
+        const float inv = l == 0.f ? 0.f : 1.f / l;
+        short *out = (short *)a.out + (size_t)(begin + tok) * a.out_stride + (size_t)head * DH;
+#pragma unroll
+        for (int d = 0; d < DH / 32; ++d)
+#pragma unroll
+            for (int i = 0; i < 16; i += 4) {
+                uint2 x;
+                x.x = pack2<BF>(w.o[d][i] * inv, w.o[d][i + 1] * inv);
+                x.y = pack2<BF>(w.o[d][i + 2] * inv, w.o[d][i + 3] * inv);
+                if (void_rows) x = make_uint2(0, 0);
+                *(uint2 *)(out + d * 32 + 2 * i + 4 * h) = x;
+            }
+    } else {
+        const size_t at = (((size_t)tile * a.kv_heads + kvh) * a.splits + split) * BM + row - row0;
+#pragma unroll
+        for (int d = 0; d < DH / 32; ++d)
+#pragma unroll
+            for (int i = 0; i < 16; i += 4)
+                *(qe_f4 *)(a.part_o + at * DH + d * 32 + 2 * i + 4 * h) = qe_f4{w.o[d][i], w.o[d][i + 1], w.o[d][i + 2], w.o[d][i + 3]};
+        if (h == 0) a.part_ml[at] = make_float2(w.m, void_rows ? -1.f : l);
     }
 }
 
@@ -369,18 +390,18 @@ __global__ __launch_bounds__(256) void k_attn_prompt_join(const QeAttnArgs a) {
     for (int e = 0; e < E; ++e) out[e * 64 + lane] = (short)pack2<BF>(none ? 0.f : o[e] * inv, 0.f);
 }
 
-template <bool BF, int DH, int WAVES, int NB>
+template <bool BF, int DH, int WAVES>
 static hipError_t launch_waves(const QeAttnArgs &a, hipStream_t st) {
-    k_attn_prompt<BF, DH, WAVES, NB><<<dim3((unsigned)(a.tiles * a.kv_heads * a.splits)), dim3(64 * WAVES), 0, st>>>(a);
+    k_attn_prompt<BF, DH, WAVES><<<dim3((unsigned)(a.tiles * a.kv_heads * a.splits)), dim3(64 * WAVES), 0, st>>>(a);
     if (a.splits > 1)
-        k_attn_prompt_join<BF, DH, 32 * WAVES * NB><<<dim3((unsigned)(a.tiles * a.kv_heads * (8 * WAVES * NB))), dim3(256), 0, st>>>(a);
+        k_attn_prompt_join<BF, DH, 32 * WAVES><<<dim3((unsigned)(a.tiles * a.kv_heads * (8 * WAVES))), dim3(256), 0, st>>>(a);
     return hipGetLastError();
 }
 template <bool BF, int DH>
 static hipError_t launch_prompt(const QeAttnArgs &a, int bm, hipStream_t st) {
     if constexpr (DH == 256)
-        if (bm == 256) return launch_waves<BF, DH, 8, 1>(a, st);
-    return launch_waves<BF, DH, 4, 1>(a, st);
+        if (bm == 256) return launch_waves<BF, DH, 8>(a, st);
+    return launch_waves<BF, DH, 4>(a, st);
 }
 
 hipError_t qe_launch_attn_prompt(const QeAttnArgs &a, int head_dim, int type, int bm, hipStream_t st) {
