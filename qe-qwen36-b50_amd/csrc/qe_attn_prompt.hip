@@ -350,39 +350,57 @@ __global__ __launch_bounds__(64 * WAVES, 2) void k_attn_prompt(const QeAttnArgs 
     }
 }
 
-// The splits' results joined, a wave per query row.
-template <bool BF, int DH, int BM>
+// The splits' results joined, W waves per query row: one up to 8 splits, and a workgroup's four over every fourth split
+// beyond (240 rows of 256 over 40 splits: 65 us the call with one wave a row, 41 with four; 16000 rows over 2: 54 and 66).
+template <bool BF, int DH, int BM, int W>
 __global__ __launch_bounds__(256) void k_attn_prompt_join(const QeAttnArgs a) {
     constexpr int E = DH / 64;
-    const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
-    const int in_tile = blockIdx.x % (BM / 4) * 4 + wave, tile = blockIdx.x / (BM / 4) / a.kv_heads, kvh = blockIdx.x / (BM / 4) % a.kv_heads;
-    int lo = 0, hi = a.n_seqs;
-    while (hi - lo > 1) {
-        const int mid = (lo + hi) >> 1;
-        if (qe_attn_first_tile(a.cu[mid], mid, a.group, BM) <= tile) lo = mid;
+    const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, item = blockIdx.x / (BM * W / 4);
+    const int in_tile = blockIdx.x % (BM * W / 4) * (4 / W) + wave / W, tile = item / a.kv_heads, kvh = item % a.kv_heads;
+    int seq = 0;
+    for (int hi = a.n_seqs; hi - seq > 1;) {
+        const int mid = (seq + hi) >> 1;
+        if (qe_attn_first_tile(scalar_load(a.cu + mid), mid, a.group, BM) <= tile) seq = mid;
         else hi = mid;
     }
     unsigned bad = 0;
-    const int begin = qe_checked(a.cu[lo], 0, a.n_tokens, 0, &bad), end = qe_checked(a.cu[lo + 1], begin, a.n_tokens, begin, &bad);
-    const int local = tile - qe_attn_first_tile(a.cu[lo], lo, a.group, BM);
+    const int cu0 = scalar_load(a.cu + seq), cu1 = scalar_load(a.cu + seq + 1);
+    const int begin = qe_checked(cu0, 0, a.n_tokens, 0, &bad), end = qe_checked(cu1, begin, a.n_tokens, begin, &bad);
+    const int local = tile - qe_attn_first_tile(cu0, seq, a.group, BM);
     const int64_t row = (int64_t)local * BM + in_tile;
+    // (of one row or of none with four waves a row: uniform there)
     if (local < 0 || row >= (int64_t)(end - begin) * a.group) return;
     const size_t at = ((size_t)tile * a.kv_heads + kvh) * a.splits * BM + in_tile;
     float m = -INFINITY;
     bool none = false;
-    for (int s = 0; s < a.splits; ++s) {
+    for (int s = lane; s < a.splits; s += 64) {
         const float2 x = a.part_ml[at + (size_t)s * BM];
         m = fmaxf(m, x.x);
         none |= x.y < 0.f;
     }
+    for (int k = 32; k; k >>= 1) m = fmaxf(m, __shfl_xor(m, k));
+    none = __any(none);
     float sum = 0, o[E];
     for (int e = 0; e < E; ++e) o[e] = 0;
-    for (int s = 0; s < a.splits; ++s) {
+#pragma unroll 4
+    for (int s = wave % W; s < a.splits; s += W) {
         const float2 x = a.part_ml[at + (size_t)s * BM];
+        float y[E];
+        for (int e = 0; e < E; ++e) y[e] = a.part_o[(at + (size_t)s * BM) * DH + e * 64 + lane];
+        const float f = x.x == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(x.x - m);
         if (x.y == 0.f) continue; // no key of that split
-        const float f = x.x == -INFINITY ? 0.f : exp2f(x.x - m);
         sum += f * x.y;
-        for (int e = 0; e < E; ++e) o[e] += f * a.part_o[(at + (size_t)s * BM) * DH + e * 64 + lane];
+        for (int e = 0; e < E; ++e) o[e] += f * y[e];
+    }
+    if constexpr (W == 4) {
+        __shared__ float o_s[4][DH], sum_s[4];
+        for (int e = 0; e < E; ++e) o_s[wave][e * 64 + lane] = o[e];
+        if (lane == 0) sum_s[wave] = sum;
+        __syncthreads();
+        if (wave) return;
+        sum = (sum_s[0] + sum_s[1]) + (sum_s[2] + sum_s[3]);
+        for (int e = 0; e < E; ++e)
+            o[e] = (o_s[0][e * 64 + lane] + o_s[1][e * 64 + lane]) + (o_s[2][e * 64 + lane] + o_s[3][e * 64 + lane]);
     }
     const float inv = none || sum == 0.f ? 0.f : 1.f / sum;
     const int tok = (int)(row / a.group), head = kvh * a.group + (int)(row - (int64_t)tok * a.group);
@@ -393,8 +411,9 @@ __global__ __launch_bounds__(256) void k_attn_prompt_join(const QeAttnArgs a) {
 template <bool BF, int DH, int WAVES>
 static hipError_t launch_waves(const QeAttnArgs &a, hipStream_t st) {
     k_attn_prompt<BF, DH, WAVES><<<dim3((unsigned)(a.tiles * a.kv_heads * a.splits)), dim3(64 * WAVES), 0, st>>>(a);
-    if (a.splits > 1)
-        k_attn_prompt_join<BF, DH, 32 * WAVES><<<dim3((unsigned)(a.tiles * a.kv_heads * (8 * WAVES))), dim3(256), 0, st>>>(a);
+    const unsigned rows = (unsigned)(a.tiles * a.kv_heads) * (32 * WAVES);
+    if (a.splits > 8) k_attn_prompt_join<BF, DH, 32 * WAVES, 4><<<dim3(rows), dim3(256), 0, st>>>(a);
+    else if (a.splits > 1) k_attn_prompt_join<BF, DH, 32 * WAVES, 1><<<dim3(rows / 4), dim3(256), 0, st>>>(a);
     return hipGetLastError();
 }
 template <bool BF, int DH>

@@ -68,10 +68,12 @@ QE_MIX_HD int qe_attn_prompt_rows(int n_tokens, int n_seqs, int group, int kv_he
     return head_dim == 256 && (int64_t)qe_attn_max_tiles(n_tokens, n_seqs, group, 256) * kv_heads >= 256 ? 256 : 128;
 }
 
-// Splits of a prompt call's keys: none if its tiles fill half the CUs.
-QE_MIX_HD int qe_attn_prompt_splits(int64_t tiles, int64_t max_len) {
+// Splits of a prompt call's keys: none if its tiles fill half the CUs, else as many workgroups as the GPU
+// holds at once (one a CU with heads of 256, whose LDS they fill: 54 us for 1000 tokens of 16 such heads, 61 with two),
+// of at least 256 keys.
+QE_MIX_HD int qe_attn_prompt_splits(int64_t tiles, int64_t max_len, int head_dim) {
     if (tiles > 128) return 1;
-    const int64_t most = (max_len + 255) / 256, want = QE_ATTN_WGS / tiles;
+    const int64_t most = (max_len + 255) / 256, want = (head_dim == 256 ? QE_ATTN_WGS / 2 : QE_ATTN_WGS) / tiles;
     const int64_t s = want < most ? want : most;
     return s < 1 ? 1 : (int)s;
 }
