@@ -17,14 +17,15 @@
  * return without a host sync; they can be captured into a HIP graph.  A
  * context is used by one host thread at a time, and calls on one context that
  * could overlap (other streams, two graphs replayed at once) race on its
- * scratch: give each its own context.  Entry points return 0 or a negative
+ * scratch, and may leave it unusable: give each its own context.  Entry points return 0 or a negative
  * QE_ERR_* code (qe_moe.h), and qe_moe_last_error() describes the calling
  * thread's last failure.  The calling thread's current device is left as it
  * was.
  *
  * What stands in device memory (lengths, page tables, slots) is checked by the
  * kernels: a bad value makes no access out of bounds, its sequence's outputs
- * are zeros, and the context remembers it.  The next call on the context
+ * are zeros (qe_attn_append leaves the token out: nothing of it is written),
+ * and the context remembers it.  The next call on the context
  * that looks returns QE_ERR_STATE for it, once, without doing its own work:
  * every entry point looks at entry without synchronising, qe_attn_check and
  * qe_delta_check after synchronising `stream`.
@@ -62,7 +63,7 @@ typedef struct {
 
 typedef struct qe_attn_ctx qe_attn_ctx;
 
-/* Create a context on `device`: scratch of a fixed size (about 140 MB at most)
+/* Create a context on `device`: scratch of a fixed size (17 to 68 MB)
  * for the partial results of calls that split a sequence's length. */
 int qe_attn_create(int device, const qe_attn_desc *desc, qe_attn_ctx **out);
 int qe_attn_destroy(qe_attn_ctx *ctx);
@@ -103,7 +104,9 @@ typedef struct {
  * NULL = the position in the sequence, on every axis.  Angles are computed in
  * 64 bits.  q and q_out may both be NULL (keys and values only); q_out may be q
  * if in_type is the context's type and the strides are equal.  Pointers are
- * 16-byte aligned and strides multiples of 16 bytes.  A page that two
+ * 16-byte aligned and strides multiples of 16 bytes.  A token before its
+ * sequence's first position (cu_q gives more tokens than kv_len) writes nothing
+ * to the cache; its q is rotated by pos or by its negative position.  A page that two
  * sequences of the call write at the same row gets one of the two. */
 int qe_attn_append(qe_attn_ctx *ctx, const qe_attn_batch *batch, const qe_kv_cache *cache, int in_type, const void *q,
                    int64_t q_stride, const void *k, int64_t k_stride, const void *v, int64_t v_stride, const int32_t *pos,
@@ -141,8 +144,9 @@ typedef struct {
 
 typedef struct qe_delta_ctx qe_delta_ctx;
 
-/* Create a context on `device`.  Scratch: 33 KiB per value head for every
- * 64 tokens of t_max and every sequence of seqs_max. */
+/* Create a context on `device`.  Scratch, for every 64 tokens of t_max and
+ * every sequence of seqs_max: 49 KiB per value head, and per key head 768 bytes
+ * of dim_k for fp32 (96 KiB of 128), 512 for fp16, none for bf16. */
 int qe_delta_create(int device, const qe_delta_desc *desc, qe_delta_ctx **out);
 int qe_delta_destroy(qe_delta_ctx *ctx);
 

@@ -33,7 +33,7 @@ __global__ __launch_bounds__(256) void k_append(const QeAppendArgs a) {
     __shared__ long row_s;
     __shared__ int seq_s[2];
     const int t = blockIdx.x, tid = threadIdx.x, half = a.rotary / 2;
-    if (tid < 64) { // the token's sequence: the last whose first row is not behind t (64 at a time)
+    if (tid < 64) { // the token's sequence: the last whose first row is not behind t
         int seq = -1;
         if (!a.cu) {
             seq = t;

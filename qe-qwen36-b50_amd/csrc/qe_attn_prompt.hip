@@ -17,10 +17,7 @@
 
 #define BN QE_ATTN_BN
 
-template <int DH>
-__device__ __forceinline__ int k_swz(int row) {
-    return row & 7;
-}
+__device__ __forceinline__ int k_swz(int row) { return row & 7; }
 template <int DH>
 __device__ __forceinline__ int v_swz(int row) {
     return DH == 64 ? ((row >> 1) & 1) << 2 : (row & 3) << 2;
@@ -50,10 +47,10 @@ __device__ __forceinline__ void load_part(const QeAttnArgs &a, int page, int kvh
     const char *from = (const char *)(IS_K ? a.kc : a.vc) + r0 * DH * 2;
     // A uniform address and a 32-bit offset: a later row's permutation differs from the first load's by a constant.
     const int lane = lane_now(), row = lane / CH, c = lane % CH;
-    const unsigned off = row * DH * 2 + ((c ^ (IS_K ? k_swz<DH>(row) : v_swz<DH>(row))) << 4);
+    const unsigned off = row * DH * 2 + ((c ^ (IS_K ? k_swz(row) : v_swz<DH>(row))) << 4);
 #pragma unroll
     for (int i = 0; i < PART / ROWS; ++i)
-        load_lds16(from + i * 1024 + (off ^ ((IS_K ? k_swz<DH>(i * ROWS) : v_swz<DH>(i * ROWS)) << 4)), lds + (wave * PART + i * ROWS) * DH);
+        load_lds16(from + i * 1024 + (off ^ ((IS_K ? k_swz(i * ROWS) : v_swz<DH>(i * ROWS)) << 4)), lds + (wave * PART + i * ROWS) * DH);
 }
 
 __device__ __forceinline__ float max3(float a, float b, float c) { return fmaxf(fmaxf(a, b), c); }
@@ -122,7 +119,7 @@ struct Rows {
     template <int KB>
     __device__ __forceinline__ void scores(const short *k_lds, int b0, Scores<KB> &x) const {
         const int lane = lane_now(), r = lane & 31, h = lane >> 5;
-        const unsigned ka = r * DH * 2 + ((h ^ k_swz<DH>(r)) << 4);
+        const unsigned ka = r * DH * 2 + ((h ^ k_swz(r)) << 4);
 #pragma unroll
         for (int b = 0; b < KB; ++b) {
 #pragma unroll

@@ -263,8 +263,9 @@ __global__ __launch_bounds__(256) void k_delta_chunks(const QeDeltaArgs a) {
         kk += __shfl_xor(kk, 32), qq += __shfl_xor(qq, 32);
         if (lane < 16) {
             kk_s[row] = kk;
-            rk_s[row] = a.l2norm ? 1.f / sqrtf(kk + 1e-6f) : 1.f;
-            rq_s[row] = (a.l2norm ? 1.f / sqrtf(qq + 1e-6f) : 1.f) * a.scale;
+            // rows behind the end stand for the last token's in k_delta_scan: factors of 0 keep them from overflowing
+            rk_s[row] = row >= n ? 0.f : a.l2norm ? 1.f / sqrtf(kk + 1e-6f) : 1.f;
+            rq_s[row] = row >= n ? 0.f : (a.l2norm ? 1.f / sqrtf(qq + 1e-6f) : 1.f) * a.scale;
         }
         __syncthreads();
 #pragma unroll
@@ -574,6 +575,7 @@ __global__ __launch_bounds__(512) void k_delta_scan(const QeDeltaArgs a) {
             // and read S while the chain is at its next product.
             load_v(t0 + ahead * QE_DELTA_C, ws, v_next, f_next);
             load_k(t0 + ahead * QE_DELTA_C, kq, k_next);
+            asm volatile("" ::: "memory"); // the count above needs M's loads behind the direct ones
             load_m(ws, m_next);
             lds_barrier();
             qe_f4 x[3] = {};

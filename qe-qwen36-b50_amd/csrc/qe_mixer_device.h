@@ -55,9 +55,6 @@ __device__ __forceinline__ float from16(short x) {
 __device__ __forceinline__ qe_s4 lds_tr(const short *p) {
     return __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) qe_s4 *)p);
 }
-__device__ __forceinline__ qe_s4 lds_tr_at(unsigned at) { // by LDS byte address
-    return __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) qe_s4 *)(uintptr_t)at);
-}
 // 64 lanes x 16 bytes from global memory straight to LDS: lane l's land at dst + 16 l
 __device__ __forceinline__ void load_lds16(const void *src, void *dst) {
     __builtin_amdgcn_global_load_lds(QE_GLOBAL(void, src), QE_LDS(void, dst), 16, 0, 0);

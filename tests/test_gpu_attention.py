@@ -93,6 +93,42 @@ def test_decode_split_over_a_long_sequence(hq, hkv, dim, page, n):
         close(out, want, off)
 
 
+def test_many_sequences():
+    """More sequences times heads than a decode call has workgroups for splits, in all three calls."""
+    n, page = 300, 32
+    lens = [1 + 37 * i % 211 for i in range(n)]
+    c = Case(8, 8, 64, page, torch.float16, lens)
+    k, v = rand(c.g, n, 8, 64, dtype=torch.float16), rand(c.g, n, 8, 64, dtype=torch.float16)
+    for b in (c.batch(), c.batch(list(range(n + 1)))):
+        kc, vc = c.kc.clone(), c.vc.clone()
+        c.att.append(b, None, k, v, kc, vc, None)
+        c.att.check()
+        for i, at in enumerate(lens):
+            p, row = int(c.table[i, (at - 1) // page]), (at - 1) % page
+            assert torch.equal(kc[p, :, row], k[i]) and torch.equal(vc[p, :, row], v[i]), i
+    q = c.q(n)
+    want, off = c.expect(q, list(range(n + 1)))
+    for attend, b in ((c.att.decode, c.batch()), (c.att.prompt, c.batch(list(range(n + 1))))):
+        out = torch.empty_like(q)
+        attend(b, q, c.kc, c.vc, out)
+        close(out, want, off)
+    c.att.check()
+
+
+def test_calls_without_tokens():
+    c = Case(4, 2, 64, 16, torch.bfloat16, [0, 20], rotary=64)
+    kc, vc = c.kc.clone(), c.vc.clone()
+    q, k = c.q(0), rand(c.g, 0, 2, 64, dtype=torch.bfloat16)
+    c.att.append(c.batch([0, 0, 0]), q, k, k, c.kc, c.vc, torch.empty_like(q))
+    c.att.prompt(c.batch([0, 0, 0]), q, c.kc, c.vc, torch.empty_like(q))
+    q, k, out = c.q(3), rand(c.g, 3, 2, 64, dtype=torch.bfloat16), torch.full((3, 4, 64), 7.0, dtype=torch.bfloat16, device="cuda")
+    c.att.append(c.batch([3, 3, 3]), q, k, k, c.kc, c.vc, out)  # rows, but of no sequence
+    c.att.prompt(c.batch([0, 0, 0]), q, c.kc, c.vc, out)
+    c.att.check()
+    assert bool((out == 7).all())
+    assert torch.equal(kc.view(torch.int16), c.kc.view(torch.int16)) and torch.equal(vc.view(torch.int16), c.vc.view(torch.int16))
+
+
 def test_decode_rows_with_strides_and_in_place():
     c = Case(16, 2, 256, 64, torch.bfloat16, [300, 20, 77])
     wide = rand(c.g, 3, 20, 256, dtype=torch.bfloat16)
@@ -397,6 +433,37 @@ def test_captured_calls_follow_the_lengths_in_device_memory():
         off = R.attend_batch(r, c.kc, c.vc, c.table, kv.tolist(), [0, 1, 2], 128 ** -0.5, 16)
         close(o1, *off)
         close(o2, *off)
+
+
+def test_two_graphs_share_a_context():
+    """One after the other, and calls of other sizes between them: what a call leaves in the scratch is of no use to the next."""
+    c = Case(16, 2, 256, 256, torch.bfloat16, [9000, 300, 2000])
+    d = [(c.batch(), c.q(3)), (qe_mixer.Batch(ints([9000]), c.table[:1]), c.q(1)), (c.batch([0, 4, 5, 40]), c.q(40))]
+    outs = [torch.empty_like(q) for _, q in d]
+    want = [c.expect(d[0][1], [0, 1, 2, 3]), R.attend_batch(d[1][1], c.kc, c.vc, c.table, [9000], [0, 1], 1 / 16, 256),
+            c.expect(d[2][1], [0, 4, 5, 40])]
+
+    def call(i, stream=None):
+        (c.att.prompt if i == 2 else c.att.decode)(*d[i], c.kc, c.vc, outs[i], stream=stream)
+
+    graphs = []
+    for i in (0, 1):
+        call(i)
+        torch.cuda.synchronize()
+        graphs.append(torch.cuda.CUDAGraph())
+        with torch.cuda.graph(graphs[-1]):
+            call(i, torch.cuda.current_stream())
+    for _ in range(4):
+        for o in outs:
+            o.fill_(7.0)
+        graphs[0].replay()
+        graphs[1].replay()
+        torch.cuda.synchronize()
+        call(2)
+        torch.cuda.synchronize()
+        for o, w in zip(outs, want):
+            close(o, *w)
+    c.att.check()
 
 
 def test_results_do_not_change_from_call_to_call():

@@ -124,6 +124,48 @@ def test_decode_of_many_sequences():
     assert bool((c.out[299] == 0).all()) and torch.equal(c.pool[34], before[34])
 
 
+def test_prompts_of_many_sequences():
+    n = 300
+    lens = [i % 4 for i in range(n)]
+    lens[7], lens[299] = 130, 65
+    c = Case(1, 2, 64, 64, torch.bfloat16, lens)
+    before = c.pool.clone()
+    into, outof = [2 * i for i in range(n)], [2 * i + 1 for i in range(n)]
+    outof[298] = 2 * 17  # what sequence 17 reads
+    c.prompt(into, outof)
+    with pytest.raises(qe_moe.QeError, match="slot"):
+        c.h.check()
+    for i in (0, 4, 7, 17, 255, 256, 299):
+        o, S = c.expect(i, before[2 * i])
+        if lens[i]:
+            c.close(c.out[c.cu[i]: c.cu[i + 1]], o, i)
+            c.close(c.pool[2 * i + 1], S, i)
+        else:
+            assert torch.equal(c.pool[2 * i + 1], before[2 * i])
+    assert bool((c.out[c.cu[298]: c.cu[299]] == 0).all()) and torch.equal(c.pool[34], before[34])
+
+
+def test_prompt_without_tokens_passes_states_on():
+    c = Case(2, 4, 64, 128, torch.float16, [0, 0, 0])
+    before = c.pool.clone()
+    c.prompt([0, -1, 4], [1, 2, -1])
+    c.h.check()
+    assert torch.equal(c.pool[1], before[0]) and bool((c.pool[2] == 0).all())
+    assert torch.equal(c.pool[[0, 3, 4, 5]], before[[0, 3, 4, 5]])
+
+
+def test_states_near_the_end_of_the_range():
+    """Nothing but the sequences' own tokens is computed from large states: no infinity out of a chunk's unused rows."""
+    c = Case(1, 2, 64, 64, torch.float32, [1, 5, 70])
+    c.pool.mul_(1e37)
+    w = [c.expect(i, c.pool[2 * i]) for i in range(3)]
+    c.prompt([0, 2, 4], [1, 3, 5])
+    c.h.check()
+    for i in range(3):
+        c.close(c.out[c.cu[i]: c.cu[i + 1]], w[i][0], i)
+        c.close(c.pool[2 * i + 1], w[i][1], i)
+
+
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
 def test_long_prompt(dtype):
     c = Case(2, 4, 128, 128, dtype, [2000])
