@@ -214,8 +214,10 @@ __device__ __forceinline__ void load8_planes(const IN *p, bool there, qe_s8 *h, 
             for (int i = 0; i < 8; ++i) h[n][i] = next_plane(x[i]);
 }
 
+// (Three workgroups a CU, as the LDS allows: 1999 fp32 tokens of 16 and 32 heads of 128 take 37 us, with the registers
+// of two 51.)
 template <typename IN, int DK>
-__global__ __launch_bounds__(256) void k_delta_chunks(const QeDeltaArgs a) {
+__global__ __launch_bounds__(256, 3) void k_delta_chunks(const QeDeltaArgs a) {
     constexpr int LD = 68, KS = DK / 32, NP = planes_of<IN>(), NO = sizeof(IN) == 4 ? 3 : 2;
     // K's planes as they are in k_delta_scan's LDS, then the heads' matrices
     constexpr int K_BYTES = NP * 64 * DK * 2, M_BYTES = 3 * 64 * LD * 4;
@@ -394,8 +396,10 @@ __global__ __launch_bounds__(256) void k_delta_chunks(const QeDeltaArgs a) {
 // while the CU's 64 bytes a cycle are taken (some 65 KiB a chunk), so the loads are few and
 // wide, and spread over the waves and over the chunk.
 // ---------------------------------------------------------------------------
+// Where the LDS holds two workgroups (bf16, and fp16 keys of 64), 128 registers let it: sequences side by side overlap
+// (16 of 500 tokens, bf16: 355 us the call with one a CU, 296 with two; one of 8192 has one a CU and takes 319 in both forms).
 template <typename IN, int DK, int DV>
-__global__ __launch_bounds__(512) void k_delta_scan(const QeDeltaArgs a) {
+__global__ __launch_bounds__(512, sizeof(IN) == 2 && (DK == 64 || __is_same(IN, __bf16)) ? 4 : 2) void k_delta_scan(const QeDeltaArgs a) {
     constexpr int KS = DK / 32, SB = DK / 64, LS = DK + 8, LT = 72, NP = planes_of<IN>(), NO = sizeof(IN) == 4 ? 3 : 2;
     constexpr int SL = DV / 16, VL = 16 / sizeof(IN); // elements of V in 16 bytes
     // what is loaded ahead has two buffers, variables of their own: else the compiler has every LDS read wait for
@@ -562,8 +566,7 @@ __global__ __launch_bounds__(512) void k_delta_scan(const QeDeltaArgs a) {
                 mf[1][p] = *(const qe_s8 *)(w + 12288 + wave * 3072 + 1536 + p * 512 + lane * 8);
             }
         };
-        IN *out[4]; // the lane's four rows
-        for (int j = 0; j < 4; ++j) out[j] = (IN *)a.out + (size_t)(begin + 16 * wave + 4 * c + j) * a.out_stride + (size_t)head * DV + col;
+        IN *out = (IN *)a.out + (size_t)(begin + 16 * wave + 4 * c) * a.out_stride + (size_t)head * DV + col; // the first of the lane's four rows
         auto step = [&](const int par, const bool whole, const float *f_s, short *k_next, IN *v_next, float *f_next, const qe_s8 (*mf)[NO], qe_s8 (*m_next)[NO], int t0) {
             const int ahead = t0 + QE_DELTA_C < end;
             kq += ahead * kq_step, ws += ahead * ws_step;
@@ -584,6 +587,7 @@ __global__ __launch_bounds__(512) void k_delta_scan(const QeDeltaArgs a) {
                 qe_s8 sf[NO];
                 for (int p = 0; p < NO; ++p) sf[p] = *(const qe_s8 *)(s_p + (p * 16 + r) * LS + 32 * s + 8 * c);
                 mul_planes<NP, NO, NO - 1>(qf[s], sf, x);
+                if (s & 1) __builtin_amdgcn_sched_barrier(0); // all of S read at once would take more than 128 registers
             }
             qe_f4 o = *(const qe_f4 *)(f_s + 256 * wave + 64 + 16 * wave + 4 * c) * (x[0] + (x[1] + x[2]));
             load_q(t0 + ahead * QE_DELTA_C, kq);
@@ -600,9 +604,9 @@ __global__ __launch_bounds__(512) void k_delta_scan(const QeDeltaArgs a) {
             o += y[0] + (y[1] + y[2]);
             for (int j = 0; j < 4; ++j) {
                 const int t = 16 * wave + 4 * c + j;
-                if (whole || t0 + t < end) *out[j] = (IN)(t < spoilt ? o[j] : NAN);
-                out[j] += QE_DELTA_C * a.out_stride;
+                if (whole || t0 + t < end) out[j * a.out_stride] = (IN)(t < spoilt ? o[j] : NAN);
             }
+            out += QE_DELTA_C * a.out_stride;
         };
         if (begin < end) {
             load_v(begin, ws, v_even, f_even);
