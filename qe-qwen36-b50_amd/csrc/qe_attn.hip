@@ -7,8 +7,9 @@
 // in 64 bits (a position of 2^18 times a pair's 24-bit rate would leave 2^-6 of a turn in
 // 32) and only the fraction goes to the 32-bit sine and cosine; they are made once per token
 // and pair, in LDS, for all of its heads.  A work item is 16 elements of a head: 8 pairs,
-// or 16 elements behind the rotated ones.  Bound by memory: q read and written, k and v
-// read and written.
+// or 16 elements behind the rotated ones.  Bound by memory: q, k and v read and written.  8192
+// tokens of 32 + 2 x 8 heads of 128, fp16, 201 MB: 31 us, 6.4 TB/s (a large copy here reaches 5.1; part of
+// it stays in the last-level cache).  8 tokens: 4 us, of which most is the launch.
 // ---------------------------------------------------------------------------
 template <typename IN>
 __device__ __forceinline__ void load8(const IN *p, float *x) {
@@ -133,7 +134,12 @@ hipError_t qe_launch_append(const QeAppendArgs &a, int in_type, int type, hipStr
 // operand, and V^T is read from LDS with the transposing read in that same order of keys, so
 // probabilities never cross lanes.  V reaches LDS by direct loads, its 64-byte units
 // permuted by row so that the four rows of a transposing read hit different banks.
-// Running maximum and sum in 32 bits per head; O is rescaled only when a maximum grew.
+// Running maximum and sum in 32 bits per head; O is rescaled only when a maximum grew.  Probabilities are
+// rounded to the cache's type for the second product (their sum is of the unrounded ones).
+// Long lengths are bound by memory: one sequence of 100,000 keys, two key-value heads of 256, bf16, 205 MB:
+// 34 us, 6.0 TB/s, and 5 for the join; 24 sequences of 1 to 8,100 keys, eight heads of 128, fp16, 339 MB: 66 us,
+// 5.1 TB/s.  Short ones by latency: 700 keys take 12 us (length and page, keys and values, the exchange through
+// memory, the join), where a launch that does nothing takes 2.
 // ---------------------------------------------------------------------------
 template <int DH>
 __device__ __forceinline__ int v_swizzle(int row) { // of the 16-byte chunk index

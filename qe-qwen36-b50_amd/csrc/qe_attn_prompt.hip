@@ -13,6 +13,14 @@
 // worked on.  16-byte chunks are permuted within their rows at the source (LDS rows
 // are contiguous for direct loads): K's by row % 8, so that the eight rows of a read's
 // phase lie in different banks, V's 64-byte units by row % 4.
+//
+// Scores, maxima and sums are in 32 bits; probabilities are rounded to the cache's type for the
+// second product.  A row's maximum is raised only where a score exceeds it by 2^8, so that O is seldom rescaled.
+// Long prompts are bound by the matrix cores, whose issue the exponentials share: 8192 tokens of 16 heads of 256 (550
+// GFLOP), bf16, 515 to 545 us, 1010 to 1070 TFLOP/s where a large library product reaches 1219.  Five
+// prompts of 1999 tokens, 32 heads of 128, fp16: 40 us, the longest row blocks' 18 steps in turn.
+// 100 tokens: 14 us, latency (lengths, pages, two tiles, the output).  Splitting the keys also where tiles fill the
+// GPU was measured too: 80 us for those five prompts.
 #include "qe_mixer_device.h"
 
 #define BN QE_ATTN_BN

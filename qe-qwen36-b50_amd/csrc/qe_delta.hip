@@ -117,7 +117,8 @@ __global__ __launch_bounds__(256) void k_delta_slots(const QeDeltaArgs a) {
 // One token per sequence: a workgroup per (sequence, value head, 32 columns of its state),
 // a thread 4 columns of DK / 32 rows.  S^T k and S^T q are summed in the one pass over the old
 // state that it needs (S'^T q = e^g S^T q + (k . q) u), so the state is read once, kept
-// in registers and written once.
+// in registers and written once.  Bound by memory: 64 sequences of 32 heads of 128 x 128, 270 MB: 46 us,
+// 5.9 TB/s (a large copy reaches 5.1; part of it stays in the last-level cache).  One sequence: 5 us, latency.
 // ---------------------------------------------------------------------------
 template <typename IN, int DK, int DV>
 __global__ __launch_bounds__(256) void k_delta_decode(const QeDeltaArgs a) {
@@ -190,6 +191,8 @@ __global__ __launch_bounds__(256) void k_delta_decode(const QeDeltaArgs a) {
 // are not written), then per token e^b / |k|, scale e^b / |q|, e^(b_last - b) / |k|, and
 // e^(b_last).  fp16 and fp32 keys and queries are cut into planes here too, for a chunk and key
 // head: K [plane][64][DK] as it lies in LDS, Q [wave][32 of DK][plane][lane][8].
+// 8192 bf16 tokens of 16 key and 32 value heads of 128: 68 us, against 52 for its reads and writes at a large copy's
+// rate; the rest is the barriers between a head's short steps.
 // ---------------------------------------------------------------------------
 template <int DK>
 __device__ __forceinline__ int key_swz(int row) { // of the 16-byte chunk index: 8 rows' pairs of chunks in different banks
@@ -394,7 +397,9 @@ __global__ __launch_bounds__(256, 3) void k_delta_chunks(const QeDeltaArgs a) {
 // What bounds it: the chain of products, exchanges and barriers of a chunk, on 256 of the
 // GPU's 1024 SIMDs for each sequence (32 heads, 8 slices).  A load stalls the wave that issues it
 // while the CU's 64 bytes a cycle are taken (some 65 KiB a chunk), so the loads are few and
-// wide, and spread over the waves and over the chunk.
+// wide, and spread over the waves and over the chunk.  8192 bf16 tokens of 32 heads of 128 x 128: 240 us, 1.9 a
+// chunk (of some 3,900 cycles K S takes 550, what is left of V to LDS 400, T times it 280, U to LDS 500,
+// the state's update and S to LDS 1,150, the rest is barriers); 1999 fp32 tokens of three prompts 90 us.
 // ---------------------------------------------------------------------------
 // Where the LDS holds two workgroups (bf16, and fp16 keys of 64), 128 registers let it: sequences side by side overlap
 // (16 of 500 tokens, bf16: 355 us the call with one a CU, 296 with two; one of 8192 has one a CU and takes 319 in both forms).
