@@ -263,11 +263,14 @@ __global__ __launch_bounds__(256, 2) void k_attn_decode(const QeAttnArgs a) {
         for (int w = 1; w < 4; ++w) top = fmaxf(top, ml[w][h].x);
         float sum = 0;
         qe_f4 r = {0, 0, 0, 0};
-        for (int w = 0; w < 4; ++w) {
-            const float mw = ml[w][h].x, f = mw == -INFINITY ? 0.f : __builtin_amdgcn_exp2f((mw - top) * a.scale_log2);
-            if (ml[w][h].y == 0.f) continue; // a wave without keys
-            sum += f * ml[w][h].y;
-            r += f * *(const qe_f4 *)((const float *)v_lds[w] + h * DH + ((d / 4) ^ h) * 4);
+#pragma unroll
+        for (int w = 0; w < 4; ++w) { // no branches: each would wait for the LDS anew
+            const float2 x = ml[w][h];
+            const float f = x.x == -INFINITY ? 0.f : __builtin_amdgcn_exp2f((x.x - top) * a.scale_log2);
+            const qe_f4 y = *(const qe_f4 *)((const float *)v_lds[w] + h * DH + ((d / 4) ^ h) * 4);
+            const bool any = x.y != 0.f; // else a wave without keys
+            sum += any ? f * x.y : 0.f;
+            for (int j = 0; j < 4; ++j) r[j] += any ? f * y[j] : 0.f;
         }
         if (active <= 1) {
             const float inv = sum == 0.f ? 0.f : 1.f / sum;
@@ -278,14 +281,15 @@ __global__ __launch_bounds__(256, 2) void k_attn_decode(const QeAttnArgs a) {
             w.y = pack2<BF>(r[2], r[3]);
             *(uint2 *)((short *)a.out + (size_t)seq * a.out_stride + ((size_t)kvh * G + h) * DH + d) = w;
         } else {
-            const size_t row = ((size_t)item * a.splits + split) * G + h;
+            const size_t part = (size_t)item * a.splits + split, row = part * G + h;
+            float2 *to_ml = a.part_ml + part * QE_ATTN_GROUP_MAX + h;
             if (a.splits <= QE_ATTN_JOIN) {
                 store_through(a.part_o + row * DH + d, qe_f2{r[0], r[1]});
                 store_through(a.part_o + row * DH + d + 2, qe_f2{r[2], r[3]});
-                if (d == 0) store_through((float *)(a.part_ml + row), qe_f2{top, bad ? -1.f : sum});
+                if (d == 0) store_through((float *)to_ml, qe_f2{top, bad ? -1.f : sum});
             } else {
                 *(qe_f4 *)(a.part_o + row * DH + d) = r;
-                if (d == 0) a.part_ml[row] = make_float2(top, bad ? -1.f : sum);
+                if (d == 0) *to_ml = make_float2(top, bad ? -1.f : sum);
             }
         }
     }
@@ -309,23 +313,33 @@ __global__ __launch_bounds__(256, 2) void k_attn_decode(const QeAttnArgs a) {
     // before in this launch, so no older copy is nearer).  Else from behind the L2s.
     const bool near_all = (count >> (8 + 7 * xcd) & 127) == (unsigned)active;
     float2 *all_ml = (float2 *)v_lds[0]; // [split][16]
-    float *sums = (float *)(all_ml + QE_ATTN_JOIN * 16);
-    for (int i = tid; i < active * 16; i += 256)
-        if ((i & 15) < a.group) {
-            const float *p = (const float *)(a.part_ml + row0 + (i >> 4) * G + (i & 15));
-            const qe_f2 x = load_through(p); // rows of others, read in this launch by their last workgroups, share its line
-            all_ml[i] = make_float2(x[0], x[1]);
+    float *sums = (float *)(all_ml + QE_ATTN_JOIN * 16), *weight = sums + 16; // [split][16]
+    float2 mine = make_float2(-INFINITY, 0.f);
+    if (tid < active * 16 && (tid & 15) < a.group) { // a split's 16 are a cache line of their own
+        const float2 *p = a.part_ml + (size_t)item * a.splits * QE_ATTN_GROUP_MAX + tid;
+        if (near_all) {
+            mine = *p;
+        } else {
+            const qe_f2 x = load_through((const float *)p);
+            mine = make_float2(x[0], x[1]);
         }
+    }
+    all_ml[tid] = mine;
     __syncthreads();
     if (tid < a.group) {
         float top = -INFINITY, sum = 0;
         bool none = false;
-        for (int s = 0; s < active; ++s) top = fmaxf(top, all_ml[s * 16 + tid].x), none |= all_ml[s * 16 + tid].y < 0.f;
-        for (int s = 0; s < active; ++s) {
-            const float2 x = all_ml[s * 16 + tid];
-            const float f = x.y == 0.f || x.x == -INFINITY ? 0.f : __builtin_amdgcn_exp2f((x.x - top) * a.scale_log2);
-            sum += x.y == 0.f ? 0.f : f * x.y;
-            all_ml[s * 16 + tid].x = f;
+        float2 x[QE_ATTN_JOIN];
+#pragma unroll
+        for (int s = 0; s < QE_ATTN_JOIN; ++s) x[s] = all_ml[s * 16 + tid];
+#pragma unroll
+        for (int s = 0; s < QE_ATTN_JOIN; ++s) top = fmaxf(top, x[s].x), none |= x[s].y < 0.f;
+#pragma unroll
+        for (int s = 0; s < QE_ATTN_JOIN; ++s) {
+            const bool any = x[s].y != 0.f;
+            const float f = x[s].x == -INFINITY ? 0.f : __builtin_amdgcn_exp2f((x[s].x - top) * a.scale_log2);
+            sum += any ? f * x[s].y : 0.f;
+            weight[s * 16 + tid] = any ? f : -1.f; // -1: nothing of that split is used
         }
         sums[tid] = none ? -1.f : sum;
     }
@@ -347,10 +361,13 @@ __global__ __launch_bounds__(256, 2) void k_attn_decode(const QeAttnArgs a) {
                 o[s] = qe_f4{x[0], x[1], y[0], y[1]};
             }
         }
+        float f[QE_ATTN_JOIN];
+#pragma unroll
+        for (int s = 0; s < QE_ATTN_JOIN; ++s) f[s] = weight[s * 16 + h]; // (as above: no branches around LDS reads)
         qe_f4 r = {0, 0, 0, 0};
 #pragma unroll
         for (int s = 0; s < QE_ATTN_JOIN; ++s)
-            if (s < active && all_ml[s * 16 + h].y != 0.f) r += all_ml[s * 16 + h].x * o[s]; // else a split without sum
+            for (int j = 0; j < 4; ++j) r[j] += s < active && !(f[s] < 0.f) ? f[s] * o[s][j] : 0.f;
         const float sum = sums[h];
         r *= sum == 0.f ? 0.f : 1.f / sum;
         if (sum < 0.f) r = qe_f4{0, 0, 0, 0};
@@ -380,7 +397,7 @@ __global__ __launch_bounds__(1024) void k_attn_join(const QeAttnArgs a) {
     if (active <= 1) return; // its one workgroup has written the row
     const size_t row0 = ((size_t)seq * a.kv_heads + kvh) * a.splits * a.group + h;
     const int d = part * 64 + tid % 16 * 4;
-    const float2 x = tid < active ? a.part_ml[row0 + (size_t)tid * a.group] : make_float2(-INFINITY, 0.f);
+    const float2 x = tid < active ? a.part_ml[(((size_t)seq * a.kv_heads + kvh) * a.splits + tid) * QE_ATTN_GROUP_MAX + h] : make_float2(-INFINITY, 0.f);
     qe_f4 o[4];
 #pragma unroll
     for (int k = 0; k < 4; ++k) { // the first 256 splits; behind the last the first again, unused

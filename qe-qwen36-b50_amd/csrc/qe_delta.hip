@@ -370,7 +370,7 @@ __global__ __launch_bounds__(256, 3) void k_delta_chunks(const QeDeltaArgs a) {
                 m[j] = M[ri * LD + cj + j];
             }
             // the lane (cj % 32) / 8 * 16 + ri % 16 of the wave's operand for columns 32 (cj / 32) .. + 31
-            short *to = (short *)ws + (wave * 2 + cj / 32) * 1536 + ((cj % 32) / 8 * 16 + ri % 16) * 8;
+            short *to = (short *)ws + (wave * 2 + cj / 32) * 3 * 512 + ((cj % 32) / 8 * 16 + ri % 16) * 8;
             for (int p = 0; p < 3; ++p) {
                 qe_s8 h;
                 for (int j = 0; j < 8; ++j) h[j] = next_plane(t[j]);
@@ -379,7 +379,7 @@ __global__ __launch_bounds__(256, 3) void k_delta_chunks(const QeDeltaArgs a) {
             for (int p = 0; p < NO; ++p) {
                 qe_s8 h;
                 for (int j = 0; j < 8; ++j) h[j] = next_plane(m[j]);
-                *(qe_s8 *)(to + 12288 + p * 512) = h;
+                *(qe_s8 *)(to + 4 * 6 * 512 + p * 512) = h;
             }
         }
     }
@@ -463,8 +463,8 @@ __global__ __launch_bounds__(512, sizeof(IN) == 2 && (DK == 64 || __is_same(IN, 
         qe_s8 tf[2][3];
         auto load = [&](const short *w) {
             for (int p = 0; p < 3; ++p) {
-                tf[0][p] = *(const qe_s8 *)(w + wave * 3072 + p * 512 + lane * 8);
-                tf[1][p] = *(const qe_s8 *)(w + wave * 3072 + 1536 + p * 512 + lane * 8);
+                tf[0][p] = *(const qe_s8 *)(w + wave * 6 * 512 + p * 512 + lane * 8);
+                tf[1][p] = *(const qe_s8 *)(w + wave * 6 * 512 + 3 * 512 + p * 512 + lane * 8);
             }
         };
         auto step = [&](const int par, const short *k_s, const IN *v_s, const float *f_s, int t0) {
@@ -567,8 +567,8 @@ __global__ __launch_bounds__(512, sizeof(IN) == 2 && (DK == 64 || __is_same(IN, 
         };
         auto load_m = [&](const short *w, qe_s8 (*mf)[NO]) {
             for (int p = 0; p < NO; ++p) {
-                mf[0][p] = *(const qe_s8 *)(w + 12288 + wave * 3072 + p * 512 + lane * 8);
-                mf[1][p] = *(const qe_s8 *)(w + 12288 + wave * 3072 + 1536 + p * 512 + lane * 8);
+                mf[0][p] = *(const qe_s8 *)(w + 4 * 6 * 512 + wave * 6 * 512 + p * 512 + lane * 8);
+                mf[1][p] = *(const qe_s8 *)(w + 4 * 6 * 512 + wave * 6 * 512 + 3 * 512 + p * 512 + lane * 8);
             }
         };
         IN *out = (IN *)a.out + (size_t)(begin + 16 * wave + 4 * c) * a.out_stride + (size_t)head * DV + col; // the first of the lane's four rows

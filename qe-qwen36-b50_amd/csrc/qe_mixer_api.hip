@@ -93,10 +93,10 @@ void release(qe_attn_ctx *c) {
     delete c;
 }
 
-// Rows of partial results: decode's splits (below QE_ATTN_PART_WGS, each `group` rows) or
+// Rows of partial results: decode's splits (below QE_ATTN_PART_WGS, each room for the rows of the largest group) or
 // prompt's (at most QE_ATTN_WGS tiles of 128 rows).
-size_t part_rows(const qe_attn_desc &d) {
-    const size_t decode = (size_t)QE_ATTN_PART_WGS * (d.q_heads / d.kv_heads), prompt = (size_t)QE_ATTN_WGS * 128;
+size_t part_rows() {
+    const size_t decode = (size_t)QE_ATTN_PART_WGS * QE_ATTN_GROUP_MAX, prompt = (size_t)QE_ATTN_WGS * 128;
     return decode > prompt ? decode : prompt;
 }
 
@@ -182,7 +182,7 @@ int qe_attn_create(int device, const qe_attn_desc *d, qe_attn_ctx **out) {
         axis[i] = d->interleaved ? (i % 3 == 1 && i < 3 * s[1] ? 1 : i % 3 == 2 && i < 3 * s[2] ? 2 : 0) : i < s[0] ? 0 : i < s[0] + s[1] ? 1 : 2;
     }
     hipError_t e = c->err.make();
-    const size_t rows = part_rows(*d);
+    const size_t rows = part_rows();
     if (e == hipSuccess) e = hipMalloc((void **)&c->turns, sizeof turns);
     if (e == hipSuccess) e = hipMalloc((void **)&c->axis, sizeof axis);
     if (e == hipSuccess) e = hipMalloc((void **)&c->part_o, rows * d->head_dim * 4);
