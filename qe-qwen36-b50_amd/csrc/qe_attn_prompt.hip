@@ -2,7 +2,7 @@
 //
 // A workgroup takes 32 query rows for each of its waves, of one sequence and one key-value head
 // (its tokens times the heads that share the key-value head, so that no key is read for one
-// head alone), and steps through the keys 64 at a time.  Per
+// head alone), and steps through the keys 64 (or 32, below) at a time.  Per
 // step S^T = K Q^T and O^T += V^T P^T on v_mfma_f32_32x32x16: a lane's column is one query
 // row, so maximum, sum and rescaling are per lane (plus one exchange between the wave's
 // halves), and the registers that hold S^T's rows are, once rounded, the second product's
@@ -19,11 +19,9 @@
 // Long prompts are bound by the matrix cores, whose issue the exponentials share: 8192 tokens of 16 heads of 256 (550
 // GFLOP), bf16, 515 to 545 us, 1010 to 1070 TFLOP/s where a large library product reaches 1219.  Five
 // prompts of 1999 tokens, 32 heads of 128, fp16: 40 us, the longest row blocks' 18 steps in turn.
-// 100 tokens: 14 us, latency (lengths, pages, two tiles, the output).  Splitting the keys also where tiles fill the
-// GPU was measured too: 80 us for those five prompts.
+// 100 tokens: 12 us, latency (lengths, pages, four steps, the output), much of it the code's first way through the
+// instruction cache: a workgroup whose code was three times as long, in steps of 64 keys with 512 registers, took 15.
 #include "qe_mixer_device.h"
-
-#define BN QE_ATTN_BN
 
 __device__ __forceinline__ int k_swz(int row) { return row & 7; }
 template <int DH>
@@ -41,13 +39,13 @@ __device__ __forceinline__ int lane_now() {
 
 // The page of a wave's part of the tile of BN keys from position k0 on: all of the part's rows lie in one.
 // Rows behind the end may lie in none, then any of the sequence's do (their probabilities are zero).
-template <int WAVES>
+template <int BN, int WAVES>
 __device__ __forceinline__ int page_of(const QeAttnArgs &a, const int32_t *table, int k0, int len, int wave) {
     const int sub = k0 + wave * (BN / WAVES);
     return scalar_load(table + ((sub < len ? sub : len - 1) >> a.page_log2));
 }
 // The part's rows of K or V to LDS.
-template <int DH, int WAVES, bool IS_K>
+template <int DH, int BN, int WAVES, bool IS_K>
 __device__ __forceinline__ void load_part(const QeAttnArgs &a, int page, int kvh, int k0, int len, int wave, short *lds, unsigned *bad) {
     constexpr int CH = DH / 8, ROWS = 64 / CH, PART = BN / WAVES; // chunks of a row, rows of one direct load, rows of a wave
     const int sub = k0 + wave * PART, at = sub < len ? sub : (len - 1) & -PART;
@@ -142,8 +140,9 @@ struct Rows {
     __device__ __forceinline__ void raise(float top) {
         if (__any(top > m + 8.f)) {
             const float mn = fmaxf(m, top), f = m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m - mn);
+            if (__any(m != -INFINITY)) // else nothing is summed yet
 #pragma unroll
-            for (int d = 0; d < DH / 32; ++d) o[d] *= f;
+                for (int d = 0; d < DH / 32; ++d) o[d] *= f;
             l *= f;
             m = mn;
         }
@@ -182,13 +181,13 @@ struct Rows {
 };
 
 // Four waves with heads of up to 128, and two or more workgroups on a CU.  With heads of 256 the tiles fill a CU's LDS, so
-// eight waves (unless the call is too small to need them) are the way to two waves a SIMD, and o and q leave
-// registers for 32 keys' scores at a time, not 64.  (Measured and not kept: the next tile's scores made among this
+// eight waves are the way to two waves a SIMD, and o and q leave registers for 32 keys' scores at a time, not 64; a call
+// too small for eight takes four, in steps of 32 keys, so that two workgroups share a CU there, too.  (Measured and not kept: the next tile's scores made among this
 // one's exponentials, 10 % slower over 4096 tokens of heads of 64 and 128; the second four waves half a tile behind the
 // first, 8 % slower over 8192 of 256; 64 rows a wave, whose 512 registers do not hold them.)
 template <bool BF, int DH, int WAVES>
 __global__ __launch_bounds__(64 * WAVES, 2) void k_attn_prompt(const QeAttnArgs a) {
-    constexpr int BM = 32 * WAVES, PART = BN / WAVES;
+    constexpr int BM = 32 * WAVES, BN = DH == 256 && WAVES == 4 ? 32 : 64, PART = BN / WAVES;
     // two buffers, variables of their own: else the compiler has every LDS read wait for the direct loads in flight
     __shared__ __align__(16) short k_a[BN * DH], v_a[BN * DH], k_b[BN * DH], v_b[BN * DH];
     // rows with an infinity or a NaN in V, of the tiles that some rows attend to in part: from `clear` on, BM tokens at most
@@ -225,10 +224,10 @@ __global__ __launch_bounds__(64 * WAVES, 2) void k_attn_prompt(const QeAttnArgs 
 
     int page = 0; // of the wave's part of the next tile
     if (lo < hi) {
-        page = page_of<WAVES>(a, table, lo * BN, len, wave);
-        load_part<DH, WAVES, true>(a, page, kvh, lo * BN, len, wave, k_a, &bad);
-        load_part<DH, WAVES, false>(a, page, kvh, lo * BN, len, wave, v_a, &bad);
-        page = page_of<WAVES>(a, table, (lo + 1) * BN, len, wave);
+        page = page_of<BN, WAVES>(a, table, lo * BN, len, wave);
+        load_part<DH, BN, WAVES, true>(a, page, kvh, lo * BN, len, wave, k_a, &bad);
+        load_part<DH, BN, WAVES, false>(a, page, kvh, lo * BN, len, wave, v_a, &bad);
+        page = page_of<BN, WAVES>(a, table, (lo + 1) * BN, len, wave);
     }
     Rows<BF, DH> w;
     {
@@ -279,14 +278,14 @@ __global__ __launch_bounds__(64 * WAVES, 2) void k_attn_prompt(const QeAttnArgs 
         lds_barrier(); // the others' loads, too, and no wave reads the other buffers any more
         const int k0 = t * BN;
         if (t + 1 < hi) {
-            load_part<DH, WAVES, true>(a, page, kvh, k0 + BN, len, wave, k_next, &bad);
-            load_part<DH, WAVES, false>(a, page, kvh, k0 + BN, len, wave, v_next, &bad);
+            load_part<DH, BN, WAVES, true>(a, page, kvh, k0 + BN, len, wave, k_next, &bad);
+            load_part<DH, BN, WAVES, false>(a, page, kvh, k0 + BN, len, wave, v_next, &bad);
         }
-        page = page_of<WAVES>(a, table, k0 + 2 * BN, len, wave); // looked up a step before it is needed
+        page = page_of<BN, WAVES>(a, table, k0 + 2 * BN, len, wave); // looked up a step before it is needed
         if (k0 >= wave_keys) return;
         constexpr int KB = DH == 256 ? 1 : 2;
 #pragma unroll
-        for (int b = 0; b < 2; b += KB) {
+        for (int b = 0; b < BN / 32; b += KB) {
             Scores<KB> s;
             w.scores(k_lds, b, s);
             schedule<4, KB * DH / 16, 1>();

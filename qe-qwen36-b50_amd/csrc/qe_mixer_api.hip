@@ -266,7 +266,7 @@ int qe_attn_prompt(qe_attn_ctx *c, const qe_attn_batch *b, const qe_kv_cache *kv
     const int bm = qe_attn_prompt_rows(b->n_tokens, b->n_seqs, a.group, a.kv_heads, c->d.head_dim);
     a.tiles = qe_attn_max_tiles(b->n_tokens, b->n_seqs, a.group, bm);
     const int64_t most = (int64_t)b->max_pages * c->d.page;
-    a.splits = qe_attn_prompt_splits((int64_t)a.tiles * a.kv_heads, b->max_len && b->max_len < most ? b->max_len : most, c->d.head_dim);
+    a.splits = qe_attn_prompt_splits((int64_t)a.tiles * a.kv_heads, b->max_len && b->max_len < most ? b->max_len : most);
     OnDevice on(c->device);
     HIP_TRY(on.e);
     HIP_TRY(qe_launch_attn_prompt(a, c->d.head_dim, c->d.type, bm, (hipStream_t)stream));

@@ -12,7 +12,6 @@
 // ---- attention ----------------------------------------------------------------
 #define QE_ATTN_SUB 16     /* keys that share one page lookup: the smallest page */
 #define QE_ATTN_TILE 32    /* keys of a decode wave's step */
-#define QE_ATTN_BN 64      /* keys of a prompt workgroup's step */
 #define QE_ATTN_WGS 512    /* workgroups a prompt call is split up to: two for each of the 256 CUs */
 #define QE_ATTN_DECODE_WGS 2048 /* and a decode call at most */
 #define QE_ATTN_DECODE_SPLITS 1024
@@ -62,18 +61,17 @@ QE_MIX_HD int qe_attn_max_tiles(int n_tokens, int n_seqs, int group, int bm) {
     return (int)((int64_t)n_tokens * group / bm) + n_seqs;
 }
 
-// Rows of a prompt workgroup.  With heads of 256 its K and V tiles fill a CU's LDS, so eight
-// waves are the way to two waves a SIMD; with smaller heads several workgroups of four share a CU.
+// Rows of a prompt workgroup.  With heads of 256 and 64 keys a step its K and V tiles fill a CU's LDS, so eight
+// waves are the way to two waves a SIMD; calls with too few rows for that, and smaller heads, take four.
 QE_MIX_HD int qe_attn_prompt_rows(int n_tokens, int n_seqs, int group, int kv_heads, int head_dim) {
     return head_dim == 256 && (int64_t)qe_attn_max_tiles(n_tokens, n_seqs, group, 256) * kv_heads >= 256 ? 256 : 128;
 }
 
-// Splits of a prompt call's keys: none if its tiles fill half the CUs, else as many workgroups as the GPU
-// holds at once (one a CU with heads of 256, whose LDS they fill: 54 us for 1000 tokens of 16 such heads, 61 with two),
-// of at least 256 keys.
-QE_MIX_HD int qe_attn_prompt_splits(int64_t tiles, int64_t max_len, int head_dim) {
+// Splits of a prompt call's keys: none if its tiles fill half the CUs (528 tiles in two splits: 80 us, 50 in one), else
+// two workgroups for each CU, of at least 256 keys.
+QE_MIX_HD int qe_attn_prompt_splits(int64_t tiles, int64_t max_len) {
     if (tiles > 128) return 1;
-    const int64_t most = (max_len + 255) / 256, want = (head_dim == 256 ? QE_ATTN_WGS / 2 : QE_ATTN_WGS) / tiles;
+    const int64_t most = (max_len + 255) / 256, want = QE_ATTN_WGS / tiles;
     const int64_t s = want < most ? want : most;
     return s < 1 ? 1 : (int)s;
 }

@@ -15,7 +15,7 @@ extern "C" {
 void decode_plan(long seqs, long heads, int dim, long len, int *steps, int *splits) { qe_attn_decode_plan(seqs, heads, dim, len, steps, splits); }
 int decode_steps(int len, int steps, int splits) { return qe_attn_decode_steps(len, steps, splits); }
 int decode_active(int len, int steps) { return qe_attn_decode_active(len, steps); }
-int prompt_splits(long tiles, long len, int dim) { return qe_attn_prompt_splits(tiles, len, dim); }
+int prompt_splits(long tiles, long len) { return qe_attn_prompt_splits(tiles, len); }
 int first_tile(int cu, int i, int g, int bm) { return qe_attn_first_tile(cu, i, g, bm); }
 int max_tiles(int n, int s, int g, int bm) { return qe_attn_max_tiles(n, s, g, bm); }
 int first_chunk(int cu, int i) { return qe_delta_first_chunk(cu, i); }
@@ -39,7 +39,7 @@ def plan(tmp_path_factory):
     subprocess.run(["g++", "-shared", "-fPIC", "-std=c++17", "-Wall", "-Wno-unused-function", "-I", os.path.join(PKG, "csrc"),
                     str(d / "shim.cpp"), "-o", str(d / "shim.so")], check=True)
     lib = ctypes.CDLL(str(d / "shim.so"))
-    lib.prompt_splits.argtypes = [ctypes.c_long, ctypes.c_long, ctypes.c_int]
+    lib.prompt_splits.argtypes = [ctypes.c_long, ctypes.c_long]
     lib.decode_plan.argtypes = [ctypes.c_long, ctypes.c_long, ctypes.c_int, ctypes.c_long, ctypes.c_void_p, ctypes.c_void_p]
     lib.slot_pair.argtypes = [ctypes.c_long, ctypes.c_int, ctypes.c_int]
     return lib
@@ -73,8 +73,8 @@ def test_partial_results_fit_their_scratch(plan):
             assert 1 <= s <= plan.decode_splits() and steps >= 2
             assert s == 1 or (seqs * heads < plan.decode_wgs() and seqs * heads * s <= plan.part_wgs())
     for tiles in list(range(1, 1200)) + [1 << 28]:
-        for n, dim in itertools.product(lens, (64, 256)):
-            s = plan.prompt_splits(tiles, n, dim)
+        for n in lens:
+            s = plan.prompt_splits(tiles, n)
             assert s >= 1 and (s == 1 or tiles * s <= plan.wgs())
 
 
