@@ -339,26 +339,33 @@ __global__ __launch_bounds__(256, 2) void k_attn_decode(const QeAttnArgs a) {
             const bool any = x[s].y != 0.f;
             const float f = x[s].x == -INFINITY ? 0.f : __builtin_amdgcn_exp2f((x[s].x - top) * a.scale_log2);
             sum += any ? f * x[s].y : 0.f;
-            weight[s * 16 + tid] = any ? f : -1.f; // -1: nothing of that split is used
+            weight[s * 16 + tid] = any ? f : 0.f; // a split without sum has left zeros
         }
         sums[tid] = none ? -1.f : sum;
     }
     __syncthreads();
     // a thread's 16 bytes of a row, all splits' in flight
     const int n = a.group * (DH / 4);
+    const float *none = (const float *)(a.arrived + QE_ATTN_DECODE_WGS);
     for (int i = tid; i < n; i += 256) {
         const int h = i / (DH / 4), d = i % (DH / 4) * 4;
         const float *p = a.part_o + (row0 + h) * DH + d;
         qe_f4 o[QE_ATTN_JOIN];
-        if (near_all) {
 #pragma unroll
-            for (int s = 0; s < QE_ATTN_JOIN; ++s) o[s] = *(const qe_f4 *)(p + (s < active ? s : 0) * G * DH); // behind the last the first again, unused
-        } else {
+        for (int g = 0; g < QE_ATTN_JOIN; g += 4) {
+            if (g >= active) { // uniform
+                o[g] = o[g + 1] = o[g + 2] = o[g + 3] = qe_f4{0, 0, 0, 0};
+                continue;
+            }
 #pragma unroll
-            for (int s = 0; s < QE_ATTN_JOIN; ++s) {
-                const float *at = p + (s < active ? s : 0) * G * DH;
-                const qe_f2 x = load_through(at), y = load_through(at + 2);
-                o[s] = qe_f4{x[0], x[1], y[0], y[1]};
+            for (int s = g; s < g + 4; ++s) {
+                const float *at = s < active ? p + s * G * DH : none; // behind the last zeros
+                if (near_all) {
+                    o[s] = *(const qe_f4 *)at;
+                } else {
+                    const qe_f2 x = load_through(at), y = load_through(at + 2);
+                    o[s] = qe_f4{x[0], x[1], y[0], y[1]};
+                }
             }
         }
         float f[QE_ATTN_JOIN];
@@ -367,7 +374,7 @@ __global__ __launch_bounds__(256, 2) void k_attn_decode(const QeAttnArgs a) {
         qe_f4 r = {0, 0, 0, 0};
 #pragma unroll
         for (int s = 0; s < QE_ATTN_JOIN; ++s)
-            for (int j = 0; j < 4; ++j) r[j] += s < active && !(f[s] < 0.f) ? f[s] * o[s][j] : 0.f;
+            for (int j = 0; j < 4; ++j) r[j] = fmaf(f[s], o[s][j], r[j]);
         const float sum = sums[h];
         r *= sum == 0.f ? 0.f : 1.f / sum;
         if (sum < 0.f) r = qe_f4{0, 0, 0, 0};

@@ -187,9 +187,9 @@ int qe_attn_create(int device, const qe_attn_desc *d, qe_attn_ctx **out) {
     if (e == hipSuccess) e = hipMalloc((void **)&c->axis, sizeof axis);
     if (e == hipSuccess) e = hipMalloc((void **)&c->part_o, rows * d->head_dim * 4);
     if (e == hipSuccess) e = hipMalloc((void **)&c->part_ml, rows * sizeof(float2));
-    if (e == hipSuccess) e = hipMalloc((void **)&c->arrived, QE_ATTN_DECODE_WGS * sizeof(unsigned long long));
+    if (e == hipSuccess) e = hipMalloc((void **)&c->arrived, (QE_ATTN_DECODE_WGS + 2) * sizeof(unsigned long long));
     const bool oom = e == hipErrorOutOfMemory;
-    if (e == hipSuccess) e = hipMemset(c->arrived, 0, QE_ATTN_DECODE_WGS * sizeof(unsigned long long));
+    if (e == hipSuccess) e = hipMemset(c->arrived, 0, (QE_ATTN_DECODE_WGS + 2) * sizeof(unsigned long long));
     if (e == hipSuccess) e = hipDeviceSynchronize();
     if (e == hipSuccess && pairs) {
         e = hipMemcpy(c->turns, turns, pairs * sizeof(double), hipMemcpyHostToDevice);
