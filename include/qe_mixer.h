@@ -91,7 +91,7 @@ typedef struct {
     const int32_t *kv_len; /* [n_seqs], each 0 .. max_pages * page */
     const int32_t *table;  /* page ids, sequence i's at table + i * table_stride */
     int table_stride;      /* >= max_pages */
-    int max_pages;         /* columns of the table, >= 1; max_pages * page < 2^31 */
+    int max_pages;         /* columns of the table, >= 1; max_pages * page <= 2^30 */
     int max_len;           /* the longest kv_len as far as the host knows, for choosing how a call is split (results do
                               not depend on it but for rounding); 0 = max_pages * page */
 } qe_attn_batch;

@@ -9,7 +9,8 @@
 // and pair, in LDS, for all of its heads.  A work item is 16 elements of a head: 8 pairs,
 // or 16 elements behind the rotated ones.  Bound by memory: q, k and v read and written.  8192
 // tokens of 32 + 2 x 8 heads of 128, fp16, 201 MB: 31 us, 6.4 TB/s (a large copy here reaches 5.1; part of
-// it stays in the last-level cache).  8 tokens: 4 us, of which most is the launch.
+// it stays in the last-level cache).  8 tokens: 4 us, of which most is the launch.  Stores that pass the caches by
+// save 2 of 40 us between calls on other data, and cost the attention that follows, which reads these rows, more.
 // ---------------------------------------------------------------------------
 template <typename IN>
 __device__ __forceinline__ void load8(const IN *p, float *x) {
@@ -146,7 +147,7 @@ __device__ __forceinline__ int v_swizzle(int row) { // of the 16-byte chunk inde
     return DH == 64 ? ((row >> 1) & 1) << 2 : (row & 3) << 2;
 }
 
-template <bool BF, int DH>
+template <bool BF, int DH, bool ONCE>
 __global__ __launch_bounds__(256, 2) void k_attn_decode(const QeAttnArgs a) {
     constexpr int CH = DH / 8;       // 16-byte chunks of a row
     constexpr int ROWS = 64 / CH;    // rows of one direct load
@@ -179,6 +180,8 @@ __global__ __launch_bounds__(256, 2) void k_attn_decode(const QeAttnArgs a) {
     for (int d = 0; d < DB; ++d) acc[d] = qe_f4{0, 0, 0, 0};
     float m = -INFINITY, l = 0;
     short *vb = v_lds[wave];
+    // keys and values of a call that exceed the L2s pass through them (qe_attn_decode_once)
+    auto load_k = [](const short *p) { return ONCE ? __builtin_nontemporal_load((const qe_s8 *)p) : *(const qe_s8 *)p; };
     const int tr_row = col >> 2, tr_el = (col & 3) * 4; // of a transposing read
     for (int t = lo + wave; t < hi; t += 4) {
         const int k0 = t * QE_ATTN_TILE;
@@ -192,14 +195,14 @@ __global__ __launch_bounds__(256, 2) void k_attn_decode(const QeAttnArgs a) {
         qe_s8 kf[2][KS];
         const short *kp0 = (const short *)a.kc + (r0 + col) * DH + c * 8, *kp1 = (const short *)a.kc + (r1 + col) * DH + c * 8;
 #pragma unroll
-        for (int s = 0; s < KS; ++s) kf[0][s] = *(const qe_s8 *)(kp0 + s * 32);
+        for (int s = 0; s < KS; ++s) kf[0][s] = load_k(kp0 + s * 32);
 #pragma unroll
-        for (int s = 0; s < KS; ++s) kf[1][s] = *(const qe_s8 *)(kp1 + s * 32);
+        for (int s = 0; s < KS; ++s) kf[1][s] = load_k(kp1 + s * 32);
 #pragma unroll
         for (int i = 0; i < QE_ATTN_TILE / ROWS; ++i) {
             const int row = i * ROWS + lane / CH, ch = (lane % CH) ^ v_swizzle<DH>(row);
             const size_t base = (i * ROWS < 16 ? r0 : r1) + (row & 15);
-            load_lds16((const short *)a.vc + base * DH + ch * 8, vb + i * 512);
+            load_lds16<ONCE>((const short *)a.vc + base * DH + ch * 8, vb + i * 512);
         }
         qe_f4 s[2] = {qe_f4{0, 0, 0, 0}, qe_f4{0, 0, 0, 0}};
 #pragma unroll
@@ -455,7 +458,8 @@ __global__ __launch_bounds__(1024) void k_attn_join(const QeAttnArgs a) {
 template <bool BF, int DH>
 static hipError_t launch_decode(const QeAttnArgs &a, hipStream_t st) {
     const unsigned units = (unsigned)(a.n_seqs * a.kv_heads), whole = a.splits > 1 && a.splits <= QE_ATTN_JOIN ? (units + 7) / 8 * 8 : units;
-    k_attn_decode<BF, DH><<<dim3(whole * a.splits), dim3(256), 0, st>>>(a);
+    if (a.once) k_attn_decode<BF, DH, true><<<dim3(whole * a.splits), dim3(256), 0, st>>>(a);
+    else k_attn_decode<BF, DH, false><<<dim3(whole * a.splits), dim3(256), 0, st>>>(a);
     if (a.splits > QE_ATTN_JOIN) k_attn_join<BF, DH><<<dim3((unsigned)(a.n_seqs * a.q_heads * (DH / 64))), dim3(1024), 0, st>>>(a);
     return hipGetLastError();
 }

@@ -117,8 +117,10 @@ __global__ __launch_bounds__(256) void k_delta_slots(const QeDeltaArgs a) {
 // One token per sequence: a workgroup per (sequence, value head, 32 columns of its state),
 // a thread 4 columns of DK / 32 rows.  S^T k and S^T q are summed in the one pass over the old
 // state that it needs (S'^T q = e^g S^T q + (k . q) u), so the state is read once, kept
-// in registers and written once.  Bound by memory: 64 sequences of 32 heads of 128 x 128, 270 MB: 46 us,
-// 5.9 TB/s (a large copy reaches 5.1; part of it stays in the last-level cache).  One sequence: 5 us, latency.
+// in registers and written once.  Bound by memory: 64 sequences of 32 heads of 128 x 128, 270 MB: 51 us,
+// 5.3 TB/s (a large copy reaches 5.1).  One sequence: 5 us, latency.  States pass the caches by: until the next
+// token the other layers' come through them.  Per call on states of many layers in turn: 16 sequences 19.2 -> 13.5 us, 64
+// 58.9 -> 53.5; on the same states over and over 15.1 -> 12.7 and 47.7 -> 50.7.
 // ---------------------------------------------------------------------------
 template <typename IN, int DK, int DV>
 __global__ __launch_bounds__(256) void k_delta_decode(const QeDeltaArgs a) {
@@ -139,7 +141,7 @@ __global__ __launch_bounds__(256) void k_delta_decode(const QeDeltaArgs a) {
     }
     qe_f4 s[ROWS];
     const float *from = a.pool + ((size_t)(in_i < 0 ? 0 : in_i) * a.v_heads + head) * DK * DV;
-    for (int i = 0; i < ROWS; ++i) s[i] = in_i < 0 ? qe_f4{0, 0, 0, 0} : *(const qe_f4 *)(from + (size_t)(row + 32 * i) * DV + col);
+    for (int i = 0; i < ROWS; ++i) s[i] = in_i < 0 ? qe_f4{0, 0, 0, 0} : __builtin_nontemporal_load((const qe_f4 *)(from + (size_t)(row + 32 * i) * DV + col));
 
     float x = 0, y = 0;
     if (tid < DK) {
@@ -172,7 +174,7 @@ __global__ __launch_bounds__(256) void k_delta_decode(const QeDeltaArgs a) {
     const qe_f4 u = beta * (v - rk * sk);
     if (out_i >= 0) {
         float *to = a.pool + ((size_t)out_i * a.v_heads + head) * DK * DV;
-        for (int i = 0; i < ROWS; ++i) *(qe_f4 *)(to + (size_t)(row + 32 * i) * DV + col) = s[i] + (rk * qk[1][row + 32 * i]) * u;
+        for (int i = 0; i < ROWS; ++i) __builtin_nontemporal_store(s[i] + (rk * qk[1][row + 32 * i]) * u, (qe_f4 *)(to + (size_t)(row + 32 * i) * DV + col));
     }
     if (tid < 8) {
         sq = (red[0][1][tid] + red[1][1][tid]) + (red[2][1][tid] + red[3][1][tid]);

@@ -107,7 +107,7 @@ int check_batch(const qe_attn_ctx *c, const qe_attn_batch *b, const qe_kv_cache 
     if (!b->cu_q && b->n_tokens != b->n_seqs)
         return qe_fail(QE_ERR_ARG, "%s: without cu_q n_tokens (%d) is n_seqs (%d)", where, b->n_tokens, b->n_seqs);
     if (!b->kv_len || !b->table) return qe_fail(QE_ERR_ARG, "%s: null kv_len or table", where);
-    if (b->max_pages < 1 || (int64_t)b->max_pages * c->d.page >= (int64_t)1 << 31 || b->table_stride < b->max_pages)
+    if (b->max_pages < 1 || (int64_t)b->max_pages * c->d.page > 1 << 30 || b->table_stride < b->max_pages)
         return qe_fail(QE_ERR_ARG, "%s: max_pages %d (of %d positions), table_stride %d", where, b->max_pages, c->d.page, b->table_stride);
     if (b->max_len < 0) return qe_fail(QE_ERR_ARG, "%s: max_len %d", where, b->max_len);
     if (!kv->k || !kv->v || !aligned16(kv->k) || !aligned16(kv->v))
@@ -280,7 +280,9 @@ int qe_attn_decode(qe_attn_ctx *c, const qe_attn_batch *b, const qe_kv_cache *kv
     if (rc != QE_OK) return rc;
     QeAttnArgs a = attn_args(c, b, kv, q, q_stride, out, out_stride);
     const int64_t most = (int64_t)b->max_pages * c->d.page;
-    qe_attn_decode_plan(b->n_seqs, a.kv_heads, c->d.head_dim, b->max_len && b->max_len < most ? b->max_len : most, &a.steps, &a.splits);
+    const int64_t max_len = b->max_len && b->max_len < most ? b->max_len : most;
+    qe_attn_decode_plan(b->n_seqs, a.kv_heads, c->d.head_dim, max_len, &a.steps, &a.splits);
+    a.once = qe_attn_decode_once(b->n_seqs, a.kv_heads, c->d.head_dim, max_len);
     OnDevice on(c->device);
     HIP_TRY(on.e);
     HIP_TRY(qe_launch_attn_decode(a, c->d.head_dim, c->d.type, (hipStream_t)stream));

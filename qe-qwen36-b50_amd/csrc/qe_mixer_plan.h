@@ -47,6 +47,12 @@ QE_MIX_HD int qe_attn_decode_steps(int len, int steps, int splits) {
     return need > steps ? need : steps;
 }
 QE_MIX_HD int qe_attn_decode_active(int len, int steps) { return ((len + QE_ATTN_TILE - 1) / QE_ATTN_TILE + steps - 1) / steps; }
+// Whether a decode call's keys and values exceed the eight L2s of 4 MB and pass through them (per call, on data of ten
+// layers in turn: 8 x 2000 keys of 8 heads of 128, 65 MB, 20.2 -> 19.1 us; 100,000 keys of 2 of 256, 205 MB, 45.4 -> 42.5; but
+// 8000 of these, 16 MB, 12.8 -> 13.6, which stay).
+QE_MIX_HD bool qe_attn_decode_once(int64_t n_seqs, int64_t kv_heads, int head_dim, int64_t max_len) {
+    return n_seqs * kv_heads * head_dim * 4 >= ((int64_t)32 << 20) / (max_len > 0 ? max_len : 1);
+}
 // Partial results that a decode call can need: with more than one split units < QE_ATTN_DECODE_WGS, and
 // units * splits < QE_ATTN_DECODE_WGS + units.
 #define QE_ATTN_PART_WGS (2 * QE_ATTN_DECODE_WGS)

@@ -392,6 +392,10 @@ def test_refusals():
         qe_mixer.Batch(ints([1, 2]).long(), c.table)
     with pytest.raises(ValueError):
         qe_mixer.Batch(ints([1, 2]), c.table, ints([0, 1]))
+    b = c.batch()
+    b.c.max_pages = b.c.table_stride = (1 << 30) // 32 + 1
+    with pytest.raises(qe_moe.QeError, match="max_pages"):
+        a.decode(b, q, c.kc, c.vc, out)
     a.check()
 
 

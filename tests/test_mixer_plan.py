@@ -24,6 +24,7 @@ void split_range(int n, int splits, int s, int *lo, int *hi) { qe_split_range(n,
 int checked(int v, int lo, int hi, int other, unsigned *bad) { return qe_checked(v, lo, hi, other, bad); }
 int slot_pair(long n, int a, int b) { return qe_slot_pair(n, a, b); }
 int slot_conflict(int i, int oi, int j, int ij, int oj) { return qe_slot_conflict(i, oi, j, ij, oj); }
+int decode_once(long s, long h, int d, long n) { return qe_attn_decode_once(s, h, d, n); }
 int wgs() { return QE_ATTN_WGS; }
 int decode_wgs() { return QE_ATTN_DECODE_WGS; }
 int decode_splits() { return QE_ATTN_DECODE_SPLITS; }
@@ -41,6 +42,7 @@ def plan(tmp_path_factory):
     lib = ctypes.CDLL(str(d / "shim.so"))
     lib.prompt_splits.argtypes = [ctypes.c_long, ctypes.c_long]
     lib.decode_plan.argtypes = [ctypes.c_long, ctypes.c_long, ctypes.c_int, ctypes.c_long, ctypes.c_void_p, ctypes.c_void_p]
+    lib.decode_once.argtypes = [ctypes.c_long, ctypes.c_long, ctypes.c_int, ctypes.c_long]
     lib.slot_pair.argtypes = [ctypes.c_long, ctypes.c_int, ctypes.c_int]
     return lib
 
@@ -63,6 +65,16 @@ def test_decode_workgroups_cover_every_length(plan):
                 assert mine >= steps and active <= splits and active * mine >= tiles and (active - 1) * mine < max(tiles, 1)
                 if n <= told:
                     assert mine == steps
+
+
+def test_large_calls_pass_the_caches_by(plan):
+    for seqs, heads, dim in itertools.product((1, 2, 7, 24, 65535), (1, 8, 256), (64, 128, 256)):
+        for n in (0, 1, 700, 8192, 100000, 1 << 30):
+            size = seqs * heads * dim * 4 * n  # of the keys and values, two bytes each
+            if size >= 32 << 20:
+                assert plan.decode_once(seqs, heads, dim, n)
+            elif size < 16 << 20 and seqs * heads * dim * 4 < 32 << 20:
+                assert not plan.decode_once(seqs, heads, dim, n)
 
 
 def test_partial_results_fit_their_scratch(plan):
