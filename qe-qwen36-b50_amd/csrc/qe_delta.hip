@@ -232,7 +232,7 @@ __global__ __launch_bounds__(256, 3) void k_delta_chunks(const QeDeltaArgs a) {
     __shared__ double b_s[64]; // in powers of two, as the hardware's exponential takes them
     __shared__ float kk_s[64], rk_s[64], rq_s[64], beta_s[64];
     const int tid = threadIdx.x, wave = tid >> 6, lane = tid & 63, r = lane & 15, c = lane >> 4;
-    const int chunk = blockIdx.x / a.k_heads, kh = blockIdx.x % a.k_heads;
+    const int parts = a.v_heads / a.heads, chunk = blockIdx.x / parts, head0 = blockIdx.x % parts * a.heads, kh = head0 / a.group;
     int seq = 0;
     for (int hi = a.n_seqs; hi - seq > 1;) {
         const int mid = (seq + hi) >> 1;
@@ -248,6 +248,11 @@ __global__ __launch_bounds__(256, 3) void k_delta_chunks(const QeDeltaArgs a) {
 
     const IN *q = (const IN *)a.q + (size_t)kh * DK + 8 * c, *k = (const IN *)a.k + (size_t)kh * DK + 8 * c;
     const int row = 16 * wave + r;
+    // the next head's, loaded a head ahead (the first's too, unless fp32's planes need the registers); behind the end the
+    // last token's, unused
+    const size_t gate = (size_t)(t0 + (lane < n ? lane : n - 1)) * a.v_heads + head0;
+    float g_next = 0, beta_next = 0;
+    if constexpr (NP < 3) g_next = a.g[gate], beta_next = a.beta[gate];
     qe_f4 gk[4], gq[4]; // K K^T and Q K^T, blocks 0 .. wave of the wave's rows
     {
         qe_s8 kr[KS][NP], qr[KS][NP];
@@ -259,7 +264,7 @@ __global__ __launch_bounds__(256, 3) void k_delta_chunks(const QeDeltaArgs a) {
             for (int i = 0; i < NP; ++i) {
                 const int at = (i * 64 + row) * DK + (((4 * s + c) ^ key_swz<DK>(row)) << 3);
                 *(qe_s8 *)(k_s + at) = kr[s][i];
-                if constexpr (NP > 1) {
+                if constexpr (NP > 1) { // (every workgroup of the key head writes the same)
                     short *ws = a.ws_kq + ((size_t)chunk * a.k_heads + kh) * 2 * NP * 64 * DK;
                     *(qe_s8 *)(ws + at) = kr[s][i];
                     *(qe_s8 *)(ws + NP * 64 * DK + ((wave * KS + s) * NP + i) * 512 + lane * 8) = qr[s][i];
@@ -291,15 +296,17 @@ __global__ __launch_bounds__(256, 3) void k_delta_chunks(const QeDeltaArgs a) {
             gq[cb] = q3[0] + (q3[1] + q3[2]);
         }
     }
-    for (int gi = 0; gi < a.group; ++gi) {
-        const int head = kh * a.group + gi;
+    if constexpr (NP == 3) g_next = a.g[gate], beta_next = a.beta[gate];
+    for (int gi = 0; gi < a.heads; ++gi) {
+        const int head = head0 + gi;
         float *ws = a.ws + ((size_t)chunk * a.v_heads + head) * QE_DELTA_WS, *factors = ws + QE_DELTA_WS - 256;
-        double b = lane < n ? (double)log_decay(a.g[(size_t)(t0 + lane) * a.v_heads + head]) * 1.4426950408889634 : 0.0;
+        double b = lane < n ? (double)log_decay(g_next) * 1.4426950408889634 : 0.0;
+        float beta = lane < n ? beta_next : 0.f;
+        if (gi + 1 < a.heads) g_next = a.g[gate + gi + 1], beta_next = a.beta[gate + gi + 1];
         for (int d = 1; d < 64; d <<= 1) {
             const double up = __shfl_up(b, d);
             if (lane >= d) b += up;
         }
-        float beta = lane < n ? a.beta[(size_t)(t0 + lane) * a.v_heads + head] : 0.f;
         __syncthreads(); // rk_s and rq_s are written, K is read; the last head's b_s, beta_s, T and M are read
         // A product of 0 and an infinity or NaN is NaN, and in a block above the diagonal's zeros it would
         // reach tokens before its own.  So from the first token whose key, gate or decay is not finite on
@@ -321,15 +328,25 @@ __global__ __launch_bounds__(256, 3) void k_delta_chunks(const QeDeltaArgs a) {
             if (lane == 0) factors[192] = __builtin_amdgcn_exp2f((float)last) + (fine < 64 ? NAN : 0.f);
         }
         __syncthreads();
+        double b_i[4], b_j[4]; // all read at once, and values that are not wanted dropped after: no branches around LDS reads
+        float q_i[4], k_i[4], k_j[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const int ri = 16 * wave + 4 * c + i, cj = 16 * i + r;
+            b_i[i] = b_s[ri], b_j[i] = b_s[cj];
+            q_i[i] = rq_s[ri], k_i[i] = rk_s[ri] * beta_s[ri], k_j[i] = rk_s[cj];
+        }
 #pragma unroll
         for (int cb = 0; cb < 4; ++cb) {
             if (cb > (wave | 1)) continue; // and zeros to the right of the diagonal in its 32 columns
+#pragma unroll
             for (int i = 0; i < 4; ++i) {
                 const int ri = 16 * wave + 4 * c + i, cj = 16 * cb + r;
                 const bool in = cb <= wave && cj <= ri && ri < fine;
-                const float fade = in ? __builtin_amdgcn_exp2f((float)(b_s[ri] - b_s[cj])) * rk_s[cj] : 0.f;
-                M[ri * LD + cj] = in ? gq[cb][i] * fade * rq_s[ri] : 0.f;
-                A[ri * LD + cj] = in && cj < ri ? gk[cb][i] * fade * (rk_s[ri] * beta_s[ri]) : 0.f;
+                const float fade = __builtin_amdgcn_exp2f((float)(b_i[i] - b_j[cb])) * k_j[cb];
+                const float m = gq[cb][i] * fade * q_i[i], x = gk[cb][i] * fade * k_i[i];
+                M[ri * LD + cj] = in ? m : 0.f;
+                A[ri * LD + cj] = in && cj < ri ? x : 0.f;
                 if (cb > wave) T[ri * LD + cj] = 0.f;
             }
         }
@@ -637,7 +654,8 @@ static hipError_t prompt(QeDeltaArgs a, hipStream_t st) {
     const unsigned chunks = (unsigned)qe_delta_max_chunks(a.n_tokens, a.n_seqs);
     if (a.n_seqs <= 256) a.skip = nullptr;
     else k_delta_slots<<<dim3((unsigned)a.n_seqs), dim3(256), 0, st>>>(a);
-    k_delta_chunks<IN, DK><<<dim3(chunks * a.k_heads), dim3(256), 0, st>>>(a);
+    a.heads = qe_delta_heads(chunks, a.v_heads, a.group);
+    k_delta_chunks<IN, DK><<<dim3(chunks * (a.v_heads / a.heads)), dim3(256), 0, st>>>(a);
     k_delta_scan<IN, DK, DV><<<dim3((unsigned)a.n_seqs * a.v_heads * (DV / 16)), dim3(512), 0, st>>>(a);
     return hipGetLastError();
 }

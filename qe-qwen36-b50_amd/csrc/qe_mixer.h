@@ -55,6 +55,7 @@ struct QeDeltaArgs {
     const int32_t *slots_in, *slots_out, *cu;
     int n_seqs, n_tokens, k_heads, v_heads, group;
     int l2norm;
+    int heads; // prompt: see qe_delta_heads
     float scale;
     float *ws;           // [chunk][v_head][QE_DELTA_WS]: see qe_delta.hip
     short *ws_kq;        // [chunk][k_head][K, Q][plane][64][dim_k], for types of more than one plane

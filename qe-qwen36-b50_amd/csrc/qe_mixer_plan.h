@@ -107,6 +107,10 @@ QE_MIX_HD int qe_checked(int v, int lo, int hi, int other, unsigned *bad) {
 QE_MIX_HD int qe_delta_first_chunk(int cu, int i) { return cu / QE_DELTA_C + i; }
 // 16-bit planes that keys and queries are cut into and kept as; bf16 ones are one as they stand.
 QE_MIX_HD int qe_delta_kept_planes(int bytes, int is_bf16) { return is_bf16 ? 0 : bytes == 4 ? 3 : 2; }
+// Value heads of a workgroup that makes a chunk's matrices: all of the key head's, which share the products of keys and
+// queries, unless a workgroup for each is no more than the GPU holds at once, three a CU (one bf16 chunk of 16 and 32
+// heads: 10 us, and 14 with two heads a workgroup).
+QE_MIX_HD int qe_delta_heads(int64_t chunks, int v_heads, int group) { return chunks * v_heads <= 768 ? 1 : group; }
 QE_MIX_HD int qe_delta_max_chunks(int n_tokens, int n_seqs) { return n_tokens / QE_DELTA_C + n_seqs; }
 
 // Whether sequence i of a call may be computed: its slots are in the pool (or -1), and nobody
