@@ -193,7 +193,7 @@ __global__ __launch_bounds__(256) void k_delta_decode(const QeDeltaArgs a) {
 // are not written), then per token e^b / |k|, scale e^b / |q|, e^(b_last - b) / |k|, and
 // e^(b_last).  fp16 and fp32 keys and queries are cut into planes here too, for a chunk and key
 // head: K [plane][64][DK] as it lies in LDS, Q [wave][32 of DK][plane][lane][8].
-// 8192 bf16 tokens of 16 key and 32 value heads of 128: 68 us, against 52 for its reads and writes at a large copy's
+// 8192 bf16 tokens of 16 key and 32 value heads of 128: 66 us, against 52 for its reads and writes at a large copy's
 // rate; the rest is the barriers between a head's short steps.
 // ---------------------------------------------------------------------------
 template <int DK>
@@ -220,7 +220,7 @@ __device__ __forceinline__ void load8_planes(const IN *p, bool there, qe_s8 *h, 
 }
 
 // (Three workgroups a CU, as the LDS allows: 1999 fp32 tokens of 16 and 32 heads of 128 take 37 us, with the registers
-// of two 51.)
+// of two 51.  One chunk: 10 us, its steps' latency.)
 template <typename IN, int DK>
 __global__ __launch_bounds__(256, 3) void k_delta_chunks(const QeDeltaArgs a) {
     constexpr int LD = 68, KS = DK / 32, NP = planes_of<IN>(), NO = sizeof(IN) == 4 ? 3 : 2;
@@ -421,7 +421,7 @@ __global__ __launch_bounds__(256, 3) void k_delta_chunks(const QeDeltaArgs a) {
 // the state's update and S to LDS 1,150, the rest is barriers); 1999 fp32 tokens of three prompts 90 us.
 // ---------------------------------------------------------------------------
 // Where the LDS holds two workgroups (bf16, and fp16 keys of 64), 128 registers let it: sequences side by side overlap
-// (16 of 500 tokens, bf16: 355 us the call with one a CU, 296 with two; one of 8192 has one a CU and takes 319 in both forms).
+// (16 of 500 tokens, bf16: 355 us the call with one a CU, 296 with two; one of 8192 has one a CU, and takes the same in both forms).
 template <typename IN, int DK, int DV>
 __global__ __launch_bounds__(512, sizeof(IN) == 2 && (DK == 64 || __is_same(IN, __bf16)) ? 4 : 2) void k_delta_scan(const QeDeltaArgs a) {
     constexpr int KS = DK / 32, SB = DK / 64, LS = DK + 8, LT = 72, NP = planes_of<IN>(), NO = sizeof(IN) == 4 ? 3 : 2;
