@@ -220,6 +220,27 @@ def test_prompt_values_that_are_not_finite_reach_their_rows_only(dim, dtype):
         assert torch.equal(out[:at], clean[:at]) and torch.equal(out[:, :2], clean[:, :2]) and bool(out[at:, 2:].isnan().all())
 
 
+def test_prompt_of_many_rows_and_heads_of_256():
+    """Enough row blocks of 256 for every CU: workgroups of eight waves."""
+    c = Case(32, 16, 256, 32, torch.bfloat16, [1600, 700, 33])
+    cu = [0, 1500, 2100, 2101]
+    q = c.q(2110)
+    clean = torch.full_like(q, 7.0)
+    c.att.prompt(c.batch(cu), q, c.kc, c.vc, clean)
+    c.att.check()
+    close(clean[:2101], *c.expect(q[:2101], cu))
+    assert bool((clean[2101:] == 7).all())
+    v = c.vc.clone()
+    for i, at, what in ((0, 1333, math.inf), (1, 699, math.nan)):  # positions: of a token in the middle, and of a last one
+        v[int(c.table[i, at // 32]), 3, at % 32, 200] = what
+    out = torch.full_like(q, 7.0)
+    c.att.prompt(c.batch(cu), q, c.kc, v, out)
+    hit = torch.zeros_like(q, dtype=torch.bool)
+    hit[1333 - 100: 1500, 6:8, 200] = hit[2099, 6:8, 200] = True  # rows from those positions on, of the two heads that read them
+    assert torch.equal(out[~hit], clean[~hit])
+    assert bool((out[:1500][hit[:1500]] == math.inf).all()) and bool(out[1500:][hit[1500:]].isnan().all())
+
+
 def test_far_offsets_in_a_large_cache():
     """Pages that start past 2^31 elements and 2^32 bytes."""
     hkv, dim, page = 2, 256, 256

@@ -145,6 +145,19 @@ def test_prompts_of_many_sequences():
     assert bool((c.out[c.cu[298]: c.cu[299]] == 0).all()) and torch.equal(c.pool[34], before[34])
 
 
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("hk,hv", [(16, 32), (10, 30)])
+def test_prompts_of_more_heads_and_chunks_than_run_at_once(hk, hv, dtype):
+    """The matrices of a key head's value heads are made one after the other then."""
+    c = Case(hk, hv, 64, 64, dtype, [1500, 300])
+    w = [c.expect(i, c.pool[2 * i]) for i in range(2)]
+    c.prompt([0, 2], [1, 3])
+    c.h.check()
+    for i in range(2):
+        c.close(c.out[c.cu[i]: c.cu[i + 1]], w[i][0], i)
+        c.close(c.pool[2 * i + 1], w[i][1], i)
+
+
 def test_prompt_without_tokens_passes_states_on():
     c = Case(2, 4, 64, 128, torch.float16, [0, 0, 0])
     before = c.pool.clone()
