@@ -14,7 +14,8 @@
  * Conventions, as in qe_moe.h: plain pointers and sizes, tensors in device
  * memory of the context's device, `stream` a hipStream_t of that device (NULL
  * = its default stream).  Calls enqueue work on `stream`, allocate nothing and
- * return without a host sync; they can be captured into a HIP graph.  A
+ * return without a host sync; they can be captured into a HIP graph.  A call
+ * that would take more threads than a launch has (2^32) is refused.  A
  * context is used by one host thread at a time, and calls on one context that
  * could overlap (other streams, two graphs replayed at once) race on its
  * scratch, and may leave it unusable: give each its own context.  Entry points return 0 or a negative
@@ -86,7 +87,7 @@ typedef struct {
  * reported, rows of the sequences beside them may hold anything. */
 typedef struct {
     int n_seqs;            /* 1 .. 65535 */
-    int n_tokens;          /* rows given; 0 .. 2^24 */
+    int n_tokens;          /* rows given; 0 .. 2^24 - 1 */
     const int32_t *cu_q;   /* [n_seqs + 1]; NULL: one token per sequence (n_tokens == n_seqs) */
     const int32_t *kv_len; /* [n_seqs], each 0 .. max_pages * page */
     const int32_t *table;  /* page ids, sequence i's at table + i * table_stride */

@@ -103,7 +103,7 @@ size_t part_rows() {
 int check_batch(const qe_attn_ctx *c, const qe_attn_batch *b, const qe_kv_cache *kv, const char *where) {
     if (!c || !b || !kv) return qe_fail(QE_ERR_ARG, "%s: null context, batch or cache", where);
     if (b->n_seqs < 1 || b->n_seqs > 65535) return qe_fail(QE_ERR_ARG, "%s: n_seqs %d is not 1 .. 65535", where, b->n_seqs);
-    if (b->n_tokens < 0 || b->n_tokens > 1 << 24) return qe_fail(QE_ERR_ARG, "%s: n_tokens %d is not 0 .. 2^24", where, b->n_tokens);
+    if (b->n_tokens < 0 || b->n_tokens >= 1 << 24) return qe_fail(QE_ERR_ARG, "%s: n_tokens %d is not 0 .. 2^24 - 1", where, b->n_tokens);
     if (!b->cu_q && b->n_tokens != b->n_seqs)
         return qe_fail(QE_ERR_ARG, "%s: without cu_q n_tokens (%d) is n_seqs (%d)", where, b->n_tokens, b->n_seqs);
     if (!b->kv_len || !b->table) return qe_fail(QE_ERR_ARG, "%s: null kv_len or table", where);
@@ -265,6 +265,8 @@ int qe_attn_prompt(qe_attn_ctx *c, const qe_attn_batch *b, const qe_kv_cache *kv
     QeAttnArgs a = attn_args(c, b, kv, q, q_stride, out, out_stride);
     const int bm = qe_attn_prompt_rows(b->n_tokens, b->n_seqs, a.group, a.kv_heads, c->d.head_dim);
     a.tiles = qe_attn_max_tiles(b->n_tokens, b->n_seqs, a.group, bm);
+    if (!qe_fits_launch((int64_t)a.tiles * a.kv_heads, 2 * bm))
+        return qe_fail(QE_ERR_ARG, "qe_attn_prompt: %d tokens of %d sequences are more threads than a launch has", b->n_tokens, b->n_seqs);
     const int64_t most = (int64_t)b->max_pages * c->d.page;
     a.splits = qe_attn_prompt_splits((int64_t)a.tiles * a.kv_heads, b->max_len && b->max_len < most ? b->max_len : most);
     OnDevice on(c->device);
@@ -393,6 +395,9 @@ int qe_delta_prompt(qe_delta_ctx *c, const qe_delta_args *x, const int32_t *cu, 
     if (rc != QE_OK) return rc;
     if (!cu) return qe_fail(QE_ERR_ARG, "%s: null cu (single tokens: qe_delta_decode)", where);
     if (x->n_tokens < 0 || x->n_tokens > c->d.t_max) return qe_fail(QE_ERR_ARG, "%s: n_tokens %d is not 0 .. %d", where, x->n_tokens, c->d.t_max);
+    const int64_t chunks = qe_delta_max_chunks(x->n_tokens, x->n_seqs);
+    if (!qe_fits_launch((int64_t)x->n_seqs * c->d.v_heads * (c->d.dim_v / 16), 512) || !qe_fits_launch(chunks * c->d.v_heads, 256))
+        return qe_fail(QE_ERR_ARG, "%s: %d tokens of %d sequences are more threads than a launch has", where, x->n_tokens, x->n_seqs);
     if ((rc = c->err.take(where)) != QE_OK) return rc;
     a.cu = cu;
     OnDevice on(c->device);
@@ -407,6 +412,8 @@ int qe_delta_decode(qe_delta_ctx *c, const qe_delta_args *x, void *stream) {
     int rc = delta_args(c, x, where, &a);
     if (rc != QE_OK) return rc;
     if (x->n_tokens != x->n_seqs) return qe_fail(QE_ERR_ARG, "%s: n_tokens %d, n_seqs %d", where, x->n_tokens, x->n_seqs);
+    if (!qe_fits_launch((int64_t)x->n_seqs * c->d.v_heads * (c->d.dim_v / 32), 256))
+        return qe_fail(QE_ERR_ARG, "%s: %d sequences are more threads than a launch has", where, x->n_seqs);
     if ((rc = c->err.take(where)) != QE_OK) return rc;
     OnDevice on(c->device);
     HIP_TRY(on.e);

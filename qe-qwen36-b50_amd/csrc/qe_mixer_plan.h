@@ -9,6 +9,9 @@
 #define QE_MIX_HD static inline
 #endif
 
+// A launch has less than 2^32 threads.
+QE_MIX_HD bool qe_fits_launch(int64_t workgroups, int threads) { return workgroups < ((int64_t)1 << 32) / threads; }
+
 // ---- attention ----------------------------------------------------------------
 #define QE_ATTN_SUB 16     /* keys that share one page lookup: the smallest page */
 #define QE_ATTN_TILE 32    /* keys of a decode wave's step */

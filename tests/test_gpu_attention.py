@@ -417,6 +417,15 @@ def test_refusals():
     b.c.max_pages = b.c.table_stride = (1 << 30) // 32 + 1
     with pytest.raises(qe_moe.QeError, match="max_pages"):
         a.decode(b, q, c.kc, c.vc, out)
+    many = qe_mixer.Attention(256, 256, 64, 16)
+    n = 65535
+    b = qe_mixer.Batch(torch.zeros(n, dtype=torch.int32, device="cuda"), torch.zeros(n, 1, dtype=torch.int32, device="cuda"),
+                       torch.zeros(n + 1, dtype=torch.int32, device="cuda"))
+    pages = torch.zeros(1, 256, 16, 64, dtype=torch.bfloat16, device="cuda")
+    rows = torch.full((256, 256, 64), 7.0, dtype=torch.bfloat16, device="cuda")
+    with pytest.raises(qe_moe.QeError, match="threads"):
+        many.prompt(b, rows, pages, pages, rows)
+    many.check()
     a.check()
 
 

@@ -25,6 +25,7 @@ int checked(int v, int lo, int hi, int other, unsigned *bad) { return qe_checked
 int slot_pair(long n, int a, int b) { return qe_slot_pair(n, a, b); }
 int slot_conflict(int i, int oi, int j, int ij, int oj) { return qe_slot_conflict(i, oi, j, ij, oj); }
 int decode_once(long s, long h, int d, long n) { return qe_attn_decode_once(s, h, d, n); }
+int fits(long wgs, int threads) { return qe_fits_launch(wgs, threads); }
 int wgs() { return QE_ATTN_WGS; }
 int decode_wgs() { return QE_ATTN_DECODE_WGS; }
 int decode_splits() { return QE_ATTN_DECODE_SPLITS; }
@@ -43,6 +44,7 @@ def plan(tmp_path_factory):
     lib.prompt_splits.argtypes = [ctypes.c_long, ctypes.c_long]
     lib.decode_plan.argtypes = [ctypes.c_long, ctypes.c_long, ctypes.c_int, ctypes.c_long, ctypes.c_void_p, ctypes.c_void_p]
     lib.decode_once.argtypes = [ctypes.c_long, ctypes.c_long, ctypes.c_int, ctypes.c_long]
+    lib.fits.argtypes = [ctypes.c_long, ctypes.c_int]
     lib.slot_pair.argtypes = [ctypes.c_long, ctypes.c_int, ctypes.c_int]
     return lib
 
@@ -65,6 +67,12 @@ def test_decode_workgroups_cover_every_length(plan):
                 assert mine >= steps and active <= splits and active * mine >= tiles and (active - 1) * mine < max(tiles, 1)
                 if n <= told:
                     assert mine == steps
+
+
+def test_launches_have_less_than_2_32_threads(plan):
+    for threads in (256, 512, 1024):
+        for n in (1, 1 << 20, (1 << 32) // threads - 1, (1 << 32) // threads, (1 << 32) // threads + 1, 1 << 40):
+            assert plan.fits(n, threads) == (n * threads < 1 << 32)
 
 
 def test_large_calls_pass_the_caches_by(plan):
