@@ -561,7 +561,7 @@ __global__ __launch_bounds__(512, sizeof(IN) == 2 && (DK == 64 || __is_same(IN, 
             for (int i = 0; i < SB; ++i)
                 for (int j = 0; j < 4; ++j) a.pool[(((size_t)out_i * a.v_heads + head) * DK + 16 * (wave * SB + i) + 4 * c + j) * DV + col] = S[i][j];
     } else {
-        qe_s8 qf[KS][NP], m_even[2][NO], m_odd[2][NO];
+        qe_s8 q_even[KS][NP], q_odd[KS][NP], mf[2][NO];
         auto load_k = [&](int t0, const short *from, short *to) {
             constexpr int ROWS = 512 / DK; // of one direct load
 #pragma unroll
@@ -578,32 +578,34 @@ __global__ __launch_bounds__(512, sizeof(IN) == 2 && (DK == 64 || __is_same(IN, 
             load_lds16((const IN *)a.v + (size_t)(t < end ? t : end - 1) * a.v_stride + (size_t)head * DV + slice * 16 + lane % PER * VL, v_to + wave * VW);
             load_lds16((const float *)w + QE_DELTA_WS - 256 + lane * 4, f_to + wave * 256);
         };
-        auto load_q = [&](int t0, const short *from) {
+        auto load_q = [&](int t0, const short *from, qe_s8 (*qf)[NP]) {
             const short *q = (const short *)a.q + (size_t)(t0 + row < end ? t0 + row : end - 1) * a.q_stride + (size_t)kh * DK + 8 * c;
             for (int s = 0; s < KS; ++s)
                 for (int p = 0; p < NP; ++p)
                     qf[s][p] = *(const qe_s8 *)(NP == 1 ? q + 32 * s : from + NP * 64 * DK + ((wave * KS + s) * NP + p) * 512 + lane * 8);
         };
-        auto load_m = [&](const short *w, qe_s8 (*mf)[NO]) {
+        auto load_m = [&](const short *w) {
             for (int p = 0; p < NO; ++p) {
                 mf[0][p] = *(const qe_s8 *)(w + 4 * 6 * 512 + wave * 6 * 512 + p * 512 + lane * 8);
                 mf[1][p] = *(const qe_s8 *)(w + 4 * 6 * 512 + wave * 6 * 512 + 3 * 512 + p * 512 + lane * 8);
             }
         };
         IN *out = (IN *)a.out + (size_t)(begin + 16 * wave + 4 * c) * a.out_stride + (size_t)head * DV + col; // the first of the lane's four rows
-        auto step = [&](const int par, const bool whole, const float *f_s, short *k_next, IN *v_next, float *f_next, const qe_s8 (*mf)[NO], qe_s8 (*m_next)[NO], int t0) {
+        auto step = [&](const int par, const bool whole, const float *f_s, short *k_next, IN *v_next, float *f_next, const qe_s8 (*qf)[NP], qe_s8 (*q_next)[NP], int t0) {
             const int ahead = t0 + QE_DELTA_C < end;
             kq += ahead * kq_step, ws += ahead * ws_step;
-            // K, V and the factors have landed: younger than their direct loads are those of M and Q, and the last chunk's stores
-            constexpr int younger = 2 * NO + KS * NP;
+            // K, V and the factors have landed, and Q: younger than the direct loads are those of Q, then of M, then the last
+            // chunk's four stores.  (A register that is still to be loaded when it is used makes the compiler wait for
+            // the direct loads in flight as well: so Q is here before the next ones begin, and M's come long before its use.)
+            constexpr int younger = 2 * NO + (KS * NP < 4 ? KS * NP : 4);
             __builtin_amdgcn_s_waitcnt(0x0f70 | (younger & 15) | (younger >> 4) << 14);
             lds_barrier();
             // The chain's waves now read all of S, which takes the LDS's bandwidth; these issue loads meanwhile,
             // and read S while the chain is at its next product.
             load_v(t0 + ahead * QE_DELTA_C, ws, v_next, f_next);
             load_k(t0 + ahead * QE_DELTA_C, kq, k_next);
-            asm volatile("" ::: "memory"); // the count above needs M's loads behind the direct ones
-            load_m(ws, m_next);
+            asm volatile("" ::: "memory"); // the count above needs Q's loads behind the direct ones
+            load_q(t0 + ahead * QE_DELTA_C, kq, q_next);
             lds_barrier();
             qe_f4 x[3] = {};
 #pragma unroll
@@ -614,7 +616,6 @@ __global__ __launch_bounds__(512, sizeof(IN) == 2 && (DK == 64 || __is_same(IN, 
                 if (s & 1) __builtin_amdgcn_sched_barrier(0); // all of S read at once would take more than 128 registers
             }
             qe_f4 o = *(const qe_f4 *)(f_s + 256 * wave + 64 + 16 * wave + 4 * c) * (x[0] + (x[1] + x[2]));
-            load_q(t0 + ahead * QE_DELTA_C, kq);
             lds_barrier();
             const int spoilt = odd_s[par][r];
             qe_f4 y[3] = {};
@@ -625,6 +626,7 @@ __global__ __launch_bounds__(512, sizeof(IN) == 2 && (DK == 64 || __is_same(IN, 
                 for (int p = 0; p < NO; ++p) uf[p] = *(const qe_s8 *)(u_p + (p * 16 + r) * LT + 32 * s + 8 * c);
                 mul_planes<NO, NO, NO - 1>(mf[s], uf, y);
             }
+            load_m(ws);
             o += y[0] + (y[1] + y[2]);
             for (int j = 0; j < 4; ++j) {
                 const int t = 16 * wave + 4 * c + j;
@@ -635,17 +637,17 @@ __global__ __launch_bounds__(512, sizeof(IN) == 2 && (DK == 64 || __is_same(IN, 
         if (begin < end) {
             load_v(begin, ws, v_even, f_even);
             load_k(begin, kq, k_even);
-            load_q(begin, kq);
-            load_m(ws, m_even);
+            load_q(begin, kq, q_even);
+            load_m(ws);
             __builtin_amdgcn_s_waitcnt(0x0f70); // in whatever order they were issued here
         }
         int t0 = begin;
         for (; t0 + 2 * QE_DELTA_C <= end; t0 += 2 * QE_DELTA_C) {
-            step(0, true, f_even, k_odd, v_odd, f_odd, m_even, m_odd, t0);
-            step(1, true, f_odd, k_even, v_even, f_even, m_odd, m_even, t0 + QE_DELTA_C);
+            step(0, true, f_even, k_odd, v_odd, f_odd, q_even, q_odd, t0);
+            step(1, true, f_odd, k_even, v_even, f_even, q_odd, q_even, t0 + QE_DELTA_C);
         }
-        if (t0 < end) step(0, false, f_even, k_odd, v_odd, f_odd, m_even, m_odd, t0);
-        if (t0 + QE_DELTA_C < end) step(1, false, f_odd, k_even, v_even, f_even, m_odd, m_even, t0 + QE_DELTA_C);
+        if (t0 < end) step(0, false, f_even, k_odd, v_odd, f_odd, q_even, q_odd, t0);
+        if (t0 + QE_DELTA_C < end) step(1, false, f_odd, k_even, v_even, f_even, q_odd, q_even, t0 + QE_DELTA_C);
     }
 }
 
