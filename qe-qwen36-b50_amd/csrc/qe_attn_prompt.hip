@@ -56,7 +56,7 @@ __device__ __forceinline__ void load_part(const QeAttnArgs &a, int page, int kvh
     const unsigned off = row * DH * 2 + ((c ^ (IS_K ? k_swz(row) : v_swz<DH>(row))) << 4);
 #pragma unroll
     for (int i = 0; i < PART / ROWS; ++i)
-        load_lds16(from + i * 1024 + (off ^ ((IS_K ? k_swz(i * ROWS) : v_swz<DH>(i * ROWS)) << 4)), lds + (wave * PART + i * ROWS) * DH);
+        load_lds16_from(from, PART * DH * 2, off ^ ((IS_K ? k_swz(i * ROWS) : v_swz<DH>(i * ROWS)) << 4), i * 1024, lds + (wave * PART + i * ROWS) * DH);
 }
 
 __device__ __forceinline__ float max3(float a, float b, float c) { return fmaxf(fmaxf(a, b), c); }
