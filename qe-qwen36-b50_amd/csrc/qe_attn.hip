@@ -201,9 +201,9 @@ __global__ __launch_bounds__(256, 2) void k_attn_decode(const QeAttnArgs a) {
 #pragma unroll
         for (int i = 0; i < QE_ATTN_TILE / ROWS; ++i) {
             const int row = i * ROWS + lane / CH, ch = (lane % CH) ^ v_swizzle<DH>(row);
-            const size_t base = (i * ROWS < 16 ? r0 : r1) + (row & 15);
-            load_lds16<ONCE>((const short *)a.vc + base * DH + ch * 8, vb + i * 512);
+            load_lds16_from<ONCE>((const short *)a.vc + (i * ROWS < 16 ? r0 : r1) * DH, 32 * DH, ((row & 15) * DH + ch * 8) * 2, 0, vb + i * 512);
         }
+        __builtin_amdgcn_sched_barrier(0); // all loads are under way before the first is waited for
         qe_f4 s[2] = {qe_f4{0, 0, 0, 0}, qe_f4{0, 0, 0, 0}};
 #pragma unroll
         for (int st = 0; st < KS; ++st) {

@@ -56,17 +56,17 @@ __device__ __forceinline__ qe_s4 lds_tr(const short *p) {
     return __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) qe_s4 *)p);
 }
 // 64 lanes x 16 bytes from global memory straight to LDS: lane l's land at dst + 16 l
-// (ONCE: the data is not expected to be read again soon, and need not stay in the caches)
-template <bool ONCE = false>
 __device__ __forceinline__ void load_lds16(const void *src, void *dst) {
-    __builtin_amdgcn_global_load_lds(QE_GLOBAL(void, src), QE_LDS(void, dst), 16, 0, ONCE ? 2 : 0);
+    __builtin_amdgcn_global_load_lds(QE_GLOBAL(void, src), QE_LDS(void, dst), 16, 0, 0);
 }
 // The same as buffer loads: `at` bytes per lane and `more` for all behind a uniform `src`, of which `bytes` may be read.
-// The compiler takes global_load_lds for one that may read LDS as well, and while one is in flight waits for all LDS reads
-// where it needs the first.
+// The compiler takes global_load_lds for one that may read LDS as well, and while one is in flight waits for all LDS reads,
+// or for all loads, where it needs the first.  (ONCE: the data is not expected to be read again soon, and need not stay in
+// the caches.)
+template <bool ONCE = false>
 __device__ __forceinline__ void load_lds16_from(const void *src, int bytes, unsigned at, unsigned more, void *dst) {
     __amdgpu_buffer_rsrc_t from = __builtin_amdgcn_make_buffer_rsrc((void *)src, 0, bytes, 0x00027000);
-    __builtin_amdgcn_raw_ptr_buffer_load_lds(from, QE_LDS(void, dst), 16, at, more, 0, 0);
+    __builtin_amdgcn_raw_ptr_buffer_load_lds(from, QE_LDS(void, dst), 16, at, more, 0, ONCE ? 2 : 0);
 }
 
 // A workgroup's barrier for what it exchanges through LDS.  __syncthreads() would also wait for
