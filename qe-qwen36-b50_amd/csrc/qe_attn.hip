@@ -138,8 +138,8 @@ hipError_t qe_launch_append(const QeAppendArgs &a, int in_type, int type, hipStr
 // Running maximum and sum in 32 bits per head; O is rescaled only when a maximum grew.  Probabilities are
 // rounded to the cache's type for the second product (their sum is of the unrounded ones).
 // Long lengths are bound by memory: one sequence of 100,000 keys, two key-value heads of 256, bf16, 205 MB:
-// 36 us, 5.7 TB/s, and 5 for the join; 24 sequences of 1 to 8,100 keys, eight heads of 128, fp16, 339 MB: 67 us,
-// 5.1 TB/s.  Short ones by latency: 700 keys take 10 us (length and page, keys and values, the exchange through
+// 36 us, 5.7 TB/s, and 5 for the join; 24 sequences of 1 to 8,100 keys, eight heads of 128, fp16, 339 MB: 66 us,
+// 5.2 TB/s.  Short ones by latency: 700 keys take 10 us (length and page, keys and values, the exchange through
 // memory, the join), where a launch that does nothing takes 2.
 // ---------------------------------------------------------------------------
 template <int DH>

@@ -17,8 +17,8 @@
 // Scores, maxima and sums are in 32 bits; probabilities are rounded to the cache's type for the
 // second product.  A row's maximum is raised only where a score exceeds it by 2^8, so that O is seldom rescaled.
 // Long prompts are bound by the matrix cores, whose issue the exponentials share: 8192 tokens of 16 heads of 256 (550
-// GFLOP), bf16, 515 to 545 us, 1010 to 1070 TFLOP/s where a large library product reaches 1219.  Five
-// prompts of 1999 tokens, 32 heads of 128, fp16: 40 us, the longest row blocks' 18 steps in turn.
+// GFLOP), bf16, 505 to 540 us, 1020 to 1090 TFLOP/s where a large library product reaches 1219.  Five
+// prompts of 1999 tokens, 32 heads of 128, fp16: 38 us, the longest row blocks' 18 steps in turn.
 // 100 tokens: 12 us, latency (lengths, pages, four steps, the output), much of it the code's first way through the
 // instruction cache: a workgroup whose code was three times as long, in steps of 64 keys with 512 registers, took 15.
 #include "qe_mixer_device.h"

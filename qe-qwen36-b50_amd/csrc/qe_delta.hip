@@ -416,9 +416,9 @@ __global__ __launch_bounds__(256, 3) void k_delta_chunks(const QeDeltaArgs a) {
 // What bounds it: the chain of products, exchanges and barriers of a chunk, on 256 of the
 // GPU's 1024 SIMDs for each sequence (32 heads, 8 slices).  A load stalls the wave that issues it
 // while the CU's 64 bytes a cycle are taken (some 65 KiB a chunk), so the loads are few and
-// wide, and spread over the waves and over the chunk.  8192 bf16 tokens of 32 heads of 128 x 128: 240 us, 1.9 a
-// chunk (of some 3,900 cycles K S takes 550, what is left of V to LDS 400, T times it 280, U to LDS 500,
-// the state's update and S to LDS 1,150, the rest is barriers); 1999 fp32 tokens of three prompts 90 us.
+// wide, and spread over the waves and over the chunk.  8192 bf16 tokens of 32 heads of 128 x 128: 226 us, 1.8 a
+// chunk (of some 3,800 cycles K S takes 550, what is left of V to LDS 400, T times it 280, U to LDS 500,
+// the state's update and S to LDS 1,150, the rest is barriers); 1999 fp32 tokens of three prompts 84 us.
 // ---------------------------------------------------------------------------
 // Where the LDS holds two workgroups (bf16, and fp16 keys of 64), 128 registers let it: sequences side by side overlap
 // (16 of 500 tokens, bf16: 355 us the call with one a CU, 296 with two; one of 8192 has one a CU, and takes the same in both forms).
