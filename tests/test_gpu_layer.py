@@ -95,7 +95,7 @@ def test_two_layers_prompt_then_tokens():
         o, S = R.delta(all_["q"].reshape(n, HK, DK), all_["k"].reshape(n, HK, DK), all_["v"].reshape(n, HV, DK), all_["g"], all_["beta"],
                        torch.zeros(HV, DK, DK, device="cuda"), True, DK ** -0.5)
         assert R.rel(all_["d"], o) <= 1e-5 and R.rel(m.pool[int(slots[i])], S) <= 1e-5
-    # the MoE block on what attention made, against the checker
+    # the MoE block on what attention made, against the oracle
     x2 = took[0][-1]["x2"].cpu().numpy()
     w = O.moe_layer(layer, x2, norm=True, residual=True)["out"]
     assert np.linalg.norm(took[0][-1]["y"].cpu().numpy() - w) <= 1e-3 * np.linalg.norm(w)
