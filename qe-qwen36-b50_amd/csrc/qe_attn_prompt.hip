@@ -354,8 +354,9 @@ __global__ __launch_bounds__(64 * WAVES, 2) void k_attn_prompt(const QeAttnArgs 
     }
 }
 
-// The splits' results joined, W waves per query row: one up to 8 splits, and a workgroup's four over every fourth split
-// beyond (240 rows of 256 over 40 splits: 65 us the call with one wave a row, 41 with four; 16000 rows over 2: 54 and 66).
+// The splits' results joined, W waves per query row: one, but for few rows over more than 8 splits a workgroup's four, each
+// over every fourth split.  (The call with one wave a row and with four: 240 rows of 256 over 40 splits 65 and 41 us, 2048 of
+// 128 over 21 60 and 54; but 6400 of 128 over 9 47 and 52, 16000 of 256 over 2 54 and 66.)
 template <bool BF, int DH, int BM, int W>
 __global__ __launch_bounds__(256) void k_attn_prompt_join(const QeAttnArgs a) {
     constexpr int E = DH / 64;
@@ -416,7 +417,7 @@ template <bool BF, int DH, int WAVES>
 static hipError_t launch_waves(const QeAttnArgs &a, hipStream_t st) {
     k_attn_prompt<BF, DH, WAVES><<<dim3((unsigned)(a.tiles * a.kv_heads * a.splits)), dim3(64 * WAVES), 0, st>>>(a);
     const unsigned rows = (unsigned)(a.tiles * a.kv_heads) * (32 * WAVES);
-    if (a.splits > 8) k_attn_prompt_join<BF, DH, 32 * WAVES, 4><<<dim3(rows), dim3(256), 0, st>>>(a);
+    if (a.splits > 8 && rows <= 4096) k_attn_prompt_join<BF, DH, 32 * WAVES, 4><<<dim3(rows), dim3(256), 0, st>>>(a);
     else if (a.splits > 1) k_attn_prompt_join<BF, DH, 32 * WAVES, 1><<<dim3(rows / 4), dim3(256), 0, st>>>(a);
     return hipGetLastError();
 }

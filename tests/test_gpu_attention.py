@@ -184,6 +184,17 @@ def test_prompt_few_rows_over_a_long_cache(dim, page):
         close(out, want, off)
 
 
+@pytest.mark.parametrize("hq,hkv,dim", [(32, 8, 128), (16, 4, 256), (24, 8, 64)])
+def test_prompt_many_rows_over_many_splits(hq, hkv, dim):
+    c = Case(hq, hkv, dim, 32, torch.bfloat16, [2600, 2700])
+    cu = [0, 100, 260]
+    q = c.q(260)
+    out = torch.empty_like(q)
+    c.att.prompt(c.batch(cu, max_len=2700), q, c.kc, c.vc, out)
+    c.att.check()
+    close(out, *c.expect(q, cu))
+
+
 def test_prompt_rows_without_positions_are_zeros():
     c = Case(8, 2, 128, 16, torch.bfloat16, [3, 0, 20])
     cu = [0, 10, 14, 34]  # ten tokens of which three are in the cache, four of which none is
