@@ -245,7 +245,8 @@ __global__ __launch_bounds__(64 * WAVES, 2) void k_attn_prompt(const QeAttnArgs 
 #pragma unroll
             for (int i = 0; i < 16; ++i) w.o[d][i] = 0;
     }
-    if (tid < BM / BN + 2) odd_rows[tid] = 0; // a barrier before the first tile's
+    if (tid < BM / BN + 2) odd_rows[tid] = 0;
+    lds_barrier(); // the first tile's marks come before its barrier
 
     // The wave's direct loads have landed.  A probability of 0 times an infinity or NaN is NaN: in its part of V's tile t rows
     // behind the end become zeros, and so do elements that are not finite, which are added in the end for the rows

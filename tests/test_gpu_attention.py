@@ -252,6 +252,45 @@ def test_prompt_of_many_rows_and_heads_of_256():
     assert bool((out[:1500][hit[:1500]] == math.inf).all()) and bool(out[1500:][hit[1500:]].isnan().all())
 
 
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("dim", [64, 128, 256])
+@pytest.mark.parametrize("extra_cols", [2, 700])  # one split; and one tile of keys each, so that some begin at their rows' own keys
+def test_prompt_values_that_are_not_finite_in_a_workgroups_first_tile(dim, dtype, extra_cols):
+    n = 150
+    c = Case(4, 2, dim, 32, dtype, [n], extra_cols=extra_cols)
+    q = c.q(n)
+    clean, out = torch.empty_like(q), torch.empty_like(q)
+    c.att.prompt(c.batch([0, n]), q, c.kc, c.vc, clean)
+    for at, what in ((0, math.nan), (1, math.inf), (15, -math.inf), (16, math.nan), (31, math.inf), (32, math.nan), (47, math.inf), (48, math.nan),
+                     (63, math.inf), (64, math.nan), (100, -math.inf), (128, math.nan), (148, math.inf)):
+        v = c.vc.clone()
+        v[int(c.table[0, at // 32]), 1, at % 32, dim - 1] = what
+        c.att.prompt(c.batch([0, n]), q, c.kc, v, out)
+        hit = torch.zeros_like(q, dtype=torch.bool)
+        hit[at:, 2:, dim - 1] = True
+        assert torch.equal(out[~hit], clean[~hit]), at
+        assert bool((out[hit].isnan() if what != what else out[hit] == what).all()), at
+    c.att.check()
+
+
+def test_prompt_values_that_are_not_finite_in_the_first_tile_of_eight_waves():
+    c = Case(32, 16, 256, 32, torch.bfloat16, [1500, 600])
+    cu = [0, 1500, 2100]
+    q = c.q(2100)
+    clean, out = torch.empty_like(q), torch.empty_like(q)
+    c.att.prompt(c.batch(cu), q, c.kc, c.vc, clean)
+    for at, what in ((0, math.nan), (7, math.inf), (8, -math.inf), (31, math.nan), (32, math.inf), (55, math.nan), (63, math.inf)):
+        v = c.vc.clone()
+        for i in range(2):
+            v[int(c.table[i, at // 32]), 5, at % 32, 129] = what
+        c.att.prompt(c.batch(cu), q, c.kc, v, out)
+        hit = torch.zeros_like(q, dtype=torch.bool)
+        hit[at:1500, 10:12, 129] = hit[1500 + at:, 10:12, 129] = True
+        assert torch.equal(out[~hit], clean[~hit]), at
+        assert bool((out[hit].isnan() if what != what else out[hit] == what).all()), at
+    c.att.check()
+
+
 def test_far_offsets_in_a_large_cache():
     """Pages that start past 2^31 elements and 2^32 bytes."""
     hkv, dim, page = 2, 256, 256
