@@ -83,8 +83,9 @@ typedef struct {
  * the work runs.  Sequence i's new tokens are rows cu_q[i] .. cu_q[i+1] - 1 of
  * q, k, v and out (0 <= cu_q[0] <= ... <= cu_q[n_seqs] <= n_tokens); they are
  * the last of its kv_len[i] positions.  kv_len counts them.  Rows of out that
- * belong to no sequence are left as they were; where offsets fall, which is
- * reported, rows of the sequences beside them may hold anything. */
+ * belong to no sequence are left as they were.  Where offsets fall, which is
+ * reported, qe_attn_prompt's rows may hold anything, and qe_attn_append leaves
+ * out the tokens of the sequences beside them. */
 typedef struct {
     int n_seqs;            /* 1 .. 65535 */
     int n_tokens;          /* rows given; 0 .. 2^24 - 1 */

@@ -35,10 +35,14 @@ __global__ __launch_bounds__(256) void k_append(const QeAppendArgs a) {
     __shared__ long row_s;
     __shared__ int seq_s[2];
     const int t = blockIdx.x, tid = threadIdx.x, half = a.rotary / 2;
+    if (a.cu && tid >= 64) // all sequences' offsets, for the report: those that are wrong may hold no token
+        for (int64_t i = (int64_t)t * 192 + tid - 64; i < a.n_seqs; i += (int64_t)gridDim.x * 192)
+            if (qe_bad_offsets(a.cu[i], a.cu[i + 1], a.n_tokens)) report(a.err, QE_BAD_LENGTH);
     if (tid < 64) { // the token's sequence: the last whose first row is not behind t
-        int seq = -1;
+        int seq = t, end = t + 1, len;
+        bool known = true;
         if (!a.cu) {
-            seq = t;
+            len = a.kv_len[seq];
         } else {
             int lo = 0, hi = a.n_seqs; // cu[lo] <= t < cu[hi], as far as cu rises
             while (hi - lo > 1) {
@@ -46,15 +50,19 @@ __global__ __launch_bounds__(256) void k_append(const QeAppendArgs a) {
                 if (a.cu[mid] <= t) lo = mid;
                 else hi = mid;
             }
-            if (a.cu[lo] <= t && t < a.cu[lo + 1]) seq = lo;
+            // next to offsets that fall, it is not known whose the token is
+            const int before = a.cu[lo ? lo - 1 : 0], begin = a.cu[lo], after = a.cu[lo + 2 <= a.n_seqs ? lo + 2 : a.n_seqs];
+            end = a.cu[lo + 1], len = a.kv_len[lo];
+            known = before <= begin && end <= after && !qe_bad_offsets(begin, end, a.n_tokens);
+            seq = begin <= t && t < end ? lo : -1;
         }
         long row = -1;
         int place = 0;
         if (seq >= 0) {
             unsigned bad = 0;
             const int most = a.max_pages << a.page_log2;
-            const int len = qe_checked(a.kv_len[seq], 0, most, -1, &bad);
-            const int end = a.cu ? qe_checked(a.cu[seq + 1], 0, a.n_tokens, -1, &bad) : t + 1;
+            len = qe_checked(len, 0, most, -1, &bad);
+            if (!known) bad = 1;
             unsigned what = QE_BAD_LENGTH;
             if (!bad) {
                 place = len - end + t;

@@ -195,6 +195,10 @@ __global__ __launch_bounds__(64 * WAVES, 2) void k_attn_prompt(const QeAttnArgs 
     const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int split = blockIdx.x % a.splits, kvh = blockIdx.x / a.splits % a.kv_heads;
     const int tile = a.tiles - 1 - blockIdx.x / a.splits / a.kv_heads; // late rows have more keys: first
+    // Workgroup i looks at sequence i's offsets, for the report: where they fall, a sequence may have no tile below.  (There
+    // are more workgroups than sequences; the others look at the last one's, so that no branch has its own wait for the loads.)
+    const int mine = blockIdx.x < (unsigned)a.n_seqs ? blockIdx.x : a.n_seqs - 1;
+    const int mine0 = scalar_load(a.cu + mine), mine1 = scalar_load(a.cu + mine + 1);
     int seq = 0;
     for (int hi = a.n_seqs; hi - seq > 1;) { // the last sequence whose first tile is not behind this one
         const int mid = (seq + hi) >> 1;
@@ -207,7 +211,7 @@ __global__ __launch_bounds__(64 * WAVES, 2) void k_attn_prompt(const QeAttnArgs 
     const int begin = qe_checked(cu0, 0, a.n_tokens, 0, &bad_len);
     const int end = qe_checked(cu1, begin, a.n_tokens, begin, &bad_len);
     const int len = qe_checked(kv, 0, a.max_pages << a.page_log2, 0, &bad_len);
-    if (bad_len && tid == 0) report(a.err, QE_BAD_LENGTH);
+    if ((bad_len || qe_bad_offsets(mine0, mine1, a.n_tokens)) && tid == 0) report(a.err, QE_BAD_LENGTH);
     const int n_rows = (end - begin) * a.group;
     if (local < 0 || (int64_t)local * BM >= n_rows) return; // uniform: no row of the sequence
     const int row0 = local * BM, first = len - (end - begin); // first: position of the sequence's first row

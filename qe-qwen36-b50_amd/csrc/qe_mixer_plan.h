@@ -102,6 +102,9 @@ QE_MIX_HD int qe_checked(int v, int lo, int hi, int other, unsigned *bad) {
     return v;
 }
 
+// Whether a sequence's offsets are not: below 0, falling, or behind the call's tokens.
+QE_MIX_HD bool qe_bad_offsets(int cu0, int cu1, int n_tokens) { return cu0 < 0 || cu1 < cu0 || cu1 > n_tokens; }
+
 // ---- gated delta rule ------------------------------------------------------------
 #define QE_DELTA_C 64                     /* tokens of a chunk */
 #define QE_DELTA_WS (6 * 64 * 64 / 2 + 4 * 64) /* floats kept per chunk and value head: six planes of 16 bits, four vectors */

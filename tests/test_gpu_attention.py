@@ -432,6 +432,51 @@ def test_bad_lengths_give_zeros_and_an_error():
         c.att.check()
 
 
+@pytest.mark.parametrize("cu", [[0, 1000, 500, 1000], [0, 1000, 0, 1000], [300, 200, 1000, 1000], [0, 10, 20, 10], [0, 1 << 30, 500, 1000]])
+def test_offsets_that_fall_are_reported(cu):
+    """Also where a sequence that they leave without rows is the only one to show it."""
+    c = Case(1, 1, 64, 16, torch.bfloat16, [1000, 1000, 1000], rotary=64)
+    q, k = c.q(1000), rand(c.g, 1000, 1, 64, dtype=torch.bfloat16)
+    out, rot, kc, vc = torch.empty_like(q), torch.full_like(q, 7.0), c.kc.clone(), c.vc.clone()
+    c.att.prompt(c.batch(cu), q, c.kc, c.vc, out)
+    with pytest.raises(qe_moe.QeError, match="offset"):
+        c.att.check()
+    c.att.append(c.batch(cu), q, k, k, kc, vc, rot)
+    with pytest.raises(qe_moe.QeError, match="offset"):
+        c.att.check()
+    # tokens of a sequence beside the fall are left out
+    for i in range(3):
+        if 0 <= cu[i] <= cu[i + 1] <= 1000 and (i == 0 or cu[i - 1] <= cu[i]) and (i == 2 or cu[i + 1] <= cu[i + 2]):
+            continue
+        p = c.table[i, : 1000 // 16].long()
+        assert torch.equal(kc[p].view(torch.int16), c.kc[p].view(torch.int16)) and torch.equal(vc[p].view(torch.int16), c.vc[p].view(torch.int16))
+    if cu[1] == 1000:  # here that is every token
+        assert bool((rot == 7).all())
+
+
+def test_offsets_of_sequences_without_tokens_are_looked_at():
+    n = 700
+    c = Case(1, 1, 64, 16, torch.float16, [20, 3] + [0] * (n - 2), rotary=64)
+    q, k = c.q(2), rand(c.g, 2, 1, 64, dtype=torch.float16)
+    want, off = R.attend_batch(q, c.kc, c.vc, c.table, [20, 3], [0, 1, 2], 64 ** -0.5, 16)
+    for at, what, word in ((None, 0, None), (n, 3, "offset"), (n - 1, 5, "offset"), (n - 100, 1, "offset"), (400, -1, "offset")):
+        cu = [0, 1] + [2] * (n - 1)
+        if at is not None:
+            cu[at] = what
+        b = c.batch(cu)
+        out, rot, kc, vc = torch.empty_like(q), torch.empty_like(q), c.kc.clone(), c.vc.clone()
+        for call in (lambda: c.att.append(b, q, k, k, kc, vc, rot), lambda: c.att.prompt(b, q, c.kc, c.vc, out)):
+            call()
+            if word:
+                with pytest.raises(qe_moe.QeError, match=word):
+                    c.att.check()
+            else:
+                c.att.check()
+        if not word:
+            close(out, want, off)
+            assert torch.equal(vc[int(c.table[0, 1]), :, 3], k[0]) and torch.equal(vc[int(c.table[1, 0]), :, 2], k[1])
+
+
 def test_refusals():
     c = Case(8, 2, 64, 32, torch.float16, [50, 60])
     q, k = c.q(2), rand(c.g, 2, 2, 64, dtype=torch.float16)

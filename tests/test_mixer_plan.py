@@ -26,6 +26,7 @@ int slot_pair(long n, int a, int b) { return qe_slot_pair(n, a, b); }
 int slot_conflict(int i, int oi, int j, int ij, int oj) { return qe_slot_conflict(i, oi, j, ij, oj); }
 int decode_once(long s, long h, int d, long n) { return qe_attn_decode_once(s, h, d, n); }
 int fits(long wgs, int threads) { return qe_fits_launch(wgs, threads); }
+int bad_offsets(int a, int b, int n) { return qe_bad_offsets(a, b, n); }
 int wgs() { return QE_ATTN_WGS; }
 int decode_wgs() { return QE_ATTN_DECODE_WGS; }
 int decode_splits() { return QE_ATTN_DECODE_SPLITS; }
@@ -145,6 +146,13 @@ def test_values_out_of_range_are_replaced_and_noted(plan):
     for v in (-1, 6, -(1 << 31), (1 << 31) - 1):
         bad.value = 0
         assert plan.checked(v, 0, 5, 3, ctypes.byref(bad)) == 3 and bad.value == 1
+
+
+def test_offsets_that_are_none_are_found(plan):
+    for a, b in ((0, 0), (0, 9), (9, 9), (3, 4)):
+        assert not plan.bad_offsets(a, b, 9)
+    for a, b in ((-1, 0), (-1, -1), (4, 3), (0, 10), (10, 10), (10, 9), (0, -1), (-(1 << 31), (1 << 31) - 1), ((1 << 31) - 1, -(1 << 31))):
+        assert plan.bad_offsets(a, b, 9)
 
 
 def test_sequences_that_are_computed_share_no_written_slot(plan):
