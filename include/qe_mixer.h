@@ -25,7 +25,8 @@
  *
  * What stands in device memory (lengths, page tables, slots) is checked by the
  * kernels: a bad value makes no access out of bounds, its sequence's outputs
- * are zeros (qe_attn_append leaves the token out: nothing of it is written),
+ * are zeros (with offsets outside the call's tokens those rows that are the
+ * call's; qe_attn_append leaves the token out: nothing of it is written),
  * and the context remembers it.  The next call on the context
  * that looks returns QE_ERR_STATE for it, once, without doing its own work:
  * every entry point looks at entry without synchronising, qe_attn_check and
@@ -180,8 +181,8 @@ typedef struct {
 
 /* Packed prompts: sequence i's tokens are rows cu[i] .. cu[i+1] - 1 (device
  * int32 [n_seqs + 1], 0 <= cu[0] <= ... <= cu[n_seqs] <= n_tokens); other rows
- * of out are left as they were.  Where offsets fall, which is reported, rows of
- * the sequences beside them may hold anything. */
+ * of out are left as they were.  Where offsets fall, which is reported, the
+ * call's rows and the states it leaves may hold anything. */
 int qe_delta_prompt(qe_delta_ctx *ctx, const qe_delta_args *args, const int32_t *cu, void *stream);
 
 /* One token per sequence: n_tokens == n_seqs, row i is sequence i's.

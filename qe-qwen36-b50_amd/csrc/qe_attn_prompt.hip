@@ -202,15 +202,16 @@ __global__ __launch_bounds__(64 * WAVES, 2) void k_attn_prompt(const QeAttnArgs 
     int seq = 0;
     for (int hi = a.n_seqs; hi - seq > 1;) { // the last sequence whose first tile is not behind this one
         const int mid = (seq + hi) >> 1;
-        if (qe_attn_first_tile(scalar_load(a.cu + mid), mid, a.group, BM) <= tile) seq = mid;
+        if (qe_attn_first_tile(qe_clamped(scalar_load(a.cu + mid), 0, a.n_tokens), mid, a.group, BM) <= tile) seq = mid;
         else hi = mid;
     }
     const int cu0 = scalar_load(a.cu + seq), cu1 = scalar_load(a.cu + seq + 1), kv = scalar_load(a.kv_len + seq);
-    const int local = tile - qe_attn_first_tile(cu0, seq, a.group, BM);
     unsigned bad_len = 0, bad = 0;
-    const int begin = qe_checked(cu0, 0, a.n_tokens, 0, &bad_len);
-    const int end = qe_checked(cu1, begin, a.n_tokens, begin, &bad_len);
-    const int len = qe_checked(kv, 0, a.max_pages << a.page_log2, 0, &bad_len);
+    int begin, end;
+    qe_rows_of(cu0, cu1, a.n_tokens, &begin, &end, &bad_len);
+    const int local = tile - qe_attn_first_tile(begin, seq, a.group, BM);
+    int len = qe_checked(kv, 0, a.max_pages << a.page_log2, 0, &bad_len);
+    if (bad_len) len = 0; // no row has a position: zeros
     if ((bad_len || qe_bad_offsets(mine0, mine1, a.n_tokens)) && tid == 0) report(a.err, QE_BAD_LENGTH);
     const int n_rows = (end - begin) * a.group;
     if (local < 0 || (int64_t)local * BM >= n_rows) return; // uniform: no row of the sequence
@@ -370,13 +371,13 @@ __global__ __launch_bounds__(256) void k_attn_prompt_join(const QeAttnArgs a) {
     int seq = 0;
     for (int hi = a.n_seqs; hi - seq > 1;) {
         const int mid = (seq + hi) >> 1;
-        if (qe_attn_first_tile(scalar_load(a.cu + mid), mid, a.group, BM) <= tile) seq = mid;
+        if (qe_attn_first_tile(qe_clamped(scalar_load(a.cu + mid), 0, a.n_tokens), mid, a.group, BM) <= tile) seq = mid;
         else hi = mid;
     }
     unsigned bad = 0;
-    const int cu0 = scalar_load(a.cu + seq), cu1 = scalar_load(a.cu + seq + 1);
-    const int begin = qe_checked(cu0, 0, a.n_tokens, 0, &bad), end = qe_checked(cu1, begin, a.n_tokens, begin, &bad);
-    const int local = tile - qe_attn_first_tile(cu0, seq, a.group, BM);
+    int begin, end;
+    qe_rows_of(scalar_load(a.cu + seq), scalar_load(a.cu + seq + 1), a.n_tokens, &begin, &end, &bad);
+    const int local = tile - qe_attn_first_tile(begin, seq, a.group, BM);
     const int64_t row = (int64_t)local * BM + in_tile;
     // (of one row or of none with four waves a row: uniform there)
     if (local < 0 || row >= (int64_t)(end - begin) * a.group) return;

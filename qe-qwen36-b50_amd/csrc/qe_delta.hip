@@ -240,9 +240,9 @@ __global__ __launch_bounds__(256, 3) void k_delta_chunks(const QeDeltaArgs a) {
         else hi = mid;
     }
     unsigned bad = 0;
-    const int cu0 = scalar_load(a.cu + seq), cu1 = scalar_load(a.cu + seq + 1);
-    const int begin = qe_checked(cu0, 0, a.n_tokens, 0, &bad), end = qe_checked(cu1, begin, a.n_tokens, begin, &bad);
-    const int64_t local = chunk - qe_delta_first_chunk(cu0, seq);
+    int begin, end;
+    qe_rows_of(scalar_load(a.cu + seq), scalar_load(a.cu + seq + 1), a.n_tokens, &begin, &end, &bad);
+    const int64_t local = chunk - qe_delta_first_chunk(begin, seq);
     if (bad || local < 0 || local * QE_DELTA_C >= end - begin) return; // uniform
     const int t0 = begin + (int)local * QE_DELTA_C, n = end - t0 < QE_DELTA_C ? end - t0 : QE_DELTA_C;
 
@@ -442,7 +442,8 @@ __global__ __launch_bounds__(512, sizeof(IN) == 2 && (DK == 64 || __is_same(IN, 
     const int slice = eights ? at / 8 % SL : at % SL, head = eights ? at / (8 * SL) * 8 + at % 8 : at / SL;
     const int kh = head / a.group, col = slice * 16 + r;
     unsigned bad = 0;
-    const int begin = qe_checked(a.cu[seq], 0, a.n_tokens, 0, &bad), end = qe_checked(a.cu[seq + 1], begin, a.n_tokens, begin, &bad);
+    int begin, end;
+    qe_rows_of(a.cu[seq], a.cu[seq + 1], a.n_tokens, &begin, &end, &bad);
     if (bad && tid == 0) report(a.err, QE_BAD_LENGTH);
     const int in_i = a.slots_in[seq], out_i = a.slots_out[seq], what = slots_of(a, seq, in_i, out_i);
     report_slots(a, what);

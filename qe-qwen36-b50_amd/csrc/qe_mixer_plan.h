@@ -104,6 +104,13 @@ QE_MIX_HD int qe_checked(int v, int lo, int hi, int other, unsigned *bad) {
 
 // Whether a sequence's offsets are not: below 0, falling, or behind the call's tokens.
 QE_MIX_HD bool qe_bad_offsets(int cu0, int cu1, int n_tokens) { return cu0 < 0 || cu1 < cu0 || cu1 > n_tokens; }
+QE_MIX_HD int qe_clamped(int v, int lo, int hi) { return v < lo ? lo : v > hi ? hi : v; }
+// The sequence's rows [*begin, *end) among the call's, whatever its offsets are; *bad is set where they are not.
+QE_MIX_HD void qe_rows_of(int cu0, int cu1, int n_tokens, int *begin, int *end, unsigned *bad) {
+    *begin = qe_clamped(cu0, 0, n_tokens);
+    *end = qe_clamped(cu1, *begin, n_tokens);
+    if (qe_bad_offsets(cu0, cu1, n_tokens)) *bad = 1;
+}
 
 // ---- gated delta rule ------------------------------------------------------------
 #define QE_DELTA_C 64                     /* tokens of a chunk */

@@ -454,6 +454,26 @@ def test_offsets_that_fall_are_reported(cu):
         assert bool((rot == 7).all())
 
 
+@pytest.mark.parametrize("hq,hkv,dim,ctx,extra_cols", [(8, 2, 64, 0, 2), (16, 1, 256, 4000, 2), (4, 4, 128, 0, 2000)])  # one split, and several
+def test_offsets_outside_the_call_give_zeros_and_an_error(hq, hkv, dim, ctx, extra_cols):
+    lens = [170, 230, 100]
+    c = Case(hq, hkv, dim, 16, torch.bfloat16, [n + ctx for n in lens], extra_cols=extra_cols)
+    q = c.q(500)
+    want, off = c.expect(q, [0, 170, 400, 500])
+    for cu, lost in (([-5, 170, 400, 500], [(0, 170)]), ([-100000, 170, 400, 500], [(0, 170)]), ([-7, -7, 400, 500], [(0, 400)]),
+                     ([0, 170, 400, 501], [(400, 500)]), ([0, 170, 1 << 30, 1 << 30], [(170, 500)]), ([-(1 << 31), 170, 400, (1 << 31) - 1], [(0, 170), (400, 500)])):
+        out = torch.full_like(q, 7.0)
+        c.att.prompt(c.batch(cu), q, c.kc, c.vc, out)
+        with pytest.raises(qe_moe.QeError, match="offset"):
+            c.att.check()
+        gone = torch.zeros(500, dtype=torch.bool, device="cuda")
+        for a, b in lost:
+            gone[a:b] = True
+        assert bool((out[gone] == 0).all()), cu
+        if cu[1] == 170:
+            close(out[~gone], want[~gone], off[~gone])
+
+
 def test_offsets_of_sequences_without_tokens_are_looked_at():
     n = 700
     c = Case(1, 1, 64, 16, torch.float16, [20, 3] + [0] * (n - 2), rotary=64)

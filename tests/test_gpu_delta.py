@@ -330,6 +330,28 @@ def test_bad_offsets_are_reported():
             c.h.check()
 
 
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_offsets_outside_the_call_give_zeros_and_an_error(dtype):
+    c = Case(2, 4, 64, 128, dtype, [70, 130, 50])
+    before = c.pool.clone()
+    w = [c.expect(i, before[2 * i]) for i in range(3)]
+    for cu, fine, lost in (([-5, 70, 200, 250], [1, 2], [(0, 70)]), ([-(1 << 31), 70, 200, 250], [1, 2], [(0, 70)]),
+                           ([0, 70, 200, 251], [0, 1], [(200, 250)]), ([0, 70, 1 << 30, (1 << 31) - 1], [0], [(70, 250)])):
+        c.pool.copy_(before)
+        c.out.fill_(7.0)
+        c.prompt([0, 2, 4], [1, 3, 5], cu=cu)
+        with pytest.raises(qe_moe.QeError, match="offset"):
+            c.h.check()
+        for a, b in lost:
+            assert bool((c.out[a:b] == 0).all()), cu
+        for i in range(3):
+            if i in fine:
+                c.close(c.out[c.cu[i]: c.cu[i + 1]], w[i][0], (cu, i))
+                c.close(c.pool[2 * i + 1], w[i][1], (cu, i))
+            else:
+                assert torch.equal(c.pool[2 * i + 1], before[2 * i + 1]), (cu, i)
+
+
 def test_refusals():
     c = Case(2, 4, 64, 64, torch.float32, [3, 4])
     a = dict(q=c.q, k=c.k, v=c.v, g=c.g, beta=c.beta, pool=c.pool, slots_in=ints([0, 2]), slots_out=ints([1, 3]), cu=ints(c.cu), out=c.out)

@@ -26,6 +26,7 @@ int slot_pair(long n, int a, int b) { return qe_slot_pair(n, a, b); }
 int slot_conflict(int i, int oi, int j, int ij, int oj) { return qe_slot_conflict(i, oi, j, ij, oj); }
 int decode_once(long s, long h, int d, long n) { return qe_attn_decode_once(s, h, d, n); }
 int fits(long wgs, int threads) { return qe_fits_launch(wgs, threads); }
+void rows_of(int a, int b, int n, int *lo, int *hi, unsigned *bad) { qe_rows_of(a, b, n, lo, hi, bad); }
 int bad_offsets(int a, int b, int n) { return qe_bad_offsets(a, b, n); }
 int wgs() { return QE_ATTN_WGS; }
 int decode_wgs() { return QE_ATTN_DECODE_WGS; }
@@ -153,6 +154,17 @@ def test_offsets_that_are_none_are_found(plan):
         assert not plan.bad_offsets(a, b, 9)
     for a, b in ((-1, 0), (-1, -1), (4, 3), (0, 10), (10, 10), (10, 9), (0, -1), (-(1 << 31), (1 << 31) - 1), ((1 << 31) - 1, -(1 << 31))):
         assert plan.bad_offsets(a, b, 9)
+
+
+def test_rows_of_any_offsets_are_the_calls(plan):
+    far = (-(1 << 31), -5, -1, 0, 1, 8, 9, 10, (1 << 31) - 1)
+    lo, hi, bad = ctypes.c_int(), ctypes.c_int(), ctypes.c_uint()
+    for a, b, n in itertools.product(far, far, (0, 1, 9)):
+        bad.value = 0
+        plan.rows_of(a, b, n, ctypes.byref(lo), ctypes.byref(hi), ctypes.byref(bad))
+        assert 0 <= lo.value <= hi.value <= n
+        assert set(range(lo.value, hi.value)) == {t for t in range(n) if a <= t < b}
+        assert bad.value == (not 0 <= a <= b <= n)
 
 
 def test_sequences_that_are_computed_share_no_written_slot(plan):
