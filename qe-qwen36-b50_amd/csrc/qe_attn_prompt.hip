@@ -46,10 +46,11 @@ __device__ __forceinline__ int page_of(const QeAttnArgs &a, const int32_t *table
 }
 // The part's rows of K or V to LDS.
 template <int DH, int BN, int WAVES, bool IS_K>
-__device__ __forceinline__ void load_part(const QeAttnArgs &a, int page, int kvh, int k0, int len, int wave, short *lds, unsigned *bad) {
+__device__ __forceinline__ void load_part(const QeAttnArgs &a, int page, int kvh, int k0, int len, int wave, short *lds) {
     constexpr int CH = DH / 8, ROWS = 64 / CH, PART = BN / WAVES; // chunks of a row, rows of one direct load, rows of a wave
     const int sub = k0 + wave * PART, at = sub < len ? sub : (len - 1) & -PART;
-    const size_t r0 = page_row(a, page, kvh, at, bad);
+    unsigned known = 0; // that a page is none: lost_pages
+    const size_t r0 = page_row(a, page, kvh, at, &known);
     const char *from = (const char *)(IS_K ? a.kc : a.vc) + r0 * DH * 2;
     // A uniform address and a 32-bit offset: a later row's permutation differs from the first load's by a constant.
     const int lane = lane_now(), row = lane / CH, c = lane % CH;
@@ -57,6 +58,21 @@ __device__ __forceinline__ void load_part(const QeAttnArgs &a, int page, int kvh
 #pragma unroll
     for (int i = 0; i < PART / ROWS; ++i)
         load_lds16_from(from, PART * DH * 2, off ^ ((IS_K ? k_swz(i * ROWS) : v_swz<DH>(i * ROWS)) << 4), i * 1024, lds + (wave * PART + i * ROWS) * DH);
+}
+
+// Whether one of the `n` pages of a sequence is none of the cache's: of the thread's share of them.  Each workgroup
+// looks at all, since the rows of all are zeros then; four at a time, the last again behind the end.
+template <int THREADS>
+__device__ __forceinline__ int lost_pages(const QeAttnArgs &a, const int32_t *table, int n, int tid) {
+    int lost = 0;
+    for (int i = tid; i < n; i += 4 * THREADS) {
+        unsigned p[4];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) p[j] = table[i + j * THREADS < n ? i + j * THREADS : n - 1];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) lost |= p[j] >= a.n_pages;
+    }
+    return lost;
 }
 
 __device__ __forceinline__ float max3(float a, float b, float c) { return fmaxf(fmaxf(a, b), c); }
@@ -206,7 +222,7 @@ __global__ __launch_bounds__(64 * WAVES, 2) void k_attn_prompt(const QeAttnArgs 
         else hi = mid;
     }
     const int cu0 = scalar_load(a.cu + seq), cu1 = scalar_load(a.cu + seq + 1), kv = scalar_load(a.kv_len + seq);
-    unsigned bad_len = 0, bad = 0;
+    unsigned bad_len = 0;
     int begin, end;
     qe_rows_of(cu0, cu1, a.n_tokens, &begin, &end, &bad_len);
     const int local = tile - qe_attn_first_tile(begin, seq, a.group, BM);
@@ -230,8 +246,8 @@ __global__ __launch_bounds__(64 * WAVES, 2) void k_attn_prompt(const QeAttnArgs 
     int page = 0; // of the wave's part of the next tile
     if (lo < hi) {
         page = page_of<BN, WAVES>(a, table, lo * BN, len, wave);
-        load_part<DH, BN, WAVES, true>(a, page, kvh, lo * BN, len, wave, k_a, &bad);
-        load_part<DH, BN, WAVES, false>(a, page, kvh, lo * BN, len, wave, v_a, &bad);
+        load_part<DH, BN, WAVES, true>(a, page, kvh, lo * BN, len, wave, k_a);
+        load_part<DH, BN, WAVES, false>(a, page, kvh, lo * BN, len, wave, v_a);
         page = page_of<BN, WAVES>(a, table, (lo + 1) * BN, len, wave);
     }
     Rows<BF, DH> w;
@@ -251,7 +267,11 @@ __global__ __launch_bounds__(64 * WAVES, 2) void k_attn_prompt(const QeAttnArgs 
             for (int i = 0; i < 16; ++i) w.o[d][i] = 0;
     }
     if (tid < BM / BN + 2) odd_rows[tid] = 0;
-    lds_barrier(); // the first tile's marks come before its barrier
+    // (A barrier, too: the first tile's marks come before its own.  It waits for the loads of that tile, as its start does.)
+    if (__syncthreads_or(lo < hi ? lost_pages<64 * WAVES>(a, table, (len + (1 << a.page_log2) - 1) >> a.page_log2, tid) : 0)) {
+        if (tid == 0) report(a.err, QE_BAD_PAGE);
+        hi = lo; // no key: zeros
+    }
 
     // The wave's direct loads have landed.  A probability of 0 times an infinity or NaN is NaN: in its part of V's tile t rows
     // behind the end become zeros, and so do elements that are not finite, which are added in the end for the rows
@@ -284,8 +304,8 @@ __global__ __launch_bounds__(64 * WAVES, 2) void k_attn_prompt(const QeAttnArgs 
         lds_barrier(); // the others' loads, too, and no wave reads the other buffers any more
         const int k0 = t * BN;
         if (t + 1 < hi) {
-            load_part<DH, BN, WAVES, true>(a, page, kvh, k0 + BN, len, wave, k_next, &bad);
-            load_part<DH, BN, WAVES, false>(a, page, kvh, k0 + BN, len, wave, v_next, &bad);
+            load_part<DH, BN, WAVES, true>(a, page, kvh, k0 + BN, len, wave, k_next);
+            load_part<DH, BN, WAVES, false>(a, page, kvh, k0 + BN, len, wave, v_next);
         }
         page = page_of<BN, WAVES>(a, table, k0 + 2 * BN, len, wave); // looked up a step before it is needed
         if (k0 >= wave_keys) return;
@@ -307,15 +327,15 @@ __global__ __launch_bounds__(64 * WAVES, 2) void k_attn_prompt(const QeAttnArgs 
         work(t, k_a, v_a, k_b, v_b);
         if (t + 1 < hi) work(t + 1, k_b, v_b, k_a, v_a);
     }
-    if (bad && (tid & 63) == 0) report(a.err, QE_BAD_PAGE);
-    const bool void_rows = __syncthreads_or(bad);
+    lds_barrier(); // all marks are made
     const int lane = lane_now(), r = lane & 31, h = lane >> 5;
     for (int t = clear / BN; t < hi; ++t) {
         unsigned long long odd = t >= lo ? odd_rows[t - clear / BN] : 0;
         while (odd) { // uniform, and empty but for values that are not finite
             const int key = t * BN + __ffsll(odd) - 1;
             odd &= odd - 1;
-            const size_t at = sub_row(a, table, kvh, __builtin_amdgcn_readfirstlane(key) & ~15, &bad) + (key & 15);
+            unsigned known = 0;
+            const size_t at = sub_row(a, table, kvh, __builtin_amdgcn_readfirstlane(key) & ~15, &known) + (key & 15);
             const short *v = (const short *)a.vc + at * DH + 4 * h;
             if (key <= w.place)
 #pragma unroll
@@ -346,7 +366,6 @@ __global__ __launch_bounds__(64 * WAVES, 2) void k_attn_prompt(const QeAttnArgs 
                 uint2 x;
                 x.x = pack2<BF>(w.o[d][i] * inv, w.o[d][i + 1] * inv);
                 x.y = pack2<BF>(w.o[d][i + 2] * inv, w.o[d][i + 3] * inv);
-                if (void_rows) x = make_uint2(0, 0);
                 *(uint2 *)(out + d * 32 + 2 * i + 4 * h) = x;
             }
     } else {
@@ -356,7 +375,7 @@ __global__ __launch_bounds__(64 * WAVES, 2) void k_attn_prompt(const QeAttnArgs 
 #pragma unroll
             for (int i = 0; i < 16; i += 4)
                 *(qe_f4 *)(a.part_o + at * DH + d * 32 + 2 * i + 4 * h) = qe_f4{w.o[d][i], w.o[d][i + 1], w.o[d][i + 2], w.o[d][i + 3]};
-        if (h == 0) a.part_ml[at] = make_float2(w.m, void_rows ? -1.f : l);
+        if (h == 0) a.part_ml[at] = make_float2(w.m, l);
     }
 }
 
@@ -383,14 +402,8 @@ __global__ __launch_bounds__(256) void k_attn_prompt_join(const QeAttnArgs a) {
     if (local < 0 || row >= (int64_t)(end - begin) * a.group) return;
     const size_t at = ((size_t)tile * a.kv_heads + kvh) * a.splits * BM + in_tile;
     float m = -INFINITY;
-    bool none = false;
-    for (int s = lane; s < a.splits; s += 64) {
-        const float2 x = a.part_ml[at + (size_t)s * BM];
-        m = fmaxf(m, x.x);
-        none |= x.y < 0.f;
-    }
+    for (int s = lane; s < a.splits; s += 64) m = fmaxf(m, a.part_ml[at + (size_t)s * BM].x);
     for (int k = 32; k; k >>= 1) m = fmaxf(m, __shfl_xor(m, k));
-    none = __any(none);
     float sum = 0, o[E];
     for (int e = 0; e < E; ++e) o[e] = 0;
 #pragma unroll 4
@@ -413,10 +426,10 @@ __global__ __launch_bounds__(256) void k_attn_prompt_join(const QeAttnArgs a) {
         for (int e = 0; e < E; ++e)
             o[e] = (o_s[0][e * 64 + lane] + o_s[1][e * 64 + lane]) + (o_s[2][e * 64 + lane] + o_s[3][e * 64 + lane]);
     }
-    const float inv = none || sum == 0.f ? 0.f : 1.f / sum;
+    const float inv = sum == 0.f ? 0.f : 1.f / sum;
     const int tok = (int)(row / a.group), head = kvh * a.group + (int)(row - (int64_t)tok * a.group);
     short *out = (short *)a.out + (size_t)(begin + tok) * a.out_stride + (size_t)head * DH;
-    for (int e = 0; e < E; ++e) out[e * 64 + lane] = (short)pack2<BF>(none ? 0.f : o[e] * inv, 0.f);
+    for (int e = 0; e < E; ++e) out[e * 64 + lane] = (short)pack2<BF>(o[e] * inv, 0.f);
 }
 
 template <bool BF, int DH, int WAVES>

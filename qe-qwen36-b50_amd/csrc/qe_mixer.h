@@ -23,7 +23,7 @@ struct QeAttnArgs {
     int steps;         // decode: see qe_attn_decode_plan
     bool once;         // decode: see qe_attn_decode_once
     float *part_o;   // partial results: [item][split][row][head_dim], unnormalised
-    float2 *part_ml; // [item][split][row] (decode: of 16): running maximum (raw scores) and sum; sum < 0: the split met a bad page
+    float2 *part_ml; // [item][split][row] (decode: of 16): running maximum and sum; decode: sum < 0: the split met a bad page
     unsigned long long *arrived; // per sequence and key-value head, 0 between calls: decode's workgroups that are done; 16 bytes of zeros behind the last
     unsigned *err;
 };

@@ -413,6 +413,31 @@ def test_bad_pages_give_zeros_and_an_error(n):
     assert torch.equal(kc.view(torch.int16), c.kc.view(torch.int16)) and torch.equal(vc.view(torch.int16), c.vc.view(torch.int16))
 
 
+@pytest.mark.parametrize("hq,hkv,dim,page,lens,extra_cols", [
+    (8, 2, 128, 16, [500, 300, 20], 2), (4, 2, 64, 32, [300, 170, 33], 1500), (16, 4, 256, 64, [300, 40, 3], 2), (16, 1, 256, 16, [5, 9, 1], 2000),
+    (32, 16, 256, 32, [1500, 600, 20], 2)])  # row blocks of four and of eight waves, one split and several
+def test_bad_pages_give_zeros_for_all_rows_of_a_prompt(hq, hkv, dim, page, lens, extra_cols):
+    ctx = [7, 1100, 0]
+    c = Case(hq, hkv, dim, page, torch.bfloat16, [a + b for a, b in zip(lens, ctx)], extra_cols=extra_cols)
+    cu = [0, lens[0], lens[0] + lens[1], sum(lens)]
+    q = c.q(cu[-1])
+    want, off = c.expect(q, cu)
+    for i in range(2):
+        pages = -(-c.kv_len[i] // page)
+        for where, what in ((0, -1), (pages // 2, c.kc.shape[0]), (pages - 1, (1 << 31) - 1)):
+            bad = c.table.clone()
+            bad[i, where] = what
+            out = torch.full_like(q, 7.0)
+            c.att.prompt(qe_mixer.Batch(ints(c.kv_len), bad, ints(cu)), q, c.kc, c.vc, out)
+            with pytest.raises(qe_moe.QeError, match="page"):
+                c.att.check()
+            assert bool((out[cu[i]: cu[i + 1]] == 0).all()), (i, where)
+            rest = torch.ones(cu[-1], dtype=torch.bool, device="cuda")
+            rest[cu[i]: cu[i + 1]] = False
+            close(out[rest], want[rest], off[rest])
+    c.att.check()
+
+
 def test_bad_lengths_give_zeros_and_an_error():
     c = Case(8, 2, 64, 32, torch.float16, [50, 60])
     q = c.q(2)
