@@ -166,7 +166,8 @@ int qe_delta_destroy(qe_delta_ctx *ctx);
  * the context remembers it.  So is one with a slot outside the pool.  A sequence
  * without tokens passes its state on as it is.  Tokens are causal: a q, k, v,
  * g or beta that is infinite or NaN reaches no token before its own and no
- * other sequence. */
+ * other sequence.  A key whose sum of squares passes the range of 32 bits (a
+ * length of 1.8e19) counts as not finite, and with l2norm so does a query. */
 typedef struct {
     int n_seqs, n_tokens;
     const void *q, *k, *v;    /* [n_tokens] rows of k_heads * dim_k, k_heads * dim_k, v_heads * dim_v, of the context's type */

@@ -42,6 +42,12 @@ __device__ __forceinline__ qe_f4 mma4(qe_f4 a, qe_f4 b, qe_f4 c) {
     return c;
 }
 
+// What a key or query with this sum of squares is multiplied by.  Where the sum passes 32 bits it is not known: NaN, in prompts
+// and single steps alike (1 / sqrt(inf) would make a silent zero of the row).
+__device__ __forceinline__ float norm_factor(float squares, bool l2norm) {
+    return !__builtin_isfinite(squares) ? NAN : l2norm ? 1.f / sqrtf(squares + 1e-6f) : 1.f;
+}
+
 __device__ __forceinline__ float log_decay(float g) { return g < -1e4f ? -1e4f : g; } // e^-1e4 is 0; a NaN stays
 
 // Planes of a type's values, and planes that the product for the outputs takes of S, M and U.
@@ -159,7 +165,7 @@ __global__ __launch_bounds__(256) void k_delta_decode(const QeDeltaArgs a) {
     xx = (part[0][0] + part[1][0]) + (part[2][0] + part[3][0]);
     yy = (part[0][1] + part[1][1]) + (part[2][1] + part[3][1]);
     xy = (part[0][2] + part[1][2]) + (part[2][2] + part[3][2]);
-    const float rq = (a.l2norm ? 1.f / sqrtf(xx + 1e-6f) : 1.f) * a.scale, rk = a.l2norm ? 1.f / sqrtf(yy + 1e-6f) : 1.f;
+    const float rq = (a.l2norm ? norm_factor(xx, true) : 1.f) * a.scale, rk = norm_factor(yy, a.l2norm);
     qe_f4 sk = {0, 0, 0, 0}, sq = {0, 0, 0, 0};
     for (int i = 0; i < ROWS; ++i) {
         s[i] *= e;
@@ -276,8 +282,8 @@ __global__ __launch_bounds__(256, 3) void k_delta_chunks(const QeDeltaArgs a) {
         if (lane < 16) {
             kk_s[row] = kk;
             // rows behind the end stand for the last token's in k_delta_scan: factors of 0 keep them from overflowing
-            rk_s[row] = row >= n ? 0.f : a.l2norm ? 1.f / sqrtf(kk + 1e-6f) : 1.f;
-            rq_s[row] = row >= n ? 0.f : (a.l2norm ? 1.f / sqrtf(qq + 1e-6f) : 1.f) * a.scale;
+            rk_s[row] = row >= n ? 0.f : norm_factor(kk, a.l2norm);
+            rq_s[row] = row >= n ? 0.f : (a.l2norm ? norm_factor(qq, true) : 1.f) * a.scale;
         }
         __syncthreads();
 #pragma unroll

@@ -405,6 +405,33 @@ def test_captured_steps_follow_the_slots_in_device_memory():
     c.h.check(), p.h.check()
 
 
+@pytest.mark.parametrize("l2norm", [True, False])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_keys_and_queries_whose_squares_pass_32_bits_are_not_finite(dtype, l2norm):
+    """In prompts and single steps alike: from the token on for a key, the token's own outputs for a query."""
+    c, one = Case(1, 2, 64, 64, dtype, [40, 30]), Case(1, 2, 64, 64, dtype, [1, 1])
+    for x in (c, one):
+        x.h = qe_mixer.GatedDelta(1, 2, 64, 64, dtype=dtype, t_max=70, seqs_max=2, l2norm=l2norm)
+        if not l2norm:
+            x.k *= 0.2
+    for x, kind, at in ((c, "prompt", 20), (one, "decode", 0)):
+        getattr(x, kind)([0, 2], [1, 3])
+        clean, pool, end = x.out.clone(), x.pool.clone(), x.cu[1]
+        assert bool(torch.isfinite(clean).all())
+        keep = x.k.clone()
+        x.k[at, 0, 5] = 3e19
+        getattr(x, kind)([0, 2], [1, 3])
+        x.k.copy_(keep)
+        assert bool(x.out[at:end].isnan().all()) and bool(x.pool[1].isnan().all()), kind
+        assert torch.equal(x.out[:at], clean[:at]) and torch.equal(x.out[end:], clean[end:]) and torch.equal(x.pool[3], pool[3])
+        if l2norm:
+            x.q[at, 0, 5] = 3e19
+            getattr(x, kind)([0, 2], [1, 3])
+            assert bool(x.out[at].isnan().all()), kind
+            assert torch.equal(x.out[:at], clean[:at]) and torch.equal(x.out[at + 1:], clean[at + 1:]) and torch.equal(x.pool[1], pool[1])
+        x.h.check()
+
+
 @pytest.mark.parametrize("what", [math.nan, math.inf])
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
 def test_values_that_are_not_finite_reach_no_earlier_token(what, dtype):
