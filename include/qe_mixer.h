@@ -120,7 +120,8 @@ int qe_attn_append(qe_attn_ctx *ctx, const qe_attn_batch *batch, const qe_kv_cac
  * to its own.  A row with none (cu_q gives more tokens than kv_len) is zeros.  q and out are of the context's type, strides
  * in elements, 16-byte aligned; out may be q (equal strides).  Scores, softmax
  * and sums are in 32 bits; probabilities are rounded to the context's type for
- * the product with V.  A V element that is infinite or NaN reaches the rows
+ * the product with V (fp16: below 2^-21 of a row's greatest, 2^-29 for single
+ * tokens, to fixed steps).  A V element that is infinite or NaN reaches the rows
  * that attend to its position, and no others. */
 int qe_attn_prompt(qe_attn_ctx *ctx, const qe_attn_batch *batch, const qe_kv_cache *cache, const void *q, int64_t q_stride,
                    void *out, int64_t out_stride, void *stream);

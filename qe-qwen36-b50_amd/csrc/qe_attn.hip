@@ -144,7 +144,7 @@ hipError_t qe_launch_append(const QeAppendArgs &a, int in_type, int type, hipStr
 // probabilities never cross lanes.  V reaches LDS by direct loads, its 64-byte units
 // permuted by row so that the four rows of a transposing read hit different banks.
 // Running maximum and sum in 32 bits per head; O is rescaled only when a maximum grew.  Probabilities are
-// rounded to the cache's type for the second product (their sum is of the unrounded ones).
+// rounded to the cache's type for the second product (exponent_base; their sum is of the unrounded ones).
 // Long lengths are bound by memory: one sequence of 100,000 keys, two key-value heads of 256, bf16, 205 MB:
 // 36 us, 5.7 TB/s, and 5 for the join; 24 sequences of 1 to 8,100 keys, eight heads of 128, fp16, 339 MB: 66 us,
 // 5.2 TB/s.  Short ones by latency: 700 keys take 10 us (length and page, keys and values, the exchange through
@@ -234,7 +234,7 @@ __global__ __launch_bounds__(256, 2) void k_attn_decode(const QeAttnArgs a) {
             l *= f;
             m = mn;
         }
-        const float base = m == -INFINITY ? 0.f : -m * a.scale_log2;
+        const float base = exponent_base<BF, 0>(m * a.scale_log2);
         float p[8];
         for (int i = 0; i < 4; ++i) {
             p[i] = __builtin_amdgcn_exp2f(fmaf(s[0][i], a.scale_log2, base));

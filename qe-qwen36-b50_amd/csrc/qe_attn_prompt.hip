@@ -15,7 +15,7 @@
 // phase lie in different banks, V's 64-byte units by row % 4.
 //
 // Scores, maxima and sums are in 32 bits; probabilities are rounded to the cache's type for the
-// second product.  A row's maximum is raised only where a score exceeds it by 2^8, so that O is seldom rescaled.
+// second product (exponent_base).  A row's maximum is raised only where a score exceeds it by 2^8, so that O is seldom rescaled.
 // Long prompts are bound by the matrix cores, whose issue the exponentials share: 8192 tokens of 16 heads of 256 (550
 // GFLOP), bf16, 505 to 540 us, 1020 to 1090 TFLOP/s where a large library product reaches 1219.  Five
 // prompts of 1999 tokens, 32 heads of 128, fp16: 38 us, the longest row blocks' 18 steps in turn.
@@ -131,6 +131,7 @@ struct Probs {
 
 template <bool BF, int DH>
 struct Rows {
+    static constexpr int LAG = 8;
     qe_f16v o[DH / 32]; // O^T
     qe_s8 q[DH / 16];
     float m, l; // running maximum of the scores (scaled, in powers of two) and sum
@@ -154,7 +155,7 @@ struct Rows {
     // The maximum that is subtracted only has to keep the powers of two in range: it follows the true one
     // when that has grown by more than 2^8, which after the first keys is rare.
     __device__ __forceinline__ void raise(float top) {
-        if (__any(top > m + 8.f)) {
+        if (__any(top > m + (float)LAG)) {
             const float mn = fmaxf(m, top), f = m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m - mn);
             if (__any(m != -INFINITY)) // else nothing is summed yet
 #pragma unroll
@@ -165,7 +166,7 @@ struct Rows {
     }
     template <int KB>
     __device__ __forceinline__ void exponentials(float scale, const Scores<KB> &x, Probs<KB> &p) {
-        const float base = m == -INFINITY ? 0.f : -m;
+        const float base = exponent_base<BF, LAG>(m);
         float sum[2] = {0, 0};
 #pragma unroll
         for (int b = 0; b < KB; ++b)

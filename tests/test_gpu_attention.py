@@ -195,6 +195,36 @@ def test_prompt_many_rows_over_many_splits(hq, hkv, dim):
     close(out, *c.expect(q, cu))
 
 
+@pytest.mark.parametrize("dim,n,below", [(64, 1 << 20, 26.0), (128, 100000, 25.1), (256, 40000, 27.0), (64, 3000, 20.0)])
+@pytest.mark.parametrize("first", [True, False])  # the great one's place
+def test_fp16_keys_far_below_the_greatest_count(dim, n, below, first):
+    """One key's score is above all others', whose weights fp16 does not hold at their own size, but together they are
+    0.03 to 1.5 % of the row's."""
+    page, scale = 256, dim ** -0.5
+    pages = -(-n // page)
+    kc, vc = (torch.zeros(pages, 1, page, dim, dtype=torch.float16, device="cuda") for _ in range(2))
+    table = torch.arange(pages, device="cuda", dtype=torch.int32)[None]
+    at = 0 if first else n - 1
+    kc[at // page, 0, at % page, 3] = 1.0
+    vc[:, 0] = torch.linspace(0.5, 2.0, dim, device="cuda").half()
+    vc[at // page, 0, at % page] = 0
+    q = torch.zeros(1, 2, dim, dtype=torch.float16, device="cuda")
+    q[:, 0, 3], q[:, 1, 3] = below * math.log(2) / scale, (below - 3) * math.log(2) / scale
+    att = qe_mixer.Attention(2, 1, dim, page, dtype=torch.float16)
+    for h in range(2):
+        want, _ = R.attend(q[:, h], kc.view(-1, dim)[:n], vc.view(-1, dim)[:n], torch.tensor([n - 1], device="cuda"), scale)
+        score = float(q[0, h, 3]) * scale
+        # as for all rows: a rounding of the result and one of the probabilities, the score's in 32 bits, the exponential's; and
+        # half of the fixed steps of fp16, 2^-25, at 2^15 and (prompts) at least 2^7 times the size, for each key
+        near = want.abs() * (2 * 2.0 ** -11 + 2 * dim * 2.0 ** -24 * score + 2.0 ** -18)
+        for up, cu in ((15, None), (7, ints([0, 1]))):
+            out = torch.empty_like(q)
+            (att.decode if cu is None else att.prompt)(qe_mixer.Batch(ints([n]), table, cu), q, kc, vc, out)
+            off = near + n * 2.0 ** (-25 - up) * 2.0
+            assert bool(((out[:, h].double() - want).abs() <= off).all()), (h, up, float(((out[:, h].double() - want).abs() / want).max()))
+    att.check()
+
+
 def test_prompt_rows_without_positions_are_zeros():
     c = Case(8, 2, 128, 16, torch.bfloat16, [3, 0, 20])
     cu = [0, 10, 14, 34]  # ten tokens of which three are in the cache, four of which none is
