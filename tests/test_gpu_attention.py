@@ -195,6 +195,20 @@ def test_prompt_many_rows_over_many_splits(hq, hkv, dim):
     close(out, *c.expect(q, cu))
 
 
+@pytest.mark.parametrize("hq,hkv,dim,lens,kv", [(32, 8, 128, (60, 70), (2600, 2700)), (24, 8, 64, (60, 110), (2700, 2500)), (16, 2, 256, (150, 151), (2560, 3000))])
+def test_prompt_more_than_eight_splits_of_more_than_4096_rows(hq, hkv, dim, lens, kv):
+    """One wave joins a row's splits there, however many they are."""
+    c = Case(hq, hkv, dim, 64, torch.float16, list(kv))
+    cu = [0, lens[0], sum(lens)]
+    tiles = (cu[2] * (hq // hkv) // 128 + 2) * hkv
+    assert tiles * 128 > 4096 and min(512 // tiles, -(-max(kv) // 256)) > 8  # the plan's, with row blocks of 128
+    q = c.q(cu[2])
+    out = torch.empty_like(q)
+    c.att.prompt(c.batch(cu, max_len=max(kv)), q, c.kc, c.vc, out)
+    c.att.check()
+    close(out, *c.expect(q, cu))
+
+
 @pytest.mark.parametrize("dim,n,below", [(64, 1 << 20, 26.0), (128, 100000, 25.1), (256, 40000, 27.0), (64, 3000, 20.0)])
 @pytest.mark.parametrize("first", [True, False])  # the great one's place
 def test_fp16_keys_far_below_the_greatest_count(dim, n, below, first):
