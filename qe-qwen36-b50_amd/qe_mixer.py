@@ -88,6 +88,13 @@ def _type(dtype, allowed):
     return TYPES[dtype]
 
 
+def _i32s(**sizes):
+    """ctypes cuts integers to 32 bits without a word: a size beyond them would be another size."""
+    for name, x in sizes.items():
+        if not -(1 << 31) <= x < 1 << 31:
+            _bad(f"{name} {x} does not fit 32 bits")
+
+
 # The checks are written for their cost: a single token's call is a few microseconds of GPU work, and a
 # tensor's shape, strides and device are fetched anew for every call.
 def _on(x, device, name):
@@ -138,6 +145,7 @@ class Batch:
             _ints(cu_q, (n + 1,), device, "cu_q")
         self.device, self.kv_len, self.table, self.cu_q, self.n_tokens = device, kv_len, table, cu_q, n_tokens
         stride = table.stride(0) if n > 1 else table.shape[1]
+        _i32s(sequences=n, table_stride=stride, pages=table.shape[1], max_len=int(max_len))
         self.c = _Batch(n, n, None if cu_q is None else cu_q.data_ptr(), kv_len.data_ptr(), table.data_ptr(), stride,
                         table.shape[1], int(max_len))
         self._ref = ctypes.byref(self.c)
@@ -162,6 +170,7 @@ class Attention:
         if len(s) > 3:
             _bad(f"sections {s}: at most three axes")
         s += (0,) * (3 - len(s))
+        _i32s(q_heads=q_heads, kv_heads=kv_heads, head_dim=head_dim, page=page, rotary=rotary, time=s[0], height=s[1], width=s[2])
         desc = _AttnDesc(q_heads, kv_heads, head_dim, page, _type(dtype, (torch.float16, torch.bfloat16)), scale, rotary, theta,
                          (_i32 * 3)(*s), int(interleaved))
         self.h = None
@@ -251,6 +260,7 @@ class GatedDelta:
     def __init__(self, k_heads, v_heads, dim_k, dim_v, dtype=torch.float32, t_max=8192, seqs_max=64, l2norm=True, scale=0.0,
                  device=0):
         lib = load()
+        _i32s(k_heads=k_heads, v_heads=v_heads, dim_k=dim_k, dim_v=dim_v, t_max=t_max, seqs_max=seqs_max)
         desc = _DeltaDesc(k_heads, v_heads, dim_k, dim_v, _type(dtype, tuple(TYPES)), int(l2norm), scale, t_max, seqs_max)
         self.h = None
         h = _vp()

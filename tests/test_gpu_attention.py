@@ -613,6 +613,14 @@ def test_refusals():
     a.check()
 
 
+def test_tables_of_far_rows_are_refused():
+    """Rows 2^32 + 8 apart are not rows 8 apart."""
+    far = torch.empty((1 << 32) + 16, dtype=torch.int32, device="cuda")
+    for kw in (dict(table=far.as_strided((2, 8), ((1 << 32) + 8, 1))), dict(table=far[:8].view(2, 4), max_len=(1 << 32) + 4)):
+        with pytest.raises(ValueError, match="32 bits"):
+            qe_mixer.Batch(ints([3, 4]), **kw)
+
+
 # -- streams, graphs ------------------------------------------------------------------
 def test_captured_calls_follow_the_lengths_in_device_memory():
     """append, prompt and decode in a graph, replayed as the sequences grow, with eager work between the replays."""

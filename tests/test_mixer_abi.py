@@ -54,6 +54,18 @@ def test_delta_geometries_that_are_refused(change):
     assert b"qe_delta_create" in lib.qe_moe_last_error()
 
 
+def test_sizes_beyond_32_bits_are_refused_by_the_binding():
+    """ctypes would cut them: a page of 2^32 + 256 positions, say, to one of 256."""
+    far = 1 << 32
+    fine = dict(q_heads=16, kv_heads=2, head_dim=256, page=256, rotary=64, theta=1e7, sections=(11, 11, 10))
+    for change in (dict(page=far + 256), dict(q_heads=far + 16), dict(rotary=far + 64), dict(sections=(far + 11, 11, 10)), dict(head_dim=256 - far)):
+        with pytest.raises(ValueError, match="32 bits"):
+            qe_mixer.Attention(**{**fine, **change})
+    for change in (dict(t_max=far + 64), dict(seqs_max=far + 1), dict(v_heads=far + 32)):
+        with pytest.raises(ValueError, match="32 bits"):
+            qe_mixer.GatedDelta(**{**dict(k_heads=16, v_heads=32, dim_k=128, dim_v=128), **change})
+
+
 def test_null_arguments():
     lib, h = qe_mixer.load(), ctypes.c_void_p()
     assert lib.qe_attn_create(0, None, ctypes.byref(h)) == qe_moe.QE_ERR_ARG
