@@ -272,6 +272,7 @@ __global__ __launch_bounds__(64 * WAVES, 2) void k_attn_prompt(const QeAttnArgs 
     if (__syncthreads_or(lo < hi ? lost_pages<64 * WAVES>(a, table, (len + (1 << a.page_log2) - 1) >> a.page_log2, tid) : 0)) {
         if (tid == 0) report(a.err, QE_BAD_PAGE);
         hi = lo; // no key: zeros
+        __builtin_amdgcn_s_waitcnt(0x0f70); // nothing reads what is on its way to LDS, but it lands before the workgroup ends
     }
 
     // The wave's direct loads have landed.  A probability of 0 times an infinity or NaN is NaN: in its part of V's tile t rows

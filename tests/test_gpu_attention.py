@@ -250,6 +250,18 @@ def test_prompt_rows_without_positions_are_zeros():
     assert bool((out[:7] == 0).all()) and bool((out[10:14] == 0).all()) and bool((out[7] != 0).any())
 
 
+@pytest.mark.parametrize("dim", [64, 128, 256])
+def test_prompt_rows_without_positions_are_zeros_in_several_splits(dim):
+    c = Case(8, 2, dim, 16, torch.float16, [3, 0, 20, 1500], extra_cols=1000)
+    cu = [0, 10, 14, 34, 40]
+    q = c.q(40)
+    out = torch.full_like(q, 7.0)
+    c.att.prompt(c.batch(cu), q, c.kc, c.vc, out)
+    c.att.check()
+    close(out, *c.expect(q, cu))
+    assert bool((out[:7] == 0).all()) and bool((out[10:14] == 0).all())
+
+
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
 @pytest.mark.parametrize("dim", [64, 128, 256])
 def test_prompt_values_that_are_not_finite_reach_their_rows_only(dim, dtype):
@@ -690,6 +702,28 @@ def test_two_graphs_share_a_context():
         for o, w in zip(outs, want):
             close(o, *w)
     c.att.check()
+
+
+def test_contexts_on_streams_of_their_own():
+    """Calls of two contexts that overlap share nothing: splits joined by the last workgroup, by a launch, and prompts'."""
+    cs = [Case(16, 2, 256, 64, torch.bfloat16, [3000, 900], seed=s) for s in (1, 2)]
+    qs, rows, streams = [c.q(2) for c in cs], [c.q(9) for c in cs], [torch.cuda.Stream() for _ in cs]
+    long_ = [Case(16, 2, 256, 64, torch.bfloat16, [20000], seed=s) for s in (3, 4)]
+    outs = [[(torch.empty_like(q), torch.empty_like(q[:1]), torch.empty_like(r)) for _ in range(6)] for q, r in zip(qs, rows)]
+    bs = [(c.batch(), l.batch(), c.batch([0, 4, 9])) for c, l in zip(cs, long_)]
+    torch.cuda.synchronize()
+    for k in range(6):
+        for i, s in enumerate(streams):
+            a, b, p = outs[i][k]
+            cs[i].att.decode(bs[i][0], qs[i], cs[i].kc, cs[i].vc, a, stream=s)
+            long_[i].att.decode(bs[i][1], qs[i][:1], long_[i].kc, long_[i].vc, b, stream=s)
+            cs[i].att.prompt(bs[i][2], rows[i], cs[i].kc, cs[i].vc, p, stream=s)
+    for i, s in enumerate(streams):
+        cs[i].att.check(s), long_[i].att.check(s)
+        want = cs[i].expect(qs[i], [0, 1, 2]), long_[i].expect(qs[i][:1], [0, 1]), cs[i].expect(rows[i], [0, 4, 9])
+        for got in outs[i]:
+            for x, w in zip(got, want):
+                close(x, *w)
 
 
 def test_results_do_not_change_from_call_to_call():
