@@ -32,57 +32,45 @@ __device__ __forceinline__ void store8(OUT *p, const float *x) {
 template <typename IN, typename OUT>
 __global__ __launch_bounds__(256) void k_append(const QeAppendArgs a) {
     __shared__ float2 cs[128];
-    __shared__ long row_s;
-    __shared__ int seq_s[2];
     const int t = blockIdx.x, tid = threadIdx.x, half = a.rotary / 2;
-    if (a.cu && tid >= 64) // all sequences' offsets, for the report: those that are wrong may hold no token
-        for (int64_t i = (int64_t)t * 192 + tid - 64; i < a.n_seqs; i += (int64_t)gridDim.x * 192)
+    if (a.cu && (int64_t)t * 256 < a.n_seqs) // all sequences' offsets, for the report: those that are wrong may hold no token
+        for (int64_t i = (int64_t)t * 256 + tid; i < a.n_seqs; i += (int64_t)gridDim.x * 256)
             if (qe_bad_offsets(a.cu[i], a.cu[i + 1], a.n_tokens)) report(a.err, QE_BAD_LENGTH);
-    if (tid < 64) { // the token's sequence: the last whose first row is not behind t
-        int seq = t, end = t + 1, len;
-        bool known = true;
-        if (!a.cu) {
-            len = a.kv_len[seq];
-        } else {
-            int lo = 0, hi = a.n_seqs; // cu[lo] <= t < cu[hi], as far as cu rises
-            while (hi - lo > 1) {
-                const int mid = (lo + hi) >> 1;
-                if (a.cu[mid] <= t) lo = mid;
-                else hi = mid;
-            }
-            // next to offsets that fall, it is not known whose the token is
-            const int before = a.cu[lo ? lo - 1 : 0], begin = a.cu[lo], after = a.cu[lo + 2 <= a.n_seqs ? lo + 2 : a.n_seqs];
-            end = a.cu[lo + 1], len = a.kv_len[lo];
-            known = before <= begin && end <= after && !qe_bad_offsets(begin, end, a.n_tokens);
-            seq = begin <= t && t < end ? lo : -1;
+    // the token's sequence, the last whose first row is not behind t, and its row in the cache: by every wave for itself, through
+    // the scalar cache, with no barrier
+    int seq = t, end = t + 1;
+    bool known = true;
+    if (a.cu) {
+        int lo = 0, hi = a.n_seqs; // cu[lo] <= t < cu[hi], as far as cu rises
+        while (hi - lo > 1) {
+            const int mid = (lo + hi) >> 1;
+            if (scalar_load(a.cu + mid) <= t) lo = mid;
+            else hi = mid;
         }
-        long row = -1;
-        int place = 0;
-        if (seq >= 0) {
-            unsigned bad = 0;
-            const int most = a.max_pages << a.page_log2;
-            len = qe_checked(len, 0, most, -1, &bad);
-            if (!known) bad = 1;
-            unsigned what = QE_BAD_LENGTH;
-            if (!bad) {
-                place = len - end + t;
-                if (place >= 0) {
-                    const unsigned p = (unsigned)a.table[(size_t)seq * a.table_stride + (place >> a.page_log2)];
-                    if (p >= a.n_pages) bad = 1, what = QE_BAD_PAGE;
-                    else row = ((long)p * a.kv_heads << a.page_log2) + (place & ((1 << a.page_log2) - 1));
-                }
-            }
-            if (bad) {
-                if (tid == 0) report(a.err, what);
-                seq = -1;
-            }
-        }
-        if (tid == 0) row_s = row, seq_s[0] = seq, seq_s[1] = place;
+        // next to offsets that fall, it is not known whose the token is
+        const int before = scalar_load(a.cu + (lo ? lo - 1 : 0)), begin = scalar_load(a.cu + lo), after = scalar_load(a.cu + (lo + 2 <= a.n_seqs ? lo + 2 : a.n_seqs));
+        end = scalar_load(a.cu + lo + 1);
+        known = before <= begin && end <= after && !qe_bad_offsets(begin, end, a.n_tokens);
+        if (t < begin || t >= end) return; // of no sequence
+        seq = lo;
     }
-    __syncthreads();
-    if (seq_s[0] < 0) return;
+    unsigned bad = 0;
+    const int len = qe_checked(scalar_load(a.kv_len + seq), 0, a.max_pages << a.page_log2, -1, &bad), place = len - end + t;
+    if (!known || bad) {
+        if (tid == 0) report(a.err, QE_BAD_LENGTH);
+        return;
+    }
+    long row = -1; // a token before the sequence's first position has none
+    if (place >= 0) {
+        const unsigned p = (unsigned)scalar_load(a.table + (size_t)seq * a.table_stride + (place >> a.page_log2));
+        if (p >= a.n_pages) {
+            if (tid == 0) report(a.err, QE_BAD_PAGE);
+            return;
+        }
+        row = ((long)p * a.kv_heads << a.page_log2) + (place & ((1 << a.page_log2) - 1));
+    }
     if (tid < half) {
-        const int pos = a.pos ? a.pos[(size_t)(a.n_axes > 1 ? a.axis[tid] : 0) * a.n_tokens + t] : seq_s[1];
+        const int pos = a.pos ? a.pos[(size_t)(a.n_axes > 1 ? a.axis[tid] : 0) * a.n_tokens + t] : place;
         const double turn = (double)pos * a.turns[tid];
         float s, c;
         sincospif((float)(2.0 * (turn - rint(turn))), &s, &c);
@@ -91,10 +79,9 @@ __global__ __launch_bounds__(256) void k_append(const QeAppendArgs a) {
     __syncthreads();
     const int per = a.head_dim / 16; // items of a head
     const int n_q = a.q ? a.q_heads * per : 0, n_k = a.kv_heads * per;
-    const long row = row_s;
     for (int it = tid; it < n_q + 2 * n_k; it += 256) {
         const int kind = it < n_q ? 0 : it < n_q + n_k ? 1 : 2, j = it - (kind == 0 ? 0 : kind == 1 ? n_q : n_q + n_k);
-        if (kind && row < 0) break; // a token before the sequence's first position
+        if (kind && row < 0) break;
         const int head = j / per, c = j - head * per;
         const bool turned = kind < 2 && c * 16 < a.rotary;
         const int e0 = turned ? c * 8 : c * 16, e1 = turned ? half + c * 8 : c * 16 + 8;
