@@ -209,6 +209,7 @@ __global__ __launch_bounds__(64 * WAVES, 2) void k_attn_prompt(const QeAttnArgs 
     __shared__ __align__(16) short k_a[BN * DH], v_a[BN * DH], k_b[BN * DH], v_b[BN * DH];
     // rows with an infinity or a NaN in V, of the tiles that some rows attend to in part: from `clear` on, BM tokens at most
     __shared__ unsigned long long odd_rows[BM / BN + 2];
+    __shared__ int lost_s[WAVES]; // a wave met a page that is none
     const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int split = blockIdx.x % a.splits, kvh = blockIdx.x / a.splits % a.kv_heads;
     const int tile = a.tiles - 1 - blockIdx.x / a.splits / a.kv_heads; // late rows have more keys: first
@@ -268,8 +269,14 @@ __global__ __launch_bounds__(64 * WAVES, 2) void k_attn_prompt(const QeAttnArgs 
             for (int i = 0; i < 16; ++i) w.o[d][i] = 0;
     }
     if (tid < BM / BN + 2) odd_rows[tid] = 0;
-    // (A barrier, too: the first tile's marks come before its own.  It waits for the loads of that tile, as its start does.)
-    if (__syncthreads_or(lo < hi ? lost_pages<64 * WAVES>(a, table, (len + (1 << a.page_log2) - 1) >> a.page_log2, tid) : 0)) {
+    const int lost = lo < hi ? lost_pages<64 * WAVES>(a, table, (len + (1 << a.page_log2) - 1) >> a.page_log2, tid) : 0;
+    if ((tid & 63) == 0) lost_s[wave] = 0;
+    if (lost) lost_s[wave] = 1;
+    lds_barrier(); // for odd_rows, too: the first tile's marks come before its own barrier
+    int any = 0;
+#pragma unroll
+    for (int i = 0; i < WAVES; ++i) any |= lost_s[i];
+    if (__builtin_amdgcn_readfirstlane(any)) {
         if (tid == 0) report(a.err, QE_BAD_PAGE);
         hi = lo; // no key: zeros
         __builtin_amdgcn_s_waitcnt(0x0f70); // nothing reads what is on its way to LDS, but it lands before the workgroup ends
