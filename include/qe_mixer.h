@@ -21,7 +21,8 @@
  * scratch, and may leave it unusable: give each its own context.  Entry points return 0 or a negative
  * QE_ERR_* code (qe_moe.h), and qe_moe_last_error() describes the calling
  * thread's last failure.  The calling thread's current device is left as it
- * was.
+ * was.  What a call writes may overlap what else it uses only where that is
+ * said below.
  *
  * What stands in device memory (lengths, page tables, slots) is checked by the
  * kernels: a bad value makes no access out of bounds, its sequence's outputs
@@ -109,8 +110,8 @@ typedef struct {
  * if in_type is the context's type and the strides are equal.  Pointers are
  * 16-byte aligned and strides multiples of 16 bytes.  A token before its
  * sequence's first position (cu_q gives more tokens than kv_len) writes nothing
- * to the cache; its q is rotated by pos or by its negative position.  A page that two
- * sequences of the call write at the same row gets one of the two. */
+ * to the cache; its q is rotated by pos or by its negative position.  A row of a
+ * page that two tokens of the call write may hold parts of both. */
 int qe_attn_append(qe_attn_ctx *ctx, const qe_attn_batch *batch, const qe_kv_cache *cache, int in_type, const void *q,
                    int64_t q_stride, const void *k, int64_t k_stride, const void *v, int64_t v_stride, const int32_t *pos,
                    void *q_out, int64_t q_out_stride, void *stream);
@@ -122,7 +123,8 @@ int qe_attn_append(qe_attn_ctx *ctx, const qe_attn_batch *batch, const qe_kv_cac
  * and sums are in 32 bits; probabilities are rounded to the context's type for
  * the product with V (fp16: below 2^-21 of a row's greatest, 2^-29 for single
  * tokens, to fixed steps).  A V element that is infinite or NaN reaches the rows
- * that attend to its position, and no others. */
+ * that attend to its position, and no others.  The last sequence's last rows are
+ * started first: a packed call is fastest with its longest sequences last. */
 int qe_attn_prompt(qe_attn_ctx *ctx, const qe_attn_batch *batch, const qe_kv_cache *cache, const void *q, int64_t q_stride,
                    void *out, int64_t out_stride, void *stream);
 
@@ -168,7 +170,9 @@ int qe_delta_destroy(qe_delta_ctx *ctx);
  * without tokens passes its state on as it is.  Tokens are causal: a q, k, v,
  * g or beta that is infinite or NaN reaches no token before its own and no
  * other sequence.  A key whose sum of squares passes the range of 32 bits (a
- * length of 1.8e19) counts as not finite, and with l2norm so does a query. */
+ * length of 1.8e19) counts as not finite, and with l2norm so does a query.  Where
+ * the rule itself leaves the range of 32 bits (g above 0 for long, or keys much
+ * longer than one without l2norm), other tokens of the same 64 may be NaN, too. */
 typedef struct {
     int n_seqs, n_tokens;
     const void *q, *k, *v;    /* [n_tokens] rows of k_heads * dim_k, k_heads * dim_k, v_heads * dim_v, of the context's type */

@@ -9,7 +9,7 @@
 // and pair, in LDS, for all of its heads.  A work item is 16 elements of a head: 8 pairs,
 // or 16 elements behind the rotated ones.  Bound by memory: q, k and v read and written.  8192
 // tokens of 32 + 2 x 8 heads of 128, fp16, 201 MB: 31 us, 6.4 TB/s (a large copy here reaches 5.1; part of
-// it stays in the last-level cache).  8 tokens: 4 us, of which most is the launch.  Stores that pass the caches by
+// it stays in the last-level cache); of 16 + 2 x 2 heads of 256 from fp32 to bf16, 252 MB: 39 us.  8 tokens: 4 us, of which most is the launch.  Stores that pass the caches by
 // save 2 of 40 us between calls on other data, and cost the attention that follows, which reads these rows, more.
 // ---------------------------------------------------------------------------
 template <typename IN>
@@ -133,8 +133,8 @@ hipError_t qe_launch_append(const QeAppendArgs &a, int in_type, int type, hipStr
 // Running maximum and sum in 32 bits per head; O is rescaled only when a maximum grew.  Probabilities are
 // rounded to the cache's type for the second product (exponent_base; their sum is of the unrounded ones).
 // Long lengths are bound by memory: one sequence of 100,000 keys, two key-value heads of 256, bf16, 205 MB:
-// 36 us, 5.7 TB/s, and 5 for the join; 24 sequences of 1 to 8,100 keys, eight heads of 128, fp16, 339 MB: 66 us,
-// 5.2 TB/s.  Short ones by latency: 700 keys take 10 us (length and page, keys and values, the exchange through
+// 37 us, 5.5 TB/s, and 5 for the join; 24 sequences of 38 to 8,095 keys, eight heads of 128, fp16, 339 MB: 70 us,
+// 4.8 TB/s.  Short ones by latency: 700 keys take 10 us (length and page, keys and values, the exchange through
 // memory, the join), where a launch that does nothing takes 2.
 // ---------------------------------------------------------------------------
 template <int DH>

@@ -17,9 +17,10 @@
 // Scores, maxima and sums are in 32 bits; probabilities are rounded to the cache's type for the
 // second product (exponent_base).  A row's maximum is raised only where a score exceeds it by 2^8, so that O is seldom rescaled.
 // Long prompts are bound by the matrix cores, whose issue the exponentials share: 8192 tokens of 16 heads of 256 (550
-// GFLOP), bf16, 505 to 540 us, 1020 to 1090 TFLOP/s where a large library product reaches 1219.  Five
+// GFLOP), bf16, 557 us on average of 30 in a row, under which the clock falls, and 511 at least: 990 and 1080 TFLOP/s where a
+// large library product reaches 1219.  Five
 // prompts of 1999 tokens, 32 heads of 128, fp16: 38 us, the longest row blocks' 18 steps in turn.
-// 100 tokens: 12 us, latency (lengths, pages, four steps, the output), much of it the code's first way through the
+// 100 tokens: 13 us, latency (lengths, pages, four steps, the output), much of it the code's first way through the
 // instruction cache: a workgroup whose code was three times as long, in steps of 64 keys with 512 registers, took 15.
 #include "qe_mixer_device.h"
 
@@ -212,7 +213,9 @@ __global__ __launch_bounds__(64 * WAVES, 2) void k_attn_prompt(const QeAttnArgs 
     __shared__ int lost_s[WAVES]; // a wave met a page that is none
     const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int split = blockIdx.x % a.splits, kvh = blockIdx.x / a.splits % a.kv_heads;
-    const int tile = a.tiles - 1 - blockIdx.x / a.splits / a.kv_heads; // late rows have more keys: first
+    // A sequence's late rows have more keys: first.  (So are the last sequence's, whatever its length: 31 prompts of 32 heads of
+    // 128, one of 1500 tokens and the others of 30, take 44 us with the long one last and 50 with it first.)
+    const int tile = a.tiles - 1 - blockIdx.x / a.splits / a.kv_heads;
     // Workgroup i looks at sequence i's offsets, for the report: where they fall, a sequence may have no tile below.  (There
     // are more workgroups than sequences; the others look at the last one's, so that no branch has its own wait for the loads.)
     const int mine = blockIdx.x < (unsigned)a.n_seqs ? blockIdx.x : a.n_seqs - 1;
@@ -389,8 +392,9 @@ __global__ __launch_bounds__(64 * WAVES, 2) void k_attn_prompt(const QeAttnArgs 
 }
 
 // The splits' results joined, W waves per query row: one, but for few rows over more than 8 splits a workgroup's four, each
-// over every fourth split.  (The call with one wave a row and with four: 240 rows of 256 over 40 splits 65 and 41 us, 2048 of
-// 128 over 21 60 and 54; but 6400 of 128 over 9 47 and 52, 16000 of 256 over 2 54 and 66.)
+// over every fourth split.  (The call with one wave a row and with four, of 16 and 2 heads of 256: 30 tokens after 10,000, 40
+// splits, 50 and 39 us, but 1000 tokens, 4 splits, 50 and 58; of 32 and 8 heads of 128: 64 after 5200, 21 splits, 42 and 36,
+// but 200 after 4000, 9 splits, 45 and 50.)
 template <bool BF, int DH, int BM, int W>
 __global__ __launch_bounds__(256) void k_attn_prompt_join(const QeAttnArgs a) {
     constexpr int E = DH / 64;

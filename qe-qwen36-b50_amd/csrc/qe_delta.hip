@@ -199,7 +199,7 @@ __global__ __launch_bounds__(256) void k_delta_decode(const QeDeltaArgs a) {
 // are not written), then per token e^b / |k|, scale e^b / |q|, e^(b_last - b) / |k|, and
 // e^(b_last).  fp16 and fp32 keys and queries are cut into planes here too, for a chunk and key
 // head: K [plane][64][DK] as it lies in LDS, Q [wave][32 of DK][plane][lane][8].
-// 8192 bf16 tokens of 16 key and 32 value heads of 128: 66 us, against 52 for its reads and writes at a large copy's
+// 8192 bf16 tokens of 16 key and 32 value heads of 128: 68 us (fp16 93, fp32 131), against 52 for its reads and writes at a large copy's
 // rate; the rest is the barriers between a head's short steps.
 // ---------------------------------------------------------------------------
 template <int DK>
@@ -225,8 +225,8 @@ __device__ __forceinline__ void load8_planes(const IN *p, bool there, qe_s8 *h, 
             for (int i = 0; i < 8; ++i) h[n][i] = next_plane(x[i]);
 }
 
-// (Three workgroups a CU, as the LDS allows: 1999 fp32 tokens of 16 and 32 heads of 128 take 37 us, with the registers
-// of two 51.  One chunk: 10 us, its steps' latency.)
+// (Three workgroups a CU, as the LDS allows: 1999 fp32 tokens of 16 and 32 heads of 128 take 38 us, with two 46, although
+// the 168 registers of three spill 14 there, in no other type or size.  One chunk: 10 us, its steps' latency.)
 template <typename IN, int DK>
 __global__ __launch_bounds__(256, 3) void k_delta_chunks(const QeDeltaArgs a) {
     constexpr int LD = 68, KS = DK / 32, NP = planes_of<IN>(), NO = sizeof(IN) == 4 ? 3 : 2;
@@ -419,15 +419,16 @@ __global__ __launch_bounds__(256, 3) void k_delta_chunks(const QeDeltaArgs a) {
 // result's registers are 4 consecutive rows of its column, an operand's 8.  K lies in LDS in
 // two buffers, the next chunk's loaded directly while this one's is used: its rows are
 // the first product's operand, and transposing reads give the third's.
-// What bounds it: the chain of products, exchanges and barriers of a chunk, on 256 of the
-// GPU's 1024 SIMDs for each sequence (32 heads, 8 slices).  A load stalls the wave that issues it
+// What bounds it: the chain of products, exchanges and barriers of a chunk, one chain wave on
+// each SIMD (a sequence of 32 heads in 8 slices is a workgroup for each of the 256 CUs).  A load stalls the wave that issues it
 // while the CU's 64 bytes a cycle are taken (some 65 KiB a chunk), so the loads are few and
-// wide, and spread over the waves and over the chunk.  8192 bf16 tokens of 32 heads of 128 x 128: 226 us, 1.8 a
-// chunk (of some 3,800 cycles K S takes 550, what is left of V to LDS 400, T times it 280, U to LDS 500,
-// the state's update and S to LDS 1,150, the rest is barriers); 1999 fp32 tokens of three prompts 84 us.
+// wide, and spread over the waves and over the chunk.  8192 bf16 tokens of 32 heads of 128 x 128: 240 us on
+// average of 30 in a row, 223 at least (fp16 303, fp32 418), 1.8 a chunk: of some 3,800 cycles K S takes 550, what is left
+// of V to LDS 400, T times it 280, U to LDS 500, the state's update and S to LDS 1,150, the rest is barriers.  1999 fp32
+// tokens of three prompts: 90 us.
 // ---------------------------------------------------------------------------
-// Where the LDS holds two workgroups (bf16, and fp16 keys of 64), 128 registers let it: sequences side by side overlap
-// (16 of 500 tokens, bf16: 355 us the call with one a CU, 296 with two; one of 8192 has one a CU, and takes the same in both forms).
+// Where the LDS holds two workgroups (bf16, and fp16 keys of 64), 128 registers let it, and the bound keeps it so: sequences
+// side by side overlap (16 of 500 tokens, bf16: 354 us the call with one a CU, 300 with two; one of 8192 has one a CU anyhow).
 template <typename IN, int DK, int DV>
 __global__ __launch_bounds__(512, sizeof(IN) == 2 && (DK == 64 || __is_same(IN, __bf16)) ? 4 : 2) void k_delta_scan(const QeDeltaArgs a) {
     constexpr int KS = DK / 32, SB = DK / 64, LS = DK + 8, LT = 72, NP = planes_of<IN>(), NO = sizeof(IN) == 4 ? 3 : 2;

@@ -23,8 +23,8 @@ QE_MIX_HD bool qe_fits_launch(int64_t workgroups, int threads) { return workgrou
 // A decode call gives a workgroup `steps` steps of QE_ATTN_TILE keys of one sequence and key-value
 // head, the same for all sequences, so that a ragged batch is even: `splits` workgroups are
 // launched for each, enough for max_len, and those behind a sequence's end do nothing.
-// One sequence: as many workgroups as the GPU holds at once, two or three a CU (LDS; one round of
-// 512 took 35 us over 100,000 keys of two heads of 256, 695 took 41), of at least two steps.
+// One sequence: as many workgroups as the GPU holds at once, two or three a CU (LDS; a round of at most
+// 512 takes 37 us over 100,000 keys of two heads of 256, 696 take 40), of at least two steps.
 // Several, which may differ in length: up to 2048, but of at least eight steps where that
 // many fill the GPU.  units = n_seqs * kv_heads.
 QE_MIX_HD void qe_attn_decode_plan(int64_t n_seqs, int64_t kv_heads, int head_dim, int64_t max_len, int *steps, int *splits) {
@@ -76,8 +76,11 @@ QE_MIX_HD int qe_attn_prompt_rows(int n_tokens, int n_seqs, int group, int kv_he
     return head_dim == 256 && (int64_t)qe_attn_max_tiles(n_tokens, n_seqs, group, 256) * kv_heads >= 256 ? 256 : 128;
 }
 
-// Splits of a prompt call's keys: none if its tiles fill half the CUs (528 tiles in two splits: 80 us, 50 in one), else
-// two workgroups for each CU, of at least 256 keys.
+// Splits of a prompt call's keys: two workgroups for each CU, of at least 256 keys; above 128 tiles none.  Where the tiles
+// fill the GPU a split only adds the join: 528 tiles take 47 us a call, and 78 in two splits.  From 129 to 255 tiles, which
+// leave half of the places empty, it is right over short keys (900 tokens of 32 and 8 heads of 128: 34 us, 45 in two
+// splits; 1200 of 24 and 8 heads of 64: 31, 39) and wrong over long ones (2000 tokens of 16 and 2 heads of 256: 92 us, 84 in
+// two; 16 x 4 after 8000 with heads of 128: 165, 123 in three; 600 after 20,000: 404, 260).
 QE_MIX_HD int qe_attn_prompt_splits(int64_t tiles, int64_t max_len) {
     if (tiles > 128) return 1;
     const int64_t most = (max_len + 255) / 256, want = QE_ATTN_WGS / tiles;
@@ -122,7 +125,7 @@ QE_MIX_HD int qe_delta_first_chunk(int cu, int i) { return cu / QE_DELTA_C + i; 
 QE_MIX_HD int qe_delta_kept_planes(int bytes, int is_bf16) { return is_bf16 ? 0 : bytes == 4 ? 3 : 2; }
 // Value heads of a workgroup that makes a chunk's matrices: all of the key head's, which share the products of keys and
 // queries, unless a workgroup for each is no more than the GPU holds at once, three a CU (one bf16 chunk of 16 and 32
-// heads: 10 us, and 14 with two heads a workgroup).
+// heads: 10 us, and 15 with two heads a workgroup).
 QE_MIX_HD int qe_delta_heads(int64_t chunks, int v_heads, int group) { return chunks * v_heads <= 768 ? 1 : group; }
 QE_MIX_HD int qe_delta_max_chunks(int n_tokens, int n_seqs) { return n_tokens / QE_DELTA_C + n_seqs; }
 

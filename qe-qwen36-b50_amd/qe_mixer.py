@@ -3,7 +3,8 @@ paged key-value cache, and the gated delta rule.
 
 Tensors are torch tensors on the context's device; types, shapes and strides
 are checked here, the rest by the library.  The calls run on the stream that is
-given (None = the default stream) and return without a synchronisation.  There is
+given (None = the default stream) and return without a synchronisation: a tensor of
+another stream is not freed before they have run (torch: record_stream).  There is
 no fallback: without the library, LibraryMissing is raised.
 """
 from __future__ import annotations
