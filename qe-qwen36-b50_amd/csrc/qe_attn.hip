@@ -9,8 +9,9 @@
 // and pair, in LDS, for all of its heads.  A work item is 16 elements of a head: 8 pairs,
 // or 16 elements behind the rotated ones.  Bound by memory: q, k and v read and written.  8192
 // tokens of 32 + 2 x 8 heads of 128, fp16, 201 MB: 31 us, 6.4 TB/s (a large copy here reaches 5.1; part of
-// it stays in the last-level cache); of 16 + 2 x 2 heads of 256 from fp32 to bf16, 252 MB: 39 us.  8 tokens: 4 us, of which most is the launch.  Stores that pass the caches by
-// save 2 of 40 us between calls on other data, and cost the attention that follows, which reads these rows, more.
+// it stays in the last-level cache); of 16 + 2 x 2 heads of 256 from fp32 to bf16, 252 MB: 39 us.  8 tokens: 4 us, of
+// which most is the launch.  Stores that pass the caches by save 2 of 40 us between calls on other data, and cost the
+// attention that follows, which reads these rows, more.
 // ---------------------------------------------------------------------------
 template <typename IN>
 __device__ __forceinline__ void load8(const IN *p, float *x) {

@@ -272,9 +272,8 @@ __global__ __launch_bounds__(64 * WAVES, 2) void k_attn_prompt(const QeAttnArgs 
             for (int i = 0; i < 16; ++i) w.o[d][i] = 0;
     }
     if (tid < BM / BN + 2) odd_rows[tid] = 0;
-    const int lost = lo < hi ? lost_pages<64 * WAVES>(a, table, (len + (1 << a.page_log2) - 1) >> a.page_log2, tid) : 0;
-    if ((tid & 63) == 0) lost_s[wave] = 0;
-    if (lost) lost_s[wave] = 1;
+    const int lost = __any(lo < hi ? lost_pages<64 * WAVES>(a, table, (len + (1 << a.page_log2) - 1) >> a.page_log2, tid) : 0);
+    if ((tid & 63) == 0) lost_s[wave] = lost;
     lds_barrier(); // for odd_rows, too: the first tile's marks come before its own barrier
     int any = 0;
 #pragma unroll

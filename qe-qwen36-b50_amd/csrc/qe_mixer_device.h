@@ -52,7 +52,7 @@ __device__ __forceinline__ float from16(short x) {
 
 // Probabilities, rounded to the cache's type for the product with V, are kept 2^UP times as large where the type is fp16,
 // and so is their sum: fp16 has fixed steps below 2^-14 and nothing below 2^-25, and of 2^20 keys at 2^-25.1 of the
-// greatest, 2.8 % of a row's weight, none would count.  Half of fp16's greatest power of two is the most they reach:
+// greatest, 2.8 % of a row's weight, none would count.  2^15, fp16's greatest power of two, is the most they reach:
 // where the subtracted maximum may lag behind the true one by 2^LAG, UP is 15 - LAG.
 template <bool BF, int LAG>
 __device__ __forceinline__ float exponent_base(float m) { return m == -INFINITY ? 0.f : (BF ? 0.f : 15.f - LAG) - m; }
