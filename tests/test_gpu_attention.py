@@ -494,6 +494,29 @@ def test_bad_pages_give_zeros_for_all_rows_of_a_prompt(hq, hkv, dim, page, lens,
     c.att.check()
 
 
+@pytest.mark.parametrize("hq,hkv,dim,rows", [(2, 1, 64, 3), (16, 16, 256, 4000)])  # workgroups of 256 and of 512 threads
+def test_bad_pages_anywhere_in_a_long_table_are_found(hq, hkv, dim, rows):
+    page, n = 16, 5000 * 16 - 5
+    kc, vc = (torch.ones(3, hkv, page, dim, dtype=torch.bfloat16, device="cuda") for _ in range(2))
+    table = torch.randint(0, 3, (1, 5001), generator=gen(1), device="cuda").to(torch.int32)
+    table[0, 5000] = -1  # behind the sequence
+    att = qe_mixer.Attention(hq, hkv, dim, page)
+    q = rand(gen(2), rows, hq, dim, dtype=torch.bfloat16)
+    out = torch.empty_like(q)
+    for at in (None, 0, 1, 255, 256, 511, 512, 767, 768, 1023, 1024, 2047, 2048, 3333, 4095, 4096, 4999):
+        bad = table.clone()
+        if at is not None:
+            bad[0, at] = 3 if at % 2 else -1
+        att.prompt(qe_mixer.Batch(ints([n]), bad, ints([0, rows]), max_len=n), q, kc, vc, out)
+        if at is None:
+            att.check()
+            assert bool(((out.float() - 1).abs() <= 2 * 2.0 ** -8).all())  # an average of ones
+        else:
+            with pytest.raises(qe_moe.QeError, match="page"):
+                att.check()
+            assert bool((out == 0).all()), at
+
+
 def test_bad_lengths_give_zeros_and_an_error():
     c = Case(8, 2, 64, 32, torch.float16, [50, 60])
     q = c.q(2)
