@@ -133,6 +133,56 @@ int qe_attn_prompt(qe_attn_ctx *ctx, const qe_attn_batch *batch, const qe_kv_cac
 int qe_attn_decode(qe_attn_ctx *ctx, const qe_attn_batch *batch, const qe_kv_cache *cache, const void *q, int64_t q_stride,
                    void *out, int64_t out_stride, void *stream);
 
+/* ---- norms with the rotation, and an 8-bit cache ---------------------------- */
+
+/* Norms of q's and k's heads before the rotation: x <- x / sqrt(mean(x^2) +
+ * eps) * weight, in 32 bits.  Weights are device memory, fp32 [head_dim],
+ * 16-byte aligned, the same for all heads; NULL: q (or k) is not normed.
+ * eps > 0.  A head whose squares sum beyond the range of 32 bits is NaN. */
+typedef struct {
+    const float *q_weight, *k_weight;
+    float eps;
+} qe_attn_norm;
+
+/* qe_attn_append with norms: q and k are normed and then rotated, v is as it is. */
+int qe_attn_append_normed(qe_attn_ctx *ctx, const qe_attn_batch *batch, const qe_kv_cache *cache, const qe_attn_norm *norm, int in_type,
+                          const void *q, int64_t q_stride, const void *k, int64_t k_stride, const void *v, int64_t v_stride,
+                          const int32_t *pos, void *q_out, int64_t q_out_stride, void *stream);
+
+/* Element types of an 8-bit cache: integers -127 .. 127, and floating point of
+ * 4 exponent bits (bias 7) and 3 more (448 is the greatest, no infinities). */
+#define QE_I8 3
+#define QE_F8 4
+
+/* An 8-bit cache: pages as in qe_kv_cache, [kv_heads][page][head_dim] codes of
+ * one byte, and a scale for each of their rows, [n_pages][kv_heads][page]: an
+ * element is code times scale.  All are 16-byte aligned.  (QE_F8: a code that is NaN is no
+ * value of a cache; where a position has one, its sequence's outputs may be NaN.) */
+typedef struct {
+    void *k, *v;
+    float *k_scale, *v_scale;
+    int64_t n_pages; /* 1 .. 2^31 - 1 */
+    int type;        /* QE_I8 or QE_F8 */
+} qe_kv_cache8;
+
+/* qe_attn_append to an 8-bit cache, with norms (norm may be NULL: none).  A row
+ * x of k or v has the scale max |x| / 127 (QE_F8: / 448) and the codes x /
+ * scale, rounded to nearest, in 32 bits: x is not rounded to 16 bits before.  A
+ * row whose greatest is below 2^-100 has the scale 0; one with an element that
+ * is not finite has the scale NaN, and all of its elements are NaN. */
+int qe_attn_append8(qe_attn_ctx *ctx, const qe_attn_batch *batch, const qe_kv_cache8 *cache, const qe_attn_norm *norm, int in_type,
+                    const void *q, int64_t q_stride, const void *k, int64_t k_stride, const void *v, int64_t v_stride,
+                    const int32_t *pos, void *q_out, int64_t q_out_stride, void *stream);
+
+/* The inverse: the keys and values that an 8-bit cache holds for the positions
+ * of the call's tokens, rounded to the context's type, in rows of kv_heads *
+ * head_dim (either of k and v may be NULL).  With cu_q the sums of kv_len all of
+ * a batch's positions are read.  A token before its sequence's first position,
+ * one whose length or page is bad, and one beside offsets that fall has rows of
+ * zeros; rows of no sequence are left as they were. */
+int qe_attn_read8(qe_attn_ctx *ctx, const qe_attn_batch *batch, const qe_kv_cache8 *cache, void *k, int64_t k_stride, void *v, int64_t v_stride,
+                  void *stream);
+
 /* Synchronise `stream` and report a bad length or page that a kernel met. */
 int qe_attn_check(qe_attn_ctx *ctx, void *stream);
 

@@ -34,44 +34,11 @@ template <typename IN, typename OUT>
 __global__ __launch_bounds__(256) void k_append(const QeAppendArgs a) {
     __shared__ float2 cs[128];
     const int t = blockIdx.x, tid = threadIdx.x, half = a.rotary / 2;
-    if (a.cu && (int64_t)t * 256 < a.n_seqs) // all sequences' offsets, for the report: those that are wrong may hold no token
-        for (int64_t i = (int64_t)t * 256 + tid; i < a.n_seqs; i += (int64_t)gridDim.x * 256)
-            if (qe_bad_offsets(a.cu[i], a.cu[i + 1], a.n_tokens)) report(a.err, QE_BAD_LENGTH);
-    // the token's sequence, the last whose first row is not behind t, and its row in the cache: by every wave for itself, through
-    // the scalar cache, with no barrier
-    int seq = t, end = t + 1;
-    bool known = true;
-    if (a.cu) {
-        int lo = 0, hi = a.n_seqs; // cu[lo] <= t < cu[hi], as far as cu rises
-        while (hi - lo > 1) {
-            const int mid = (lo + hi) >> 1;
-            if (scalar_load(a.cu + mid) <= t) lo = mid;
-            else hi = mid;
-        }
-        // next to offsets that fall, it is not known whose the token is
-        const int before = scalar_load(a.cu + (lo ? lo - 1 : 0)), begin = scalar_load(a.cu + lo), after = scalar_load(a.cu + (lo + 2 <= a.n_seqs ? lo + 2 : a.n_seqs));
-        end = scalar_load(a.cu + lo + 1);
-        known = before <= begin && end <= after && !qe_bad_offsets(begin, end, a.n_tokens);
-        if (t < begin || t >= end) return; // of no sequence
-        seq = lo;
-    }
-    unsigned bad = 0;
-    const int len = qe_checked(scalar_load(a.kv_len + seq), 0, a.max_pages << a.page_log2, -1, &bad), place = len - end + t;
-    if (!known || bad) {
-        if (tid == 0) report(a.err, QE_BAD_LENGTH);
-        return;
-    }
-    long row = -1; // a token before the sequence's first position has none
-    if (place >= 0) {
-        const unsigned p = (unsigned)scalar_load(a.table + (size_t)seq * a.table_stride + (place >> a.page_log2));
-        if (p >= a.n_pages) {
-            if (tid == 0) report(a.err, QE_BAD_PAGE);
-            return;
-        }
-        row = ((long)p * a.kv_heads << a.page_log2) + (place & ((1 << a.page_log2) - 1));
-    }
+    report_offsets(a);
+    QeToken at;
+    if (!token_place(a, t, tid == 0, at)) return;
     if (tid < half) {
-        const int pos = a.pos ? a.pos[(size_t)(a.n_axes > 1 ? a.axis[tid] : 0) * a.n_tokens + t] : place;
+        const int pos = a.pos ? a.pos[(size_t)(a.n_axes > 1 ? a.axis[tid] : 0) * a.n_tokens + t] : at.place;
         const double turn = (double)pos * a.turns[tid];
         float s, c;
         sincospif((float)(2.0 * (turn - rint(turn))), &s, &c);
@@ -82,7 +49,7 @@ __global__ __launch_bounds__(256) void k_append(const QeAppendArgs a) {
     const int n_q = a.q ? a.q_heads * per : 0, n_k = a.kv_heads * per;
     for (int it = tid; it < n_q + 2 * n_k; it += 256) {
         const int kind = it < n_q ? 0 : it < n_q + n_k ? 1 : 2, j = it - (kind == 0 ? 0 : kind == 1 ? n_q : n_q + n_k);
-        if (kind && row < 0) break;
+        if (kind && at.row < 0) break;
         const int head = j / per, c = j - head * per;
         const bool turned = kind < 2 && c * 16 < a.rotary;
         const int e0 = turned ? c * 8 : c * 16, e1 = turned ? half + c * 8 : c * 16 + 8;
@@ -101,7 +68,7 @@ __global__ __launch_bounds__(256) void k_append(const QeAppendArgs a) {
                 y[i] = fmaf(w, r.x, u * r.y);
             }
         OUT *dst = kind == 0 ? (OUT *)a.q_out + (size_t)t * a.q_out_stride + (size_t)head * a.head_dim
-                             : (OUT *)(kind == 1 ? a.kc : a.vc) + (row + ((long)head << a.page_log2)) * a.head_dim;
+                             : (OUT *)(kind == 1 ? a.kc : a.vc) + (at.row + ((long)head << a.page_log2)) * a.head_dim;
         store8(dst + e0, x);
         store8(dst + e1, y);
     }

@@ -41,6 +41,26 @@ struct QeAppendArgs {
     unsigned *err;
 };
 
+// Norms, and an 8-bit cache: `a` with kc and vc codes (or 16-bit elements).
+struct QeAppend8Args {
+    QeAppendArgs a;
+    const float *wq, *wk; // norms' weights, or null
+    float eps;
+    float *ks, *vs; // scales
+};
+struct QeRead8Args {
+    const void *kc, *vc;
+    const float *ks, *vs;
+    void *k, *v;
+    int64_t k_stride, v_stride;
+    const int32_t *cu, *kv_len, *table;
+    int n_seqs, n_tokens, table_stride, max_pages, kv_heads, head_dim, page_log2;
+    unsigned n_pages;
+    unsigned *err;
+};
+
+hipError_t qe_launch_append8(const QeAppend8Args &a, int in_type, int type, int cache_type, hipStream_t st);
+hipError_t qe_launch_read8(const QeRead8Args &a, int type, int cache_type, hipStream_t st);
 hipError_t qe_launch_append(const QeAppendArgs &a, int in_type, int type, hipStream_t st);
 hipError_t qe_launch_attn_decode(const QeAttnArgs &a, int head_dim, int type, hipStream_t st);
 hipError_t qe_launch_attn_prompt(const QeAttnArgs &a, int head_dim, int type, int bm, hipStream_t st);

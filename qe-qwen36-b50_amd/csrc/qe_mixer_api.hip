@@ -100,8 +100,7 @@ size_t part_rows() {
     return decode > prompt ? decode : prompt;
 }
 
-int check_batch(const qe_attn_ctx *c, const qe_attn_batch *b, const qe_kv_cache *kv, const char *where) {
-    if (!c || !b || !kv) return qe_fail(QE_ERR_ARG, "%s: null context, batch or cache", where);
+int check_seqs(const qe_attn_ctx *c, const qe_attn_batch *b, const char *where) {
     if (b->n_seqs < 1 || b->n_seqs > 65535) return qe_fail(QE_ERR_ARG, "%s: n_seqs %d is not 1 .. 65535", where, b->n_seqs);
     if (b->n_tokens < 0 || b->n_tokens >= 1 << 24) return qe_fail(QE_ERR_ARG, "%s: n_tokens %d is not 0 .. 2^24 - 1", where, b->n_tokens);
     if (!b->cu_q && b->n_tokens != b->n_seqs)
@@ -110,9 +109,25 @@ int check_batch(const qe_attn_ctx *c, const qe_attn_batch *b, const qe_kv_cache 
     if (b->max_pages < 1 || (int64_t)b->max_pages * c->d.page > 1 << 30 || b->table_stride < b->max_pages)
         return qe_fail(QE_ERR_ARG, "%s: max_pages %d (of %d positions), table_stride %d", where, b->max_pages, c->d.page, b->table_stride);
     if (b->max_len < 0) return qe_fail(QE_ERR_ARG, "%s: max_len %d", where, b->max_len);
-    if (!kv->k || !kv->v || !aligned16(kv->k) || !aligned16(kv->v))
-        return qe_fail(QE_ERR_ARG, "%s: cache arrays are null or not 16-byte aligned", where);
-    if (kv->n_pages < 1 || kv->n_pages > 0x7fffffff) return qe_fail(QE_ERR_ARG, "%s: n_pages %lld", where, (long long)kv->n_pages);
+    return QE_OK;
+}
+int check_pages(const void *k, const void *v, int64_t n_pages, const char *where) {
+    if (!k || !v || !aligned16(k) || !aligned16(v)) return qe_fail(QE_ERR_ARG, "%s: cache arrays are null or not 16-byte aligned", where);
+    if (n_pages < 1 || n_pages > 0x7fffffff) return qe_fail(QE_ERR_ARG, "%s: n_pages %lld", where, (long long)n_pages);
+    return QE_OK;
+}
+int check_batch(const qe_attn_ctx *c, const qe_attn_batch *b, const qe_kv_cache *kv, const char *where) {
+    if (!c || !b || !kv) return qe_fail(QE_ERR_ARG, "%s: null context, batch or cache", where);
+    const int rc = check_seqs(c, b, where);
+    return rc != QE_OK ? rc : check_pages(kv->k, kv->v, kv->n_pages, where);
+}
+int check_batch(const qe_attn_ctx *c, const qe_attn_batch *b, const qe_kv_cache8 *kv, const char *where) {
+    if (!c || !b || !kv) return qe_fail(QE_ERR_ARG, "%s: null context, batch or cache", where);
+    int rc = check_seqs(c, b, where);
+    if (rc != QE_OK || (rc = check_pages(kv->k, kv->v, kv->n_pages, where)) != QE_OK) return rc;
+    if (kv->type != QE_I8 && kv->type != QE_F8) return qe_fail(QE_ERR_ARG, "%s: cache type %d is neither QE_I8 nor QE_F8", where, kv->type);
+    if (!kv->k_scale || !kv->v_scale || !aligned16(kv->k_scale) || !aligned16(kv->v_scale))
+        return qe_fail(QE_ERR_ARG, "%s: the cache's scales are null or not 16-byte aligned", where);
     return QE_OK;
 }
 
@@ -211,11 +226,10 @@ int qe_attn_destroy(qe_attn_ctx *c) {
     return QE_OK;
 }
 
-int qe_attn_append(qe_attn_ctx *c, const qe_attn_batch *b, const qe_kv_cache *kv, int in_type, const void *q, int64_t q_stride, const void *k,
-                   int64_t k_stride, const void *v, int64_t v_stride, const int32_t *pos, void *q_out, int64_t q_out_stride, void *stream) {
-    static const char *const where = "qe_attn_append";
-    int rc = check_batch(c, b, kv, where);
-    if (rc != QE_OK) return rc;
+// What the three calls that write a cache share; kv (or kv8) is checked.
+static int append_args(const qe_attn_ctx *c, const qe_attn_batch *b, int in_type, const void *q, int64_t q_stride, const void *k, int64_t k_stride,
+                       const void *v, int64_t v_stride, const int32_t *pos, void *q_out, int64_t q_out_stride, const char *where, QeAppendArgs *a) {
+    int rc;
     if (in_type != QE_F32 && in_type != c->d.type) return qe_fail(QE_ERR_ARG, "%s: in_type %d, the cache has type %d", where, in_type, c->d.type);
     if (!q != !q_out) return qe_fail(QE_ERR_ARG, "%s: q and q_out go together", where);
     const int64_t qw = (int64_t)c->d.q_heads * c->d.head_dim, kw = (int64_t)c->d.kv_heads * c->d.head_dim;
@@ -227,20 +241,95 @@ int qe_attn_append(qe_attn_ctx *c, const qe_attn_batch *b, const qe_kv_cache *kv
         if ((rc = check_rows(k, k_stride, kw, in_type, "k", where)) != QE_OK) return rc;
         if ((rc = check_rows(v, v_stride, kw, in_type, "v", where)) != QE_OK) return rc;
     }
-    if ((rc = c->err.take(where)) != QE_OK) return rc;
-    if (b->n_tokens == 0) return QE_OK;
+    a->q = q; a->k = k; a->v = v; a->q_out = q_out;
+    a->q_stride = q_stride; a->k_stride = k_stride; a->v_stride = v_stride; a->q_out_stride = q_out_stride;
+    a->pos = pos; a->cu = b->cu_q; a->kv_len = b->kv_len; a->table = b->table;
+    a->turns = c->turns; a->axis = c->axis;
+    a->n_axes = c->n_axes; a->n_seqs = b->n_seqs; a->n_tokens = b->n_tokens; a->table_stride = b->table_stride; a->max_pages = b->max_pages;
+    a->q_heads = c->d.q_heads; a->kv_heads = c->d.kv_heads; a->head_dim = c->d.head_dim; a->page_log2 = log2_of(c->d.page); a->rotary = c->d.rotary;
+    a->err = c->err.dev;
+    return QE_OK;
+}
+
+int qe_attn_append(qe_attn_ctx *c, const qe_attn_batch *b, const qe_kv_cache *kv, int in_type, const void *q, int64_t q_stride, const void *k,
+                   int64_t k_stride, const void *v, int64_t v_stride, const int32_t *pos, void *q_out, int64_t q_out_stride, void *stream) {
+    static const char *const where = "qe_attn_append";
     QeAppendArgs a{};
-    a.q = q; a.k = k; a.v = v; a.q_out = q_out; a.kc = kv->k; a.vc = kv->v;
-    a.q_stride = q_stride; a.k_stride = k_stride; a.v_stride = v_stride; a.q_out_stride = q_out_stride;
-    a.pos = pos; a.cu = b->cu_q; a.kv_len = b->kv_len; a.table = b->table;
-    a.turns = c->turns; a.axis = c->axis;
-    a.n_axes = c->n_axes; a.n_seqs = b->n_seqs; a.n_tokens = b->n_tokens; a.table_stride = b->table_stride; a.max_pages = b->max_pages;
-    a.q_heads = c->d.q_heads; a.kv_heads = c->d.kv_heads; a.head_dim = c->d.head_dim; a.page_log2 = log2_of(c->d.page); a.rotary = c->d.rotary;
+    int rc = check_batch(c, b, kv, where);
+    if (rc != QE_OK || (rc = append_args(c, b, in_type, q, q_stride, k, k_stride, v, v_stride, pos, q_out, q_out_stride, where, &a)) != QE_OK) return rc;
+    if ((rc = c->err.take(where)) != QE_OK || b->n_tokens == 0) return rc;
+    a.kc = kv->k; a.vc = kv->v; a.n_pages = (unsigned)kv->n_pages;
+    OnDevice on(c->device);
+    HIP_TRY(on.e);
+    HIP_TRY(qe_launch_append(a, in_type, c->d.type, (hipStream_t)stream));
+    return QE_OK;
+}
+
+static int check_norm(const qe_attn_norm *n, const char *where) {
+    if (!aligned16(n->q_weight) || !aligned16(n->k_weight)) return qe_fail(QE_ERR_ARG, "%s: the norms' weights are not 16-byte aligned", where);
+    if (!(n->eps >= 1e-30f) || !isfinite(n->eps)) return qe_fail(QE_ERR_ARG, "%s: eps %g is not 1e-30 or more", where, n->eps);
+    return QE_OK;
+}
+
+int qe_attn_append_normed(qe_attn_ctx *c, const qe_attn_batch *b, const qe_kv_cache *kv, const qe_attn_norm *norm, int in_type, const void *q,
+                          int64_t q_stride, const void *k, int64_t k_stride, const void *v, int64_t v_stride, const int32_t *pos, void *q_out,
+                          int64_t q_out_stride, void *stream) {
+    static const char *const where = "qe_attn_append_normed";
+    QeAppend8Args x{};
+    int rc = check_batch(c, b, kv, where);
+    if (rc != QE_OK || (rc = append_args(c, b, in_type, q, q_stride, k, k_stride, v, v_stride, pos, q_out, q_out_stride, where, &x.a)) != QE_OK) return rc;
+    if (!norm) return qe_fail(QE_ERR_ARG, "%s: null norm (without norms: qe_attn_append)", where);
+    if ((rc = check_norm(norm, where)) != QE_OK) return rc;
+    if ((rc = c->err.take(where)) != QE_OK || b->n_tokens == 0) return rc;
+    x.a.kc = kv->k; x.a.vc = kv->v; x.a.n_pages = (unsigned)kv->n_pages;
+    x.wq = norm->q_weight; x.wk = norm->k_weight; x.eps = norm->eps;
+    OnDevice on(c->device);
+    HIP_TRY(on.e);
+    HIP_TRY(qe_launch_append8(x, in_type, c->d.type, c->d.type, (hipStream_t)stream));
+    return QE_OK;
+}
+
+int qe_attn_append8(qe_attn_ctx *c, const qe_attn_batch *b, const qe_kv_cache8 *kv, const qe_attn_norm *norm, int in_type, const void *q,
+                    int64_t q_stride, const void *k, int64_t k_stride, const void *v, int64_t v_stride, const int32_t *pos, void *q_out,
+                    int64_t q_out_stride, void *stream) {
+    static const char *const where = "qe_attn_append8";
+    QeAppend8Args x{};
+    int rc = check_batch(c, b, kv, where);
+    if (rc != QE_OK || (rc = append_args(c, b, in_type, q, q_stride, k, k_stride, v, v_stride, pos, q_out, q_out_stride, where, &x.a)) != QE_OK) return rc;
+    if (norm && (rc = check_norm(norm, where)) != QE_OK) return rc;
+    if ((rc = c->err.take(where)) != QE_OK || b->n_tokens == 0) return rc;
+    x.a.kc = kv->k; x.a.vc = kv->v; x.a.n_pages = (unsigned)kv->n_pages;
+    x.ks = kv->k_scale; x.vs = kv->v_scale;
+    if (norm) x.wq = norm->q_weight, x.wk = norm->k_weight, x.eps = norm->eps;
+    OnDevice on(c->device);
+    HIP_TRY(on.e);
+    HIP_TRY(qe_launch_append8(x, in_type, c->d.type, kv->type, (hipStream_t)stream));
+    return QE_OK;
+}
+
+int qe_attn_read8(qe_attn_ctx *c, const qe_attn_batch *b, const qe_kv_cache8 *kv, void *k, int64_t k_stride, void *v, int64_t v_stride, void *stream) {
+    static const char *const where = "qe_attn_read8";
+    int rc = check_batch(c, b, kv, where);
+    if (rc != QE_OK) return rc;
+    const int64_t kw = (int64_t)c->d.kv_heads * c->d.head_dim;
+    if (!k && !v) return qe_fail(QE_ERR_ARG, "%s: k and v are null", where);
+    if (b->n_tokens) {
+        if (k && (rc = check_rows(k, k_stride, kw, c->d.type, "k", where)) != QE_OK) return rc;
+        if (v && (rc = check_rows(v, v_stride, kw, c->d.type, "v", where)) != QE_OK) return rc;
+        if (k == v) return qe_fail(QE_ERR_ARG, "%s: k and v are one array", where);
+    }
+    if ((rc = c->err.take(where)) != QE_OK || b->n_tokens == 0) return rc;
+    QeRead8Args a{};
+    a.kc = kv->k; a.vc = kv->v; a.ks = kv->k_scale; a.vs = kv->v_scale;
+    a.k = k; a.v = v; a.k_stride = k_stride; a.v_stride = v_stride;
+    a.cu = b->cu_q; a.kv_len = b->kv_len; a.table = b->table;
+    a.n_seqs = b->n_seqs; a.n_tokens = b->n_tokens; a.table_stride = b->table_stride; a.max_pages = b->max_pages;
+    a.kv_heads = c->d.kv_heads; a.head_dim = c->d.head_dim; a.page_log2 = log2_of(c->d.page);
     a.n_pages = (unsigned)kv->n_pages;
     a.err = c->err.dev;
     OnDevice on(c->device);
     HIP_TRY(on.e);
-    HIP_TRY(qe_launch_append(a, in_type, c->d.type, (hipStream_t)stream));
+    HIP_TRY(qe_launch_read8(a, c->d.type, kv->type, (hipStream_t)stream));
     return QE_OK;
 }
 

@@ -107,3 +107,71 @@ __device__ __forceinline__ size_t page_row(const QeAttnArgs &a, int page, int kv
 __device__ __forceinline__ size_t sub_row(const QeAttnArgs &a, const int32_t *table, int kvh, int pos16, unsigned *bad) {
     return page_row(a, scalar_load(table + (pos16 >> a.page_log2)), kvh, pos16, bad);
 }
+
+// ---- a token of an append or read: its sequence, and its row in the cache --------------------------------
+struct QeToken {
+    int place;    // position in its sequence; below 0: before the first
+    long row;     // of key-value head 0 among all rows of the cache; -1 where place is below 0
+    bool in_call; // of a sequence, as far as is known
+};
+// All sequences' offsets are looked at, for the report: those that are wrong may hold no token.
+template <typename ARGS>
+__device__ __forceinline__ void report_offsets(const ARGS &a) {
+    if (a.cu)
+        for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < a.n_seqs; i += (int64_t)gridDim.x * 256)
+            if (qe_bad_offsets(a.cu[i], a.cu[i + 1], a.n_tokens)) report(a.err, QE_BAD_LENGTH);
+}
+// Token t's, by every wave for itself, through the scalar cache, with no barrier.  False: it has none; `teller` reports why.
+template <typename ARGS>
+__device__ __forceinline__ bool token_place(const ARGS &a, int t, bool teller, QeToken &x) {
+    // the last sequence whose first row is not behind t
+    int seq = t, end = t + 1;
+    bool known = true;
+    x.in_call = true;
+    if (a.cu) {
+        int lo = 0, hi = a.n_seqs; // cu[lo] <= t < cu[hi], as far as cu rises
+        while (hi - lo > 1) {
+            const int mid = (lo + hi) >> 1;
+            if (scalar_load(a.cu + mid) <= t) lo = mid;
+            else hi = mid;
+        }
+        // next to offsets that fall, it is not known whose the token is
+        const int before = scalar_load(a.cu + (lo ? lo - 1 : 0)), begin = scalar_load(a.cu + lo), after = scalar_load(a.cu + (lo + 2 <= a.n_seqs ? lo + 2 : a.n_seqs));
+        end = scalar_load(a.cu + lo + 1);
+        known = before <= begin && end <= after && !qe_bad_offsets(begin, end, a.n_tokens);
+        if (t < begin || t >= end) { // of no sequence
+            x.in_call = false;
+            return false;
+        }
+        seq = lo;
+    }
+    unsigned bad = 0;
+    const int len = qe_checked(scalar_load(a.kv_len + seq), 0, a.max_pages << a.page_log2, -1, &bad);
+    x.place = len - end + t;
+    x.row = -1;
+    if (!known || bad) {
+        if (teller) report(a.err, QE_BAD_LENGTH);
+        return false;
+    }
+    if (x.place >= 0) {
+        const unsigned p = (unsigned)scalar_load(a.table + (size_t)seq * a.table_stride + (x.place >> a.page_log2));
+        if (p >= a.n_pages) {
+            if (teller) report(a.err, QE_BAD_PAGE);
+            return false;
+        }
+        x.row = ((long)p * a.kv_heads << a.page_log2) + (x.place & ((1 << a.page_log2) - 1));
+    }
+    return true;
+}
+
+// ---- codes of 8 bits ------------------------------------------------------------------------------------
+// a word's four codes in 32 bits
+template <int CT>
+__device__ __forceinline__ void floats_of(unsigned w, float *y) {
+    if constexpr (CT == QE_I8) {
+        for (int i = 0; i < 4; ++i) y[i] = (float)(signed char)(w >> (8 * i));
+    } else {
+        const qe_f2 a = __builtin_amdgcn_cvt_pk_f32_fp8((int)w, false), b = __builtin_amdgcn_cvt_pk_f32_fp8((int)w, true);
+        y[0] = a[0], y[1] = a[1], y[2] = b[0], y[3] = b[1];
+    }
+}

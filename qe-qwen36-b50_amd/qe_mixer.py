@@ -20,6 +20,7 @@ from qe_moe import QeError, _check, _stream  # noqa: F401  (QeError is what call
 HEADER = os.path.join(os.path.dirname(qe_moe.HERE), "include", "qe_mixer.h")
 QE_ATTN_GROUP_MAX = 16  # include/qe_mixer.h
 TYPES = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}  # QE_F32, QE_F16, QE_BF16
+CODES = {torch.int8: 3, torch.float8_e4m3fn: 4}  # QE_I8, QE_F8
 
 _vp, _i32, _i64, _f32 = ctypes.c_void_p, ctypes.c_int, ctypes.c_int64, ctypes.c_float
 
@@ -38,6 +39,14 @@ class _Batch(ctypes.Structure):
                 ("max_pages", _i32), ("max_len", _i32)]
 
 
+class _Cache8(ctypes.Structure):
+    _fields_ = [("k", _vp), ("v", _vp), ("k_scale", _vp), ("v_scale", _vp), ("n_pages", _i64), ("type", _i32)]
+
+
+class _Norm(ctypes.Structure):
+    _fields_ = [("q_weight", _vp), ("k_weight", _vp), ("eps", _f32)]
+
+
 class _DeltaDesc(ctypes.Structure):
     _fields_ = [("k_heads", _i32), ("v_heads", _i32), ("dim_k", _i32), ("dim_v", _i32), ("type", _i32), ("l2norm", _i32),
                 ("scale", _f32), ("t_max", _i32), ("seqs_max", _i32)]
@@ -54,6 +63,11 @@ _SIGNATURES = {
     "qe_attn_destroy": [_vp],
     "qe_attn_append": [_vp, ctypes.POINTER(_Batch), ctypes.POINTER(_Cache), _i32, _vp, _i64, _vp, _i64, _vp, _i64, _vp, _vp, _i64,
                        _vp],
+    "qe_attn_append_normed": [_vp, ctypes.POINTER(_Batch), ctypes.POINTER(_Cache), ctypes.POINTER(_Norm), _i32, _vp, _i64, _vp, _i64, _vp,
+                              _i64, _vp, _vp, _i64, _vp],
+    "qe_attn_append8": [_vp, ctypes.POINTER(_Batch), ctypes.POINTER(_Cache8), ctypes.POINTER(_Norm), _i32, _vp, _i64, _vp, _i64, _vp, _i64,
+                        _vp, _vp, _i64, _vp],
+    "qe_attn_read8": [_vp, ctypes.POINTER(_Batch), ctypes.POINTER(_Cache8), _vp, _i64, _vp, _i64, _vp],
     "qe_attn_prompt": [_vp, ctypes.POINTER(_Batch), ctypes.POINTER(_Cache), _vp, _i64, _vp, _i64, _vp],
     "qe_attn_decode": [_vp, ctypes.POINTER(_Batch), ctypes.POINTER(_Cache), _vp, _i64, _vp, _i64, _vp],
     "qe_attn_check": [_vp, _vp],
@@ -161,6 +175,42 @@ class Batch:
         return self._ref
 
 
+class Norms:
+    """Norms of q's and k's heads before the rotation: float32 weights [head_dim] (None: not normed)."""
+
+    def __init__(self, q_weight, k_weight, eps=1e-6):
+        self.q_weight, self.k_weight = q_weight, k_weight
+        self.device, self.dim = None, None
+        for x, name in ((q_weight, "q_weight"), (k_weight, "k_weight")):
+            if x is None:
+                continue
+            if x.dtype != torch.float32 or x.dim() != 1 or not x.is_contiguous() or (self.dim is not None and x.shape[0] != self.dim):
+                _bad(f"{name}: contiguous float32 [head_dim] is wanted, got {x.dtype} {tuple(x.shape)}")
+            if self.device is not None:
+                _on(x, self.device, name)
+            self.device, self.dim = x.get_device(), x.shape[0]
+        self.c = _Norm(None if q_weight is None else q_weight.data_ptr(), None if k_weight is None else k_weight.data_ptr(), eps)
+        self._ref = ctypes.byref(self.c)
+
+
+class Cache8:
+    """An 8-bit cache: codes [pages, kv_heads, page, head_dim] of int8 or float8_e4m3fn, and float32 scales [pages, kv_heads,
+    page] of their rows."""
+
+    def __init__(self, kc, vc, k_scale, v_scale):
+        if kc.dtype not in CODES:
+            _bad(f"type {kc.dtype}: one of {', '.join(str(x) for x in CODES)} is taken")
+        self.device, self.shape = kc.get_device(), tuple(kc.shape)
+        for x, name, dtype, shape in ((kc, "k cache", kc.dtype, self.shape), (vc, "v cache", kc.dtype, self.shape),
+                                      (k_scale, "k_scale", torch.float32, self.shape[:3]), (v_scale, "v_scale", torch.float32, self.shape[:3])):
+            _on(x, self.device, name)
+            if x.dtype != dtype or x.dim() != len(shape) or tuple(x.shape) != shape or len(self.shape) != 4 or not x.is_contiguous():
+                _bad(f"{name}: contiguous {dtype} {shape} is wanted, got {x.dtype} {tuple(x.shape)}")
+        self.kc, self.vc, self.k_scale, self.v_scale = kc, vc, k_scale, v_scale
+        self.c = _Cache8(kc.data_ptr(), vc.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr(), kc.shape[0], CODES[kc.dtype])
+        self._ref = ctypes.byref(self.c)
+
+
 class Attention:
     """One attention geometry on one GPU: rotary positions and cache write, prompts, single tokens."""
 
@@ -214,8 +264,31 @@ class Attention:
             _bad(f"the batch is on cuda:{batch.device}, the context on cuda:{self.device}")
         return batch._with(n)
 
-    def append(self, batch, q, k, v, kc, vc, q_out, pos=None, stream=None):
-        """Rotate q into q_out (both None: keys and values only), rotate k and write k and v to their pages."""
+    def _cache8(self, cache):
+        if cache.shape[1:] != self._pages or cache.device != self.device:
+            _on(cache.kc, self.device, "the cache")
+            _bad(f"the cache: [pages, {', '.join(map(str, self._pages))}] is wanted, got {cache.shape}")
+        return cache._ref
+
+    def _norms(self, norms):
+        if norms.dim is not None and (norms.dim != self.head_dim or norms.device != self.device):
+            _bad(f"the norms are of {norms.dim} elements on cuda:{norms.device}, the heads of {self.head_dim} on cuda:{self.device}")
+        return norms._ref
+
+    def append(self, batch, q, k, v, kc, vc, q_out, pos=None, norms=None, stream=None):
+        """Rotate q into q_out (both None: keys and values only), rotate k and write k and v to their pages.  norms: Norms of q and
+        k before the rotation."""
+        if norms is None:
+            self._append(self._lib.qe_attn_append, (self._cache(kc, vc),), batch, q, k, v, q_out, pos, stream)
+        else:
+            self._append(self._lib.qe_attn_append_normed, (self._cache(kc, vc), self._norms(norms)), batch, q, k, v, q_out, pos, stream)
+
+    def append8(self, batch, q, k, v, cache, q_out, pos=None, norms=None, stream=None):
+        """The same to an 8-bit cache (Cache8)."""
+        self._append(self._lib.qe_attn_append8, (self._cache8(cache), None if norms is None else self._norms(norms)), batch, q, k, v, q_out,
+                     pos, stream)
+
+    def _append(self, entry, where, batch, q, k, v, q_out, pos, stream):
         n, dt, dev = k.shape[0], k.dtype, self.device
         if dt is not self.dtype:
             _type(dt, (torch.float32, self.dtype))
@@ -230,7 +303,23 @@ class Attention:
             op, os_ = _rows(q_out, self.q_heads, self.head_dim, self.dtype, dev, "q_out", n)
         b = self._batch(batch, n)
         pp = None if pos is None else _ints(pos, (self.n_axes, batch.c.n_tokens), dev, "pos")
-        rc = self._lib.qe_attn_append(self.h, b, self._cache(kc, vc), TYPES[dt], qp, qs, kp, ks, vp, vs, pp, op, os_, _stream(stream))
+        rc = entry(self.h, b, *where, TYPES[dt], qp, qs, kp, ks, vp, vs, pp, op, os_, _stream(stream))
+        if rc:
+            _check(rc)
+
+    def read8(self, batch, cache, k, v, stream=None):
+        """The keys and values that an 8-bit cache holds for the positions of the batch's tokens (either may be None)."""
+        x = k if k is not None else v
+        if x is None:
+            _bad("k and v are None")
+        n = x.shape[0]
+        kp = vp = None
+        ks = vs = 0
+        if k is not None:
+            kp, ks = _rows(k, self.kv_heads, self.head_dim, self.dtype, self.device, "k", n)
+        if v is not None:
+            vp, vs = _rows(v, self.kv_heads, self.head_dim, self.dtype, self.device, "v", n)
+        rc = self._lib.qe_attn_read8(self.h, self._batch(batch, n), self._cache8(cache), kp, ks, vp, vs, _stream(stream))
         if rc:
             _check(rc)
 
