@@ -183,6 +183,13 @@ int qe_attn_append8(qe_attn_ctx *ctx, const qe_attn_batch *batch, const qe_kv_ca
 int qe_attn_read8(qe_attn_ctx *ctx, const qe_attn_batch *batch, const qe_kv_cache8 *cache, void *k, int64_t k_stride, void *v, int64_t v_stride,
                   void *stream);
 
+/* qe_attn_decode over an 8-bit cache.  Products are as exact as with a
+ * 16-bit cache, since codes are numbers of both 16-bit types; a key's scale multiplies its
+ * score and a value's its probability, which is then rounded to bf16 (in contexts
+ * of QE_F16, too). */
+int qe_attn_decode8(qe_attn_ctx *ctx, const qe_attn_batch *batch, const qe_kv_cache8 *cache, const void *q, int64_t q_stride, void *out,
+                    int64_t out_stride, void *stream);
+
 /* Synchronise `stream` and report a bad length or page that a kernel met. */
 int qe_attn_check(qe_attn_ctx *ctx, void *stream);
 

@@ -134,7 +134,7 @@ __global__ __launch_bounds__(256) void k_append8(const QeAppend8Args x) {
                 u[8 + i] = fmaf(q, r.x, p * r.y);
             }
         const size_t row = (size_t)(at.row + ((long)m.head << a.page_log2));
-        if (CT == QE_F32 || m.kind == 0) { // 16 bits
+        if (CT == QE_CACHE16 || m.kind == 0) { // 16 bits
             OUT *dst = m.kind == 0 ? (OUT *)a.q_out + (size_t)t * a.q_out_stride + (size_t)m.head * DH : (OUT *)(m.kind == 1 ? a.kc : a.vc) + row * DH;
             OUT8 lo, hi;
 #pragma unroll
@@ -174,7 +174,7 @@ static hipError_t launch_append8(const QeAppend8Args &a, hipStream_t st) {
 template <typename IN, typename OUT>
 static hipError_t launch_append8(const QeAppend8Args &a, int cache_type, hipStream_t st) {
     if (cache_type == QE_I8) return launch_append8<IN, OUT, QE_I8>(a, st);
-    return cache_type == QE_F8 ? launch_append8<IN, OUT, QE_F8>(a, st) : launch_append8<IN, OUT, QE_F32>(a, st);
+    return cache_type == QE_F8 ? launch_append8<IN, OUT, QE_F8>(a, st) : launch_append8<IN, OUT, QE_CACHE16>(a, st);
 }
 hipError_t qe_launch_append8(const QeAppend8Args &a, int in_type, int type, int cache_type, hipStream_t st) {
     if (a.a.n_tokens == 0) return hipSuccess;

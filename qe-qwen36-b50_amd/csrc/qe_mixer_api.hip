@@ -140,7 +140,8 @@ int check_rows(const void *p, int64_t stride, int64_t width, int type, const cha
     return QE_OK;
 }
 
-QeAttnArgs attn_args(const qe_attn_ctx *c, const qe_attn_batch *b, const qe_kv_cache *kv, const void *q, int64_t q_stride, void *out,
+template <typename CACHE>
+QeAttnArgs attn_args(const qe_attn_ctx *c, const qe_attn_batch *b, const CACHE *kv, const void *q, int64_t q_stride, void *out,
                      int64_t out_stride) {
     QeAttnArgs a{};
     a.q = q; a.out = out; a.kc = kv->k; a.vc = kv->v;
@@ -285,7 +286,7 @@ int qe_attn_append_normed(qe_attn_ctx *c, const qe_attn_batch *b, const qe_kv_ca
     x.wq = norm->q_weight; x.wk = norm->k_weight; x.eps = norm->eps;
     OnDevice on(c->device);
     HIP_TRY(on.e);
-    HIP_TRY(qe_launch_append8(x, in_type, c->d.type, c->d.type, (hipStream_t)stream));
+    HIP_TRY(qe_launch_append8(x, in_type, c->d.type, QE_CACHE16, (hipStream_t)stream));
     return QE_OK;
 }
 
@@ -333,7 +334,10 @@ int qe_attn_read8(qe_attn_ctx *c, const qe_attn_batch *b, const qe_kv_cache8 *kv
     return QE_OK;
 }
 
-static int check_attend(qe_attn_ctx *c, const qe_attn_batch *b, const qe_kv_cache *kv, const void *q, int64_t q_stride, const void *out,
+}  // extern "C"
+
+template <typename CACHE>
+static int check_attend(qe_attn_ctx *c, const qe_attn_batch *b, const CACHE *kv, const void *q, int64_t q_stride, const void *out,
                         int64_t out_stride, const char *where) {
     int rc = check_batch(c, b, kv, where);
     if (rc != QE_OK) return rc;
@@ -345,6 +349,8 @@ static int check_attend(qe_attn_ctx *c, const qe_attn_batch *b, const qe_kv_cach
     }
     return c->err.take(where);
 }
+
+extern "C" {
 
 int qe_attn_prompt(qe_attn_ctx *c, const qe_attn_batch *b, const qe_kv_cache *kv, const void *q, int64_t q_stride, void *out, int64_t out_stride,
                    void *stream) {
@@ -377,6 +383,24 @@ int qe_attn_decode(qe_attn_ctx *c, const qe_attn_batch *b, const qe_kv_cache *kv
     OnDevice on(c->device);
     HIP_TRY(on.e);
     HIP_TRY(qe_launch_attn_decode(a, c->d.head_dim, c->d.type, (hipStream_t)stream));
+    return QE_OK;
+}
+
+int qe_attn_decode8(qe_attn_ctx *c, const qe_attn_batch *b, const qe_kv_cache8 *kv, const void *q, int64_t q_stride, void *out, int64_t out_stride,
+                    void *stream) {
+    if (b && b->cu_q) return qe_fail(QE_ERR_ARG, "qe_attn_decode8: cu_q given (several tokens: qe_attn_prompt8)");
+    const int rc = check_attend(c, b, kv, q, q_stride, out, out_stride, "qe_attn_decode8");
+    if (rc != QE_OK) return rc;
+    QeAttn8Args x{};
+    x.a = attn_args(c, b, kv, q, q_stride, out, out_stride);
+    x.ks = kv->k_scale; x.vs = kv->v_scale;
+    const int64_t most = (int64_t)b->max_pages * c->d.page;
+    const int64_t max_len = b->max_len && b->max_len < most ? b->max_len : most;
+    qe_attn_decode_plan(b->n_seqs, x.a.kv_heads, c->d.head_dim, max_len, &x.a.steps, &x.a.splits);
+    x.a.once = qe_attn_decode_once(b->n_seqs, x.a.kv_heads, c->d.head_dim, max_len / 2);
+    OnDevice on(c->device);
+    HIP_TRY(on.e);
+    HIP_TRY(qe_launch_attn_decode8(x, c->d.head_dim, c->d.type, kv->type, (hipStream_t)stream));
     return QE_OK;
 }
 

@@ -175,3 +175,42 @@ __device__ __forceinline__ void floats_of(unsigned w, float *y) {
         y[0] = a[0], y[1] = a[1], y[2] = b[0], y[3] = b[1];
     }
 }
+
+// eight codes as the matrix cores' 16-bit type; exact, a code has at most 8 bits
+template <int CT, bool BF>
+__device__ __forceinline__ qe_s8 elements_of(unsigned lo, unsigned hi) {
+    unsigned r[4];
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+        const unsigned w = h ? hi : lo;
+        if constexpr (CT == QE_F8 && BF) {
+            r[2 * h] = __builtin_bit_cast(unsigned, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w, 1.f, false));
+            r[2 * h + 1] = __builtin_bit_cast(unsigned, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w, 1.f, true));
+        } else if constexpr (CT == QE_F8) {
+            r[2 * h] = __builtin_bit_cast(unsigned, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(w, 1.f, false));
+            r[2 * h + 1] = __builtin_bit_cast(unsigned, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(w, 1.f, true));
+        } else if constexpr (BF) {
+            float y[4];
+            floats_of<QE_I8>(w, y);
+            r[2 * h] = pack2<true>(y[0], y[1]);
+            r[2 * h + 1] = pack2<true>(y[2], y[3]);
+        } else { // 1024 + (code + 128), by a byte before it, less 1152
+            const unsigned u = w ^ 0x80808080u;
+            const qe_h2 off = {(_Float16)-1152.f, (_Float16)-1152.f};
+            r[2 * h] = __builtin_bit_cast(unsigned, __builtin_bit_cast(qe_h2, __builtin_amdgcn_perm(0x64646464u, u, 0x04010400u)) + off);
+            r[2 * h + 1] = __builtin_bit_cast(unsigned, __builtin_bit_cast(qe_h2, __builtin_amdgcn_perm(0x64646464u, u, 0x04030402u)) + off);
+        }
+    }
+    return __builtin_bit_cast(qe_s8, make_uint4(r[0], r[1], r[2], r[3]));
+}
+// Lane I of each 16's value, to all of them: the compiler makes it an operand of the instruction that uses it.
+template <int I>
+__device__ __forceinline__ float of_lane(float x) {
+    return __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(x), 0x150 + I, 0xf, 0xf, true));
+}
+// Transposing LDS read of bytes: of each 16 lanes, lane l addresses 8 bytes of row l / 2 (columns 8 (l % 2) .. + 7) and gets
+// column l of the eight rows.
+__device__ __forceinline__ uint2 lds_tr8(const uint8_t *p) {
+    typedef int i2 __attribute__((ext_vector_type(2)));
+    return __builtin_bit_cast(uint2, __builtin_amdgcn_ds_read_tr8_b64_v2i32((__attribute__((address_space(3))) i2 *)p));
+}

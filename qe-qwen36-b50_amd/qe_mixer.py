@@ -70,6 +70,7 @@ _SIGNATURES = {
     "qe_attn_read8": [_vp, ctypes.POINTER(_Batch), ctypes.POINTER(_Cache8), _vp, _i64, _vp, _i64, _vp],
     "qe_attn_prompt": [_vp, ctypes.POINTER(_Batch), ctypes.POINTER(_Cache), _vp, _i64, _vp, _i64, _vp],
     "qe_attn_decode": [_vp, ctypes.POINTER(_Batch), ctypes.POINTER(_Cache), _vp, _i64, _vp, _i64, _vp],
+    "qe_attn_decode8": [_vp, ctypes.POINTER(_Batch), ctypes.POINTER(_Cache8), _vp, _i64, _vp, _i64, _vp],
     "qe_attn_check": [_vp, _vp],
     "qe_delta_create": [_i32, ctypes.POINTER(_DeltaDesc), ctypes.POINTER(_vp)],
     "qe_delta_destroy": [_vp],
@@ -323,21 +324,25 @@ class Attention:
         if rc:
             _check(rc)
 
-    def _attend(self, entry, batch, q, kc, vc, out, stream):
+    def _attend(self, entry, batch, q, cache, out, stream):
         qp, qs = _rows(q, self.q_heads, self.head_dim, self.dtype, self.device, "q")
         n = q.shape[0]
         op, os_ = _rows(out, self.q_heads, self.head_dim, self.dtype, self.device, "out", n)
-        rc = entry(self.h, self._batch(batch, n), self._cache(kc, vc), qp, qs, op, os_, _stream(stream))
+        rc = entry(self.h, self._batch(batch, n), cache, qp, qs, op, os_, _stream(stream))
         if rc:
             _check(rc)
 
     def prompt(self, batch, q, kc, vc, out, stream=None):
         """Causal attention of the batch's new tokens, which are in the cache, over their sequences."""
-        self._attend(self._lib.qe_attn_prompt, batch, q, kc, vc, out, stream)
+        self._attend(self._lib.qe_attn_prompt, batch, q, self._cache(kc, vc), out, stream)
 
     def decode(self, batch, q, kc, vc, out, stream=None):
         """The same for one new token per sequence (a batch without cu_q)."""
-        self._attend(self._lib.qe_attn_decode, batch, q, kc, vc, out, stream)
+        self._attend(self._lib.qe_attn_decode, batch, q, self._cache(kc, vc), out, stream)
+
+    def decode8(self, batch, q, cache, out, stream=None):
+        """decode over an 8-bit cache (Cache8)."""
+        self._attend(self._lib.qe_attn_decode8, batch, q, self._cache8(cache), out, stream)
 
     def check(self, stream=None):
         """Synchronise `stream`; raise QeError if a kernel met a bad length or page."""

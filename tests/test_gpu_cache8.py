@@ -8,71 +8,12 @@ import cache8_ref as Q  # noqa: E402
 import mixer_ref as R  # noqa: E402
 import qe_mixer  # noqa: E402
 import qe_moe  # noqa: E402
+from cache8_ref import Case8, bits, gen, ints, rand, same  # noqa: E402
 
 pytestmark = pytest.mark.gpu
 EPS = 1e-6
 GEOMETRIES = [(16, 2, 256, 256, 64, (11, 11, 10), True), (4, 2, 128, 16, 128, (64,), False), (3, 3, 64, 32, 48, (10, 8, 6), False),
               (40, 8, 64, 16, 64, (14, 9, 9), True), (2, 2, 64, 16, 0, (0,), False)]
-
-
-def gen(seed):
-    g = torch.Generator(device="cuda")
-    g.manual_seed(seed)
-    return g
-
-
-def rand(g, *shape, dtype=torch.float32, std=1.0):
-    return (torch.randn(*shape, generator=g, device="cuda") * std).to(dtype)
-
-
-def ints(v):
-    return torch.tensor(v, dtype=torch.int32, device="cuda")
-
-
-class Case8:
-    """Sequences in an 8-bit cache of shuffled pages, with junk wherever no position is."""
-
-    def __init__(self, hq, hkv, dim, page, dtype, codes, kv_len, seed=0, extra_cols=2, **desc):
-        g = gen(seed)
-        self.hq, self.hkv, self.dim, self.page, self.dtype, self.kv_len = hq, hkv, dim, page, dtype, kv_len
-        per = [-(-n // page) for n in kv_len]
-        total = sum(per) + 3
-        order = torch.randperm(total, generator=g, device="cuda")[: sum(per)].to(torch.int32)
-        # columns behind a sequence's pages name no page of the cache
-        self.table = torch.full((len(kv_len), max(per + [1]) + extra_cols), 1 << 30, dtype=torch.int32, device="cuda")
-        used = torch.zeros(total, page, dtype=torch.bool, device="cuda")
-        at = 0
-        for i, (n, p) in enumerate(zip(kv_len, per)):
-            self.table[i, :p] = order[at: at + p]
-            for c in range(p):
-                used[order[at + c], : min(page, n - c * page)] = True
-            at += p
-        (self.kc, self.ks), (self.vc, self.vs) = (Q.quantised(rand(g, total, hkv, page, dim), codes) for _ in range(2))
-        Q.poison(self.kc, self.ks, used, g)
-        Q.poison(self.vc, self.vs, used, g)
-        self.att = qe_mixer.Attention(hq, hkv, dim, page, dtype=dtype, **desc)
-        self.g = g
-
-    def cache(self):
-        return qe_mixer.Cache8(self.kc, self.vc, self.ks, self.vs)
-
-    def copy(self):
-        return qe_mixer.Cache8(self.kc.clone(), self.vc.clone(), self.ks.clone(), self.vs.clone())
-
-    def batch(self, cu=None, **kw):
-        return qe_mixer.Batch(ints(self.kv_len), self.table, None if cu is None else ints(cu), **kw)
-
-    def q(self, T, std=2.0):
-        return rand(self.g, T, self.hq, self.dim, dtype=self.dtype, std=std)
-
-
-def bits(x):
-    return x.view({1: torch.int8, 2: torch.int16, 4: torch.int32}[x.element_size()])
-
-
-def same(a, b):
-    """Whether two caches hold the same bits."""
-    return all(torch.equal(bits(x), bits(y)) for x, y in ((a.kc, b.kc), (a.vc, b.vc), (a.k_scale, b.k_scale), (a.v_scale, b.v_scale)))
 
 
 @pytest.mark.parametrize("normed", [True, False])
