@@ -183,10 +183,13 @@ int qe_attn_append8(qe_attn_ctx *ctx, const qe_attn_batch *batch, const qe_kv_ca
 int qe_attn_read8(qe_attn_ctx *ctx, const qe_attn_batch *batch, const qe_kv_cache8 *cache, void *k, int64_t k_stride, void *v, int64_t v_stride,
                   void *stream);
 
-/* qe_attn_decode over an 8-bit cache.  Products are as exact as with a
- * 16-bit cache, since codes are numbers of both 16-bit types; a key's scale multiplies its
- * score and a value's its probability, which is then rounded to bf16 (in contexts
- * of QE_F16, too). */
+/* qe_attn_prompt and qe_attn_decode over an 8-bit cache.  Products are as exact
+ * as with a 16-bit cache, since codes are numbers of both 16-bit types; a key's
+ * scale multiplies its score and a value's its probability, which is then
+ * rounded to bf16 (in contexts of QE_F16, too).  A scale that is not finite
+ * reaches the rows that attend to its position, and no others. */
+int qe_attn_prompt8(qe_attn_ctx *ctx, const qe_attn_batch *batch, const qe_kv_cache8 *cache, const void *q, int64_t q_stride, void *out,
+                    int64_t out_stride, void *stream);
 int qe_attn_decode8(qe_attn_ctx *ctx, const qe_attn_batch *batch, const qe_kv_cache8 *cache, const void *q, int64_t q_stride, void *out,
                     int64_t out_stride, void *stream);
 

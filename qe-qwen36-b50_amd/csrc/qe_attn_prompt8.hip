@@ -1,0 +1,205 @@
+// Causal attention of packed prompts over an 8-bit paged cache.
+//
+// As k_attn_prompt (qe_attn_prompt.hip), whose products, softmax and split of the work these are: 32 query rows a wave, S^T = K
+// Q^T and O^T += V^T P^T on v_mfma_f32_32x32x16 from tiles in LDS.  The tiles hold the codes as 16-bit numbers, exactly: each
+// wave loads its part of the next tile's codes while this one is worked on, turns them to 16 bits when its work is done,
+// and writes them to the other of two buffers, so that a code is turned once for all rows of a workgroup.  With heads of 256
+// the registers are full: there the codes wait in a few KB of LDS, by direct loads.  A key's scale multiplies its scores and a
+// value's its probabilities (to bf16, as in k_attn_decode8), from one register: lane n of 16 has the scale of the n-th
+// of the 16 keys in the lane's registers.
+#include "qe_attn_rows.h"
+
+template <int CT, bool BF, int DH, int WAVES>
+struct Stage {
+    static constexpr int BN = DH == 256 ? 32 : 64, PART = BN / WAVES, NL = PART * DH / 1024; // 16-byte loads of a lane
+    static constexpr int CH = DH / 16;                                                       // chunks of a row
+    static constexpr bool WAIT_IN_LDS = DH == 256;
+    typedef unsigned u4 __attribute__((ext_vector_type(4)));
+    u4 k[WAIT_IN_LDS ? 1 : NL], v[WAIT_IN_LDS ? 1 : NL];
+    float scale; // lanes 0 .. PART - 1: of the part's keys, 32 .. 32 + PART - 1: of its values
+
+    // The codes of the wave's part of the tile of BN keys from k0 on.
+    __device__ __forceinline__ void issue(const QeAttn8Args &x, int page, int kvh, int k0, int len, int wave, uint8_t *raw) {
+        const int sub = k0 + wave * PART, at = sub < len ? sub : (len - 1) & -PART;
+        unsigned known = 0; // that a page is none: lost_pages
+        const size_t r0 = page_row(x.a, page, kvh, at, &known);
+        const int lane = lane_now(), n = lane & 31;
+        scale = (lane < 32 ? x.ks : x.vs)[r0 + (n < PART ? n : 0)];
+        const uint8_t *kp = (const uint8_t *)x.a.kc + r0 * DH, *vp = (const uint8_t *)x.a.vc + r0 * DH;
+        if constexpr (WAIT_IN_LDS) {
+#pragma unroll
+            for (int i = 0; i < NL; ++i) load_lds16_from(kp, PART * DH, lane * 16, i * 1024, raw + i * 1024);
+#pragma unroll
+            for (int i = 0; i < NL; ++i) load_lds16_from(vp, PART * DH, lane * 16, i * 1024, raw + (NL + i) * 1024);
+        } else {
+#pragma unroll
+            for (int i = 0; i < NL; ++i) k[i] = *(const u4 *)(kp + i * 1024 + lane * 16);
+#pragma unroll
+            for (int i = 0; i < NL; ++i) v[i] = *(const u4 *)(vp + i * 1024 + lane * 16);
+        }
+    }
+    // They have come: to the tiles, as 16-bit numbers.  Behind the end, where codes and scales may be anything, zeros.
+    __device__ __forceinline__ void land(int k0, int len, int wave, const uint8_t *raw, short *k_lds, short *v_lds, float *ks, float *vs) {
+        if constexpr (WAIT_IN_LDS) __builtin_amdgcn_s_waitcnt(0x0f70);
+        const int lane = lane_now(), n = lane & 31;
+        const bool cut = k0 + BN > len;
+        if (n < PART) (lane < 32 ? ks : vs)[wave * PART + n] = cut && k0 + wave * PART + n >= len ? 0.f : scale;
+#pragma unroll
+        for (int i = 0; i < NL; ++i) {
+            const int row = wave * PART + i * (64 / CH) + lane / CH, c = lane % CH * 2;
+            u4 a, b;
+            if constexpr (WAIT_IN_LDS) {
+                a = *(const u4 *)(raw + i * 1024 + lane * 16);
+                b = *(const u4 *)(raw + (NL + i) * 1024 + lane * 16);
+            } else {
+                a = k[i];
+                b = v[i];
+            }
+            if (CT == QE_F8 && cut && k0 + row >= len) a = b = u4{0, 0, 0, 0};
+            short *kr = k_lds + row * DH, *vr = v_lds + row * DH;
+            *(qe_s8 *)(kr + ((c ^ k_swz(row)) << 3)) = elements_of<CT, BF>(a[0], a[1]);
+            *(qe_s8 *)(kr + (((c + 1) ^ k_swz(row)) << 3)) = elements_of<CT, BF>(a[2], a[3]);
+            *(qe_s8 *)(vr + ((c ^ v_swz<DH>(row)) << 3)) = elements_of<CT, true>(b[0], b[1]);
+            *(qe_s8 *)(vr + (((c + 1) ^ v_swz<DH>(row)) << 3)) = elements_of<CT, true>(b[2], b[3]);
+        }
+    }
+};
+
+// x[i] times lane i's scale, of each 16 lanes
+template <int I = 0>
+__device__ __forceinline__ void scaled(qe_f16v &x, float s) {
+    if constexpr (I < 16) {
+        x[I] *= of_lane<I>(s);
+        scaled<I + 1>(x, s);
+    }
+}
+
+template <bool BF, int DH, int CT, int WAVES>
+__global__ __launch_bounds__(64 * WAVES, 2) void k_attn_prompt8(const QeAttn8Args x) {
+    const QeAttnArgs &a = x.a;
+    typedef Stage<CT, BF, DH, WAVES> ST;
+    constexpr int BM = 32 * WAVES, BN = ST::BN, KB = DH == 256 ? 1 : 2;
+    static_assert(BN == 32 * KB, "a tile is a step");
+    __shared__ __align__(16) short k_a[BN * DH], v_a[BN * DH], k_b[BN * DH], v_b[BN * DH];
+    __shared__ __align__(16) uint8_t raw_s[ST::WAIT_IN_LDS ? 2 * BN * DH : 16];
+    __shared__ float s_a[2][BN], s_b[2][BN];
+    const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int split = blockIdx.x % a.splits, kvh = blockIdx.x / a.splits % a.kv_heads;
+    const int tile = a.tiles - 1 - blockIdx.x / a.splits / a.kv_heads; // a sequence's late rows have more keys: first
+    // workgroup i looks at sequence i's offsets, for the report: where they fall, a sequence may have no tile below
+    const int mine = blockIdx.x < (unsigned)a.n_seqs ? blockIdx.x : a.n_seqs - 1;
+    const int mine0 = scalar_load(a.cu + mine), mine1 = scalar_load(a.cu + mine + 1);
+    int seq = 0;
+    for (int hi = a.n_seqs; hi - seq > 1;) { // the last sequence whose first tile is not behind this one
+        const int mid = (seq + hi) >> 1;
+        if (qe_attn_first_tile(qe_clamped(scalar_load(a.cu + mid), 0, a.n_tokens), mid, a.group, BM) <= tile) seq = mid;
+        else hi = mid;
+    }
+    const int cu0 = scalar_load(a.cu + seq), cu1 = scalar_load(a.cu + seq + 1), kv = scalar_load(a.kv_len + seq);
+    unsigned bad_len = 0;
+    int begin, end;
+    qe_rows_of(cu0, cu1, a.n_tokens, &begin, &end, &bad_len);
+    const int local = tile - qe_attn_first_tile(begin, seq, a.group, BM);
+    int len = qe_checked(kv, 0, a.max_pages << a.page_log2, 0, &bad_len);
+    if (bad_len) len = 0; // no row has a position: zeros
+    if ((bad_len || qe_bad_offsets(mine0, mine1, a.n_tokens)) && tid == 0) report(a.err, QE_BAD_LENGTH);
+    const int n_rows = (end - begin) * a.group;
+    if (local < 0 || (int64_t)local * BM >= n_rows) return; // uniform: no row of the sequence
+    const int row0 = local * BM, first = len - (end - begin); // first: position of the sequence's first row
+    const int32_t *table = a.table + (size_t)seq * a.table_stride;
+
+    const int last_tok = (row0 + BM < n_rows ? row0 + BM - 1 : n_rows - 1) / a.group, keys = first + last_tok + 1;
+    const int wave_row = row0 + wave * 32, wave_end = wave_row + 32 < n_rows ? wave_row + 32 : n_rows;
+    const int wave_keys = wave_row < n_rows ? first + (wave_end - 1) / a.group + 1 : 0, wave_clear = first + wave_row / a.group + 1;
+    int lo, hi;
+    qe_split_range(keys > 0 ? (keys + BN - 1) / BN : 0, a.splits, split, &lo, &hi);
+
+    ST stage;
+    uint8_t *raw = raw_s + (ST::WAIT_IN_LDS ? wave * (2 * ST::PART * DH) : 0);
+    int page = 0; // of the wave's part of the tile after the one that is loaded
+    if (lo < hi) {
+        page = page_of<BN, WAVES>(a, table, lo * BN, len, wave);
+        stage.issue(x, page, kvh, lo * BN, len, wave, raw);
+        page = page_of<BN, WAVES>(a, table, (lo + 1) * BN, len, wave);
+    }
+    Rows<BF, DH, true> w;
+    {
+        const int row = wave_row + (tid & 31), h = tid >> 5 & 1;
+        const bool there = row < n_rows;
+        const int tok = there ? row / a.group : 0, head = kvh * a.group + (there ? row - tok * a.group : 0);
+        w.place = there ? first + tok : -1;
+        const short *q = (const short *)a.q + (size_t)(begin + tok) * a.q_stride + (size_t)head * DH + h * 8;
+#pragma unroll
+        for (int s = 0; s < DH / 16; ++s) w.q[s] = there ? *(const qe_s8 *)(q + s * 16) : qe_s8{};
+        w.m = -INFINITY;
+        w.l = 0;
+#pragma unroll
+        for (int d = 0; d < DH / 32; ++d)
+#pragma unroll
+            for (int i = 0; i < 16; ++i) w.o[d][i] = 0;
+    }
+    if (lo < hi) {
+        const int lost = lost_pages<64 * WAVES>(a, table, (len + (1 << a.page_log2) - 1) >> a.page_log2, tid);
+        if (__syncthreads_or(lost)) { // (it waits for what is on its way to LDS, too)
+            if (tid == 0) report(a.err, QE_BAD_PAGE);
+            hi = lo; // no key: zeros
+        }
+    }
+    if (lo < hi) {
+        stage.land(lo * BN, len, wave, raw, k_a, v_a, s_a[0], s_a[1]);
+        if (lo + 1 < hi) stage.issue(x, page, kvh, (lo + 1) * BN, len, wave, raw);
+        page = page_of<BN, WAVES>(a, table, (lo + 2) * BN, len, wave);
+    }
+    auto work = [&](int t, const short *k_lds, const short *v_lds, const float (*s_lds)[BN], short *k_next, short *v_next, float (*s_next)[BN]) {
+        lds_barrier(); // the tile is there, and no wave reads the other buffers any more
+        const int k0 = t * BN;
+        if (k0 < wave_keys) {
+            const int lane = lane_now(), at = 8 * (lane >> 2 & 3) + 4 * (lane >> 5) + (lane & 3);
+            Scores<KB> s;
+            w.scores(k_lds, 0, s);
+            schedule<4, KB * DH / 16, 1>();
+#pragma unroll
+            for (int b = 0; b < KB; ++b) scaled(s.s[b], s_lds[0][b * 32 + at]);
+            const bool cut = k0 + BN > wave_clear;
+            const int limit = w.place - k0 - 4 * (lane >> 5);
+            if (cut) s.mask(limit);
+            w.raise(s.top() * a.scale_log2);
+            Probs<KB> p;
+            w.weigh(a.scale_log2, s);
+#pragma unroll
+            for (int b = 0; b < KB; ++b) scaled(s.s[b], s_lds[1][b * 32 + at]);
+            if (cut) s.clear(limit); // a scale that is not finite reaches the rows that attend to its position
+            s.pack(p);
+            w.values(v_lds, 0, p);
+            schedule<3, KB * DH / 16, 2>();
+        }
+        if (t + 1 < hi) {
+            stage.land(k0 + BN, len, wave, raw, k_next, v_next, s_next[0], s_next[1]);
+            if (t + 2 < hi) stage.issue(x, page, kvh, k0 + 2 * BN, len, wave, raw);
+            page = page_of<BN, WAVES>(a, table, k0 + 3 * BN, len, wave);
+        }
+    };
+    for (int t = lo; t < hi; t += 2) {
+        work(t, k_a, v_a, s_a, k_b, v_b, s_b);
+        if (t + 1 < hi) work(t + 1, k_b, v_b, s_b, k_a, v_a, s_a);
+    }
+    w.template finish<BM>(a, begin, n_rows, row0, wave_row, tile, kvh, split);
+}
+
+template <bool BF, int DH, int CT, int WAVES>
+static hipError_t launch_waves8(const QeAttn8Args &x, hipStream_t st) {
+    k_attn_prompt8<BF, DH, CT, WAVES><<<dim3((unsigned)(x.a.tiles * x.a.kv_heads * x.a.splits)), dim3(64 * WAVES), 0, st>>>(x);
+    launch_prompt_join<BF, DH, 32 * WAVES>(x.a, st);
+    return hipGetLastError();
+}
+template <bool BF, int CT>
+static hipError_t launch_prompt8(const QeAttn8Args &x, int head_dim, int bm, hipStream_t st) {
+    if (head_dim == 64) return launch_waves8<BF, 64, CT, 4>(x, st);
+    if (head_dim == 128) return launch_waves8<BF, 128, CT, 4>(x, st);
+    return bm == 256 ? launch_waves8<BF, 256, CT, 8>(x, st) : launch_waves8<BF, 256, CT, 4>(x, st);
+}
+
+hipError_t qe_launch_attn_prompt8(const QeAttn8Args &x, int head_dim, int type, int cache_type, int bm, hipStream_t st) {
+    if (type == QE_BF16) return cache_type == QE_I8 ? launch_prompt8<true, QE_I8>(x, head_dim, bm, st) : launch_prompt8<true, QE_F8>(x, head_dim, bm, st);
+    return cache_type == QE_I8 ? launch_prompt8<false, QE_I8>(x, head_dim, bm, st) : launch_prompt8<false, QE_F8>(x, head_dim, bm, st);
+}

@@ -352,21 +352,44 @@ static int check_attend(qe_attn_ctx *c, const qe_attn_batch *b, const CACHE *kv,
 
 extern "C" {
 
+// How a prompt call is cut up: a->tiles and a->splits, and the rows of a workgroup.
+static int plan_prompt(const qe_attn_ctx *c, const qe_attn_batch *b, const char *where, QeAttnArgs *a, int *bm) {
+    *bm = qe_attn_prompt_rows(b->n_tokens, b->n_seqs, a->group, a->kv_heads, c->d.head_dim);
+    a->tiles = qe_attn_max_tiles(b->n_tokens, b->n_seqs, a->group, *bm);
+    if (!qe_fits_launch((int64_t)a->tiles * a->kv_heads, 2 * *bm))
+        return qe_fail(QE_ERR_ARG, "%s: %d tokens of %d sequences are more threads than a launch has", where, b->n_tokens, b->n_seqs);
+    const int64_t most = (int64_t)b->max_pages * c->d.page;
+    a->splits = qe_attn_prompt_splits((int64_t)a->tiles * a->kv_heads, b->max_len && b->max_len < most ? b->max_len : most);
+    return QE_OK;
+}
+
 int qe_attn_prompt(qe_attn_ctx *c, const qe_attn_batch *b, const qe_kv_cache *kv, const void *q, int64_t q_stride, void *out, int64_t out_stride,
                    void *stream) {
-    if (b && !b->cu_q) return qe_fail(QE_ERR_ARG, "qe_attn_prompt: null cu_q (single tokens: qe_attn_decode)");
-    const int rc = check_attend(c, b, kv, q, q_stride, out, out_stride, "qe_attn_prompt");
+    static const char *const where = "qe_attn_prompt";
+    if (b && !b->cu_q) return qe_fail(QE_ERR_ARG, "%s: null cu_q (single tokens: qe_attn_decode)", where);
+    int rc = check_attend(c, b, kv, q, q_stride, out, out_stride, where), bm;
     if (rc != QE_OK || b->n_tokens == 0) return rc;
     QeAttnArgs a = attn_args(c, b, kv, q, q_stride, out, out_stride);
-    const int bm = qe_attn_prompt_rows(b->n_tokens, b->n_seqs, a.group, a.kv_heads, c->d.head_dim);
-    a.tiles = qe_attn_max_tiles(b->n_tokens, b->n_seqs, a.group, bm);
-    if (!qe_fits_launch((int64_t)a.tiles * a.kv_heads, 2 * bm))
-        return qe_fail(QE_ERR_ARG, "qe_attn_prompt: %d tokens of %d sequences are more threads than a launch has", b->n_tokens, b->n_seqs);
-    const int64_t most = (int64_t)b->max_pages * c->d.page;
-    a.splits = qe_attn_prompt_splits((int64_t)a.tiles * a.kv_heads, b->max_len && b->max_len < most ? b->max_len : most);
+    if ((rc = plan_prompt(c, b, where, &a, &bm)) != QE_OK) return rc;
     OnDevice on(c->device);
     HIP_TRY(on.e);
     HIP_TRY(qe_launch_attn_prompt(a, c->d.head_dim, c->d.type, bm, (hipStream_t)stream));
+    return QE_OK;
+}
+
+int qe_attn_prompt8(qe_attn_ctx *c, const qe_attn_batch *b, const qe_kv_cache8 *kv, const void *q, int64_t q_stride, void *out, int64_t out_stride,
+                    void *stream) {
+    static const char *const where = "qe_attn_prompt8";
+    if (b && !b->cu_q) return qe_fail(QE_ERR_ARG, "%s: null cu_q (single tokens: qe_attn_decode8)", where);
+    int rc = check_attend(c, b, kv, q, q_stride, out, out_stride, where), bm;
+    if (rc != QE_OK || b->n_tokens == 0) return rc;
+    QeAttn8Args x{};
+    x.a = attn_args(c, b, kv, q, q_stride, out, out_stride);
+    x.ks = kv->k_scale; x.vs = kv->v_scale;
+    if ((rc = plan_prompt(c, b, where, &x.a, &bm)) != QE_OK) return rc;
+    OnDevice on(c->device);
+    HIP_TRY(on.e);
+    HIP_TRY(qe_launch_attn_prompt8(x, c->d.head_dim, c->d.type, kv->type, bm, (hipStream_t)stream));
     return QE_OK;
 }
 

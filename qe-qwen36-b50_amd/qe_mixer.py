@@ -70,6 +70,7 @@ _SIGNATURES = {
     "qe_attn_read8": [_vp, ctypes.POINTER(_Batch), ctypes.POINTER(_Cache8), _vp, _i64, _vp, _i64, _vp],
     "qe_attn_prompt": [_vp, ctypes.POINTER(_Batch), ctypes.POINTER(_Cache), _vp, _i64, _vp, _i64, _vp],
     "qe_attn_decode": [_vp, ctypes.POINTER(_Batch), ctypes.POINTER(_Cache), _vp, _i64, _vp, _i64, _vp],
+    "qe_attn_prompt8": [_vp, ctypes.POINTER(_Batch), ctypes.POINTER(_Cache8), _vp, _i64, _vp, _i64, _vp],
     "qe_attn_decode8": [_vp, ctypes.POINTER(_Batch), ctypes.POINTER(_Cache8), _vp, _i64, _vp, _i64, _vp],
     "qe_attn_check": [_vp, _vp],
     "qe_delta_create": [_i32, ctypes.POINTER(_DeltaDesc), ctypes.POINTER(_vp)],
@@ -339,6 +340,10 @@ class Attention:
     def decode(self, batch, q, kc, vc, out, stream=None):
         """The same for one new token per sequence (a batch without cu_q)."""
         self._attend(self._lib.qe_attn_decode, batch, q, self._cache(kc, vc), out, stream)
+
+    def prompt8(self, batch, q, cache, out, stream=None):
+        """prompt over an 8-bit cache (Cache8)."""
+        self._attend(self._lib.qe_attn_prompt8, batch, q, self._cache8(cache), out, stream)
 
     def decode8(self, batch, q, cache, out, stream=None):
         """decode over an 8-bit cache (Cache8)."""

@@ -127,3 +127,196 @@ def test_decode_bad_pages_and_lengths_give_zeros_and_an_error(n):
             c.att.check()
         assert bool((out[1] == 0).all())
         close(out[0], want[0], off[0])
+
+
+def offsets(lens):
+    cu = [0]
+    for n in lens:
+        cu.append(cu[-1] + n)
+    return cu
+
+
+@pytest.mark.parametrize("codes", CODES)
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("hq,hkv,dim,page", HEADS)
+def test_prompt(hq, hkv, dim, page, dtype, codes):
+    lens, ctx = [1, 0, 17, 200, 64, 5, 130], [0, 30, 40, 0, 64, 1000, 3]
+    c = Case8(hq, hkv, dim, page, dtype, codes, [a + b for a, b in zip(lens, ctx)])
+    cu = offsets(lens)
+    q = c.q(cu[-1] + 3)  # rows behind the last sequence
+    out = torch.full_like(q, 7.0)
+    c.att.prompt8(c.batch(cu), q, c.cache(), out)
+    c.att.check()
+    want, off = Q.attend_batch(c, q[: cu[-1]], cu)
+    close(out[: cu[-1]], want, off)
+    assert bool((out[cu[-1]:] == 7).all())
+
+
+@pytest.mark.parametrize("codes", CODES)
+@pytest.mark.parametrize("hq,hkv,dim,page,lens", [(16, 2, 256, 256, [1500, 600]), (32, 16, 256, 32, [900, 333]), (32, 8, 128, 64, [1500, 600]),
+                                                  (24, 8, 64, 16, [1500, 600])])
+def test_prompt_long(hq, hkv, dim, page, lens, codes):
+    c = Case8(hq, hkv, dim, page, torch.bfloat16, codes, [lens[0], lens[1] + 300])
+    cu = offsets(lens)
+    q = c.q(cu[-1])
+    out = torch.empty_like(q)
+    c.att.prompt8(c.batch(cu), q, c.cache(), out)
+    close(out, *Q.attend_batch(c, q, cu))
+
+
+@pytest.mark.parametrize("codes", CODES)
+@pytest.mark.parametrize("dim,page", [(256, 256), (128, 16), (64, 64)])
+def test_prompt_few_rows_over_a_long_cache(dim, page, codes):
+    c = Case8(8, 2, dim, page, torch.float16, codes, [9000, 4097])
+    cu = [0, 5, 6]
+    q = c.q(6)
+    want, off = Q.attend_batch(c, q, cu)
+    for max_len in (0, 9000, 300):
+        out = torch.empty_like(q)
+        c.att.prompt8(c.batch(cu, max_len=max_len), q, c.cache(), out)
+        close(out, want, off)
+
+
+@pytest.mark.parametrize("dim", [64, 128, 256])
+def test_prompt_rows_without_positions_are_zeros(dim):
+    for extra in (2, 1000):  # one split, and several
+        c = Case8(8, 2, dim, 16, torch.float16, torch.float8_e4m3fn, [3, 0, 20, 1500], extra_cols=extra)
+        cu = [0, 10, 14, 34, 40]
+        q = c.q(40)
+        out = torch.full_like(q, 7.0)
+        c.att.prompt8(c.batch(cu), q, c.cache(), out)
+        c.att.check()
+        close(out, *Q.attend_batch(c, q, cu))
+        assert bool((out[:7] == 0).all()) and bool((out[10:14] == 0).all()) and bool((out[7] != 0).any())
+
+
+@pytest.mark.parametrize("codes", CODES)
+@pytest.mark.parametrize("hq,hkv,dim,rows", [(8, 2, 64, 200), (8, 2, 128, 200), (16, 2, 256, 200), (32, 16, 256, 900)])
+@pytest.mark.parametrize("which", ["k", "v"])
+def test_prompt_scales_that_are_not_finite_reach_their_rows_only(hq, hkv, dim, rows, which, codes):
+    c = Case8(hq, hkv, dim, 16, torch.bfloat16, codes, [rows, 40])
+    cu = [0, rows, rows + 40]
+    q = c.q(cu[-1])
+    want, off = Q.attend_batch(c, q, cu)
+    for at in (0, 77, rows - 1):
+        s = c.ks if which == "k" else c.vs
+        place = int(c.table[0, at // 16]), 1, at % 16
+        kept = s[place].clone()
+        s[place] = math.nan if at else math.inf
+        out = torch.empty_like(q)
+        c.att.prompt8(c.batch(cu), q, c.cache(), out)
+        group = hq // hkv
+        gone = torch.zeros(cu[-1], hq, dtype=torch.bool, device="cuda")
+        gone[at: rows, group: 2 * group] = True
+        assert not bool(torch.isfinite(out[gone]).all(-1).any()) if which == "v" else bool(torch.isnan(out[gone][:, 0]).any())
+        close(out[~gone], want[~gone], off[~gone])
+        s[place] = kept
+
+
+@pytest.mark.parametrize("codes", CODES)
+def test_prompt_scales_of_any_size(codes):
+    for dim in (64, 128, 256):
+        c = Case8(8, 2, dim, 32, torch.float16, codes, [300, 200])
+        cu = [0, 300, 310]
+        q = c.q(310)
+        c.ks *= torch.where(torch.arange(c.page, device="cuda") % 3 == 0, 2.0 ** -40, 1.0)
+        c.vs *= torch.exp2(torch.arange(c.page, device="cuda") % 7 * 4.0 - 30.0)
+        out = torch.empty_like(q)
+        c.att.prompt8(c.batch(cu), q, c.cache(), out)
+        close(out, *Q.attend_batch(c, q, cu))
+
+
+@pytest.mark.parametrize("hq,hkv,dim,page,lens,extra_cols", [
+    (8, 2, 128, 16, [500, 300, 20], 2), (4, 2, 64, 32, [300, 170, 33], 1500), (16, 4, 256, 64, [300, 40, 3], 2), (16, 1, 256, 16, [5, 9, 1], 2000),
+    (32, 16, 256, 32, [1500, 600, 20], 2)])  # row blocks of four and of eight waves, one split and several
+def test_bad_pages_give_zeros_for_all_rows_of_a_prompt(hq, hkv, dim, page, lens, extra_cols):
+    ctx = [7, 1100, 0]
+    c = Case8(hq, hkv, dim, page, torch.bfloat16, torch.int8, [a + b for a, b in zip(lens, ctx)], extra_cols=extra_cols)
+    cu = offsets(lens)
+    q = c.q(cu[-1])
+    want, off = Q.attend_batch(c, q, cu)
+    for i in range(2):
+        pages = -(-c.kv_len[i] // page)
+        for where, what in ((0, -1), (pages // 2, c.kc.shape[0]), (pages - 1, (1 << 31) - 1)):
+            bad = c.table.clone()
+            bad[i, where] = what
+            out = torch.full_like(q, 7.0)
+            c.att.prompt8(qe_mixer.Batch(ints(c.kv_len), bad, ints(cu)), q, c.cache(), out)
+            with pytest.raises(qe_moe.QeError, match="page"):
+                c.att.check()
+            assert bool((out[cu[i]: cu[i + 1]] == 0).all()), (i, where)
+            rest = torch.ones(cu[-1], dtype=torch.bool, device="cuda")
+            rest[cu[i]: cu[i + 1]] = False
+            close(out[rest], want[rest], off[rest])
+    c.att.check()
+
+
+@pytest.mark.parametrize("hq,hkv,dim,ctx,extra_cols", [(8, 2, 64, 0, 2), (16, 1, 256, 4000, 2), (4, 4, 128, 0, 2000)])  # one split, and several
+def test_prompt_bad_lengths_and_offsets_give_zeros_and_an_error(hq, hkv, dim, ctx, extra_cols):
+    lens = [170, 230, 100]
+    c = Case8(hq, hkv, dim, 16, torch.bfloat16, torch.float8_e4m3fn, [n + ctx for n in lens], extra_cols=extra_cols)
+    q = c.q(500)
+    want, off = Q.attend_batch(c, q, [0, 170, 400, 500])
+    for cu, kv1, lost in (([-5, 170, 400, 500], 0, [(0, 170)]), ([-7, -7, 400, 500], 0, [(0, 400)]), ([0, 170, 400, 501], 0, [(400, 500)]),
+                          ([0, 170, 1 << 30, 1 << 30], 0, [(170, 500)]), ([0, 170, 400, 500], -1, [(170, 400)]), ([0, 170, 400, 500], 1 << 30, [(170, 400)])):
+        out = torch.full_like(q, 7.0)
+        kv = list(c.kv_len)
+        kv[1] = kv1 or kv[1]
+        c.att.prompt8(qe_mixer.Batch(ints(kv), c.table, ints(cu)), q, c.cache(), out)
+        with pytest.raises(qe_moe.QeError, match="length or token offset"):
+            c.att.check()
+        gone = torch.zeros(500, dtype=torch.bool, device="cuda")
+        for a, b in lost:
+            gone[a:b] = True
+        assert bool((out[gone] == 0).all()), cu
+        if cu[1] == 170:
+            close(out[~gone], want[~gone], off[~gone])
+
+
+def test_far_offsets_in_a_large_cache():
+    """Pages whose codes start past 2^32 bytes."""
+    hkv, dim, page = 2, 256, 256
+    pages = (1 << 32) // (hkv * page * dim) + 40
+    c = Case8(16, hkv, dim, page, torch.bfloat16, torch.int8, [700, 513])
+    kc, vc = (torch.empty(pages, hkv, page, dim, dtype=torch.int8, device="cuda") for _ in range(2))
+    ks, vs = (torch.empty(pages, hkv, page, device="cuda") for _ in range(2))
+    far = ints([[pages - 1, 5, pages - 7], [3, pages - 2, 0]])
+    for p, to in zip(c.table[:, :3].flatten().tolist(), far.flatten().tolist()):
+        for a, b in ((kc, c.kc), (vc, c.vc), (ks, c.ks), (vs, c.vs)):
+            a[to] = b[p]
+    cache = qe_mixer.Cache8(kc, vc, ks, vs)
+    q = c.q(90)
+    want, off = Q.attend_batch(c, q[:2], [0, 1, 2])
+    out = torch.empty_like(q)
+    c.att.decode8(qe_mixer.Batch(ints(c.kv_len), far), q[:2], cache, out[:2])
+    close(out[:2], want, off)
+    c.att.prompt8(qe_mixer.Batch(ints(c.kv_len), far, ints([0, 60, 90])), q, cache, out)
+    close(out, *Q.attend_batch(c, q, [0, 60, 90]))
+
+
+def test_refusals():
+    c = Case8(8, 2, 64, 32, torch.float16, torch.int8, [50, 60])
+    q = c.q(2)
+    out, a = torch.empty_like(q), c.att
+    with pytest.raises(qe_moe.QeError, match="cu_q"):
+        a.prompt8(c.batch(), q, c.cache(), out)
+    with pytest.raises(qe_moe.QeError, match="cu_q"):
+        a.decode8(c.batch([0, 1, 2]), q, c.cache(), out)
+    other = Case8(8, 4, 64, 32, torch.float16, torch.int8, [50, 60])
+    for call, b in ((a.prompt8, c.batch([0, 1, 2])), (a.decode8, c.batch())):
+        for bad in (dict(q=q.float()), dict(q=q.cpu()), dict(q=q[:, :4]), dict(out=out.bfloat16()), dict(cache=other.cache())):
+            with pytest.raises(ValueError):
+                call(b, **{**dict(q=q, cache=c.cache(), out=out), **bad})
+        cache = c.cache()
+        cache.c.type = 1
+        with pytest.raises(qe_moe.QeError, match="cache type"):
+            call(b, q, cache, out)
+        cache = c.cache()
+        cache.c.k_scale = None
+        with pytest.raises(qe_moe.QeError, match="scales"):
+            call(b, q, cache, out)
+        cache = c.cache()
+        cache.c.v += 8
+        with pytest.raises(qe_moe.QeError, match="aligned"):
+            call(b, q, cache, out)
+    a.check()
