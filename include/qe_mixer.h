@@ -193,6 +193,36 @@ int qe_attn_prompt8(qe_attn_ctx *ctx, const qe_attn_batch *batch, const qe_kv_ca
 int qe_attn_decode8(qe_attn_ctx *ctx, const qe_attn_batch *batch, const qe_kv_cache8 *cache, const void *q, int64_t q_stride, void *out,
                     int64_t out_stride, void *stream);
 
+/* ---- sequences that share their beginnings ----------------------------------- */
+
+/* Groups of a call's sequences.  Group g's are seqs[g] .. seqs[g+1] - 1 (0 <=
+ * seqs[0] <= ... <= seqs[n_groups] <= n_seqs); their first prefix[g] positions
+ * are the same, and stand in the pages of the group's first sequence.  kv_len
+ * counts them.  Of another sequence's table the entries of pages that lie wholly
+ * before position prefix[g] are not used, and of the page that the position lies in
+ * only the rows from it on.  A sequence of no group has all positions to itself.
+ * Where a prefix is out of range (0 .. max_pages * page), a group's offsets
+ * leave the call's sequences, or a sequence is shorter than its group's prefix,
+ * those sequences' outputs are zeros; where offsets fall, the call's outputs may
+ * hold anything.  Either is reported as a bad length. */
+typedef struct {
+    int n_groups;          /* 1 .. 65535 */
+    const int32_t *seqs;   /* device [n_groups + 1] */
+    const int32_t *prefix; /* device [n_groups] */
+    int max_prefix;        /* the greatest prefix as far as the host knows, for choosing splits; 0 = the longest length */
+} qe_attn_shared;
+
+/* qe_attn_decode and qe_attn_decode8 of such sequences: a group's shared keys and
+ * values are read once for all of its queries.  The results are those of the
+ * plain calls on tables whose first entries are the shared pages, but for
+ * rounding (fp16: probabilities below 2^-21 of a row's greatest to fixed steps).
+ * A bad page among the shared ones makes zeros of all of its
+ * group's outputs. */
+int qe_attn_decode_shared(qe_attn_ctx *ctx, const qe_attn_batch *batch, const qe_attn_shared *shared, const qe_kv_cache *cache, const void *q,
+                          int64_t q_stride, void *out, int64_t out_stride, void *stream);
+int qe_attn_decode8_shared(qe_attn_ctx *ctx, const qe_attn_batch *batch, const qe_attn_shared *shared, const qe_kv_cache8 *cache,
+                           const void *q, int64_t q_stride, void *out, int64_t out_stride, void *stream);
+
 /* Synchronise `stream` and report a bad length or page that a kernel met. */
 int qe_attn_check(qe_attn_ctx *ctx, void *stream);
 

@@ -14,11 +14,6 @@
 // Probabilities are rounded to bf16 for the second product, with either type: scaled by V's they have no bounded
 // range, which fp16 would need, and a rounding of 2^-9 is half a step of the cache's integers.
 // ---------------------------------------------------------------------------
-template <int DH>
-__device__ __forceinline__ int swz8(int row) { // of the 16-byte chunk index
-    return DH == 256 ? (row & 7) | (row >> 4 & 1) << 3 : DH == 128 ? (row >> 1 & 3) | (row >> 4 & 1) << 2 : (row >> 2 & 1) | (row >> 4 & 1) << 1;
-}
-
 template <bool BF, int DH, int CT, bool ONCE>
 __global__ __launch_bounds__(256, DH == 256 ? 2 : DH == 128 ? 3 : 4) void k_attn_decode8(const QeAttn8Args x) {
     const QeAttnArgs &a = x.a;

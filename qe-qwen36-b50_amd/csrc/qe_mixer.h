@@ -65,9 +65,19 @@ struct QeAttn8Args {
     const float *ks, *vs; // scales
 };
 
+// Sequences that share beginnings: `x` with kc, vc and, of an 8-bit cache, scales; x.a.splits and x.a.steps of their own
+// positions, x.a.tiles of QE_ATTN_SHARED_BM rows.
+struct QeSharedArgs {
+    QeAttn8Args x;
+    const int32_t *seqs, *prefix; // [n_groups + 1], [n_groups]
+    int n_groups, psplits;
+    int seq0, seq1; // of this launch
+};
+
 #define QE_CACHE16 0 /* a cache of the context's type, beside QE_I8 and QE_F8 */
 hipError_t qe_launch_attn_prompt8(const QeAttn8Args &a, int head_dim, int type, int cache_type, int bm, hipStream_t st);
 hipError_t qe_launch_attn_decode8(const QeAttn8Args &a, int head_dim, int type, int cache_type, hipStream_t st);
+hipError_t qe_launch_attn_shared(const QeSharedArgs &a, int head_dim, int type, int cache_type, hipStream_t st);
 hipError_t qe_launch_append8(const QeAppend8Args &a, int in_type, int type, int cache_type, hipStream_t st);
 hipError_t qe_launch_read8(const QeRead8Args &a, int type, int cache_type, hipStream_t st);
 hipError_t qe_launch_append(const QeAppendArgs &a, int in_type, int type, hipStream_t st);

@@ -427,6 +427,52 @@ int qe_attn_decode8(qe_attn_ctx *c, const qe_attn_batch *b, const qe_kv_cache8 *
     return QE_OK;
 }
 
+}  // extern "C"
+
+// Both calls with shared beginnings; kv8 is null for a 16-bit cache.
+template <typename CACHE>
+static int decode_shared(qe_attn_ctx *c, const qe_attn_batch *b, const qe_attn_shared *sh, const CACHE *kv, const qe_kv_cache8 *kv8, const void *q,
+                         int64_t q_stride, void *out, int64_t out_stride, const char *where, void *stream) {
+    if (b && b->cu_q) return qe_fail(QE_ERR_ARG, "%s: cu_q given (single tokens only)", where);
+    if (!sh || !sh->seqs || !sh->prefix) return qe_fail(QE_ERR_ARG, "%s: null shared, seqs or prefix", where);
+    if (sh->n_groups < 1 || sh->n_groups > 65535) return qe_fail(QE_ERR_ARG, "%s: n_groups %d is not 1 .. 65535", where, sh->n_groups);
+    if (sh->max_prefix < 0) return qe_fail(QE_ERR_ARG, "%s: max_prefix %d", where, sh->max_prefix);
+    int rc = check_attend(c, b, kv, q, q_stride, out, out_stride, where);
+    if (rc != QE_OK) return rc;
+    QeSharedArgs y{};
+    y.x.a = attn_args(c, b, kv, q, q_stride, out, out_stride);
+    if (kv8) y.x.ks = kv8->k_scale, y.x.vs = kv8->v_scale;
+    y.seqs = sh->seqs; y.prefix = sh->prefix; y.n_groups = sh->n_groups;
+    const int64_t most = (int64_t)b->max_pages * c->d.page;
+    const int64_t max_len = b->max_len && b->max_len < most ? b->max_len : most, max_prefix = sh->max_prefix && sh->max_prefix < max_len ? sh->max_prefix : max_len;
+    // a launch's sequences, and their groups as far as they reach into it
+    const int n = qe_attn_shared_seqs(b->n_seqs, y.x.a.q_heads);
+    y.x.a.tiles = qe_attn_max_tiles(n, sh->n_groups, y.x.a.group, QE_ATTN_SHARED_BM);
+    qe_attn_shared_plan(n, sh->n_groups, y.x.a.q_heads, y.x.a.kv_heads, c->d.head_dim, max_prefix, max_len > max_prefix ? max_len - max_prefix : 1, &y.psplits,
+                        &y.x.a.steps, &y.x.a.splits);
+    if (!qe_fits_launch((int64_t)y.x.a.tiles * y.x.a.kv_heads * y.psplits, 256) || !qe_fits_launch((int64_t)n * y.x.a.q_heads * y.x.a.splits, 256))
+        return qe_fail(QE_ERR_ARG, "%s: %d sequences of %d groups are more threads than a launch has", where, b->n_seqs, sh->n_groups);
+    OnDevice on(c->device);
+    HIP_TRY(on.e);
+    for (y.seq0 = 0; y.seq0 < b->n_seqs; y.seq0 = y.seq1) {
+        y.seq1 = y.seq0 + n < b->n_seqs ? y.seq0 + n : b->n_seqs;
+        HIP_TRY(qe_launch_attn_shared(y, c->d.head_dim, c->d.type, kv8 ? kv8->type : QE_CACHE16, (hipStream_t)stream));
+    }
+    return QE_OK;
+}
+
+extern "C" {
+
+int qe_attn_decode_shared(qe_attn_ctx *c, const qe_attn_batch *b, const qe_attn_shared *shared, const qe_kv_cache *kv, const void *q, int64_t q_stride,
+                          void *out, int64_t out_stride, void *stream) {
+    return decode_shared(c, b, shared, kv, nullptr, q, q_stride, out, out_stride, "qe_attn_decode_shared", stream);
+}
+
+int qe_attn_decode8_shared(qe_attn_ctx *c, const qe_attn_batch *b, const qe_attn_shared *shared, const qe_kv_cache8 *kv, const void *q, int64_t q_stride,
+                           void *out, int64_t out_stride, void *stream) {
+    return decode_shared(c, b, shared, kv, kv, q, q_stride, out, out_stride, "qe_attn_decode8_shared", stream);
+}
+
 int qe_attn_check(qe_attn_ctx *c, void *stream) {
     if (!c) return qe_fail(QE_ERR_ARG, "qe_attn_check: null context");
     OnDevice on(c->device);

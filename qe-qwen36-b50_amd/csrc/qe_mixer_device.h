@@ -214,3 +214,8 @@ __device__ __forceinline__ uint2 lds_tr8(const uint8_t *p) {
     typedef int i2 __attribute__((ext_vector_type(2)));
     return __builtin_bit_cast(uint2, __builtin_amdgcn_ds_read_tr8_b64_v2i32((__attribute__((address_space(3))) i2 *)p));
 }
+// Permutation of a row's 16-byte chunks of codes in LDS: the 16 rows that half a wave reads with lds_tr8 lie in different banks.
+template <int DH>
+__device__ __forceinline__ int swz8(int row) { // of the 16-byte chunk index
+    return DH == 256 ? (row & 7) | (row >> 4 & 1) << 3 : DH == 128 ? (row >> 1 & 3) | (row >> 4 & 1) << 2 : (row >> 2 & 1) | (row >> 4 & 1) << 1;
+}

@@ -88,6 +88,35 @@ QE_MIX_HD int qe_attn_prompt_splits(int64_t tiles, int64_t max_len) {
     return s < 1 ? 1 : (int)s;
 }
 
+// A call of single tokens whose sequences share beginnings: `psplits` workgroups for every 128 rows of a group's queries and
+// key-value head over the shared keys, and `splits` of `steps` steps for a sequence's own (as qe_attn_decode_plan has them).
+// Each leaves partial results, psplits + splits for a row of n_seqs * q_heads, which have room for QE_ATTN_SHARED_ROWS.  At
+// most 2^15 rows are in a launch (qe_attn_shared_seqs), so that each has room for two.
+#define QE_ATTN_SHARED_ROWS 65536
+#define QE_ATTN_SHARED_BM 128 /* rows of a workgroup */
+QE_MIX_HD int qe_attn_shared_seqs(int n_seqs, int q_heads) {
+    const int most = QE_ATTN_SHARED_ROWS / 2 / q_heads;
+    return n_seqs < most ? n_seqs : most;
+}
+QE_MIX_HD void qe_attn_shared_plan(int n_seqs, int n_groups, int q_heads, int kv_heads, int head_dim, int64_t max_prefix, int64_t max_own, int *psplits,
+                                   int *steps, int *splits) {
+    const int64_t room = QE_ATTN_SHARED_ROWS / ((int64_t)n_seqs * q_heads);
+    qe_attn_decode_plan(n_seqs, kv_heads, head_dim, max_own, steps, splits);
+    if (*splits > (room + 1) / 2) *splits = (int)((room + 1) / 2);
+    const int64_t tiles = ((int64_t)n_seqs * (q_heads / kv_heads) + (int64_t)n_groups * (QE_ATTN_SHARED_BM - 1)) / QE_ATTN_SHARED_BM * kv_heads;
+    const int64_t most = (max_prefix + 255) / 256;
+    int64_t s = 256 / (tiles > 0 ? tiles : 1);
+    if (s > most) s = most;
+    if (s > room - *splits) s = room - *splits;
+    *psplits = s < 1 ? 1 : (int)s;
+}
+// Steps of `step` keys of a shared beginning in each of its splits, and how many of those have any.
+QE_MIX_HD int qe_attn_shared_per(int prefix, int step, int psplits) { return ((prefix + step - 1) / step + psplits - 1) / psplits; }
+QE_MIX_HD int qe_attn_shared_active(int prefix, int step, int psplits) {
+    const int per = qe_attn_shared_per(prefix, step, psplits);
+    return per ? ((prefix + step - 1) / step + per - 1) / per : 0;
+}
+
 // The part [*lo, *hi) of n steps that split s of `splits` takes.
 QE_MIX_HD void qe_split_range(int n, int splits, int s, int *lo, int *hi) {
     const int per = (n + splits - 1) / splits;

@@ -47,6 +47,10 @@ class _Norm(ctypes.Structure):
     _fields_ = [("q_weight", _vp), ("k_weight", _vp), ("eps", _f32)]
 
 
+class _Shared(ctypes.Structure):
+    _fields_ = [("n_groups", _i32), ("seqs", _vp), ("prefix", _vp), ("max_prefix", _i32)]
+
+
 class _DeltaDesc(ctypes.Structure):
     _fields_ = [("k_heads", _i32), ("v_heads", _i32), ("dim_k", _i32), ("dim_v", _i32), ("type", _i32), ("l2norm", _i32),
                 ("scale", _f32), ("t_max", _i32), ("seqs_max", _i32)]
@@ -72,6 +76,8 @@ _SIGNATURES = {
     "qe_attn_decode": [_vp, ctypes.POINTER(_Batch), ctypes.POINTER(_Cache), _vp, _i64, _vp, _i64, _vp],
     "qe_attn_prompt8": [_vp, ctypes.POINTER(_Batch), ctypes.POINTER(_Cache8), _vp, _i64, _vp, _i64, _vp],
     "qe_attn_decode8": [_vp, ctypes.POINTER(_Batch), ctypes.POINTER(_Cache8), _vp, _i64, _vp, _i64, _vp],
+    "qe_attn_decode_shared": [_vp, ctypes.POINTER(_Batch), ctypes.POINTER(_Shared), ctypes.POINTER(_Cache), _vp, _i64, _vp, _i64, _vp],
+    "qe_attn_decode8_shared": [_vp, ctypes.POINTER(_Batch), ctypes.POINTER(_Shared), ctypes.POINTER(_Cache8), _vp, _i64, _vp, _i64, _vp],
     "qe_attn_check": [_vp, _vp],
     "qe_delta_create": [_i32, ctypes.POINTER(_DeltaDesc), ctypes.POINTER(_vp)],
     "qe_delta_destroy": [_vp],
@@ -213,6 +219,21 @@ class Cache8:
         self._ref = ctypes.byref(self.c)
 
 
+class Shared:
+    """Groups of a batch's sequences that share their beginnings: int32 seqs [groups + 1], group g's first sequence and one
+    behind its last, and prefix [groups], how many positions it shares (in the pages of its first sequence).  Both may be
+    updated in place between calls.  max_prefix: the greatest as far as is known, for choosing splits."""
+
+    def __init__(self, seqs, prefix, max_prefix=0):
+        n, device = prefix.shape[0], prefix.get_device()
+        _ints(prefix, (n,), device, "prefix")
+        _ints(seqs, (n + 1,), device, "seqs")
+        _i32s(groups=n, max_prefix=int(max_prefix))
+        self.device, self.seqs, self.prefix = device, seqs, prefix
+        self.c = _Shared(n, seqs.data_ptr(), prefix.data_ptr(), int(max_prefix))
+        self._ref = ctypes.byref(self.c)
+
+
 class Attention:
     """One attention geometry on one GPU: rotary positions and cache write, prompts, single tokens."""
 
@@ -325,11 +346,11 @@ class Attention:
         if rc:
             _check(rc)
 
-    def _attend(self, entry, batch, q, cache, out, stream):
+    def _attend(self, entry, batch, q, cache, out, stream, *shared):
         qp, qs = _rows(q, self.q_heads, self.head_dim, self.dtype, self.device, "q")
         n = q.shape[0]
         op, os_ = _rows(out, self.q_heads, self.head_dim, self.dtype, self.device, "out", n)
-        rc = entry(self.h, self._batch(batch, n), cache, qp, qs, op, os_, _stream(stream))
+        rc = entry(self.h, self._batch(batch, n), *shared, cache, qp, qs, op, os_, _stream(stream))
         if rc:
             _check(rc)
 
@@ -348,6 +369,19 @@ class Attention:
     def decode8(self, batch, q, cache, out, stream=None):
         """decode over an 8-bit cache (Cache8)."""
         self._attend(self._lib.qe_attn_decode8, batch, q, self._cache8(cache), out, stream)
+
+    def _shared(self, shared):
+        if shared.device != self.device:
+            _bad(f"the groups are on cuda:{shared.device}, the context on cuda:{self.device}")
+        return shared._ref
+
+    def decode_shared(self, batch, shared, q, kc, vc, out, stream=None):
+        """decode of sequences that share their beginnings (Shared)."""
+        self._attend(self._lib.qe_attn_decode_shared, batch, q, self._cache(kc, vc), out, stream, self._shared(shared))
+
+    def decode8_shared(self, batch, shared, q, cache, out, stream=None):
+        """The same over an 8-bit cache (Cache8)."""
+        self._attend(self._lib.qe_attn_decode8_shared, batch, q, self._cache8(cache), out, stream, self._shared(shared))
 
     def check(self, stream=None):
         """Synchronise `stream`; raise QeError if a kernel met a bad length or page."""
