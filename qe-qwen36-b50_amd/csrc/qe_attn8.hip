@@ -11,8 +11,7 @@
 // transposing reads of bytes; its 16-byte chunks are permuted by row so that the 16 rows that half a wave reads lie in
 // different banks.  A key's scale multiplies its scores, a value's its probabilities, each from one register: lane n of
 // 16 has the scale of their n-th key, which the multiplication takes from there.
-// Probabilities are rounded to bf16 for the second product, with either type: scaled by V's they have no bounded
-// range, which fp16 would need, and a rounding of 2^-9 is half a step of the cache's integers.
+// Probabilities, times their values' scales, are rounded to the context's type for the second product (fp16: Units).
 // ---------------------------------------------------------------------------
 template <bool BF, int DH, int CT, bool ONCE>
 __global__ __launch_bounds__(256, DH == 256 ? 2 : DH == 128 ? 3 : 4) void k_attn_decode8(const QeAttn8Args x) {
@@ -48,6 +47,7 @@ __global__ __launch_bounds__(256, DH == 256 ? 2 : DH == 128 ? 3 : 4) void k_attn
 #pragma unroll
     for (int d = 0; d < DB; ++d) acc[d] = qe_f4{0, 0, 0, 0};
     float m = -INFINITY, l = 0;
+    Units units;
     uint8_t *vb = (uint8_t *)lds[wave];
     auto load16 = [](const void *p) {
         typedef unsigned u4 __attribute__((ext_vector_type(4)));
@@ -72,7 +72,8 @@ __global__ __launch_bounds__(256, DH == 256 ? 2 : DH == 128 ? 3 : 4) void k_attn
 #pragma unroll
         for (int s = 0; s < KL; ++s) kr[1][s] = load16(kp1 + s * 64);
         const size_t sr = (col & 4 ? r1 : r0) + 4 * c + (col & 3);
-        const float ks = x.ks[sr], vs = x.vs[sr];
+        const float ks = x.ks[sr];
+        float vs = x.vs[sr];
 #pragma unroll
         for (int i = 0; i < QE_ATTN_TILE / ROWS; ++i) {
             const int row = i * ROWS + lane / CH, ch = (lane % CH) ^ swz8<DH>(row);
@@ -108,7 +109,14 @@ __global__ __launch_bounds__(256, DH == 256 ? 2 : DH == 128 ? 3 : 4) void k_attn
             l *= f;
             m = mn;
         }
-        const float base = exponent_base<true, 0>(m * a.scale_log2);
+        if constexpr (!BF) {
+            const float f = units.raise(!cut || (col & 4 ? k0 + 16 : k0) + 4 * c + (col & 3) < len ? vs : 0.f);
+            if (f != 1.f)
+#pragma unroll
+                for (int d = 0; d < DB; ++d) acc[d] *= f;
+            vs *= units.inverse;
+        }
+        const float base = exponent_base<BF, 0>(m * a.scale_log2);
         float p[8];
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
@@ -130,7 +138,7 @@ __global__ __launch_bounds__(256, DH == 256 ? 2 : DH == 128 ? 3 : 4) void k_attn
             qe_s8 v;
         } pf;
 #pragma unroll
-        for (int i = 0; i < 4; ++i) pf.u[i] = pack2<true>(w[2 * i], w[2 * i + 1]);
+        for (int i = 0; i < 4; ++i) pf.u[i] = pack2<BF>(w[2 * i], w[2 * i + 1]);
         __builtin_amdgcn_s_waitcnt(0x0f70); // the direct loads have landed (vmcnt 0)
         if (CT == QE_F8 && cut) {            // codes behind the end may be NaN: a probability of 0 times NaN is NaN
             for (int i = lane; i < QE_ATTN_TILE * CH; i += 64)
@@ -139,9 +147,12 @@ __global__ __launch_bounds__(256, DH == 256 ? 2 : DH == 128 ? 3 : 4) void k_attn
 #pragma unroll
         for (int d = 0; d < DB; ++d) {
             const uint2 v = lds_tr8(tr + ((d ^ swz8<DH>(tr_key)) << 4));
-            acc[d] = mfma16<true>(elements_of<CT, true>(v.x, v.y), pf.v, acc[d]);
+            acc[d] = mfma16<BF>(elements_of<CT, BF>(v.x, v.y), pf.v, acc[d]);
         }
     }
+    if constexpr (!BF)
+#pragma unroll
+        for (int d = 0; d < DB; ++d) acc[d] *= units.unit;
     finish_decode<BF, DH>(a, item, split, active, acc, m, l, bad, bad_len, &lds[0][0], LDS, ml);
 }
 

@@ -5,7 +5,7 @@
 // wave loads its part of the next tile's codes while this one is worked on, turns them to 16 bits when its work is done,
 // and writes them to the other of two buffers, so that a code is turned once for all rows of a workgroup.  With heads of 256
 // the registers are full: there the codes wait in a few KB of LDS, by direct loads.  A key's scale multiplies its scores and a
-// value's its probabilities (to bf16, as in k_attn_decode8), from one register: lane n of 16 has the scale of the n-th
+// value's its probabilities (in fp16 in units of theirs: Units), from one register: lane n of 16 has the scale of the n-th
 // of the 16 keys in the lane's registers.
 #include "qe_attn_stage8.h"
 
@@ -57,7 +57,8 @@ __global__ __launch_bounds__(64 * WAVES, 2) void k_attn_prompt8(const QeAttn8Arg
         stage.issue(x, page, kvh, lo * BN, len, wave, raw);
         page = page_of<BN, WAVES>(a, table, (lo + 1) * BN, len, wave);
     }
-    Rows<BF, DH, true> w;
+    Rows<BF, DH> w;
+    Units units;
     {
         const int row = wave_row + (tid & 31), h = tid >> 5 & 1;
         const bool there = row < n_rows;
@@ -99,12 +100,13 @@ __global__ __launch_bounds__(64 * WAVES, 2) void k_attn_prompt8(const QeAttn8Arg
             const int limit = w.place - k0 - 4 * (lane >> 5);
             if (cut) s.mask(limit);
             w.raise(s.top() * a.scale_log2);
+            if constexpr (!BF) w.times(units.raise(s_lds[1][lane & (BN - 1)]));
             Probs<KB> p;
             w.weigh(a.scale_log2, s);
 #pragma unroll
-            for (int b = 0; b < KB; ++b) scaled(s.s[b], s_lds[1][b * 32 + at]);
+            for (int b = 0; b < KB; ++b) scaled(s.s[b], BF ? s_lds[1][b * 32 + at] : s_lds[1][b * 32 + at] * units.inverse);
             if (cut) s.clear(limit); // a scale that is not finite reaches the rows that attend to its position
-            s.pack(p);
+            s.template pack<BF>(p);
             w.values(v_lds, 0, p);
             schedule<3, KB * DH / 16, 2>();
         }
@@ -118,6 +120,7 @@ __global__ __launch_bounds__(64 * WAVES, 2) void k_attn_prompt8(const QeAttn8Arg
         work(t, k_a, v_a, s_a, k_b, v_b, s_b);
         if (t + 1 < hi) work(t + 1, k_b, v_b, s_b, k_a, v_a, s_a);
     }
+    if constexpr (!BF) w.times(units.unit);
     w.template finish<BM>(a, begin, n_rows, row0, wave_row, tile, kvh, split);
 }
 

@@ -104,11 +104,12 @@ struct Scores {
             for (int i = 0; i < 16; ++i)
                 if (b * 32 + 8 * (i / 4) + i % 4 > limit) s[b][i] = 0;
     }
-    __device__ __forceinline__ void pack(Probs<KB> &p) const { // to bf16
+    template <bool BF>
+    __device__ __forceinline__ void pack(Probs<KB> &p) const {
 #pragma unroll
         for (int b = 0; b < KB; ++b)
 #pragma unroll
-            for (int i = 0; i < 16; i += 2) p.p[b][i / 8].u[i % 8 / 2] = pack2<true>(s[b][i], s[b][i + 1]);
+            for (int i = 0; i < 16; i += 2) p.p[b][i / 8].u[i % 8 / 2] = pack2<BF>(s[b][i], s[b][i + 1]);
     }
     __device__ __forceinline__ float top() const { // of the row
         float t = s[0][0];
@@ -123,8 +124,7 @@ struct Scores {
         return max_halves(t);
     }
 };
-// BF: Q's and K's type; PBF: that of the probabilities and V.
-template <bool BF, int DH, bool PBF = BF>
+template <bool BF, int DH>
 struct Rows {
     static constexpr int LAG = 8;
     qe_f16v o[DH / 32]; // O^T
@@ -161,7 +161,7 @@ struct Rows {
     }
     template <int KB>
     __device__ __forceinline__ void exponentials(float scale, const Scores<KB> &x, Probs<KB> &p) {
-        const float base = exponent_base<PBF, LAG>(m);
+        const float base = exponent_base<BF, LAG>(m);
         float sum[2] = {0, 0};
 #pragma unroll
         for (int b = 0; b < KB; ++b)
@@ -171,14 +171,20 @@ struct Rows {
                 const float z = __builtin_amdgcn_exp2f(fmaf(x.s[b][i + 1], scale, base));
                 sum[0] += y;
                 sum[1] += z;
-                p.p[b][i / 8].u[i % 8 / 2] = pack2<PBF>(y, z);
+                p.p[b][i / 8].u[i % 8 / 2] = pack2<BF>(y, z);
             }
         l += sum[0] + sum[1];
+    }
+    // O counts other units: Units::raise
+    __device__ __forceinline__ void times(float f) {
+        if (f != 1.f)
+#pragma unroll
+            for (int d = 0; d < DH / 32; ++d) o[d] *= f;
     }
     // the scores become probabilities, not rounded yet
     template <int KB>
     __device__ __forceinline__ void weigh(float scale, Scores<KB> &x) {
-        const float base = exponent_base<PBF, LAG>(m);
+        const float base = exponent_base<BF, LAG>(m);
         float sum[2] = {0, 0};
 #pragma unroll
         for (int b = 0; b < KB; ++b)
@@ -201,7 +207,7 @@ struct Rows {
             for (int d = 0; d < DH / 32; ++d) {
                 const unsigned vp = (va ^ (d & 3) << 6) + (b0 * 2 + ks) * 32 * DH + (d >> 2) * 256;
                 const qe_s4 x = lds_tr((const short *)((const char *)v_lds + vp)), y = lds_tr((const short *)((const char *)v_lds + (vp + 16 * DH))); // 8 rows on the permutation is the same
-                o[d] = mfma32<PBF>(qe_s8{x[0], x[1], x[2], x[3], y[0], y[1], y[2], y[3]}, p.p[ks / 2][ks % 2].v, o[d]);
+                o[d] = mfma32<BF>(qe_s8{x[0], x[1], x[2], x[3], y[0], y[1], y[2], y[3]}, p.p[ks / 2][ks % 2].v, o[d]);
             }
     }
     // The rows to `out`, or as a split's partial results.

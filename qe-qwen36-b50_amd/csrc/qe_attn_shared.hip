@@ -95,7 +95,8 @@ __global__ __launch_bounds__(256, 2) void k_shared_prefix(const QeSharedArgs y) 
         }
     };
     load(lo, k_a, v_a);
-    Rows<BF, DH, CODES || BF> w;
+    Rows<BF, DH> w;
+    Units units;
     {
         const short *q = (const short *)a.q + (size_t)seq * a.q_stride + (size_t)head * DH + (tid >> 5 & 1) * 8;
 #pragma unroll
@@ -133,10 +134,11 @@ __global__ __launch_bounds__(256, 2) void k_shared_prefix(const QeSharedArgs y) 
             w.raise(s.top() * a.scale_log2);
             Probs<KB> p;
             if constexpr (CODES) {
+                if constexpr (!BF) w.times(units.raise(s_lds[1][lane & (BN - 1)]));
                 w.weigh(a.scale_log2, s);
 #pragma unroll
-                for (int b = 0; b < KB; ++b) scaled(s.s[b], s_lds[1][b * 32 + at]);
-                s.pack(p);
+                for (int b = 0; b < KB; ++b) scaled(s.s[b], BF ? s_lds[1][b * 32 + at] : s_lds[1][b * 32 + at] * units.inverse);
+                s.template pack<BF>(p);
             } else {
                 w.exponentials(a.scale_log2, s, p);
             }
@@ -153,6 +155,7 @@ __global__ __launch_bounds__(256, 2) void k_shared_prefix(const QeSharedArgs y) 
         work(t, k_a, v_a, s_a, k_b, v_b, s_b);
         if (t + 1 < hi) work(t + 1, k_b, v_b, s_b, k_a, v_a, s_a);
     }
+    if constexpr (CODES && !BF) w.times(units.unit);
     bad = __syncthreads_or(bad);
     if (bad && tid == 0) report(a.err, QE_BAD_PAGE);
     const float sum = w.l + __shfl_xor(w.l, 32);
@@ -172,7 +175,7 @@ __global__ __launch_bounds__(256, 2) void k_shared_prefix(const QeSharedArgs y) 
 template <bool BF, int DH, int CT>
 __global__ __launch_bounds__(256, DH == 256 ? 2 : 3) void k_shared_own(const QeSharedArgs y) {
     const QeAttnArgs &a = y.x.a;
-    constexpr bool CODES = CT != QE_CACHE16, PBF = CODES || BF;
+    constexpr bool CODES = CT != QE_CACHE16;
     constexpr int SIZE = CODES ? 1 : 2;                // bytes of an element
     constexpr int CH = DH * SIZE / 16, ROWS = 64 / CH; // 16-byte chunks of a row, rows of one direct load
     constexpr int KL = DH * SIZE / 64, DB = DH / 16;
@@ -198,6 +201,7 @@ __global__ __launch_bounds__(256, DH == 256 ? 2 : 3) void k_shared_own(const QeS
 #pragma unroll
     for (int d = 0; d < DB; ++d) acc[d] = qe_f4{0, 0, 0, 0};
     float m = -INFINITY, l = 0;
+    Units units;
     uint8_t *vb = (uint8_t *)lds[wave];
     const int tr_key = CODES ? 4 * c + (col >> 1 & 3) + (col & 8) * 2 : 4 * c + (col >> 2);
     auto swz = [](int r) { return CODES ? swz8<DH>(r) : v_swz<DH>(r); };
@@ -261,7 +265,14 @@ __global__ __launch_bounds__(256, DH == 256 ? 2 : 3) void k_shared_own(const QeS
             l *= f;
             m = mn;
         }
-        const float base = exponent_base<PBF, Rows<BF, DH>::LAG>(m * a.scale_log2); // as large as the prefix's are kept
+        if constexpr (CODES && !BF) {
+            const float f = units.raise(cut && outside((col & 4 ? 16 : 0) + 4 * c + (col & 3)) ? 0.f : vs);
+            if (f != 1.f)
+#pragma unroll
+                for (int d = 0; d < DB; ++d) acc[d] *= f;
+            vs *= units.inverse;
+        }
+        const float base = exponent_base<BF, Rows<BF, DH>::LAG>(m * a.scale_log2); // as large as the prefix's are kept
         float p[8];
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
@@ -285,7 +296,7 @@ __global__ __launch_bounds__(256, DH == 256 ? 2 : 3) void k_shared_own(const QeS
             qe_s8 v;
         } pf;
 #pragma unroll
-        for (int i = 0; i < 4; ++i) pf.u[i] = pack2<PBF>(p[2 * i], p[2 * i + 1]);
+        for (int i = 0; i < 4; ++i) pf.u[i] = pack2<BF>(p[2 * i], p[2 * i + 1]);
         __builtin_amdgcn_s_waitcnt(0x0f70); // the direct loads have landed (vmcnt 0)
         if (CT != QE_I8 && cut) {            // V there may be anything: a probability of 0 times NaN is NaN
             for (int i = lane; i < QE_ATTN_TILE * CH; i += 64)
@@ -295,7 +306,7 @@ __global__ __launch_bounds__(256, DH == 256 ? 2 : 3) void k_shared_own(const QeS
         for (int d = 0; d < DB; ++d) {
             if constexpr (CODES) {
                 const uint2 v = lds_tr8(vb + tr_key * DH + ((d ^ swz(tr_key)) << 4) + (col & 1) * 8);
-                acc[d] = mfma16<true>(elements_of<CT, true>(v.x, v.y), pf.v, acc[d]);
+                acc[d] = mfma16<BF>(elements_of<CT, BF>(v.x, v.y), pf.v, acc[d]);
             } else {
                 const int el = d * 16 + (col & 3) * 4, at = (((el >> 3) ^ swz(tr_key)) << 3) + (el & 7); // 16 rows on the permutation is the same
                 const qe_s4 x = lds_tr((const short *)vb + tr_key * DH + at), z = lds_tr((const short *)vb + (tr_key + 16) * DH + at);
@@ -303,6 +314,9 @@ __global__ __launch_bounds__(256, DH == 256 ? 2 : 3) void k_shared_own(const QeS
             }
         }
     }
+    if constexpr (CODES && !BF)
+#pragma unroll
+        for (int d = 0; d < DB; ++d) acc[d] *= units.unit;
     // the four waves' results joined (as in finish_decode), and left as a partial one
     l += __shfl_xor(l, 16);
     l += __shfl_xor(l, 32);

@@ -54,8 +54,8 @@ struct Stage {
             short *kr = k_lds + row * DH, *vr = v_lds + row * DH;
             *(qe_s8 *)(kr + ((c ^ k_swz(row)) << 3)) = elements_of<CT, BF>(a[0], a[1]);
             *(qe_s8 *)(kr + (((c + 1) ^ k_swz(row)) << 3)) = elements_of<CT, BF>(a[2], a[3]);
-            *(qe_s8 *)(vr + ((c ^ v_swz<DH>(row)) << 3)) = elements_of<CT, true>(b[0], b[1]);
-            *(qe_s8 *)(vr + (((c + 1) ^ v_swz<DH>(row)) << 3)) = elements_of<CT, true>(b[2], b[3]);
+            *(qe_s8 *)(vr + ((c ^ v_swz<DH>(row)) << 3)) = elements_of<CT, BF>(b[0], b[1]);
+            *(qe_s8 *)(vr + (((c + 1) ^ v_swz<DH>(row)) << 3)) = elements_of<CT, BF>(b[2], b[3]);
         }
     }
 };

@@ -208,6 +208,33 @@ template <int I>
 __device__ __forceinline__ float of_lane(float x) {
     return __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(x), 0x150 + I, 0xf, 0xf, true));
 }
+// The value scales of an 8-bit cache as fp16 probabilities can take them: a probability times a scale has no bounded range, but
+// times scale / unit it has, where unit is a power of two that is above all scales so far.  The sums with V count units; they are
+// brought to a new one where a tile has a greater scale.  (bf16 has the range of 32 bits and needs none.)
+struct Units {
+    float unit = 0, inverse = 0;
+    // `scale`, over all lanes: a tile's; those of fewer lanes are in others, too.  What sums so far are to be multiplied by.
+    __device__ __forceinline__ float raise(float scale) {
+        float top = fabsf(scale) < INFINITY ? fabsf(scale) : 0.f; // one that is not finite reaches the rows that attend to it without this
+        top = fmaxf(top, __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(top), 0xb1, 0xf, 0xf, true)));
+        top = fmaxf(top, __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(top), 0x4e, 0xf, 0xf, true)));
+        top = fmaxf(top, __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(top), 0x141, 0xf, 0xf, true)));
+        top = fmaxf(top, __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(top), 0x140, 0xf, 0xf, true)));
+        const auto a = __builtin_amdgcn_permlane16_swap(__float_as_uint(top), __float_as_uint(top), false, false);
+        top = fmaxf(__uint_as_float(a[0]), __uint_as_float(a[1]));
+        const auto b = __builtin_amdgcn_permlane32_swap(__float_as_uint(top), __float_as_uint(top), false, false);
+        const unsigned bits = __builtin_amdgcn_readfirstlane(__float_as_uint(fmaxf(__uint_as_float(b[0]), __uint_as_float(b[1]))));
+        if (__uint_as_float(bits) <= unit) return 1.f;
+        // two to four times the greatest, so that it seldom changes; within 2^-100 .. 2^100
+        unsigned e = (bits >> 23) + 2;
+        e = e < 27 ? 27 : e > 227 ? 227 : e;
+        const float was = unit, next = __uint_as_float(e << 23);
+        if (next <= was) return 1.f;
+        unit = next;
+        inverse = __uint_as_float((254 - e) << 23);
+        return was * inverse;
+    }
+};
 // Transposing LDS read of bytes: of each 16 lanes, lane l addresses 8 bytes of row l / 2 (columns 8 (l % 2) .. + 7) and gets
 // column l of the eight rows.
 __device__ __forceinline__ uint2 lds_tr8(const uint8_t *p) {

@@ -59,7 +59,9 @@ def poison(codes, scale, used, g):
 def attend(q, k, v, place, scale):
     """q [rows, dim] of one head, k and v [keys, dim] in 64 bits, place [rows] -> (out, how far it may be off).  As with a 16-bit
     cache: a score is a sum of dim products in 32 bits, and its key's scale; a probability takes the score's error twice, the
-    exponential's, and one rounding to bf16."""
+    exponential's, and with its value's scale one rounding to the type.  fp16 has fixed steps of 2^-24 there: a probability of
+    1 is kept at 2^7 at least, and a scale in units of at most four times the greatest, so that half a step is 2^-25 2^-7 4
+    = 2^-30 of the greatest value for each key."""
     u, dim = U[q.dtype], q.shape[1]
     if k.shape[0] == 0:
         z = torch.zeros_like(q, dtype=torch.float64)
@@ -73,7 +75,10 @@ def attend(q, k, v, place, scale):
     div = torch.where(total == 0, 1.0, total)
     o, size = p @ v / div, p @ v.abs() / div
     ds = (dim + 2) * 2.0 ** -24 * scale * ((q.abs() @ k.abs().T) * seen).amax(-1, keepdim=True)
-    return o, u * o.abs() + (2.0 ** -8 + 2 * ds + 2.0 ** -18) * size + 1e-7
+    off = u * o.abs() + (u + 2 * ds + 2.0 ** -18) * size + 1e-7
+    if u < 2.0 ** -8:
+        off += 2.0 ** -30 * v.abs().max() * seen.sum(-1, keepdim=True) / div
+    return o, off
 
 
 def rows_of(c, cache, i, h, n, first=None, shared=0):
