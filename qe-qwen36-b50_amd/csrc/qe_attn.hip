@@ -214,7 +214,7 @@ __global__ __launch_bounds__(256, 2) void k_attn_decode(const QeAttnArgs a) {
             acc[d] = mfma16<BF>(qe_s8{x[0], x[1], x[2], x[3], y[0], y[1], y[2], y[3]}, pf.v, acc[d]);
         }
     }
-    finish_decode<BF, DH>(a, item, split, active, acc, m, l, bad, bad_len, &v_lds[0][0], QE_ATTN_TILE * DH, ml);
+    finish_decode<BF, DH, 16>(a, item, split, active, acc, m, l, bad, bad_len, [&](int w, int h) { return (float *)v_lds[w] + h * DH; }, v_lds[0], ml);
 }
 
 template <bool BF, int DH>

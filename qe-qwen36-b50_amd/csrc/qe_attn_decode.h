@@ -4,10 +4,11 @@
 
 // Four waves' results (acc: O^T, column the head; m, l: running maximum and sum of the lane's keys) of split `split` of
 // sequence and key-value head `item`: joined, and written where there is one active split, else left as a partial result,
-// which with few splits the last workgroup to arrive joins.  `lds`: `stride` shorts a wave, room for 16 heads x DH floats.
-template <bool BF, int DH>
+// which with few splits the last workgroup to arrive joins.  row(w, h): DH floats of LDS for wave w's head h, of HEADS at a time;
+// lds: some of it, 4 KB.
+template <bool BF, int DH, int HEADS, typename ROW>
 __device__ __forceinline__ void finish_decode(const QeAttnArgs &a, int item, int split, int active, const qe_f4 *acc, float m, float l, unsigned bad,
-                                              unsigned bad_len, short *lds, int stride, float2 (*ml)[16]) {
+                                              unsigned bad_len, const ROW &row, void *lds, float2 (*ml)[16]) {
     constexpr int DB = DH / 16;
     const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63, col = lane & 15, c = lane >> 4;
     const int seq = item / a.kv_heads, kvh = item % a.kv_heads;
@@ -15,44 +16,56 @@ __device__ __forceinline__ void finish_decode(const QeAttnArgs &a, int item, int
     l += __shfl_xor(l, 16);
     l += __shfl_xor(l, 32);
     if (lane < 16) ml[wave][lane] = make_float2(m, l);
-    // the waves' results through LDS (a wave's own V buffer holds 16 heads x DH floats)
-    float *o = (float *)(lds + wave * stride);
-    for (int d = 0; d < DB; ++d) *(qe_f4 *)(o + col * DH + ((d * 4 + c) ^ col) * 4) = acc[d]; // 16-byte units permuted by row: rows lie in the same banks
-    bad = __syncthreads_or(bad) ? 1 : 0;
-    if (tid == 0 && (bad | bad_len)) report(a.err, bad ? QE_BAD_PAGE : QE_BAD_LENGTH);
-    for (int i = tid; i < a.group * (DH / 4); i += 256) {
-        const int h = i / (DH / 4), d = i % (DH / 4) * 4;
-        float top = ml[0][h].x;
-        for (int w = 1; w < 4; ++w) top = fmaxf(top, ml[w][h].x);
-        float sum = 0;
-        qe_f4 r = {0, 0, 0, 0};
 #pragma unroll
-        for (int w = 0; w < 4; ++w) { // no branches: each would wait for the LDS anew
-            const float2 x = ml[w][h];
-            const float f = x.x == -INFINITY ? 0.f : __builtin_amdgcn_exp2f((x.x - top) * a.scale_log2);
-            const qe_f4 y = *(const qe_f4 *)((const float *)(lds + w * stride) + h * DH + ((d / 4) ^ h) * 4);
-            const bool any = x.y != 0.f; // else a wave without keys
-            sum += any ? f * x.y : 0.f;
-            for (int j = 0; j < 4; ++j) r[j] += any ? f * y[j] : 0.f;
+    for (int h0 = 0; h0 < 16; h0 += HEADS) {
+        if (h0 && h0 >= a.group) break;
+        // the waves' results through LDS
+        if (h0) __syncthreads();
+        if (HEADS == 16 || col / HEADS == h0 / HEADS) {
+            float *o = row(wave, col - h0);
+            for (int d = 0; d < DB; ++d) *(qe_f4 *)(o + ((d * 4 + c) ^ col) * 4) = acc[d]; // 16-byte units permuted by row: rows lie in the same banks
         }
-        if (active <= 1) {
-            const float inv = sum == 0.f ? 0.f : 1.f / sum;
-            r *= inv;
-            if (bad) r = qe_f4{0, 0, 0, 0};
-            uint2 w;
-            w.x = pack2<BF>(r[0], r[1]);
-            w.y = pack2<BF>(r[2], r[3]);
-            *(uint2 *)((short *)a.out + (size_t)seq * a.out_stride + ((size_t)kvh * G + h) * DH + d) = w;
+        if (h0) {
+            __syncthreads();
         } else {
-            const size_t part = (size_t)item * a.splits + split, row = part * G + h;
-            float2 *to_ml = a.part_ml + part * QE_ATTN_GROUP_MAX + h;
-            if (a.splits <= QE_ATTN_JOIN) {
-                store_through(a.part_o + row * DH + d, qe_f2{r[0], r[1]});
-                store_through(a.part_o + row * DH + d + 2, qe_f2{r[2], r[3]});
-                if (d == 0) store_through((float *)to_ml, qe_f2{top, bad ? -1.f : sum});
+            bad = __syncthreads_or(bad) ? 1 : 0;
+            if (tid == 0 && (bad | bad_len)) report(a.err, bad ? QE_BAD_PAGE : QE_BAD_LENGTH);
+        }
+        const int heads = a.group - h0 < HEADS ? a.group - h0 : HEADS;
+        for (int i = tid; i < heads * (DH / 4); i += 256) {
+            const int h = h0 + i / (DH / 4), d = i % (DH / 4) * 4;
+            float top = ml[0][h].x;
+            for (int w = 1; w < 4; ++w) top = fmaxf(top, ml[w][h].x);
+            float sum = 0;
+            qe_f4 r = {0, 0, 0, 0};
+#pragma unroll
+            for (int w = 0; w < 4; ++w) { // no branches: each would wait for the LDS anew
+                const float2 x = ml[w][h];
+                const float f = x.x == -INFINITY ? 0.f : __builtin_amdgcn_exp2f((x.x - top) * a.scale_log2);
+                const qe_f4 y = *(const qe_f4 *)(row(w, h - h0) + ((d / 4) ^ h) * 4);
+                const bool any = x.y != 0.f; // else a wave without keys
+                sum += any ? f * x.y : 0.f;
+                for (int j = 0; j < 4; ++j) r[j] += any ? f * y[j] : 0.f;
+            }
+            if (active <= 1) {
+                const float inv = sum == 0.f ? 0.f : 1.f / sum;
+                r *= inv;
+                if (bad) r = qe_f4{0, 0, 0, 0};
+                uint2 w;
+                w.x = pack2<BF>(r[0], r[1]);
+                w.y = pack2<BF>(r[2], r[3]);
+                *(uint2 *)((short *)a.out + (size_t)seq * a.out_stride + ((size_t)kvh * G + h) * DH + d) = w;
             } else {
-                *(qe_f4 *)(a.part_o + row * DH + d) = r;
-                if (d == 0) *to_ml = make_float2(top, bad ? -1.f : sum);
+                const size_t part = (size_t)item * a.splits + split, place = part * G + h;
+                float2 *to_ml = a.part_ml + part * QE_ATTN_GROUP_MAX + h;
+                if (a.splits <= QE_ATTN_JOIN) {
+                    store_through(a.part_o + place * DH + d, qe_f2{r[0], r[1]});
+                    store_through(a.part_o + place * DH + d + 2, qe_f2{r[2], r[3]});
+                    if (d == 0) store_through((float *)to_ml, qe_f2{top, bad ? -1.f : sum});
+                } else {
+                    *(qe_f4 *)(a.part_o + place * DH + d) = r;
+                    if (d == 0) *to_ml = make_float2(top, bad ? -1.f : sum);
+                }
             }
         }
     }

@@ -1,11 +1,12 @@
 // Attention of single tokens whose sequences share their beginnings: a shared key and value is read once for all rows of its
 // group, not once a sequence.
 //
-// Three launches.  k_shared_prefix: 128 rows of a group (its sequences' heads of one key-value head) over a split of the shared
-// positions, by the products of a prompt (qe_attn_rows.h) without a causal mask.  k_shared_own: a sequence's own positions, by
-// those of k_attn_decode.  Both leave unnormalised partial results with their maximum and sum, in 32 bits, and k_shared_join
-// joins a row's.  Positions are read through the table of the group's first sequence below the group's length, and
-// through a sequence's own from there on.
+// One launch for all keys, whose workgroups are of two kinds, and one for the join.  Prefix workgroups take 128 rows of a group
+// (its sequences' heads of one key-value head) over a split of the shared positions, by the products of a prompt
+// (qe_attn_rows.h) without a causal mask; the others a sequence's own positions, by those of k_attn_decode.  Both leave
+// unnormalised partial results with their maximum and sum, in 32 bits, and k_shared_join joins a row's.  Positions are read
+// through the table of the group's first sequence below the group's length, and through a sequence's own from there on.
+#include "qe_attn_keys.h"
 #include "qe_attn_stage8.h"
 
 // ---- groups --------------------------------------------------------------------------------------------
@@ -39,7 +40,7 @@ __device__ __forceinline__ bool own_positions(const QeSharedArgs &y, int seq, in
     *len = *start = 0;
     return false;
 }
-// 32-key steps from the one that start lies in on
+// from the step on that start lies in
 __device__ __forceinline__ int own_length(int start, int len) { return len > start ? len - (start & -QE_ATTN_TILE) : 0; }
 
 template <int DH>
@@ -52,17 +53,14 @@ __device__ __forceinline__ size_t part_of(const QeSharedArgs &y, int seq, int he
 
 // ---- the shared positions ---------------------------------------------------------------------------------
 template <bool BF, int DH, int CT>
-__global__ __launch_bounds__(256, 2) void k_shared_prefix(const QeSharedArgs y) {
+__device__ __forceinline__ void shared_prefix(const QeSharedArgs &y, int tile, int kvh, int split, short *k_a, short *v_a, short *k_b, short *v_b,
+                                              uint8_t *raw_s, float (*s_a)[shared_step<DH>()], float (*s_b)[shared_step<DH>()]) {
     const QeAttnArgs &a = y.x.a;
     constexpr bool CODES = CT != QE_CACHE16;
     typedef Stage<CODES ? CT : QE_I8, BF, DH, 4> ST;
     constexpr int BM = QE_ATTN_SHARED_BM, BN = shared_step<DH>(), KB = BN / 32, PART = BN / 4;
     static_assert(ST::BN == BN, "a stage is a step");
-    __shared__ __align__(16) short k_a[BN * DH], v_a[BN * DH], k_b[BN * DH], v_b[BN * DH];
-    __shared__ __align__(16) uint8_t raw_s[CODES && ST::WAIT_IN_LDS ? 2 * BN * DH : 16];
-    __shared__ float s_a[2][BN], s_b[2][BN];
     const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-    const int split = blockIdx.x % y.psplits, kvh = blockIdx.x / y.psplits % a.kv_heads, tile = blockIdx.x / y.psplits / a.kv_heads;
     // the group: the last one whose first tile is not behind this one, among this launch's sequences
     int g = 0;
     for (int hi = y.n_groups; hi - g > 1;) {
@@ -84,8 +82,15 @@ __global__ __launch_bounds__(256, 2) void k_shared_prefix(const QeSharedArgs y) 
     unsigned bad = 0; // a page of the wave's that is none
     ST stage;
     uint8_t *raw = raw_s + (CODES && ST::WAIT_IN_LDS ? wave * (2 * PART * DH) : 0);
+    // pages of the wave's parts of 64 tiles, a lane each, looked up together
+    int pages = 0, pages_lo = lo - 64;
     auto load = [&](int t, short *k_lds, short *v_lds) { // the wave's part of tile t
-        const int k0 = t * BN, page = page_of<BN, 4>(a, table, k0, len, wave);
+        if (t >= pages_lo + 64) {
+            pages_lo = t;
+            const int at = (t + lane_now()) * BN + wave * PART;
+            pages = table[(at < len ? at : len - 1) >> a.page_log2];
+        }
+        const int k0 = t * BN, page = __builtin_amdgcn_readlane(pages, t - pages_lo);
         bad |= (unsigned)page >= a.n_pages;
         if constexpr (CODES) {
             stage.issue(y.x, page, kvh, k0, len, wave, raw);
@@ -172,172 +177,48 @@ __global__ __launch_bounds__(256, 2) void k_shared_prefix(const QeSharedArgs y) 
 
 // ---- a sequence's own positions -----------------------------------------------------------------------------
 // As k_attn_decode and k_attn_decode8, from a position on that may lie within a step.
-template <bool BF, int DH, int CT>
-__global__ __launch_bounds__(256, DH == 256 ? 2 : 3) void k_shared_own(const QeSharedArgs y) {
+// vb: a wave's LDS, for its steps; row(w, h): DH floats of LDS for wave w's head h.
+template <bool BF, int DH, int CT, typename ROW>
+__device__ __forceinline__ void shared_own(const QeSharedArgs &y, int item, int split, uint8_t *vb, const ROW &row, float2 (*ml)[16]) {
     const QeAttnArgs &a = y.x.a;
-    constexpr bool CODES = CT != QE_CACHE16;
-    constexpr int SIZE = CODES ? 1 : 2;                // bytes of an element
-    constexpr int CH = DH * SIZE / 16, ROWS = 64 / CH; // 16-byte chunks of a row, rows of one direct load
-    constexpr int KL = DH * SIZE / 64, DB = DH / 16;
-    constexpr int LDS = QE_ATTN_TILE * DH; // shorts of a wave: room for 16 heads x DH floats
-    typedef unsigned u4 __attribute__((ext_vector_type(4)));
-    __shared__ __align__(16) short lds[4][LDS];
-    __shared__ float2 ml[4][16];
+    typedef KeyWave<BF, DH, CT, Rows<BF, DH>::LAG, false> Wave; // probabilities as large as the prefix's are kept
     const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63, col = lane & 15, c = lane >> 4;
-    const int split = blockIdx.x % a.splits, item = blockIdx.x / a.splits, seq = y.seq0 + item / a.kv_heads, kvh = item % a.kv_heads;
-    const short *q = (const short *)a.q + (size_t)seq * a.q_stride + ((size_t)kvh * a.group + col) * DH;
-    qe_s8 qf[DH / 32]; // in the order of the codes (k_attn_decode8), or of K
-#pragma unroll
-    for (int s = 0; s < DH / 32; ++s) qf[s] = col < a.group ? *(const qe_s8 *)(q + (CODES ? s / 2 * 64 + c * 16 + s % 2 * 8 : s * 32 + c * 8)) : qe_s8{};
+    const int seq = y.seq0 + item / a.kv_heads, kvh = item % a.kv_heads;
+    Wave w;
+    w.begin(a, seq, kvh, lane);
     int start, len;
     own_positions(y, seq, &start, &len);
-    const int own = own_length(start, len), base0 = start & -QE_ATTN_TILE;
+    const int own = own_length(start, len), base = start & -Wave::TILE;
     const int steps = qe_attn_decode_steps(own, a.steps, a.splits);
     if (split >= qe_attn_decode_active(own, steps)) return;
     const int32_t *table = a.table + (size_t)seq * a.table_stride;
-    const int tiles = (own + QE_ATTN_TILE - 1) / QE_ATTN_TILE, lo = split * steps, hi = lo + steps < tiles ? lo + steps : tiles;
-    unsigned bad = 0;
-    qe_f4 acc[DB];
-#pragma unroll
-    for (int d = 0; d < DB; ++d) acc[d] = qe_f4{0, 0, 0, 0};
-    float m = -INFINITY, l = 0;
-    Units units;
-    uint8_t *vb = (uint8_t *)lds[wave];
-    const int tr_key = CODES ? 4 * c + (col >> 1 & 3) + (col & 8) * 2 : 4 * c + (col >> 2);
-    auto swz = [](int r) { return CODES ? swz8<DH>(r) : v_swz<DH>(r); };
-    for (int t = lo + wave; t < hi; t += 4) {
-        const int k0 = base0 + t * QE_ATTN_TILE;
-        // 16 positions that all lie before the first, or behind the last, may have no page: any of the sequence's own does
-        const int p0 = k0 + 16 > start ? k0 : start & -16, p1 = k0 + 16 < len ? k0 + 16 : p0;
-        const size_t r0 = sub_row(a, table, kvh, p0, &bad), r1 = sub_row(a, table, kvh, p1, &bad);
-        const uint8_t *kp0 = (const uint8_t *)a.kc + (r0 + col) * DH * SIZE + c * 16, *kp1 = (const uint8_t *)a.kc + (r1 + col) * DH * SIZE + c * 16;
-        u4 kr[2][KL];
-#pragma unroll
-        for (int s = 0; s < KL; ++s) kr[0][s] = *(const u4 *)(kp0 + s * 64);
-#pragma unroll
-        for (int s = 0; s < KL; ++s) kr[1][s] = *(const u4 *)(kp1 + s * 64);
-        float ks = 0, vs = 0;
-        if constexpr (CODES) {
-            const size_t sr = (col & 4 ? r1 : r0) + 4 * c + (col & 3);
-            ks = y.x.ks[sr], vs = y.x.vs[sr];
-        }
-#pragma unroll
-        for (int i = 0; i < QE_ATTN_TILE / ROWS; ++i) {
-            const int row = i * ROWS + lane / CH, ch = (lane % CH) ^ swz(row);
-            load_lds16_from((const uint8_t *)a.vc + (i * ROWS < 16 ? r0 : r1) * DH * SIZE, 16 * DH * SIZE, (row & 15) * DH * SIZE + ch * 16, 0, vb + i * 1024);
-        }
-        __builtin_amdgcn_sched_barrier(0); // all loads are under way before the first is waited for
-        qe_f4 s[2] = {qe_f4{0, 0, 0, 0}, qe_f4{0, 0, 0, 0}};
-#pragma unroll
-        for (int st = 0; st < KL; ++st) {
-            if constexpr (CODES) {
-#pragma unroll
-                for (int h = 0; h < 2; ++h) {
-                    s[0] = mfma16<BF>(elements_of<CT, BF>(kr[0][st][2 * h], kr[0][st][2 * h + 1]), qf[2 * st + h], s[0]);
-                    s[1] = mfma16<BF>(elements_of<CT, BF>(kr[1][st][2 * h], kr[1][st][2 * h + 1]), qf[2 * st + h], s[1]);
-                }
-            } else {
-                s[0] = mfma16<BF>(__builtin_bit_cast(qe_s8, kr[0][st]), qf[st], s[0]);
-                s[1] = mfma16<BF>(__builtin_bit_cast(qe_s8, kr[1][st]), qf[st], s[1]);
-            }
-        }
-        if constexpr (CODES) {
-            s[0] = qe_f4{s[0][0] * of_lane<0>(ks), s[0][1] * of_lane<1>(ks), s[0][2] * of_lane<2>(ks), s[0][3] * of_lane<3>(ks)};
-            s[1] = qe_f4{s[1][0] * of_lane<4>(ks), s[1][1] * of_lane<5>(ks), s[1][2] * of_lane<6>(ks), s[1][3] * of_lane<7>(ks)};
-        }
-        const bool cut = k0 < start || k0 + QE_ATTN_TILE > len;
-        auto outside = [&](int key) { return k0 + key < start || k0 + key >= len; };
-        if (cut) {
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                if (outside(4 * c + i)) s[0][i] = -INFINITY;
-                if (outside(16 + 4 * c + i)) s[1][i] = -INFINITY;
-            }
-        }
-        float top = fmaxf(fmaxf(fmaxf(s[0][0], s[0][1]), fmaxf(s[0][2], s[0][3])),
-                          fmaxf(fmaxf(s[1][0], s[1][1]), fmaxf(s[1][2], s[1][3])));
-        top = fmaxf(top, __shfl_xor(top, 16));
-        top = fmaxf(top, __shfl_xor(top, 32));
-        if (__any(top > m)) {
-            const float mn = fmaxf(m, top), f = m == -INFINITY ? 0.f : exp2f((m - mn) * a.scale_log2);
-#pragma unroll
-            for (int d = 0; d < DB; ++d) acc[d] *= f;
-            l *= f;
-            m = mn;
-        }
-        if constexpr (CODES && !BF) {
-            const float f = units.raise(cut && outside((col & 4 ? 16 : 0) + 4 * c + (col & 3)) ? 0.f : vs);
-            if (f != 1.f)
-#pragma unroll
-                for (int d = 0; d < DB; ++d) acc[d] *= f;
-            vs *= units.inverse;
-        }
-        const float base = exponent_base<BF, Rows<BF, DH>::LAG>(m * a.scale_log2); // as large as the prefix's are kept
-        float p[8];
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            p[i] = __builtin_amdgcn_exp2f(fmaf(s[0][i], a.scale_log2, base));
-            p[4 + i] = __builtin_amdgcn_exp2f(fmaf(s[1][i], a.scale_log2, base));
-        }
-        l += ((p[0] + p[1]) + (p[2] + p[3])) + ((p[4] + p[5]) + (p[6] + p[7]));
-        if constexpr (CODES) {
-            p[0] *= of_lane<0>(vs), p[1] *= of_lane<1>(vs), p[2] *= of_lane<2>(vs), p[3] *= of_lane<3>(vs);
-            p[4] *= of_lane<4>(vs), p[5] *= of_lane<5>(vs), p[6] *= of_lane<6>(vs), p[7] *= of_lane<7>(vs);
-            if (cut) { // a scale there may be anything
-#pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    if (outside(4 * c + i)) p[i] = 0;
-                    if (outside(16 + 4 * c + i)) p[4 + i] = 0;
-                }
-            }
-        }
-        union {
-            unsigned u[4];
-            qe_s8 v;
-        } pf;
-#pragma unroll
-        for (int i = 0; i < 4; ++i) pf.u[i] = pack2<BF>(p[2 * i], p[2 * i + 1]);
-        __builtin_amdgcn_s_waitcnt(0x0f70); // the direct loads have landed (vmcnt 0)
-        if (CT != QE_I8 && cut) {            // V there may be anything: a probability of 0 times NaN is NaN
-            for (int i = lane; i < QE_ATTN_TILE * CH; i += 64)
-                if (outside(i / CH)) *(uint4 *)(vb + i * 16) = make_uint4(0, 0, 0, 0);
-        }
-#pragma unroll
-        for (int d = 0; d < DB; ++d) {
-            if constexpr (CODES) {
-                const uint2 v = lds_tr8(vb + tr_key * DH + ((d ^ swz(tr_key)) << 4) + (col & 1) * 8);
-                acc[d] = mfma16<BF>(elements_of<CT, BF>(v.x, v.y), pf.v, acc[d]);
-            } else {
-                const int el = d * 16 + (col & 3) * 4, at = (((el >> 3) ^ swz(tr_key)) << 3) + (el & 7); // 16 rows on the permutation is the same
-                const qe_s4 x = lds_tr((const short *)vb + tr_key * DH + at), z = lds_tr((const short *)vb + (tr_key + 16) * DH + at);
-                acc[d] = mfma16<BF>(qe_s8{x[0], x[1], x[2], x[3], z[0], z[1], z[2], z[3]}, pf.v, acc[d]);
-            }
-        }
-    }
-    if constexpr (CODES && !BF)
-#pragma unroll
-        for (int d = 0; d < DB; ++d) acc[d] *= units.unit;
+    const int tiles = (len - base + Wave::TILE - 1) / Wave::TILE, lo = split * steps + wave, hi = split * steps + steps < tiles ? split * steps + steps : tiles;
+    typename Wave::Pages pages = {};
+    if (lo < hi) pages = Wave::look_up(a, table, base + lo * Wave::TILE, start, len);
+    run_steps(w, a, y.x.ks, y.x.vs, table, kvh, base, start, len, lo, hi, pages, vb);
+    w.end();
     // the four waves' results joined (as in finish_decode), and left as a partial one
+    float l = w.l;
     l += __shfl_xor(l, 16);
     l += __shfl_xor(l, 32);
-    if (lane < 16) ml[wave][lane] = make_float2(m, l);
-    float *o = (float *)lds[wave];
+    if (lane < 16) ml[wave][lane] = make_float2(w.m, l);
+    float *o = row(wave, col);
 #pragma unroll
-    for (int d = 0; d < DB; ++d) *(qe_f4 *)(o + col * DH + ((d * 4 + c) ^ col) * 4) = acc[d];
-    bad = __syncthreads_or(bad);
+    for (int d = 0; d < DH / 16; ++d) *(qe_f4 *)(o + ((d * 4 + c) ^ col) * 4) = w.acc[d];
+    const int bad = __syncthreads_or(w.bad);
     if (bad && tid == 0) report(a.err, QE_BAD_PAGE);
     for (int i = tid; i < a.group * (DH / 4); i += 256) {
         const int h = i / (DH / 4), d = i % (DH / 4) * 4;
         float top = ml[0][h].x;
 #pragma unroll
-        for (int w = 1; w < 4; ++w) top = fmaxf(top, ml[w][h].x);
+        for (int v = 1; v < 4; ++v) top = fmaxf(top, ml[v][h].x);
         float sum = 0;
         qe_f4 r = {0, 0, 0, 0};
 #pragma unroll
-        for (int w = 0; w < 4; ++w) {
-            const float2 x = ml[w][h];
+        for (int u = 0; u < 4; ++u) {
+            const float2 x = ml[u][h];
             const float f = x.x == -INFINITY ? 0.f : __builtin_amdgcn_exp2f((x.x - top) * a.scale_log2);
-            const qe_f4 v = *(const qe_f4 *)((const float *)lds[w] + h * DH + ((d / 4) ^ h) * 4);
+            const qe_f4 v = *(const qe_f4 *)(row(u, h) + ((d / 4) ^ h) * 4);
             const bool any = x.y != 0.f; // else a wave without keys
             sum += any ? f * x.y : 0.f;
 #pragma unroll
@@ -349,7 +230,30 @@ __global__ __launch_bounds__(256, DH == 256 ? 2 : 3) void k_shared_own(const QeS
     }
 }
 
-// ---- a row's partial results joined: a wave a row -----------------------------------------------------------
+// Prefix workgroups come first, since they are the longest; those of the same keys, one for each 128 rows, go to one XCD, whose
+// L2 has the keys from the first one's reading on (workgroups go to the eight in turn).
+template <bool BF, int DH, int CT>
+__global__ __launch_bounds__(256, 2) void k_shared(const QeSharedArgs y) {
+    const QeAttnArgs &a = y.x.a;
+    constexpr int BN = shared_step<DH>();
+    constexpr bool CODES = CT != QE_CACHE16;
+    __shared__ __align__(16) short k_a[BN * DH], v_a[BN * DH], k_b[BN * DH], v_b[BN * DH];
+    __shared__ __align__(16) uint8_t raw_s[CODES && DH == 256 ? 2 * BN * DH : 16];
+    __shared__ __align__(16) float s_a[2][BN], s_b[2][BN];
+    const int units = y.psplits * a.kv_heads, prefix = (units + 7) / 8 * 8 * a.tiles;
+    if ((int)blockIdx.x < prefix) {
+        const int unit = blockIdx.x / 8 / a.tiles * 8 + blockIdx.x % 8;
+        if (unit < units) shared_prefix<BF, DH, CT>(y, blockIdx.x / 8 % a.tiles, unit / y.psplits, unit % y.psplits, k_a, v_a, k_b, v_b, raw_s, s_a, s_b);
+    } else {
+        static_assert(sizeof k_a >= 64 * DH, "room for a wave's values of a step, and its results");
+        __shared__ float2 ml[4][16];
+        const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), at = blockIdx.x - prefix;
+        auto buffer = [&](int w) { return w < 2 ? w == 0 ? k_a : v_a : w == 2 ? k_b : v_b; }; // a wave's own
+        shared_own<BF, DH, CT>(y, at / a.splits, at % a.splits, (uint8_t *)buffer(wave), [&](int w, int h) { return (float *)buffer(w) + h * DH; }, ml);
+    }
+}
+
+// ---- a row's partial results joined: a workgroup a row, its four waves every fourth split -------------------------
 template <bool BF, int DH>
 __global__ __launch_bounds__(256) void k_shared_join(const QeSharedArgs y) {
     const QeAttnArgs &a = y.x.a;
@@ -357,12 +261,10 @@ __global__ __launch_bounds__(256) void k_shared_join(const QeSharedArgs y) {
     // all groups' offsets are looked at, for the report: those that are wrong may hold no sequence
     for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < y.n_groups; i += (int64_t)gridDim.x * 256)
         if (qe_bad_offsets(y.seqs[i], y.seqs[i + 1], a.n_seqs) || y.prefix[i] < 0 || y.prefix[i] > a.max_pages << a.page_log2) report(a.err, QE_BAD_LENGTH);
-    const int lane = threadIdx.x & 63, row = __builtin_amdgcn_readfirstlane(blockIdx.x * 4 + (threadIdx.x >> 6));
-    if (row >= (y.seq1 - y.seq0) * a.q_heads) return;
-    const int seq = y.seq0 + row / a.q_heads, head = row % a.q_heads;
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, seq = y.seq0 + blockIdx.x / a.q_heads, head = blockIdx.x % a.q_heads;
     int start, len;
     const bool good = own_positions(y, seq, &start, &len);
-    if (!good && lane == 0) report(a.err, QE_BAD_LENGTH);
+    if (!good && threadIdx.x == 0) report(a.err, QE_BAD_LENGTH);
     const int own = own_length(start, len), np = qe_attn_shared_active(start, shared_step<DH>(), y.psplits);
     const int n = np + qe_attn_decode_active(own, qe_attn_decode_steps(own, a.steps, a.splits));
     const size_t at = part_of(y, seq, head, 0);
@@ -380,31 +282,40 @@ __global__ __launch_bounds__(256) void k_shared_join(const QeSharedArgs y) {
 #pragma unroll
     for (int e = 0; e < E; ++e) o[e] = 0;
 #pragma unroll 4
-    for (int s = 0; s < n; ++s) {
+    for (int s = wave; s < n; s += 4) {
         const size_t i = at + s + (s < np ? 0 : gap);
         const float2 x = a.part_ml[i];
         float v[E];
 #pragma unroll
         for (int e = 0; e < E; ++e) v[e] = a.part_o[i * DH + e * 64 + lane];
         const float f = x.x == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(x.x - m);
-        if (x.y == 0.f) continue;
-        sum += f * x.y;
+        const bool any = x.y != 0.f; // else no key
+        sum += any ? f * x.y : 0.f;
 #pragma unroll
-        for (int e = 0; e < E; ++e) o[e] += f * v[e];
+        for (int e = 0; e < E; ++e) o[e] += any ? f * v[e] : 0.f;
     }
+    __shared__ float o_s[4][DH], sum_s[4];
+#pragma unroll
+    for (int e = 0; e < E; ++e) o_s[wave][e * 64 + lane] = o[e];
+    if (lane == 0) sum_s[wave] = sum;
+    __syncthreads();
+    if (wave) return;
+    sum = (sum_s[0] + sum_s[1]) + (sum_s[2] + sum_s[3]);
     const float inv = sum == 0.f ? 0.f : 1.f / sum;
     short *out = (short *)a.out + (size_t)seq * a.out_stride + (size_t)head * DH;
 #pragma unroll
-    for (int e = 0; e < E; ++e) out[e * 64 + lane] = bad ? 0 : (short)pack2<BF>(o[e] * inv, 0.f);
+    for (int e = 0; e < E; ++e) {
+        const float r = (o_s[0][e * 64 + lane] + o_s[1][e * 64 + lane]) + (o_s[2][e * 64 + lane] + o_s[3][e * 64 + lane]);
+        out[e * 64 + lane] = bad ? 0 : (short)pack2<BF>(r * inv, 0.f);
+    }
 }
 
 template <bool BF, int DH, int CT>
 static hipError_t launch_shared(const QeSharedArgs &y, hipStream_t st) {
     const QeAttnArgs &a = y.x.a;
-    const int n = y.seq1 - y.seq0;
-    k_shared_prefix<BF, DH, CT><<<dim3((unsigned)(a.tiles * a.kv_heads * y.psplits)), dim3(256), 0, st>>>(y);
-    k_shared_own<BF, DH, CT><<<dim3((unsigned)(n * a.kv_heads * a.splits)), dim3(256), 0, st>>>(y);
-    k_shared_join<BF, DH><<<dim3((unsigned)((n * a.q_heads + 3) / 4)), dim3(256), 0, st>>>(y);
+    const unsigned n = y.seq1 - y.seq0, prefix = (unsigned)(y.psplits * a.kv_heads + 7) / 8 * 8 * a.tiles;
+    k_shared<BF, DH, CT><<<dim3(prefix + n * a.kv_heads * a.splits), dim3(256), 0, st>>>(y);
+    k_shared_join<BF, DH><<<dim3(n * a.q_heads), dim3(256), 0, st>>>(y);
     return hipGetLastError();
 }
 template <bool BF, int CT>

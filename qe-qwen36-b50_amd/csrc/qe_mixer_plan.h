@@ -27,13 +27,14 @@ QE_MIX_HD bool qe_fits_launch(int64_t workgroups, int threads) { return workgrou
 // 512 takes 37 us over 100,000 keys of two heads of 256, 696 take 40), of at least two steps.
 // Several, which may differ in length: up to 2048, but of at least eight steps where that
 // many fill the GPU.  units = n_seqs * kv_heads.
-QE_MIX_HD void qe_attn_decode_plan(int64_t n_seqs, int64_t kv_heads, int head_dim, int64_t max_len, int *steps, int *splits) {
+// `round`: the workgroups that the GPU holds at once; `least`: steps of one where there are several sequences.
+QE_MIX_HD void qe_attn_decode_cut(int64_t n_seqs, int64_t kv_heads, int round, int least, int64_t max_len, int *steps, int *splits) {
     const int64_t tiles = (max_len + QE_ATTN_TILE - 1) / QE_ATTN_TILE, units = n_seqs * kv_heads, total = tiles * units;
-    const int64_t round = head_dim == 256 ? 512 : 768, once = (total + round - 1) / round;
+    const int64_t once = (total + round - 1) / round;
     int64_t per = once;
     if (n_seqs > 1) {
         per = (total + QE_ATTN_DECODE_WGS - 1) / QE_ATTN_DECODE_WGS;
-        if (per < 8) per = once < 8 ? once : 8;
+        if (per < least) per = once < least ? once : least;
     }
     if (per > tiles) per = tiles; // one workgroup for each
     if (per < 2) per = 2;
@@ -42,6 +43,15 @@ QE_MIX_HD void qe_attn_decode_plan(int64_t n_seqs, int64_t kv_heads, int head_di
     if (s < 1 || units >= QE_ATTN_DECODE_WGS) s = 1;
     *steps = (int)per;
     *splits = (int)s;
+}
+QE_MIX_HD void qe_attn_decode_plan(int64_t n_seqs, int64_t kv_heads, int head_dim, int64_t max_len, int *steps, int *splits) {
+    qe_attn_decode_cut(n_seqs, kv_heads, head_dim == 256 ? 512 : 768, 8, max_len, steps, splits);
+}
+// Over an 8-bit cache at least six steps (24 ragged sequences up to 8095 keys, 2 heads of 256: 32.5 us a call, 39.8 with
+// eight, 32.5 with four; 8 x 8000: 24.9, 22.1 and 25.9).  Fewer and longer ones, so that the last workgroup joins all
+// 16, are 5 to 10 % faster for sequences of one length, and a third slower where they differ much.
+QE_MIX_HD void qe_attn_decode8_plan(int64_t n_seqs, int64_t kv_heads, int64_t max_len, int *steps, int *splits) {
+    qe_attn_decode_cut(n_seqs, kv_heads, 512, 6, max_len, steps, splits);
 }
 // Steps of a sequence of `len` keys in each of its workgroups (more than planned where the host's max_len was short
 // of it), and how many of those have any.
