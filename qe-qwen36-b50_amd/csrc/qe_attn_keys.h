@@ -56,6 +56,7 @@ struct KeyWave {
         u4 k[NB][KL];
         float ks[NB / 2], vs[NB / 2];
     };
+    static constexpr int LOADS = NB * KL + (CODES ? NB : 0) + TILE / ROWS; // of a step
     // The step of keys from k0 on, of which those in [start, len) count, in the pages given.
     __device__ __forceinline__ void issue(const QeAttnArgs &a, const float *k_scale, const float *v_scale, int kvh, int k0, int start, int len, const Pages pages,
                                           uint8_t *vb, Step &x) {
@@ -82,7 +83,8 @@ struct KeyWave {
         }
         __builtin_amdgcn_sched_barrier(0); // all loads are under way before the first is waited for
     }
-    // The step that `x` and vb hold, or will.
+    // The step that `x` and vb hold, or will.  MORE: another one was issued after it.
+    template <bool MORE>
     __device__ __forceinline__ void work(const QeAttnArgs &a, int k0, int start, int len, uint8_t *vb, Step &x) {
         const int lane = lane_now(), col = lane & 15, c = lane >> 4;
         auto swz = [](int row) { return CODES ? swz8<DH>(row) : v_swz<DH>(row); };
@@ -158,7 +160,8 @@ struct KeyWave {
             }
             pf[j] = __builtin_bit_cast(qe_s8, u4{pack2<BF>(p[0], p[1]), pack2<BF>(p[2], p[3]), pack2<BF>(z[0], z[1]), pack2<BF>(z[2], z[3])});
         }
-        __builtin_amdgcn_s_waitcnt(0x0f70); // the direct loads have landed (vmcnt 0)
+        constexpr int LATER = MORE ? LOADS : 0;
+        __builtin_amdgcn_s_waitcnt(0x0f70 | (LATER & 15) | LATER >> 4 << 14); // its direct loads have landed (vmcnt LATER)
         if (CT != QE_I8 && cut)              // V there may be anything: a probability of 0 times NaN is NaN
             for (int i = lane; i < TILE * CH; i += 64)
                 if (outside(i / CH)) *(uint4 *)(vb + i * 16) = make_uint4(0, 0, 0, 0);
@@ -194,8 +197,8 @@ struct KeyWave {
 };
 
 // A wave's steps from t on, every fourth one up to `hi`, of keys counted from `base` (a multiple of the step's).  `pages` are the
-// first one's.  (Measured and not kept: the next step's loads issued before this one's work, into two buffers, 42 -> 47 us for 24
-// ragged sequences of 8 heads of 128, since fewer waves fit; steps of 64 keys, 42 -> 48.)
+// first one's.  (In k_attn_decode8 these; issuing the next step before this one's work took it from 42 to 47 us for 24 ragged
+// sequences of 8 heads of 128, since fewer waves fit; steps of 64 keys, to 48.)
 template <typename WAVE>
 __device__ __forceinline__ void run_steps(WAVE &w, const QeAttnArgs &a, const float *ks, const float *vs, const int32_t *table, int kvh, int base, int start, int len,
                                           int t, int hi, typename WAVE::Pages pages, uint8_t *vb) {
@@ -204,6 +207,31 @@ __device__ __forceinline__ void run_steps(WAVE &w, const QeAttnArgs &a, const fl
         const int k0 = base + t * WAVE::TILE;
         w.issue(a, ks, vs, kvh, k0, start, len, pages, vb, x);
         if (t + 4 < hi) pages = WAVE::look_up(a, table, k0 + 4 * WAVE::TILE, start, len);
-        w.work(a, k0, start, len, vb, x);
+        w.template work<false>(a, k0, start, len, vb, x);
     }
+}
+// The same with the next step on its way to the other of two buffers while one is worked on, where registers are there anyway.
+// (The buffers are in variables of their own: else the compiler has LDS reads wait for all direct loads in flight.)
+template <typename WAVE>
+__device__ __forceinline__ void run_steps_ahead(WAVE &w, const QeAttnArgs &a, const float *ks, const float *vs, const int32_t *table, int kvh, int base, int start,
+                                                int len, int t, int hi, typename WAVE::Pages pages, uint8_t *buf_a, uint8_t *buf_b) {
+    constexpr int TILE = WAVE::TILE;
+    if (t >= hi) return;
+    typename WAVE::Step x, y;
+    auto pages_of = [&](int i) { return WAVE::look_up(a, table, base + (i < hi ? i : t) * TILE, start, len); };
+    w.issue(a, ks, vs, kvh, base + t * TILE, start, len, pages, buf_a, x);
+    pages = pages_of(t + 4);
+    for (; t + 4 < hi; t += 8) {
+        w.issue(a, ks, vs, kvh, base + (t + 4) * TILE, start, len, pages, buf_b, y);
+        pages = pages_of(t + 8);
+        w.template work<true>(a, base + t * TILE, start, len, buf_a, x);
+        if (t + 8 >= hi) {
+            w.template work<false>(a, base + (t + 4) * TILE, start, len, buf_b, y);
+            return;
+        }
+        w.issue(a, ks, vs, kvh, base + (t + 8) * TILE, start, len, pages, buf_a, x);
+        pages = pages_of(t + 12);
+        w.template work<true>(a, base + (t + 4) * TILE, start, len, buf_b, y);
+    }
+    w.template work<false>(a, base + t * TILE, start, len, buf_a, x);
 }

@@ -16,7 +16,7 @@ __global__ __launch_bounds__(64 * WAVES, 2) void k_attn_prompt8(const QeAttn8Arg
     constexpr int BM = 32 * WAVES, BN = ST::BN, KB = DH == 256 ? 1 : 2;
     static_assert(BN == 32 * KB, "a tile is a step");
     __shared__ __align__(16) short k_a[BN * DH], v_a[BN * DH], k_b[BN * DH], v_b[BN * DH];
-    __shared__ __align__(16) uint8_t raw_s[ST::WAIT_IN_LDS ? 2 * BN * DH : 16];
+    __shared__ __align__(16) uint8_t raw_s[ST::RAW ? WAVES * ST::RAW : 16];
     __shared__ float s_a[2][BN], s_b[2][BN];
     const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int split = blockIdx.x % a.splits, kvh = blockIdx.x / a.splits % a.kv_heads;
@@ -50,7 +50,7 @@ __global__ __launch_bounds__(64 * WAVES, 2) void k_attn_prompt8(const QeAttn8Arg
     qe_split_range(keys > 0 ? (keys + BN - 1) / BN : 0, a.splits, split, &lo, &hi);
 
     ST stage;
-    uint8_t *raw = raw_s + (ST::WAIT_IN_LDS ? wave * (2 * ST::PART * DH) : 0);
+    uint8_t *raw = raw_s + wave * ST::RAW;
     int page = 0; // of the wave's part of the tile after the one that is loaded
     if (lo < hi) {
         page = page_of<BN, WAVES>(a, table, lo * BN, len, wave);

@@ -81,7 +81,7 @@ __device__ __forceinline__ void shared_prefix(const QeSharedArgs &y, int tile, i
 
     unsigned bad = 0; // a page of the wave's that is none
     ST stage;
-    uint8_t *raw = raw_s + (CODES && ST::WAIT_IN_LDS ? wave * (2 * PART * DH) : 0);
+    uint8_t *raw = raw_s + (CODES ? wave * ST::RAW : 0);
     // pages of the wave's parts of 64 tiles, a lane each, looked up together
     int pages = 0, pages_lo = lo - 64;
     auto load = [&](int t, short *k_lds, short *v_lds) { // the wave's part of tile t
@@ -177,9 +177,9 @@ __device__ __forceinline__ void shared_prefix(const QeSharedArgs &y, int tile, i
 
 // ---- a sequence's own positions -----------------------------------------------------------------------------
 // As k_attn_decode and k_attn_decode8, from a position on that may lie within a step.
-// vb: a wave's LDS, for its steps; row(w, h): DH floats of LDS for wave w's head h.
-template <bool BF, int DH, int CT, typename ROW>
-__device__ __forceinline__ void shared_own(const QeSharedArgs &y, int item, int split, uint8_t *vb, const ROW &row, float2 (*ml)[16]) {
+// buf_a, buf_b: a wave's LDS, for its steps; row(w, h): DH floats of LDS for wave w's head h.
+template <bool BF, int DH, int CT, bool AHEAD, typename ROW>
+__device__ __forceinline__ void shared_own(const QeSharedArgs &y, int item, int split, uint8_t *buf_a, uint8_t *buf_b, const ROW &row, float2 (*ml)[16]) {
     const QeAttnArgs &a = y.x.a;
     typedef KeyWave<BF, DH, CT, Rows<BF, DH>::LAG, false> Wave; // probabilities as large as the prefix's are kept
     const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63, col = lane & 15, c = lane >> 4;
@@ -195,7 +195,8 @@ __device__ __forceinline__ void shared_own(const QeSharedArgs &y, int item, int 
     const int tiles = (len - base + Wave::TILE - 1) / Wave::TILE, lo = split * steps + wave, hi = split * steps + steps < tiles ? split * steps + steps : tiles;
     typename Wave::Pages pages = {};
     if (lo < hi) pages = Wave::look_up(a, table, base + lo * Wave::TILE, start, len);
-    run_steps(w, a, y.x.ks, y.x.vs, table, kvh, base, start, len, lo, hi, pages, vb);
+    if constexpr (AHEAD) run_steps_ahead(w, a, y.x.ks, y.x.vs, table, kvh, base, start, len, lo, hi, pages, buf_a, buf_b);
+    else run_steps(w, a, y.x.ks, y.x.vs, table, kvh, base, start, len, lo, hi, pages, buf_a);
     w.end();
     // the four waves' results joined (as in finish_decode), and left as a partial one
     float l = w.l;
@@ -238,7 +239,7 @@ __global__ __launch_bounds__(256, 2) void k_shared(const QeSharedArgs y) {
     constexpr int BN = shared_step<DH>();
     constexpr bool CODES = CT != QE_CACHE16;
     __shared__ __align__(16) short k_a[BN * DH], v_a[BN * DH], k_b[BN * DH], v_b[BN * DH];
-    __shared__ __align__(16) uint8_t raw_s[CODES && DH == 256 ? 2 * BN * DH : 16];
+    __shared__ __align__(16) uint8_t raw_s[CODES && DH == 256 ? 4 * Stage<QE_I8, BF, DH, 4>::RAW : 16];
     __shared__ __align__(16) float s_a[2][BN], s_b[2][BN];
     const int units = y.psplits * a.kv_heads, prefix = (units + 7) / 8 * 8 * a.tiles;
     if ((int)blockIdx.x < prefix) {
@@ -248,12 +249,24 @@ __global__ __launch_bounds__(256, 2) void k_shared(const QeSharedArgs y) {
         static_assert(sizeof k_a >= 64 * DH, "room for a wave's values of a step, and its results");
         __shared__ float2 ml[4][16];
         const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), at = blockIdx.x - prefix;
-        auto buffer = [&](int w) { return w < 2 ? w == 0 ? k_a : v_a : w == 2 ? k_b : v_b; }; // a wave's own
-        shared_own<BF, DH, CT>(y, at / a.splits, at % a.splits, (uint8_t *)buffer(wave), [&](int w, int h) { return (float *)buffer(w) + h * DH; }, ml);
+        // a wave's own: two, for the values of a step each (of 16 bits and heads of 256 one)
+        constexpr bool AHEAD = DH < 256; // (with 256 registers spill, and buffers of 16 bits would not fit)
+        auto buffer = [&](int w, int second) {
+            if (!AHEAD) return (uint8_t *)(w < 2 ? w == 0 ? k_a : v_a : w == 2 ? k_b : v_b);
+            return (uint8_t *)(second ? w < 2 ? k_b : v_b : w < 2 ? k_a : v_a) + (w & 1) * (sizeof k_a / 2);
+        };
+        // and for its results: sixteen heads' in one, or eight in each
+        auto row = [&](int w, int h) {
+            if (!AHEAD || sizeof k_a / 2 >= 64 * DH) return (float *)buffer(w, 0) + h * DH;
+            return (float *)buffer(w, h >> 3) + (h & 7) * DH;
+        };
+        shared_own<BF, DH, CT, AHEAD>(y, at / a.splits, at % a.splits, buffer(wave, 0), buffer(wave, 1), row, ml);
     }
 }
 
 // ---- a row's partial results joined: a workgroup a row, its four waves every fourth split -------------------------
+// (6 us, of which most is the launch and the look-ups.  Measured and not kept: sixteen waves a row where there are few rows and many
+// splits; the first 32 results read while it is looked up which there are.)
 template <bool BF, int DH>
 __global__ __launch_bounds__(256) void k_shared_join(const QeSharedArgs y) {
     const QeAttnArgs &a = y.x.a;

@@ -8,9 +8,11 @@ template <int CT, bool BF, int DH, int WAVES>
 struct Stage {
     static constexpr int BN = DH == 256 ? 32 : 64, PART = BN / WAVES, NL = PART * DH / 1024; // 16-byte loads of a lane
     static constexpr int CH = DH / 16;                                                       // chunks of a row
-    static constexpr bool WAIT_IN_LDS = DH == 256;
+    // of heads of 256: V, and with eight waves K, too (with four, two workgroups fit a CU's LDS only without)
+    static constexpr bool V_IN_LDS = DH == 256, K_IN_LDS = DH == 256 && WAVES == 8;
+    static constexpr int RAW = (V_IN_LDS + K_IN_LDS) * PART * DH; // bytes of LDS a wave
     typedef unsigned u4 __attribute__((ext_vector_type(4)));
-    u4 k[WAIT_IN_LDS ? 1 : NL], v[WAIT_IN_LDS ? 1 : NL];
+    u4 k[K_IN_LDS ? 1 : NL], v[V_IN_LDS ? 1 : NL];
     float scale; // lanes 0 .. PART - 1: of the part's keys, 32 .. 32 + PART - 1: of its values
 
     // The codes of the wave's part of the tile of BN keys from k0 on.
@@ -21,21 +23,20 @@ struct Stage {
         const int lane = lane_now(), n = lane & 31;
         scale = (lane < 32 ? x.ks : x.vs)[r0 + (n < PART ? n : 0)];
         const uint8_t *kp = (const uint8_t *)x.a.kc + r0 * DH, *vp = (const uint8_t *)x.a.vc + r0 * DH;
-        if constexpr (WAIT_IN_LDS) {
 #pragma unroll
-            for (int i = 0; i < NL; ++i) load_lds16_from(kp, PART * DH, lane * 16, i * 1024, raw + i * 1024);
+        for (int i = 0; i < NL; ++i) {
+            if constexpr (K_IN_LDS) load_lds16_from(kp, PART * DH, lane * 16, i * 1024, raw + (NL + i) * 1024);
+            else k[i] = *(const u4 *)(kp + i * 1024 + lane * 16);
+        }
 #pragma unroll
-            for (int i = 0; i < NL; ++i) load_lds16_from(vp, PART * DH, lane * 16, i * 1024, raw + (NL + i) * 1024);
-        } else {
-#pragma unroll
-            for (int i = 0; i < NL; ++i) k[i] = *(const u4 *)(kp + i * 1024 + lane * 16);
-#pragma unroll
-            for (int i = 0; i < NL; ++i) v[i] = *(const u4 *)(vp + i * 1024 + lane * 16);
+        for (int i = 0; i < NL; ++i) {
+            if constexpr (V_IN_LDS) load_lds16_from(vp, PART * DH, lane * 16, i * 1024, raw + i * 1024);
+            else v[i] = *(const u4 *)(vp + i * 1024 + lane * 16);
         }
     }
     // They have come: to the tiles, as 16-bit numbers.  Behind the end, where codes and scales may be anything, zeros.
     __device__ __forceinline__ void land(int k0, int len, int wave, const uint8_t *raw, short *k_lds, short *v_lds, float *ks, float *vs) {
-        if constexpr (WAIT_IN_LDS) __builtin_amdgcn_s_waitcnt(0x0f70);
+        if constexpr (V_IN_LDS) __builtin_amdgcn_s_waitcnt(0x0f70);
         const int lane = lane_now(), n = lane & 31;
         const bool cut = k0 + BN > len;
         if (n < PART) (lane < 32 ? ks : vs)[wave * PART + n] = cut && k0 + wave * PART + n >= len ? 0.f : scale;
@@ -43,13 +44,10 @@ struct Stage {
         for (int i = 0; i < NL; ++i) {
             const int row = wave * PART + i * (64 / CH) + lane / CH, c = lane % CH * 2;
             u4 a, b;
-            if constexpr (WAIT_IN_LDS) {
-                a = *(const u4 *)(raw + i * 1024 + lane * 16);
-                b = *(const u4 *)(raw + (NL + i) * 1024 + lane * 16);
-            } else {
-                a = k[i];
-                b = v[i];
-            }
+            if constexpr (K_IN_LDS) a = *(const u4 *)(raw + (NL + i) * 1024 + lane * 16);
+            else a = k[i];
+            if constexpr (V_IN_LDS) b = *(const u4 *)(raw + i * 1024 + lane * 16);
+            else b = v[i];
             if (CT == QE_F8 && cut && k0 + row >= len) a = b = u4{0, 0, 0, 0};
             short *kr = k_lds + row * DH, *vr = v_lds + row * DH;
             *(qe_s8 *)(kr + ((c ^ k_swz(row)) << 3)) = elements_of<CT, BF>(a[0], a[1]);

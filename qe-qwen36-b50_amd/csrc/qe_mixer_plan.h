@@ -99,7 +99,10 @@ QE_MIX_HD int qe_attn_prompt_splits(int64_t tiles, int64_t max_len) {
 }
 
 // A call of single tokens whose sequences share beginnings: `psplits` workgroups for every 128 rows of a group's queries and
-// key-value head over the shared keys, and `splits` of `steps` steps for a sequence's own (as qe_attn_decode_plan has them).
+// key-value head over the shared keys, and `splits` of `steps` steps for a sequence's own (qe_attn_decode_cut).
+// A split of the shared keys costs its partial results, and saves the others time: P splits take about a prefix / P + b rows
+// P, which is least where P^2 is a / b times prefix / rows.  With a / b = 40, at most one workgroup a CU, and at least 64 keys,
+// 32 sequences of 16 heads of 256 behind 8000 take 34 us a call (36 with 60, 39 with 100), 8 behind 16,000 30 (29, 29).
 // Each leaves partial results, psplits + splits for a row of n_seqs * q_heads, which have room for QE_ATTN_SHARED_ROWS.  At
 // most 2^15 rows are in a launch (qe_attn_shared_seqs), so that each has room for two.
 #define QE_ATTN_SHARED_ROWS 65536
@@ -108,15 +111,14 @@ QE_MIX_HD int qe_attn_shared_seqs(int n_seqs, int q_heads) {
     const int most = QE_ATTN_SHARED_ROWS / 2 / q_heads;
     return n_seqs < most ? n_seqs : most;
 }
-QE_MIX_HD void qe_attn_shared_plan(int n_seqs, int n_groups, int q_heads, int kv_heads, int head_dim, int64_t max_prefix, int64_t max_own, int *psplits,
-                                   int *steps, int *splits) {
-    const int64_t room = QE_ATTN_SHARED_ROWS / ((int64_t)n_seqs * q_heads);
-    qe_attn_decode_plan(n_seqs, kv_heads, head_dim, max_own, steps, splits);
+QE_MIX_HD void qe_attn_shared_plan(int n_seqs, int q_heads, int kv_heads, int64_t max_prefix, int64_t max_own, int *psplits, int *steps, int *splits) {
+    const int64_t rows = (int64_t)n_seqs * q_heads, room = QE_ATTN_SHARED_ROWS / rows;
+    qe_attn_decode_cut(n_seqs, kv_heads, 512, 12, max_own, steps, splits);
     if (*splits > (room + 1) / 2) *splits = (int)((room + 1) / 2);
-    const int64_t tiles = ((int64_t)n_seqs * (q_heads / kv_heads) + (int64_t)n_groups * (QE_ATTN_SHARED_BM - 1)) / QE_ATTN_SHARED_BM * kv_heads;
-    const int64_t most = (max_prefix + 255) / 256;
-    int64_t s = 256 / (tiles > 0 ? tiles : 1);
-    if (s > most) s = most;
+    const int64_t tiles = ((int64_t)n_seqs * (q_heads / kv_heads) + QE_ATTN_SHARED_BM - 1) / QE_ATTN_SHARED_BM * kv_heads;
+    const int64_t most = (max_prefix + 63) / 64, fill = (256 + tiles - 1) / tiles;
+    int64_t s = 1;
+    while (s * s * rows < 40 * max_prefix && s < most && s < fill) ++s;
     if (s > room - *splits) s = room - *splits;
     *psplits = s < 1 ? 1 : (int)s;
 }
