@@ -81,6 +81,9 @@ __global__ __launch_bounds__(64 * WAVES, 2) void k_attn_prompt8(const QeAttn8Arg
             hi = lo; // no key: zeros
         }
     }
+    // Q and the first tile have come, on every way to the loop: else the compiler has each step wait for Q, and with it for the
+    // loads in flight.
+    __builtin_amdgcn_s_waitcnt(0x0f70);
     if (lo < hi) {
         stage.land(lo * BN, len, wave, raw, k_a, v_a, s_a[0], s_a[1]);
         if (lo + 1 < hi) stage.issue(x, page, kvh, (lo + 1) * BN, len, wave, raw);

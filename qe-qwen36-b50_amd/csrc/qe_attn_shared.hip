@@ -113,6 +113,8 @@ __device__ __forceinline__ void shared_prefix(const QeSharedArgs &y, int tile, i
 #pragma unroll
             for (int i = 0; i < 16; ++i) w.o[d][i] = 0;
     }
+    // Q and the first tile have come: else the compiler has each step wait for Q, and with it for the loads in flight
+    __builtin_amdgcn_s_waitcnt(0x0f70);
     if constexpr (CODES) {
         stage.land(lo * BN, len, wave, raw, k_a, v_a, s_a[0], s_a[1]);
         if (lo + 1 < hi) load(lo + 1, nullptr, nullptr);

@@ -13,15 +13,16 @@ struct Stage {
     static constexpr int RAW = (V_IN_LDS + K_IN_LDS) * PART * DH; // bytes of LDS a wave
     typedef unsigned u4 __attribute__((ext_vector_type(4)));
     u4 k[K_IN_LDS ? 1 : NL], v[V_IN_LDS ? 1 : NL];
-    float scale; // lanes 0 .. PART - 1: of the part's keys, 32 .. 32 + PART - 1: of its values
+    float ks, vs; // lane n: the scales of the part's key n % PART
 
     // The codes of the wave's part of the tile of BN keys from k0 on.
     __device__ __forceinline__ void issue(const QeAttn8Args &x, int page, int kvh, int k0, int len, int wave, uint8_t *raw) {
         const int sub = k0 + wave * PART, at = sub < len ? sub : (len - 1) & -PART;
         unsigned known = 0; // that a page is none: lost_pages
         const size_t r0 = page_row(x.a, page, kvh, at, &known);
-        const int lane = lane_now(), n = lane & 31;
-        scale = (lane < 32 ? x.ks : x.vs)[r0 + (n < PART ? n : 0)];
+        const unsigned lane = lane_now(), n = lane % PART;
+        ks = (x.ks + r0)[n];
+        vs = (x.vs + r0)[n];
         const uint8_t *kp = (const uint8_t *)x.a.kc + r0 * DH, *vp = (const uint8_t *)x.a.vc + r0 * DH;
 #pragma unroll
         for (int i = 0; i < NL; ++i) {
@@ -34,26 +35,37 @@ struct Stage {
             else v[i] = *(const u4 *)(vp + i * 1024 + lane * 16);
         }
     }
+    // A load's registers, not looked at before this place: the compiler would begin to take codes apart where they are loaded,
+    // and wait for them there.
+    static __device__ __forceinline__ u4 come(u4 x) {
+        asm volatile("" : "+v"(x));
+        return x;
+    }
     // They have come: to the tiles, as 16-bit numbers.  Behind the end, where codes and scales may be anything, zeros.
-    __device__ __forceinline__ void land(int k0, int len, int wave, const uint8_t *raw, short *k_lds, short *v_lds, float *ks, float *vs) {
+    __device__ __forceinline__ void land(int k0, int len, int wave, const uint8_t *raw, short *k_lds, short *v_lds, float *ks_lds, float *vs_lds) {
         if constexpr (V_IN_LDS) __builtin_amdgcn_s_waitcnt(0x0f70);
-        const int lane = lane_now(), n = lane & 31;
-        const bool cut = k0 + BN > len;
-        if (n < PART) (lane < 32 ? ks : vs)[wave * PART + n] = cut && k0 + wave * PART + n >= len ? 0.f : scale;
+        const unsigned lane = lane_now(), n = lane % PART;
+        // Lanes 0 .. PART - 1 write the part's keys' scales, the next PART its values', the others again what these did.
+        const bool of_v = lane / PART & 1;
+        (of_v ? vs_lds : ks_lds)[wave * PART + n] = k0 + wave * PART + (int)n < len ? (of_v ? vs : ks) : 0.f;
 #pragma unroll
         for (int i = 0; i < NL; ++i) {
-            const int row = wave * PART + i * (64 / CH) + lane / CH, c = lane % CH * 2;
             u4 a, b;
             if constexpr (K_IN_LDS) a = *(const u4 *)(raw + (NL + i) * 1024 + lane * 16);
-            else a = k[i];
+            else a = come(k[i]);
             if constexpr (V_IN_LDS) b = *(const u4 *)(raw + i * 1024 + lane * 16);
-            else b = v[i];
-            if (CT == QE_F8 && cut && k0 + row >= len) a = b = u4{0, 0, 0, 0};
-            short *kr = k_lds + row * DH, *vr = v_lds + row * DH;
-            *(qe_s8 *)(kr + ((c ^ k_swz(row)) << 3)) = elements_of<CT, BF>(a[0], a[1]);
-            *(qe_s8 *)(kr + (((c + 1) ^ k_swz(row)) << 3)) = elements_of<CT, BF>(a[2], a[3]);
-            *(qe_s8 *)(vr + ((c ^ v_swz<DH>(row)) << 3)) = elements_of<CT, BF>(b[0], b[1]);
-            *(qe_s8 *)(vr + (((c + 1) ^ v_swz<DH>(row)) << 3)) = elements_of<CT, BF>(b[2], b[3]);
+            else b = come(v[i]);
+            const int row = wave * PART + i * (64 / CH) + lane / CH;
+            if (CT == QE_F8 && k0 + BN > len) { // uniform
+                if (k0 + row >= len) a = b = u4{0, 0, 0, 0};
+            }
+            // a lane's two chunks: of K neighbours but for the permutation, of V side by side
+            char *kr = (char *)k_lds + row * DH * 2, *vr = (char *)v_lds + row * DH * 2;
+            const unsigned ko = (lane % CH * 2 ^ k_swz(row)) << 4, vo = (lane % CH * 2 ^ v_swz<DH>(row)) << 4;
+            *(qe_s8 *)(kr + ko) = elements_of<CT, BF>(a[0], a[1]);
+            *(qe_s8 *)(kr + (ko ^ 16)) = elements_of<CT, BF>(a[2], a[3]);
+            *(qe_s8 *)(vr + vo) = elements_of<CT, BF>(b[0], b[1]);
+            *(qe_s8 *)(vr + vo + 16) = elements_of<CT, BF>(b[2], b[3]);
         }
     }
 };
