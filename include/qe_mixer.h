@@ -66,7 +66,7 @@ typedef struct {
 
 typedef struct qe_attn_ctx qe_attn_ctx;
 
-/* Create a context on `device`: scratch of a fixed size (17 to 68 MB)
+/* Create a context on `device`: scratch of a fixed size (35 to 135 MB)
  * for the partial results of calls that split a sequence's length. */
 int qe_attn_create(int device, const qe_attn_desc *desc, qe_attn_ctx **out);
 int qe_attn_destroy(qe_attn_ctx *ctx);

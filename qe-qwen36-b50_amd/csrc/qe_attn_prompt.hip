@@ -189,7 +189,7 @@ __global__ __launch_bounds__(64 * WAVES, 2) void k_attn_prompt(const QeAttnArgs 
                     }
         }
     }
-    w.template finish<BM>(a, begin, n_rows, row0, wave_row, tile, kvh, split);
+    w.template finish<BM>(a, begin, n_rows, row0, wave_row, tile, kvh, split, a.splits == 1);
 }
 
 template <bool BF, int DH, int WAVES>

@@ -43,11 +43,12 @@ __global__ __launch_bounds__(64 * WAVES, 2) void k_attn_prompt8(const QeAttn8Arg
     const int row0 = local * BM, first = len - (end - begin); // first: position of the sequence's first row
     const int32_t *table = a.table + (size_t)seq * a.table_stride;
 
-    const int last_tok = (row0 + BM < n_rows ? row0 + BM - 1 : n_rows - 1) / a.group, keys = first + last_tok + 1;
     const int wave_row = row0 + wave * 32, wave_end = wave_row + 32 < n_rows ? wave_row + 32 : n_rows;
     const int wave_keys = wave_row < n_rows ? first + (wave_end - 1) / a.group + 1 : 0, wave_clear = first + wave_row / a.group + 1;
+    const int steps = qe_attn_tile_steps(len, begin, end, row0, a.group, BM, BN), splits = qe_attn_tile_splits(steps, a.steps, a.splits);
+    if (split >= splits) return;
     int lo, hi;
-    qe_split_range(keys > 0 ? (keys + BN - 1) / BN : 0, a.splits, split, &lo, &hi);
+    qe_split_range(steps, splits, split, &lo, &hi);
 
     ST stage;
     uint8_t *raw = raw_s + wave * ST::RAW;
@@ -124,13 +125,68 @@ __global__ __launch_bounds__(64 * WAVES, 2) void k_attn_prompt8(const QeAttn8Arg
         if (t + 1 < hi) work(t + 1, k_b, v_b, s_b, k_a, v_a, s_a);
     }
     if constexpr (!BF) w.times(units.unit);
-    w.template finish<BM>(a, begin, n_rows, row0, wave_row, tile, kvh, split);
+    w.template finish<BM>(a, begin, n_rows, row0, wave_row, tile, kvh, split, splits == 1);
+}
+
+// The splits' results joined, of the tiles that have several: a workgroup for ROWS of a tile's rows and a key-value head, each wave
+// one row after the other, all of a row's reads (and the next rows') in flight.
+template <bool BF, int DH, int BM, int BN, int ROWS>
+__global__ __launch_bounds__(256) void k_attn_prompt8_join(const QeAttnArgs a) {
+    constexpr int E = DH / 64;
+    const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, item = blockIdx.x / (BM / ROWS), tile = item / a.kv_heads, kvh = item % a.kv_heads;
+    int seq = 0;
+    for (int hi = a.n_seqs; hi - seq > 1;) {
+        const int mid = (seq + hi) >> 1;
+        if (qe_attn_first_tile(qe_clamped(scalar_load(a.cu + mid), 0, a.n_tokens), mid, a.group, BM) <= tile) seq = mid;
+        else hi = mid;
+    }
+    unsigned bad = 0;
+    int begin, end;
+    qe_rows_of(scalar_load(a.cu + seq), scalar_load(a.cu + seq + 1), a.n_tokens, &begin, &end, &bad);
+    const int len = qe_checked(scalar_load(a.kv_len + seq), 0, a.max_pages << a.page_log2, 0, &bad);
+    const int local = tile - qe_attn_first_tile(begin, seq, a.group, BM), n_rows = (end - begin) * a.group;
+    if (local < 0 || (int64_t)local * BM >= n_rows) return;
+    const int splits = qe_attn_tile_splits(qe_attn_tile_steps(bad ? 0 : len, begin, end, local * BM, a.group, BM, BN), a.steps, a.splits);
+    if (splits <= 1) return; // its one workgroup has written the rows
+    const size_t at0 = ((size_t)tile * a.kv_heads + kvh) * a.splits * BM;
+    const int first = blockIdx.x % (BM / ROWS) * ROWS, left = n_rows - local * BM - first;
+#pragma unroll 2
+    for (int r = wave; r < ROWS; r += 4) {
+        if (r >= left) return;
+        const size_t at = at0 + first + r;
+        float m = -INFINITY, sum = 0, o[E];
+#pragma unroll
+        for (int e = 0; e < E; ++e) o[e] = 0;
+        for (int s = lane; s < splits; s += 64) m = fmaxf(m, a.part_ml[at + (size_t)s * BM].x);
+        for (int k = 32; k; k >>= 1) m = fmaxf(m, __shfl_xor(m, k));
+#pragma unroll 4
+        for (int s = 0; s < splits; ++s) {
+            const float2 x = a.part_ml[at + (size_t)s * BM];
+            float y[E];
+#pragma unroll
+            for (int e = 0; e < E; ++e) y[e] = a.part_o[(at + (size_t)s * BM) * DH + e * 64 + lane];
+            const float f = x.x == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(x.x - m);
+            const bool any = x.y != 0.f; // else no key of that split
+            sum += any ? f * x.y : 0.f;
+#pragma unroll
+            for (int e = 0; e < E; ++e) o[e] += any ? f * y[e] : 0.f;
+        }
+        const float inv = sum == 0.f ? 0.f : 1.f / sum;
+        const int row = local * BM + first + r, tok = row / a.group, head = kvh * a.group + row - tok * a.group;
+        short *out = (short *)a.out + (size_t)(begin + tok) * a.out_stride + (size_t)head * DH;
+#pragma unroll
+        for (int e = 0; e < E; ++e) out[e * 64 + lane] = (short)pack2<BF>(o[e] * inv, 0.f);
+    }
 }
 
 template <bool BF, int DH, int CT, int WAVES>
 static hipError_t launch_waves8(const QeAttn8Args &x, hipStream_t st) {
-    k_attn_prompt8<BF, DH, CT, WAVES><<<dim3((unsigned)(x.a.tiles * x.a.kv_heads * x.a.splits)), dim3(64 * WAVES), 0, st>>>(x);
-    launch_prompt_join<BF, DH, 32 * WAVES>(x.a, st);
+    constexpr int BM = 32 * WAVES, BN = Stage<CT, BF, DH, WAVES>::BN;
+    const unsigned items = (unsigned)(x.a.tiles * x.a.kv_heads);
+    k_attn_prompt8<BF, DH, CT, WAVES><<<dim3(items * x.a.splits), dim3(64 * WAVES), 0, st>>>(x);
+    // few tiles: fewer rows a workgroup
+    if (x.a.splits > 1 && items >= 128) k_attn_prompt8_join<BF, DH, BM, BN, 32><<<dim3(items * (BM / 32)), dim3(256), 0, st>>>(x.a);
+    else if (x.a.splits > 1) k_attn_prompt8_join<BF, DH, BM, BN, 4><<<dim3(items * (BM / 4)), dim3(256), 0, st>>>(x.a);
     return hipGetLastError();
 }
 template <bool BF, int CT>

@@ -210,13 +210,13 @@ struct Rows {
                 o[d] = mfma32<BF>(qe_s8{x[0], x[1], x[2], x[3], y[0], y[1], y[2], y[3]}, p.p[ks / 2][ks % 2].v, o[d]);
             }
     }
-    // The rows to `out`, or as a split's partial results.
+    // The rows to `out` (direct), or as a split's partial results.
     template <int BM>
-    __device__ __forceinline__ void finish(const QeAttnArgs &a, int begin, int n_rows, int row0, int wave_row, int tile, int kvh, int split) const {
+    __device__ __forceinline__ void finish(const QeAttnArgs &a, int begin, int n_rows, int row0, int wave_row, int tile, int kvh, int split, bool direct) const {
         const int lane = lane_now(), r = lane & 31, h = lane >> 5;
         const float sum = l + __shfl_xor(l, 32);
         const int row = wave_row + r;
-        if (a.splits == 1) {
+        if (direct) {
             if (row >= n_rows) return;
             const int tok = row / a.group, head = kvh * a.group + row - tok * a.group;
             const float inv = sum == 0.f ? 0.f : 1.f / sum;

@@ -2,6 +2,7 @@
 #include <math.h>
 #include <string.h>
 
+#include <initializer_list>
 #include <new>
 
 #include "qe_mixer.h"
@@ -93,11 +94,13 @@ void release(qe_attn_ctx *c) {
     delete c;
 }
 
-// Rows of partial results: decode's splits (below QE_ATTN_PART_WGS, each room for the rows of the largest group) or
-// prompt's (at most QE_ATTN_WGS tiles of 128 rows).
+// Rows of partial results: decode's splits (below QE_ATTN_PART_WGS, each room for the rows of the largest group), prompt's (at
+// most QE_ATTN_WGS tiles of 128 rows, over an 8-bit cache QE_ATTN_PROMPT8_ROWS) or those of shared beginnings.
 size_t part_rows() {
-    const size_t decode = (size_t)QE_ATTN_PART_WGS * QE_ATTN_GROUP_MAX, prompt = (size_t)QE_ATTN_WGS * 128;
-    return decode > prompt ? decode : prompt;
+    size_t most = (size_t)QE_ATTN_PART_WGS * QE_ATTN_GROUP_MAX;
+    for (size_t rows : {(size_t)QE_ATTN_WGS * 128, (size_t)QE_ATTN_PROMPT8_ROWS, (size_t)QE_ATTN_SHARED_ROWS})
+        if (rows > most) most = rows;
+    return most;
 }
 
 int check_seqs(const qe_attn_ctx *c, const qe_attn_batch *b, const char *where) {
@@ -352,14 +355,14 @@ static int check_attend(qe_attn_ctx *c, const qe_attn_batch *b, const CACHE *kv,
 
 extern "C" {
 
-// How a prompt call is cut up: a->tiles and a->splits, and the rows of a workgroup.
-static int plan_prompt(const qe_attn_ctx *c, const qe_attn_batch *b, const char *where, QeAttnArgs *a, int *bm) {
+// A prompt call's a->tiles, the rows of a workgroup, and the longest length.
+static int plan_prompt(const qe_attn_ctx *c, const qe_attn_batch *b, const char *where, QeAttnArgs *a, int *bm, int64_t *max_len) {
     *bm = qe_attn_prompt_rows(b->n_tokens, b->n_seqs, a->group, a->kv_heads, c->d.head_dim);
     a->tiles = qe_attn_max_tiles(b->n_tokens, b->n_seqs, a->group, *bm);
     if (!qe_fits_launch((int64_t)a->tiles * a->kv_heads, 2 * *bm))
         return qe_fail(QE_ERR_ARG, "%s: %d tokens of %d sequences are more threads than a launch has", where, b->n_tokens, b->n_seqs);
     const int64_t most = (int64_t)b->max_pages * c->d.page;
-    a->splits = qe_attn_prompt_splits((int64_t)a->tiles * a->kv_heads, b->max_len && b->max_len < most ? b->max_len : most);
+    *max_len = b->max_len && b->max_len < most ? b->max_len : most;
     return QE_OK;
 }
 
@@ -370,7 +373,9 @@ int qe_attn_prompt(qe_attn_ctx *c, const qe_attn_batch *b, const qe_kv_cache *kv
     int rc = check_attend(c, b, kv, q, q_stride, out, out_stride, where), bm;
     if (rc != QE_OK || b->n_tokens == 0) return rc;
     QeAttnArgs a = attn_args(c, b, kv, q, q_stride, out, out_stride);
-    if ((rc = plan_prompt(c, b, where, &a, &bm)) != QE_OK) return rc;
+    int64_t max_len;
+    if ((rc = plan_prompt(c, b, where, &a, &bm, &max_len)) != QE_OK) return rc;
+    a.splits = qe_attn_prompt_splits((int64_t)a.tiles * a.kv_heads, max_len);
     OnDevice on(c->device);
     HIP_TRY(on.e);
     HIP_TRY(qe_launch_attn_prompt(a, c->d.head_dim, c->d.type, bm, (hipStream_t)stream));
@@ -386,7 +391,9 @@ int qe_attn_prompt8(qe_attn_ctx *c, const qe_attn_batch *b, const qe_kv_cache8 *
     QeAttn8Args x{};
     x.a = attn_args(c, b, kv, q, q_stride, out, out_stride);
     x.ks = kv->k_scale; x.vs = kv->v_scale;
-    if ((rc = plan_prompt(c, b, where, &x.a, &bm)) != QE_OK) return rc;
+    int64_t max_len;
+    if ((rc = plan_prompt(c, b, where, &x.a, &bm, &max_len)) != QE_OK) return rc;
+    qe_attn_prompt8_plan((int64_t)x.a.tiles * x.a.kv_heads, bm, c->d.head_dim == 256 ? 32 : 64, max_len, &x.a.steps, &x.a.splits);
     OnDevice on(c->device);
     HIP_TRY(on.e);
     HIP_TRY(qe_launch_attn_prompt8(x, c->d.head_dim, c->d.type, kv->type, bm, (hipStream_t)stream));

@@ -98,6 +98,36 @@ QE_MIX_HD int qe_attn_prompt_splits(int64_t tiles, int64_t max_len) {
     return s < 1 ? 1 : (int)s;
 }
 
+// A prompt call over an 8-bit cache splits a tile's keys by how many it has, so that a long tile among short ones is cut and these
+// are not: `steps` steps a workgroup, at most `splits` for a tile and key-value head, as many as there is scratch for.
+// Workgroups that a tile has no use for end at once, and one that has all of a tile's keys writes its rows itself.  At
+// least eight steps, and as many as let twice the places of the GPU hold all tiles if each were as long as the longest (32 / 8 heads
+// of 128, int8: 600 tokens after 20,000 337 us with 1.5 times, 307 with twice and with three times, 599 without; 50, 700 and 20
+// after 5000, 0 and 19,000 of 24 / 8 heads of 64 107, 87 and 88, 406 without).  Where tiles fill half of the places and none has 40
+// steps the join costs as much as it saves: 1500 tokens 53 us without, 65 with; 4 x 400 after 2000 103 and 122; but 200, 333 and
+// 967 after 0, 1700 and 0 81 and 76.
+#define QE_ATTN_PROMPT8_ROWS 131072 /* of partial results */
+QE_MIX_HD void qe_attn_prompt8_plan(int64_t tiles, int bm, int bn, int64_t max_len, int *steps, int *splits) {
+    const int64_t longest = (max_len + bn - 1) / bn, places = bm == 256 ? 256 : 512, room = QE_ATTN_PROMPT8_ROWS / (tiles * bm);
+    int64_t per = (longest * tiles + 2 * places - 1) / (2 * places);
+    if (per < 8) per = 8;
+    int64_t s = (longest + per - 1) / per;
+    if (s > room) s = room;
+    if (s < 1 || (2 * tiles > places && longest < 40)) s = 1;
+    *steps = (int)per;
+    *splits = (int)s;
+}
+// Steps of `bn` keys of the tile of rows from row0 on, up to the place of its last row.  (The sequence's rows are tokens begin ..
+// end - 1 times `group`, and its last position is the last token's.)
+QE_MIX_HD int qe_attn_tile_steps(int len, int begin, int end, int row0, int group, int bm, int bn) {
+    const int n_rows = (end - begin) * group, last = (row0 + bm < n_rows ? row0 + bm - 1 : n_rows - 1) / group, keys = len - (end - begin) + last + 1;
+    return keys > 0 ? (keys + bn - 1) / bn : 0;
+}
+QE_MIX_HD int qe_attn_tile_splits(int n, int steps, int splits) {
+    const int s = (n + steps - 1) / steps;
+    return s < 1 ? 1 : s < splits ? s : splits;
+}
+
 // A call of single tokens whose sequences share beginnings: `psplits` workgroups for every 128 rows of a group's queries and
 // key-value head over the shared keys, and `splits` of `steps` steps for a sequence's own (qe_attn_decode_cut).
 // A split of the shared keys costs its partial results, and saves the others time: P splits take about a prefix / P + b rows
