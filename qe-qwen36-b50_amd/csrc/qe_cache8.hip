@@ -217,8 +217,10 @@ __global__ __launch_bounds__(256) void k_read8(const QeRead8Args a) {
             o[0] = make_uint4(r[0], r[1], r[2], r[3]);
             o[1] = make_uint4(r[4], r[5], r[6], r[7]);
         }
-        *(uint4 *)dst = o[0];
-        *(uint4 *)(dst + 8) = o[1];
+        // (past the caches: 18,178 positions 28.8 -> 25.5 us)
+        typedef unsigned u4 __attribute__((ext_vector_type(4)));
+        __builtin_nontemporal_store(u4{o[0].x, o[0].y, o[0].z, o[0].w}, (u4 *)dst);
+        __builtin_nontemporal_store(u4{o[1].x, o[1].y, o[1].z, o[1].w}, (u4 *)(dst + 8));
     }
 }
 

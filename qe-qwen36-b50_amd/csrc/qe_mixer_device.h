@@ -118,7 +118,7 @@ struct QeToken {
 template <typename ARGS>
 __device__ __forceinline__ void report_offsets(const ARGS &a) {
     if (a.cu)
-        for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < a.n_seqs; i += (int64_t)gridDim.x * 256)
+        for (int64_t i = (int64_t)blockIdx.x * blockDim.x + threadIdx.x; i < a.n_seqs; i += (int64_t)gridDim.x * blockDim.x)
             if (qe_bad_offsets(a.cu[i], a.cu[i + 1], a.n_tokens)) report(a.err, QE_BAD_LENGTH);
 }
 // Token t's, by every wave for itself, through the scalar cache, with no barrier.  False: it has none; `teller` reports why.
