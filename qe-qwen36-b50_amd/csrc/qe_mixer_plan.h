@@ -110,6 +110,7 @@ QE_MIX_HD int qe_attn_prompt_splits(int64_t tiles, int64_t max_len) {
 QE_MIX_HD void qe_attn_prompt8_plan(int64_t tiles, int bm, int bn, int64_t max_len, int *steps, int *splits) {
     const int64_t longest = (max_len + bn - 1) / bn, places = bm == 256 ? 256 : 512, room = QE_ATTN_PROMPT8_ROWS / (tiles * bm);
     int64_t per = (longest * tiles + 2 * places - 1) / (2 * places);
+    if (per > longest) per = longest;
     if (per < 8) per = 8;
     int64_t s = (longest + per - 1) / per;
     if (s > room) s = room;
