@@ -109,7 +109,11 @@ __global__ __launch_bounds__(64 * WAVES, 2) void k_attn_prompt8(const QeAttn8Arg
             w.weigh(a.scale_log2, s);
 #pragma unroll
             for (int b = 0; b < KB; ++b) scaled(s.s[b], BF ? s_lds[1][b * 32 + at] : s_lds[1][b * 32 + at] * units.inverse);
-            if (cut) s.clear(limit); // a scale that is not finite reaches the rows that attend to its position
+            if (cut) { // a scale that is not finite reaches the rows that attend to its position
+                int again = limit;
+                asm volatile("" : "+v"(again)); // else the compiler makes these comparisons in every step: 637 us for 614 at 8000 tokens
+                s.clear(again);
+            }
             s.template pack<BF>(p);
             w.values(v_lds, 0, p);
             schedule<3, KB * DH / 16, 2>();

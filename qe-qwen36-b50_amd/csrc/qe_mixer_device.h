@@ -215,15 +215,17 @@ struct Units {
     float unit = 0, inverse = 0;
     // `scale`, over all lanes: a tile's; those of fewer lanes are in others, too.  What sums so far are to be multiplied by.
     __device__ __forceinline__ float raise(float scale) {
-        float top = fabsf(scale) < INFINITY ? fabsf(scale) : 0.f; // one that is not finite reaches the rows that attend to it without this
-        top = fmaxf(top, __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(top), 0xb1, 0xf, 0xf, true)));
-        top = fmaxf(top, __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(top), 0x4e, 0xf, 0xf, true)));
-        top = fmaxf(top, __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(top), 0x141, 0xf, 0xf, true)));
-        top = fmaxf(top, __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(top), 0x140, 0xf, 0xf, true)));
-        const auto a = __builtin_amdgcn_permlane16_swap(__float_as_uint(top), __float_as_uint(top), false, false);
-        top = fmaxf(__uint_as_float(a[0]), __uint_as_float(a[1]));
-        const auto b = __builtin_amdgcn_permlane32_swap(__float_as_uint(top), __float_as_uint(top), false, false);
-        const unsigned bits = __builtin_amdgcn_readfirstlane(__float_as_uint(fmaxf(__uint_as_float(b[0]), __uint_as_float(b[1]))));
+        // (one that is not finite reaches the rows that attend to it without this; positive numbers' bits are in their order)
+        unsigned top = __float_as_uint(scale) & 0x7fffffffu;
+        if (top >= 0x7f800000u) top = 0;
+        top = max(top, (unsigned)__builtin_amdgcn_update_dpp(0, (int)top, 0xb1, 0xf, 0xf, true));
+        top = max(top, (unsigned)__builtin_amdgcn_update_dpp(0, (int)top, 0x4e, 0xf, 0xf, true));
+        top = max(top, (unsigned)__builtin_amdgcn_update_dpp(0, (int)top, 0x141, 0xf, 0xf, true));
+        top = max(top, (unsigned)__builtin_amdgcn_update_dpp(0, (int)top, 0x140, 0xf, 0xf, true));
+        const auto a = __builtin_amdgcn_permlane16_swap(top, top, false, false);
+        top = max(a[0], a[1]);
+        const auto b = __builtin_amdgcn_permlane32_swap(top, top, false, false);
+        const unsigned bits = __builtin_amdgcn_readfirstlane(max(b[0], b[1]));
         if (__uint_as_float(bits) <= unit) return 1.f;
         // two to four times the greatest, so that it seldom changes; within 2^-100 .. 2^100
         unsigned e = (bits >> 23) + 2;
