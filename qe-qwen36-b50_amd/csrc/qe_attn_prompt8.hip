@@ -6,19 +6,21 @@
 // and writes them to the other of two buffers, so that a code is turned once for all rows of a workgroup.  With heads of 256
 // the registers are full: there the codes wait in a few KB of LDS, by direct loads.  A key's scale multiplies its scores and a
 // value's its probabilities (in fp16 in units of theirs: Units), from one register: lane n of 16 has the scale of the n-th
-// of the 16 keys in the lane's registers.
+// of the 16 keys in the lane's registers.  Where tiles are few, eight waves share a tile's rows, four for the even steps and four for
+// the odd ones (HALVES, qe_attn_prompt8_halves), and join their sums in LDS.
 #include "qe_attn_stage8.h"
 
-template <bool BF, int DH, int CT, int WAVES>
-__global__ __launch_bounds__(64 * WAVES, 2) void k_attn_prompt8(const QeAttn8Args x) {
+template <bool BF, int DH, int CT, int WAVES, int HALVES>
+__global__ __launch_bounds__(64 * WAVES * HALVES, 2) void k_attn_prompt8(const QeAttn8Args x) {
     const QeAttnArgs &a = x.a;
     typedef Stage<CT, BF, DH, WAVES> ST;
     constexpr int BM = 32 * WAVES, BN = ST::BN, KB = DH == 256 ? 1 : 2;
     static_assert(BN == 32 * KB, "a tile is a step");
-    __shared__ __align__(16) short k_a[BN * DH], v_a[BN * DH], k_b[BN * DH], v_b[BN * DH];
-    __shared__ __align__(16) uint8_t raw_s[ST::RAW ? WAVES * ST::RAW : 16];
-    __shared__ float s_a[2][BN], s_b[2][BN];
-    const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    __shared__ __align__(16) short k_a[HALVES][BN * DH], v_a[HALVES][BN * DH], k_b[HALVES][BN * DH], v_b[HALVES][BN * DH];
+    __shared__ __align__(16) uint8_t raw_s[ST::RAW ? WAVES * HALVES * ST::RAW : 16];
+    __shared__ float s_a[HALVES][2][BN], s_b[HALVES][2][BN];
+    const int tid = threadIdx.x, thread_wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int half = HALVES == 1 ? 0 : thread_wave / WAVES, wave = thread_wave - half * WAVES;
     const int split = blockIdx.x % a.splits, kvh = blockIdx.x / a.splits % a.kv_heads;
     const int tile = a.tiles - 1 - blockIdx.x / a.splits / a.kv_heads; // a sequence's late rows have more keys: first
     // workgroup i looks at sequence i's offsets, for the report: where they fall, a sequence may have no tile below
@@ -51,12 +53,13 @@ __global__ __launch_bounds__(64 * WAVES, 2) void k_attn_prompt8(const QeAttn8Arg
     qe_split_range(steps, splits, split, &lo, &hi);
 
     ST stage;
-    uint8_t *raw = raw_s + wave * ST::RAW;
+    uint8_t *raw = raw_s + thread_wave * ST::RAW;
     int page = 0; // of the wave's part of the tile after the one that is loaded
-    if (lo < hi) {
-        page = page_of<BN, WAVES>(a, table, lo * BN, len, wave);
-        stage.issue(x, page, kvh, lo * BN, len, wave, raw);
-        page = page_of<BN, WAVES>(a, table, (lo + 1) * BN, len, wave);
+    const int t0 = lo + half; // the half's first step
+    if (t0 < hi) {
+        page = page_of<BN, WAVES>(a, table, t0 * BN, len, wave);
+        stage.issue(x, page, kvh, t0 * BN, len, wave, raw);
+        page = page_of<BN, WAVES>(a, table, (t0 + HALVES) * BN, len, wave);
     }
     Rows<BF, DH> w;
     Units units;
@@ -76,7 +79,7 @@ __global__ __launch_bounds__(64 * WAVES, 2) void k_attn_prompt8(const QeAttn8Arg
             for (int i = 0; i < 16; ++i) w.o[d][i] = 0;
     }
     if (lo < hi) {
-        const int lost = lost_pages<64 * WAVES>(a, table, (len + (1 << a.page_log2) - 1) >> a.page_log2, tid);
+        const int lost = lost_pages<64 * WAVES * HALVES>(a, table, (len + (1 << a.page_log2) - 1) >> a.page_log2, tid);
         if (__syncthreads_or(lost)) { // (it waits for what is on its way to LDS, too)
             if (tid == 0) report(a.err, QE_BAD_PAGE);
             hi = lo; // no key: zeros
@@ -85,15 +88,15 @@ __global__ __launch_bounds__(64 * WAVES, 2) void k_attn_prompt8(const QeAttn8Arg
     // Q and the first tile have come, on every way to the loop: else the compiler has each step wait for Q, and with it for the
     // loads in flight.
     __builtin_amdgcn_s_waitcnt(0x0f70);
-    if (lo < hi) {
-        stage.land(lo * BN, len, wave, raw, k_a, v_a, s_a[0], s_a[1]);
-        if (lo + 1 < hi) stage.issue(x, page, kvh, (lo + 1) * BN, len, wave, raw);
-        page = page_of<BN, WAVES>(a, table, (lo + 2) * BN, len, wave);
+    if (t0 < hi) {
+        stage.land(t0 * BN, len, wave, raw, k_a[half], v_a[half], s_a[half][0], s_a[half][1]);
+        if (t0 + HALVES < hi) stage.issue(x, page, kvh, (t0 + HALVES) * BN, len, wave, raw);
+        page = page_of<BN, WAVES>(a, table, (t0 + 2 * HALVES) * BN, len, wave);
     }
     auto work = [&](int t, const short *k_lds, const short *v_lds, const float (*s_lds)[BN], short *k_next, short *v_next, float (*s_next)[BN]) {
         lds_barrier(); // the tile is there, and no wave reads the other buffers any more
         const int k0 = t * BN;
-        if (k0 < wave_keys) {
+        if ((HALVES == 1 || t < hi) && k0 < wave_keys) {
             const int lane = lane_now(), at = 8 * (lane >> 2 & 3) + 4 * (lane >> 5) + (lane & 3);
             Scores<KB> s;
             w.scores(k_lds, 0, s);
@@ -118,17 +121,43 @@ __global__ __launch_bounds__(64 * WAVES, 2) void k_attn_prompt8(const QeAttn8Arg
             w.values(v_lds, 0, p);
             schedule<3, KB * DH / 16, 2>();
         }
-        if (t + 1 < hi) {
-            stage.land(k0 + BN, len, wave, raw, k_next, v_next, s_next[0], s_next[1]);
-            if (t + 2 < hi) stage.issue(x, page, kvh, k0 + 2 * BN, len, wave, raw);
-            page = page_of<BN, WAVES>(a, table, k0 + 3 * BN, len, wave);
+        if (t + HALVES < hi) {
+            stage.land(k0 + HALVES * BN, len, wave, raw, k_next, v_next, s_next[0], s_next[1]);
+            if (t + 2 * HALVES < hi) stage.issue(x, page, kvh, k0 + 2 * HALVES * BN, len, wave, raw);
+            page = page_of<BN, WAVES>(a, table, k0 + 3 * HALVES * BN, len, wave);
         }
     };
-    for (int t = lo; t < hi; t += 2) {
-        work(t, k_a, v_a, s_a, k_b, v_b, s_b);
-        if (t + 1 < hi) work(t + 1, k_b, v_b, s_b, k_a, v_a, s_a);
+    for (int t = lo; t < hi; t += 2 * HALVES) { // both halves pass all barriers
+        work(t + half, k_a[half], v_a[half], s_a[half], k_b[half], v_b[half], s_b[half]);
+        if (t + HALVES < hi) work(t + HALVES + half, k_b[half], v_b[half], s_b[half], k_a[half], v_a[half], s_a[half]);
     }
     if constexpr (!BF) w.times(units.unit);
+    if constexpr (HALVES == 2) { // the second half's sums, through the tiles' LDS
+        constexpr int LOT = 64 * WAVES * 16, LOTS = HALVES * BN * DH / 2 / LOT; // floats of 32 columns; these that an array has room for
+        static_assert(LOTS >= 1 && 4 * LOTS * 32 >= DH, "room for all columns");
+        __shared__ float ml_s[2][64 * WAVES];
+        float *const room[4] = {(float *)k_a, (float *)v_a, (float *)k_b, (float *)v_b};
+        const int at = wave * 64 + (tid & 63);
+        lds_barrier(); // no wave reads a tile any more
+        if (half) {
+#pragma unroll
+            for (int d = 0; d < DH / 32; ++d)
+#pragma unroll
+                for (int i = 0; i < 16; ++i) room[d / LOTS][d % LOTS * LOT + i * 64 * WAVES + at] = w.o[d][i];
+            ml_s[0][at] = w.m;
+            ml_s[1][at] = w.l;
+        }
+        lds_barrier();
+        if (half) return;
+        const float m1 = ml_s[0][at], m = fmaxf(w.m, m1);
+        const float f0 = w.m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(w.m - m), f1 = m1 == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m1 - m);
+        w.l = w.l * f0 + ml_s[1][at] * f1;
+        w.m = m;
+#pragma unroll
+        for (int d = 0; d < DH / 32; ++d)
+#pragma unroll
+            for (int i = 0; i < 16; ++i) w.o[d][i] = w.o[d][i] * f0 + room[d / LOTS][d % LOTS * LOT + i * 64 * WAVES + at] * f1;
+    }
     w.template finish<BM>(a, begin, n_rows, row0, wave_row, tile, kvh, split, splits == 1);
 }
 
@@ -183,24 +212,25 @@ __global__ __launch_bounds__(256) void k_attn_prompt8_join(const QeAttnArgs a) {
     }
 }
 
-template <bool BF, int DH, int CT, int WAVES>
+template <bool BF, int DH, int CT, int WAVES, int HALVES>
 static hipError_t launch_waves8(const QeAttn8Args &x, hipStream_t st) {
     constexpr int BM = 32 * WAVES, BN = Stage<CT, BF, DH, WAVES>::BN;
     const unsigned items = (unsigned)(x.a.tiles * x.a.kv_heads);
-    k_attn_prompt8<BF, DH, CT, WAVES><<<dim3(items * x.a.splits), dim3(64 * WAVES), 0, st>>>(x);
+    k_attn_prompt8<BF, DH, CT, WAVES, HALVES><<<dim3(items * x.a.splits), dim3(64 * WAVES * HALVES), 0, st>>>(x);
     // few tiles: fewer rows a workgroup
     if (x.a.splits > 1 && items >= 128) k_attn_prompt8_join<BF, DH, BM, BN, 32><<<dim3(items * (BM / 32)), dim3(256), 0, st>>>(x.a);
     else if (x.a.splits > 1) k_attn_prompt8_join<BF, DH, BM, BN, 4><<<dim3(items * (BM / 4)), dim3(256), 0, st>>>(x.a);
     return hipGetLastError();
 }
 template <bool BF, int CT>
-static hipError_t launch_prompt8(const QeAttn8Args &x, int head_dim, int bm, hipStream_t st) {
-    if (head_dim == 64) return launch_waves8<BF, 64, CT, 4>(x, st);
-    if (head_dim == 128) return launch_waves8<BF, 128, CT, 4>(x, st);
-    return bm == 256 ? launch_waves8<BF, 256, CT, 8>(x, st) : launch_waves8<BF, 256, CT, 4>(x, st);
+static hipError_t launch_prompt8(const QeAttn8Args &x, int head_dim, int bm, bool halves, hipStream_t st) {
+    if (head_dim == 64) return halves ? launch_waves8<BF, 64, CT, 4, 2>(x, st) : launch_waves8<BF, 64, CT, 4, 1>(x, st);
+    if (head_dim == 128) return halves ? launch_waves8<BF, 128, CT, 4, 2>(x, st) : launch_waves8<BF, 128, CT, 4, 1>(x, st);
+    if (bm == 256) return launch_waves8<BF, 256, CT, 8, 1>(x, st);
+    return launch_waves8<BF, 256, CT, 4, 1>(x, st);
 }
 
-hipError_t qe_launch_attn_prompt8(const QeAttn8Args &x, int head_dim, int type, int cache_type, int bm, hipStream_t st) {
-    if (type == QE_BF16) return cache_type == QE_I8 ? launch_prompt8<true, QE_I8>(x, head_dim, bm, st) : launch_prompt8<true, QE_F8>(x, head_dim, bm, st);
-    return cache_type == QE_I8 ? launch_prompt8<false, QE_I8>(x, head_dim, bm, st) : launch_prompt8<false, QE_F8>(x, head_dim, bm, st);
+hipError_t qe_launch_attn_prompt8(const QeAttn8Args &x, int head_dim, int type, int cache_type, int bm, bool halves, hipStream_t st) {
+    if (type == QE_BF16) return cache_type == QE_I8 ? launch_prompt8<true, QE_I8>(x, head_dim, bm, halves, st) : launch_prompt8<true, QE_F8>(x, head_dim, bm, halves, st);
+    return cache_type == QE_I8 ? launch_prompt8<false, QE_I8>(x, head_dim, bm, halves, st) : launch_prompt8<false, QE_F8>(x, head_dim, bm, halves, st);
 }

@@ -75,7 +75,7 @@ struct QeSharedArgs {
 };
 
 #define QE_CACHE16 0 /* a cache of the context's type, beside QE_I8 and QE_F8 */
-hipError_t qe_launch_attn_prompt8(const QeAttn8Args &a, int head_dim, int type, int cache_type, int bm, hipStream_t st);
+hipError_t qe_launch_attn_prompt8(const QeAttn8Args &a, int head_dim, int type, int cache_type, int bm, bool halves, hipStream_t st);
 hipError_t qe_launch_attn_decode8(const QeAttn8Args &a, int head_dim, int type, int cache_type, hipStream_t st);
 hipError_t qe_launch_attn_shared(const QeSharedArgs &a, int head_dim, int type, int cache_type, hipStream_t st);
 hipError_t qe_launch_append8(const QeAppend8Args &a, int in_type, int type, int cache_type, hipStream_t st);

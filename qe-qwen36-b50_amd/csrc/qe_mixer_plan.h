@@ -98,14 +98,26 @@ QE_MIX_HD int qe_attn_prompt_splits(int64_t tiles, int64_t max_len) {
     return s < 1 ? 1 : (int)s;
 }
 
+// Whether a prompt workgroup over an 8-bit cache has eight waves, of which four work on a tile's even steps and four on its odd
+// ones: with heads of up to 128, where the tiles are too few for two workgroups on each CU, or have unequal numbers of steps, and are
+// worth no split's join (below).  A wave alone on its SIMD takes 1.9 us a step of 64 keys and heads of 128, two side by side 2.5.  int8, 32 / 8
+// heads of 128: 900 tokens 28 us a call (two splits 40), 1500 40 (four waves, no split 49), 200, 333 and 967 after 0, 1700 and 0 63 (75),
+// 3 x 300 after 1500 47 (73 in splits), but 4 x 400 after 2000, equal tiles, 108 (97).  16 / 16 of 64: 1100 24 (36).  Behind
+// 64 steps a long tile among short ones needs splits (256 and 800 after 4500 and 0 83 us in splits, 107 with halves);
+// with less than 16 in more than 256 tiles the halves' join is what they save (6 x 256 after 256 30 us without, 36 with); so it is in
+// up to 128 tiles, where splits are as good (300 after 1000 29, 35).  Tiles that fill the GPU are 11% slower (8000 tokens), and heads of 256 are, too:
+// their join is 128 KB of LDS (1000 tokens of 16 / 2 44 us, 54).
+QE_MIX_HD bool qe_attn_prompt8_halves(int64_t tiles, int bn, int64_t max_len) {
+    const int64_t longest = (max_len + bn - 1) / bn;
+    return bn == 64 && longest < 64 && (tiles <= 256 ? tiles > 128 && longest > 4 : tiles <= 512 && longest >= 16);
+}
 // A prompt call over an 8-bit cache splits a tile's keys by how many it has, so that a long tile among short ones is cut and these
 // are not: `steps` steps a workgroup, at most `splits` for a tile and key-value head, as many as there is scratch for.
 // Workgroups that a tile has no use for end at once, and one that has all of a tile's keys writes its rows itself.  At
 // least eight steps, and as many as let twice the places of the GPU hold all tiles if each were as long as the longest (32 / 8 heads
 // of 128, int8: 600 tokens after 20,000 337 us with 1.5 times, 307 with twice and with three times, 599 without; 50, 700 and 20
 // after 5000, 0 and 19,000 of 24 / 8 heads of 64 107, 87 and 88, 406 without).  Where tiles fill half of the places and none has 40
-// steps the join costs as much as it saves: 1500 tokens 53 us without, 65 with; 4 x 400 after 2000 103 and 122; but 200, 333 and
-// 967 after 0, 1700 and 0 81 and 76.
+// steps the join costs as much as it saves (4 x 400 after 2000 103 us without, 122 with; 1500 tokens 53 and 65).
 #define QE_ATTN_PROMPT8_ROWS 131072 /* of partial results */
 QE_MIX_HD void qe_attn_prompt8_plan(int64_t tiles, int bm, int bn, int64_t max_len, int *steps, int *splits) {
     const int64_t longest = (max_len + bn - 1) / bn, places = bm == 256 ? 256 : 512, room = QE_ATTN_PROMPT8_ROWS / (tiles * bm);
@@ -114,7 +126,7 @@ QE_MIX_HD void qe_attn_prompt8_plan(int64_t tiles, int bm, int bn, int64_t max_l
     if (per < 8) per = 8;
     int64_t s = (longest + per - 1) / per;
     if (s > room) s = room;
-    if (s < 1 || (2 * tiles > places && longest < 40)) s = 1;
+    if (s < 1 || (2 * tiles > places && longest < 40) || qe_attn_prompt8_halves(tiles, bn, max_len)) s = 1;
     *steps = (int)per;
     *splits = (int)s;
 }

@@ -15,6 +15,7 @@ extern "C" {
 void decode8_plan(long seqs, long heads, long len, int *steps, int *splits) { qe_attn_decode8_plan(seqs, heads, len, steps, splits); }
 int decode_steps(int len, int steps, int splits) { return qe_attn_decode_steps(len, steps, splits); }
 int decode_active(int len, int steps) { return qe_attn_decode_active(len, steps); }
+int prompt8_halves(long tiles, int bn, long len) { return qe_attn_prompt8_halves(tiles, bn, len); }
 void prompt8_plan(long tiles, int bm, int bn, long len, int *steps, int *splits) { qe_attn_prompt8_plan(tiles, bm, bn, len, steps, splits); }
 int tile_steps(int len, int b, int e, int r, int g, int bm, int bn) { return qe_attn_tile_steps(len, b, e, r, g, bm, bn); }
 int tile_splits(int n, int steps, int splits) { return qe_attn_tile_splits(n, steps, splits); }
@@ -41,6 +42,7 @@ def plan(tmp_path_factory):
                     str(d / "shim.cpp"), "-o", str(d / "shim.so")], check=True)
     lib = ctypes.CDLL(str(d / "shim.so"))
     lib.decode8_plan.argtypes = [ctypes.c_long] * 3 + [ctypes.c_void_p] * 2
+    lib.prompt8_halves.argtypes = [ctypes.c_long, ctypes.c_int, ctypes.c_long]
     lib.prompt8_plan.argtypes = [ctypes.c_long, ctypes.c_int, ctypes.c_int, ctypes.c_long, ctypes.c_void_p, ctypes.c_void_p]
     lib.shared_plan.argtypes = [ctypes.c_int] * 3 + [ctypes.c_long] * 2 + [ctypes.c_void_p] * 3
     return lib
@@ -81,6 +83,8 @@ def test_prompt8_splits_fit_their_scratch_and_cover_a_tiles_steps(plan):
         steps, splits = steps.value, splits.value
         assert steps >= 8 and splits >= 1
         assert splits == 1 or tiles * splits * bm <= plan.prompt8_rows()
+        if plan.prompt8_halves(tiles, bn, longest):  # eight waves join in LDS, and have all of a tile's steps
+            assert splits == 1 and dim < 256 and bm == 128 and 128 < tiles <= 512
         for own in (0, 1, 7, 8, 9, steps, steps + 1, int(rng.integers(0, 3 * steps * splits + 2))):
             mine = plan.tile_splits(own, steps, splits)
             assert 1 <= mine <= splits and (mine == 1) == (own <= steps or splits == 1)

@@ -273,6 +273,86 @@ def test_prompt_bad_lengths_and_offsets_give_zeros_and_an_error(hq, hkv, dim, ct
             close(out[~gone], want[~gone], off[~gone])
 
 
+def in_halves(c, T, n_seqs, max_len):
+    """Whether eight waves share a tile of such a call, as its plan has it."""
+    tiles = (T * (c.hq // c.hkv) // 128 + n_seqs) * c.hkv
+    return -(-max_len // 64) > 4 and 128 < tiles <= 256 or -(-max_len // 64) >= 16 and 256 < tiles <= 512
+
+
+@pytest.mark.parametrize("codes", CODES)
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("hq,hkv,dim,page,lens,ctx", [
+    (32, 8, 128, 16, [1, 33, 0, 700, 129], [0, 900, 5, 0, 63]), (32, 8, 128, 64, [1000, 200, 5], [24, 900, 1]),
+    (12, 12, 64, 32, [1, 33, 0, 900, 513], [0, 1900, 5, 0, 64]), (24, 8, 64, 256, [300, 64, 65, 128, 40], [1000, 0, 0, 0, 3000]),
+    (14, 2, 128, 16, [1, 1, 1, 1300], [0, 62, 63, 64])])
+def test_prompt_in_halves(hq, hkv, dim, page, lens, ctx, dtype, codes):
+    c = Case8(hq, hkv, dim, page, dtype, codes, [a + b for a, b in zip(lens, ctx)])
+    cu = offsets(lens)
+    q = c.q(cu[-1] + 3)
+    want, off = Q.attend_batch(c, q[: cu[-1]], cu)
+    for max_len in (3900, 1030):  # the host may have believed less
+        assert in_halves(c, cu[-1] + 3, len(lens), max_len)
+        out, again = torch.full_like(q, 7.0), torch.empty_like(q)
+        c.att.prompt8(c.batch(cu, max_len=max_len), q, c.cache(), out)
+        c.att.prompt8(c.batch(cu, max_len=max_len), q, c.cache(), again)
+        c.att.check()
+        close(out[: cu[-1]], want, off)
+        assert bool((out[cu[-1]:] == 7).all()) and torch.equal(out[: cu[-1]], again[: cu[-1]])
+
+
+@pytest.mark.parametrize("hq,hkv,dim", [(32, 8, 128), (24, 8, 64)])
+@pytest.mark.parametrize("which", ["k", "v"])
+def test_prompt_in_halves_scales_that_are_not_finite(hq, hkv, dim, which):
+    rows = 700
+    c = Case8(hq, hkv, dim, 16, torch.float16, torch.int8, [rows, 40])
+    cu = [0, rows, rows + 40]
+    q = c.q(cu[-1])
+    want, off = Q.attend_batch(c, q, cu)
+    for at in (0, 77, rows - 1):  # of either half's steps
+        s = c.ks if which == "k" else c.vs
+        place = int(c.table[0, at // 16]), 1, at % 16
+        kept = s[place].clone()
+        s[place] = math.nan
+        out = torch.empty_like(q)
+        assert in_halves(c, cu[-1], 2, rows)
+        c.att.prompt8(c.batch(cu, max_len=rows), q, c.cache(), out)
+        gone = torch.zeros(cu[-1], hq, dtype=torch.bool, device="cuda")
+        gone[at: rows, hq // hkv: 2 * (hq // hkv)] = True
+        assert bool(torch.isnan(out[gone]).any(-1).all())
+        close(out[~gone], want[~gone], off[~gone])
+        s[place] = kept
+
+
+@pytest.mark.parametrize("hq,hkv,dim", [(32, 8, 128), (24, 8, 64)])
+def test_prompt_in_halves_bad_pages_lengths_and_scales_of_any_size(hq, hkv, dim):
+    lens, ctx = [500, 300, 20, 30], [7, 1100, 0, -20]  # the last's first rows have no position
+    c = Case8(hq, hkv, dim, 16, torch.float16, torch.int8, [a + b for a, b in zip(lens, ctx)])
+    c.vs *= torch.exp2(torch.arange(c.page, device="cuda") % 7 * 4.0 - 30.0)
+    cu = offsets(lens)
+    q = c.q(cu[-1])
+    assert in_halves(c, cu[-1], 4, 1400)
+    want, off = Q.attend_batch(c, q, cu)
+    out = torch.full_like(q, 7.0)
+    c.att.prompt8(c.batch(cu, max_len=1400), q, c.cache(), out)
+    c.att.check()
+    close(out, want, off)
+    assert bool((out[cu[3]: cu[3] + 20] == 0).all())
+    for i, kv, where in ((0, None, 31), (1, None, 0), (1, -1, None), (0, 1 << 30, None)):
+        bad, lengths = c.table.clone(), list(c.kv_len)
+        if kv is None:
+            bad[i, where] = c.kc.shape[0]
+        else:
+            lengths[i] = kv
+        out = torch.full_like(q, 7.0)
+        c.att.prompt8(qe_mixer.Batch(ints(lengths), bad, ints(cu), max_len=1400), q, c.cache(), out)
+        with pytest.raises(qe_moe.QeError, match="page" if kv is None else "length"):
+            c.att.check()
+        rest = torch.ones(cu[-1], dtype=torch.bool, device="cuda")
+        rest[cu[i]: cu[i + 1]] = False
+        assert bool((out[~rest] == 0).all())
+        close(out[rest], want[rest], off[rest])
+
+
 def test_far_offsets_in_a_large_cache():
     """Pages whose codes start past 2^32 bytes."""
     hkv, dim, page = 2, 256, 256
