@@ -138,7 +138,7 @@ int qe_attn_decode(qe_attn_ctx *ctx, const qe_attn_batch *batch, const qe_kv_cac
 /* Norms of q's and k's heads before the rotation: x <- x / sqrt(mean(x^2) +
  * eps) * weight, in 32 bits.  Weights are device memory, fp32 [head_dim],
  * 16-byte aligned, the same for all heads; NULL: q (or k) is not normed.
- * eps > 0.  A head whose squares sum beyond the range of 32 bits is NaN. */
+ * eps is 1e-30 or more.  A head whose squares sum beyond the range of 32 bits is NaN. */
 typedef struct {
     const float *q_weight, *k_weight;
     float eps;

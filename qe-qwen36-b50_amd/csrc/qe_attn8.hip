@@ -4,7 +4,11 @@
 
 // ---------------------------------------------------------------------------
 // As k_attn_decode: a workgroup per (sequence, key-value head, split of its length), its four waves each over their own steps
-// (KeyWave), no barrier before the end.  
+// (KeyWave), no barrier before the end.
+//
+// Bound by memory where lengths are long: 24 ragged sequences of up to 8,095 keys, 8 heads of 128 of e4m3, are 175 MB and take 42 us, 4.2 TB/s
+// (the longest sequences' last steps find half of the GPU done).  900 keys of one sequence, 2 heads of 256, take 10 us: length and page, keys and
+// values, the exchange and the join, one after the other.  Steps of 64 keys in place of 32: 48 us for 42.
 // ---------------------------------------------------------------------------
 template <bool BF, int DH, int CT, bool ONCE>
 __global__ __launch_bounds__(256, DH == 64 ? 4 : 3) void k_attn_decode8(const QeAttn8Args x) {

@@ -7,6 +7,10 @@
 // element are a few exchanges between lanes, and everything stays in registers from the load to the codes:
 //   y = x / sqrt(mean(x^2) + eps) w, rotated;  scale = max |y| / 127 or / 448;  codes = y / scale, to nearest.
 // The greatest is found among the bits without sign, where what is not finite is greater than all else.
+//
+// Bound by memory: 8000 tokens of 32 + 2 x 8 heads of 128, fp16 to e4m3, are 213 MB and take 40 us, 5.3 TB/s; 2000 tokens of 16 + 2 x 2
+// heads of 256 with norms, bf16 to 16 bits, 41 MB, 12 us.  Eight single tokens take 4.9 us, a launch and one round trip each for length, page and
+// data.  A thread for each item, up to 512 a token, is slower than turns of 256 (42 us for 8000 tokens).
 // ---------------------------------------------------------------------------
 template <typename IN>
 __device__ __forceinline__ void load8(const IN *p, float *x) {
@@ -183,7 +187,9 @@ hipError_t qe_launch_append8(const QeAppend8Args &a, int in_type, int type, int 
 }
 
 // ---------------------------------------------------------------------------
-// An 8-bit cache read back: a wave per token, 16 codes a lane and turn.
+// An 8-bit cache read back: a wave per token, 16 codes a lane and turn.  y = code times scale, rounded to 32 bits and then to 16.
+// Bound by memory: 18,178 positions of 8 heads of 128, e4m3 to fp16, are 113 MB and take 26 us, 4.3 TB/s.  Two or four tokens a wave: 31 and
+// 32 us (with ordinary stores, when one took 29).
 // ---------------------------------------------------------------------------
 template <bool BF, int CT>
 __global__ __launch_bounds__(256) void k_read8(const QeRead8Args a) {

@@ -98,15 +98,16 @@ QE_MIX_HD int qe_attn_prompt_splits(int64_t tiles, int64_t max_len) {
     return s < 1 ? 1 : (int)s;
 }
 
-// Whether a prompt workgroup over an 8-bit cache has eight waves, of which four work on a tile's even steps and four on its odd
-// ones: with heads of up to 128, where the tiles are too few for two workgroups on each CU, or have unequal numbers of steps, and are
-// worth no split's join (below).  A wave alone on its SIMD takes 1.9 us a step of 64 keys and heads of 128, two side by side 2.5.  int8, 32 / 8
-// heads of 128: 900 tokens 28 us a call (two splits 40), 1500 40 (four waves, no split 49), 200, 333 and 967 after 0, 1700 and 0 63 (75),
-// 3 x 300 after 1500 47 (73 in splits), but 4 x 400 after 2000, equal tiles, 108 (97).  16 / 16 of 64: 1100 24 (36).  Behind
-// 64 steps a long tile among short ones needs splits (256 and 800 after 4500 and 0 83 us in splits, 107 with halves);
-// with less than 16 in more than 256 tiles the halves' join is what they save (6 x 256 after 256 30 us without, 36 with); so it is in
-// up to 128 tiles, where splits are as good (300 after 1000 29, 35).  Tiles that fill the GPU are 11% slower (8000 tokens), and heads of 256 are, too:
-// their join is 128 KB of LDS (1000 tokens of 16 / 2 44 us, 54).
+// Whether a prompt workgroup over an 8-bit cache has eight waves, four for a tile's even steps and four for its odd ones, which join
+// in LDS.  A wave alone on its SIMD takes 1.9 us for a step of 64 keys and heads of 128, two side by side 2.5: where a CU has one
+// workgroup for most of the time, since tiles are few or unequal, eight waves take less.  Microseconds a call, int8, 32 / 8 heads
+// of 128 unless other heads are named:
+//   129 to 256 tiles and more than 4 steps: 900 tokens 28 (two splits 40); 3 x 300 after 1500 47 (splits 73); 1100 of 16 / 16 heads
+//     of 64 24 (36).  Up to 128 tiles splits are as good (300 after 1000 30, 35 with eight waves);
+//   257 to 512 tiles and at least 16 steps: 1500 tokens 40 (four waves 49); 200, 333 and 967 after 0, 1700 and 0 63 (75); but equal
+//     tiles, 4 x 400 after 2000, 108 (97).  With less steps the join is what they save: 6 x 256 after 256 36 (30);
+//   from 64 steps on a long tile among short ones needs splits: 256 and 800 after 4500 and 0 107 (splits 83);
+//   tiles that fill the GPU: 8000 tokens 702 (625);  heads of 256, whose join is 128 KB: 1000 tokens of 16 / 2 54 (44).
 QE_MIX_HD bool qe_attn_prompt8_halves(int64_t tiles, int bn, int64_t max_len) {
     const int64_t longest = (max_len + bn - 1) / bn;
     return bn == 64 && longest < 64 && (tiles <= 256 ? tiles > 128 && longest > 4 : tiles <= 512 && longest >= 16);
