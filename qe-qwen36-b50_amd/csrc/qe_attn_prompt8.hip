@@ -13,7 +13,7 @@
 //
 // Bound by the matrix cores and by the vector instructions beside them, which turn codes, apply scales and make exponentials: 8192
 // tokens of 16 / 2 heads of 256, e4m3, take 557 us of a pass, 980 TFLOP/s (16-bit tiles, which come by direct loads: 489); 8000 of 32 / 8 of 128
-// 614 us a call, 850 TFLOP/s.  Packed prompts of 200, 333 and 967 tokens after 0, 1700 and 0 take 62: the longest tiles' 32 steps, on a GPU half
+// 614 us a call, 850 TFLOP/s.  Packed prompts of 200, 333 and 967 tokens after 0, 1700 and 0 take 54: the longest tiles' 32 steps, on a GPU half
 // full.  Eight waves and 256 rows for heads of 128: 8000 tokens 613 us for 635, but 5000 of 14 / 2 185 for 158.
 template <bool BF, int DH, int CT, int WAVES, int HALVES>
 __global__ __launch_bounds__(64 * WAVES * HALVES, 2) void k_attn_prompt8(const QeAttn8Args x) {
@@ -27,21 +27,43 @@ __global__ __launch_bounds__(64 * WAVES * HALVES, 2) void k_attn_prompt8(const Q
     const int tid = threadIdx.x, thread_wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int half = HALVES == 1 ? 0 : thread_wave / WAVES, wave = thread_wave - half * WAVES;
     const int split = blockIdx.x % a.splits, kvh = blockIdx.x / a.splits % a.kv_heads;
-    const int tile = a.tiles - 1 - blockIdx.x / a.splits / a.kv_heads; // a sequence's late rows have more keys: first
+    const int rank = blockIdx.x / a.splits / a.kv_heads; // of the workgroup's tile, in the order in which they are begun
     // workgroup i looks at sequence i's offsets, for the report: where they fall, a sequence may have no tile below
     const int mine = blockIdx.x < (unsigned)a.n_seqs ? blockIdx.x : a.n_seqs - 1;
     const int mine0 = scalar_load(a.cu + mine), mine1 = scalar_load(a.cu + mine + 1);
-    int seq = 0;
-    for (int hi = a.n_seqs; hi - seq > 1;) { // the last sequence whose first tile is not behind this one
-        const int mid = (seq + hi) >> 1;
-        if (qe_attn_first_tile(qe_clamped(scalar_load(a.cu + mid), 0, a.n_tokens), mid, a.group, BM) <= tile) seq = mid;
-        else hi = mid;
+    int cu0, cu1, kv, seq, local;
+    // The longest sequence's last rows first, from a sequence for each lane and the tiles of all longer ones: 200, 333 and 967 tokens after 0, 1700 and 0 take 54 us
+    // in place of 62, and 500, 60, 40, 20, 300 and 1000 after 0, 9000, 0, 3000, 0 and 0 of 16 / 2 heads of 256 133 in place of 170.
+    if (a.n_seqs <= 64) {
+        const int lane = lane_now(), i = lane < a.n_seqs ? lane : a.n_seqs - 1;
+        const int c0 = a.cu[i], c1 = a.cu[i + 1], length = a.kv_len[i];
+        unsigned any = 0;
+        int begin, end, before = 0;
+        qe_rows_of(c0, c1, a.n_tokens, &begin, &end, &any);
+        const int n = ((end - begin) * a.group + BM - 1) / BM;
+        for (int j = 0; j < a.n_seqs; ++j) {
+            const int other = __builtin_amdgcn_readlane(length, j);
+            before += other > length || (other == length && j < lane) ? __builtin_amdgcn_readlane(n, j) : 0;
+        }
+        const uint64_t here = __ballot(lane < a.n_seqs && rank >= before && rank < before + n);
+        seq = here ? __builtin_ctzll(here) : 0;
+        cu0 = __builtin_amdgcn_readlane(c0, seq), cu1 = __builtin_amdgcn_readlane(c1, seq), kv = __builtin_amdgcn_readlane(length, seq);
+        local = here ? __builtin_amdgcn_readlane(before + n, seq) - 1 - rank : -1;
+    } else { // the last sequence's last rows first
+        const int place = a.tiles - 1 - rank;
+        seq = 0;
+        for (int hi = a.n_seqs; hi - seq > 1;) { // the last sequence whose first tile is not behind this one
+            const int mid = (seq + hi) >> 1;
+            if (qe_attn_first_tile(qe_clamped(scalar_load(a.cu + mid), 0, a.n_tokens), mid, a.group, BM) <= place) seq = mid;
+            else hi = mid;
+        }
+        cu0 = scalar_load(a.cu + seq), cu1 = scalar_load(a.cu + seq + 1), kv = scalar_load(a.kv_len + seq);
+        local = place - qe_attn_first_tile(qe_clamped(cu0, 0, a.n_tokens), seq, a.group, BM);
     }
-    const int cu0 = scalar_load(a.cu + seq), cu1 = scalar_load(a.cu + seq + 1), kv = scalar_load(a.kv_len + seq);
     unsigned bad_len = 0;
     int begin, end;
     qe_rows_of(cu0, cu1, a.n_tokens, &begin, &end, &bad_len);
-    const int local = tile - qe_attn_first_tile(begin, seq, a.group, BM);
+    const int tile = qe_attn_first_tile(begin, seq, a.group, BM) + local;
     int len = qe_checked(kv, 0, a.max_pages << a.page_log2, 0, &bad_len);
     if (bad_len) len = 0; // no row has a position: zeros
     if ((bad_len || qe_bad_offsets(mine0, mine1, a.n_tokens)) && tid == 0) report(a.err, QE_BAD_LENGTH);

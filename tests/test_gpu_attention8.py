@@ -273,6 +273,42 @@ def test_prompt_bad_lengths_and_offsets_give_zeros_and_an_error(hq, hkv, dim, ct
             close(out[~gone], want[~gone], off[~gone])
 
 
+@pytest.mark.parametrize("n", [64, 65, 150])
+@pytest.mark.parametrize("hq,hkv,dim,codes", [(8, 2, 128, torch.int8), (4, 4, 64, torch.float8_e4m3fn), (16, 1, 256, torch.int8)])
+def test_prompt_of_many_sequences(hq, hkv, dim, codes, n):
+    """Tiles are begun in the order of their sequences' lengths, among up to 64 sequences: equal ones, and ones without rows."""
+    lens = [(7 * i) % 23 if i % 5 else 40 for i in range(n)]
+    ctx = [(31 * i) % 400 if i % 3 else 100 - lens[i] for i in range(n)]
+    c = Case8(hq, hkv, dim, 32, torch.bfloat16, codes, [a + b for a, b in zip(lens, ctx)])
+    cu = offsets(lens)
+    q = c.q(cu[-1])
+    want, off = Q.attend_batch(c, q, cu)
+    for max_len in (450, 20000):
+        out = torch.full_like(q, 7.0)
+        c.att.prompt8(c.batch(cu, max_len=max_len), q, c.cache(), out)
+        c.att.check()
+        close(out, want, off)
+
+
+@pytest.mark.parametrize("hq,hkv,dim,lens,ctx", [(32, 8, 128, [300, 500], [40, 0]), (8, 2, 64, [20, 300], [5000, 0]), (16, 2, 256, [30, 7], [6000, 0])])
+def test_prompt_and_decode_in_place(hq, hkv, dim, lens, ctx):
+    c = Case8(hq, hkv, dim, 64, torch.bfloat16, torch.int8, [a + b for a, b in zip(lens, ctx)])
+    cu = offsets(lens)
+    q = c.q(cu[-1])
+    out = torch.empty_like(q)
+    c.att.prompt8(c.batch(cu), q, c.cache(), out)
+    both = q.clone()
+    c.att.prompt8(c.batch(cu), both, c.cache(), both)
+    assert torch.equal(both, out)
+    q = c.q(2)
+    out = torch.empty_like(q)
+    c.att.decode8(c.batch(), q, c.cache(), out)
+    both = q.clone()
+    c.att.decode8(c.batch(), both, c.cache(), both)
+    assert torch.equal(both, out)
+    c.att.check()
+
+
 def in_halves(c, T, n_seqs, max_len):
     """Whether eight waves share a tile of such a call, as its plan has it."""
     tiles = (T * (c.hq // c.hkv) // 128 + n_seqs) * c.hkv
