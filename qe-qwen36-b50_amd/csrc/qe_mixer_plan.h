@@ -147,6 +147,10 @@ QE_MIX_HD int qe_attn_tile_splits(int n, int steps, int splits) {
 // A split of the shared keys costs its partial results, and saves the others time: P splits take about a prefix / P + b rows
 // P, which is least where P^2 is a / b times prefix / rows.  With a / b = 40, at most one workgroup a CU, and at least 64 keys,
 // 32 sequences of 16 heads of 256 behind 8000 take 34 us a call (36 with 60, 39 with 100), 8 behind 16,000 30 (29, 29).
+// A sequence's own positions: at least twelve steps a workgroup, or as few as make 768 workgroups if all are as long as the longest.
+// (32 sequences of 16 / 2 heads of 256 with up to 1500 of their own: 31.8 us a call, 33.4 with 512, 37.9 with 1024; 50 of 8 / 1 with up to
+// 1000: 25.9, 27.0, 26.4.  At least eight steps: 64 of 32 / 8 heads of 128 with up to 1000 46.9 for 42.2, but 40 of 24 / 8 of 64 with up to
+// 1500 26.7 for 29.1.)
 // Each leaves partial results, psplits + splits for a row of n_seqs * q_heads, which have room for QE_ATTN_SHARED_ROWS.  At
 // most 2^15 rows are in a launch (qe_attn_shared_seqs), so that each has room for two.
 #define QE_ATTN_SHARED_ROWS 65536
@@ -157,7 +161,7 @@ QE_MIX_HD int qe_attn_shared_seqs(int n_seqs, int q_heads) {
 }
 QE_MIX_HD void qe_attn_shared_plan(int n_seqs, int q_heads, int kv_heads, int64_t max_prefix, int64_t max_own, int *psplits, int *steps, int *splits) {
     const int64_t rows = (int64_t)n_seqs * q_heads, room = QE_ATTN_SHARED_ROWS / rows;
-    qe_attn_decode_cut(n_seqs, kv_heads, 512, 12, max_own, steps, splits);
+    qe_attn_decode_cut(n_seqs, kv_heads, 768, 12, max_own, steps, splits);
     if (*splits > (room + 1) / 2) *splits = (int)((room + 1) / 2);
     const int64_t tiles = ((int64_t)n_seqs * (q_heads / kv_heads) + QE_ATTN_SHARED_BM - 1) / QE_ATTN_SHARED_BM * kv_heads;
     const int64_t most = (max_prefix + 63) / 64, fill = (256 + tiles - 1) / tiles;
