@@ -185,9 +185,10 @@ int qe_attn_read8(qe_attn_ctx *ctx, const qe_attn_batch *batch, const qe_kv_cach
 
 /* qe_attn_prompt and qe_attn_decode over an 8-bit cache.  Products are as exact
  * as with a 16-bit cache, since codes are numbers of both 16-bit types; a key's
- * scale multiplies its score and a value's its probability, which is then
- * rounded to the context's type (fp16: to fixed steps below 2^-20, 2^-28 for
- * single tokens, of a row's greatest probability and the greatest scale).  A scale that is
+ * scale multiplies its score and a value's its probability, which is then, in
+ * prompts, rounded to the context's type (fp16: to fixed steps below 2^-20 of
+ * a row's greatest probability and the greatest scale), and for single tokens
+ * taken as two numbers of it.  A scale that is
  * not finite reaches the rows that attend to its position, and no others.  Of up to 64
  * sequences the longest are started first, in whatever order they are given. */
 int qe_attn_prompt8(qe_attn_ctx *ctx, const qe_attn_batch *batch, const qe_kv_cache8 *cache, const void *q, int64_t q_stride, void *out,

@@ -120,6 +120,7 @@ __global__ __launch_bounds__(64 * WAVES * HALVES, 2) void k_attn_prompt8(const Q
         if (t0 + HALVES < hi) stage.issue(x, page, kvh, (t0 + HALVES) * BN, len, wave, raw);
         page = page_of<BN, WAVES>(a, table, (t0 + 2 * HALVES) * BN, len, wave);
     }
+    const bool few = n_rows < BM && steps <= 8; // few rows of few keys: sum_rounded
     auto work = [&](int t, const short *k_lds, const short *v_lds, const float (*s_lds)[BN], short *k_next, short *v_next, float (*s_next)[BN]) {
         lds_barrier(); // the tile is there, and no wave reads the other buffers any more
         const int k0 = t * BN;
@@ -145,6 +146,10 @@ __global__ __launch_bounds__(64 * WAVES * HALVES, 2) void k_attn_prompt8(const Q
                 s.clear(again);
             }
             s.template pack<BF>(p);
+            if (few || (cut && k0 == 0)) // (in all cut tiles it would cost 4 to 8 % of 1000 tokens, for few rows of many keys 13 %)
+#pragma unroll
+                for (int b = 0; b < KB; ++b)
+                    sum_rounded<BF>(w.l, s, p, b, inverse_of<BF>(BF ? s_lds[1][b * 32 + at] : s_lds[1][b * 32 + at] * units.inverse));
             w.values(v_lds, 0, p);
             schedule<3, KB * DH / 16, 2>();
         }

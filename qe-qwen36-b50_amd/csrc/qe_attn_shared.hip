@@ -124,6 +124,7 @@ __device__ __forceinline__ void shared_prefix(const QeSharedArgs &y, int tile, i
         stage.land(lo * BN, len, wave, raw, k_a, v_a, s_a[0], s_a[1]);
         if (lo + 1 < hi) load(lo + 1, nullptr, nullptr);
     }
+    const bool few = n_rows < BM; // sum_rounded
     auto work = [&](int t, const short *k_lds, short *v_lds, const float (*s_lds)[BN], short *k_next, short *v_next, float (*s_next)[BN]) {
         const int k0 = t * BN;
         if constexpr (!CODES) {
@@ -151,6 +152,10 @@ __device__ __forceinline__ void shared_prefix(const QeSharedArgs &y, int tile, i
 #pragma unroll
                 for (int b = 0; b < KB; ++b) scaled(s.s[b], BF ? s_lds[1][b * 32 + at] : s_lds[1][b * 32 + at] * units.inverse);
                 s.template pack<BF>(p);
+                if (few)
+#pragma unroll
+                    for (int b = 0; b < KB; ++b)
+                        sum_rounded<BF>(w.l, s, p, b, inverse_of<BF>(BF ? s_lds[1][b * 32 + at] : s_lds[1][b * 32 + at] * units.inverse));
             } else {
                 w.exponentials(a.scale_log2, s, p);
             }

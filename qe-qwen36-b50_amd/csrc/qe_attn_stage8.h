@@ -78,3 +78,17 @@ __device__ __forceinline__ void scaled(qe_f16v &x, float s) {
         scaled<I + 1>(x, s);
     }
 }
+// The sum of the probabilities as they are rounded, in place of as they were: x are they times their values' scales s, p is x rounded.
+// A row's weights then sum to 1, and where one probability is nearly all, its rounding is in both and none of it in the result; a row
+// of one key is its value.  (Over many rows with many keys it changes little.)  Scales far below the greatest, whose products may be
+// too small for the type, are left out.
+template <bool BF, int I = 0, int KB>
+__device__ __forceinline__ void sum_rounded(float &l, const Scores<KB> &x, const Probs<KB> &p, int b, float inverse) {
+    if constexpr (I < 16) {
+        const float2 r = rest_of<BF>(p.p[b][I / 8].u[I % 8 / 2], x.s[b][I], x.s[b][I + 1]);
+        l = fmaf(-r.x, of_lane<I>(inverse), fmaf(-r.y, of_lane<I + 1>(inverse), l));
+        sum_rounded<BF, I + 2>(l, x, p, b, inverse);
+    }
+}
+template <bool BF>
+__device__ __forceinline__ float inverse_of(float s) { return s > (BF ? 0x1p-60f : 0x1p-6f) ? __builtin_amdgcn_rcpf(s) : 0.f; }

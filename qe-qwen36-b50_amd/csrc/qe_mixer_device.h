@@ -49,6 +49,11 @@ __device__ __forceinline__ float from16(short x) {
     else
         return (float)__builtin_bit_cast(_Float16, x);
 }
+// what pack2's rounding leaves of them, in 32 bits
+template <bool BF>
+__device__ __forceinline__ float2 rest_of(unsigned packed, float a, float b) {
+    return make_float2(a - from16<BF>((short)packed), b - from16<BF>((short)(packed >> 16)));
+}
 
 // Probabilities, rounded to the cache's type for the product with V, are kept 2^UP times as large where the type is fp16,
 // and so is their sum: fp16 has fixed steps below 2^-14 and nothing below 2^-25, and of 2^20 keys at 2^-25.1 of the

@@ -309,6 +309,30 @@ def test_prompt_and_decode_in_place(hq, hkv, dim, lens, ctx):
     c.att.check()
 
 
+@pytest.mark.parametrize("codes", CODES)
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("hq,hkv,dim", [(8, 2, 64), (32, 8, 128), (16, 1, 256)])
+def test_a_row_of_one_key_is_its_value(hq, hkv, dim, dtype, codes):
+    """But for the result's rounding.  Single tokens: a probability as two numbers of the type is off by U^2.  Prompts: its rounding is in the
+    weights' sum, too, which has a few roundings of 2^-24 and a reciprocal's 2^-23."""
+    n = 9
+    c = Case8(hq, hkv, dim, 16, dtype, codes, [1] * n)
+    q = c.q(n)
+    want = torch.stack([torch.cat([Q.rows_of(c, ((c.vc, c.vs),), i, h, 1)[0] for h in range(hkv)]) for i in range(n)]).repeat_interleave(hq // hkv, 1)
+    out = torch.empty_like(q)
+    c.att.decode8(c.batch(), q, c.cache(), out)
+    assert bool(((out.double() - want).abs() <= (Q.U[dtype] + 2 * Q.U[dtype] ** 2 + 2.0 ** -20) * want.abs() + 1e-7).all())
+    c.att.prompt8(c.batch(list(range(n + 1))), q, c.cache(), out)
+    assert bool(((out.double() - want).abs() <= (Q.U[dtype] + 2.0 ** -20) * want.abs() + 1e-7).all())
+    # the first rows of prompts, beside rows of more keys
+    c = Case8(hq, hkv, dim, 16, dtype, codes, [300, 70])
+    q, out = c.q(370), torch.empty(370, hq, dim, dtype=dtype, device="cuda")
+    c.att.prompt8(c.batch([0, 300, 370]), q, c.cache(), out)
+    for i, row in ((0, 0), (1, 300)):
+        want = torch.cat([Q.rows_of(c, ((c.vc, c.vs),), i, h, 1)[0] for h in range(hkv)]).repeat_interleave(hq // hkv, 0)
+        assert bool(((out[row].double() - want).abs() <= (Q.U[dtype] + 2.0 ** -20) * want.abs() + 1e-7).all())
+
+
 def in_halves(c, T, n_seqs, max_len):
     """Whether eight waves share a tile of such a call, as its plan has it."""
     tiles = (T * (c.hq // c.hkv) // 128 + n_seqs) * c.hkv
