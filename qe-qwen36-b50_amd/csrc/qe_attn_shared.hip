@@ -9,7 +9,7 @@
 //
 // A shared key has 2 group n flops for a byte or two (n sequences), so that the prefix is bound by its products from some hundred rows
 // on, and the own positions by memory.  Neither fills the GPU for long: 32 sequences behind 8000 positions, 16 / 2 heads of 256 in bf16, take
-// 27 us and 6 for the join, where their 69 MB take 14 and the sequences alone would read 577; 64 in three groups, 32 / 8 of 128, e4m3, 36
+// 26 us and 6 for the join, where their 69 MB take 14 and the sequences alone would read 577; 64 in three groups, 32 / 8 of 128, e4m3, 36
 // and 7 (90 MB); four behind 1000, int8, 8 and 4.  Launches of their own for the two kinds of work: 60 us for 34.
 #include "qe_attn_keys.h"
 #include "qe_attn_stage8.h"

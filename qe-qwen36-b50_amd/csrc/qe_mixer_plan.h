@@ -104,9 +104,9 @@ QE_MIX_HD int qe_attn_prompt_splits(int64_t tiles, int64_t max_len) {
 // of 128 unless other heads are named:
 //   129 to 256 tiles and more than 4 steps: 900 tokens 28 (two splits 40); 3 x 300 after 1500 47 (splits 73); 1100 of 16 / 16 heads
 //     of 64 24 (36).  Up to 128 tiles splits are as good (300 after 1000 30, 35 with eight waves);
-//   257 to 512 tiles and at least 16 steps: 1500 tokens 40 (four waves 49); 200, 333 and 967 after 0, 1700 and 0 63 (75); but equal
+//   257 to 512 tiles and at least 16 steps: 1500 tokens 40 (four waves 49); 200, 333 and 967 after 0, 1700 and 0 54 (65); but equal
 //     tiles, 4 x 400 after 2000, 108 (97).  With less steps the join is what they save: 6 x 256 after 256 36 (30);
-//   from 64 steps on a long tile among short ones needs splits: 256 and 800 after 4500 and 0 107 (splits 83);
+//   from 64 steps on a long tile among short ones needs splits: 256 and 800 after 4500 and 0 104 (splits 65);
 //   tiles that fill the GPU: 8000 tokens 702 (625);  heads of 256, whose join is 128 KB: 1000 tokens of 16 / 2 54 (44).
 QE_MIX_HD bool qe_attn_prompt8_halves(int64_t tiles, int bn, int64_t max_len) {
     const int64_t longest = (max_len + bn - 1) / bn;
