@@ -413,6 +413,52 @@ def test_prompt_in_halves_bad_pages_lengths_and_scales_of_any_size(hq, hkv, dim)
         close(out[rest], want[rest], off[rest])
 
 
+@pytest.mark.parametrize("hq,hkv,dim,max_len", [(32, 8, 128, 2000), (24, 8, 64, 2000), (16, 2, 256, 0), (8, 2, 128, 2000)])  # halves, and splits
+def test_prompts_captured_follow_lengths_and_offsets(hq, hkv, dim, max_len):
+    """Rows of 900 tokens, shared out anew among three sequences before each replay: the order in which tiles are begun changes, too."""
+    plans = [([300, 500, 100], [0, 0, 1500]), ([100, 0, 800], [1200, 300, 0]), ([1, 898, 1], [0, 900, 1990]), ([300, 500, 100], [0, 0, 1500])]
+    most = [max(p[0][i] + p[1][i] for p in plans) for i in range(3)]
+    c = Case8(hq, hkv, dim, 32, torch.float16, torch.int8, most)
+    kv, cu = ints(most), ints([0, 300, 800, 900])
+    batch = qe_mixer.Batch(kv, c.table, cu, max_len=max_len)
+    q = c.q(900)
+    out = torch.empty_like(q)
+    c.att.prompt8(batch, q, c.cache(), out)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        c.att.prompt8(batch, q, c.cache(), out, stream=torch.cuda.current_stream())
+    for lens, ctx in plans:
+        c.kv_len = [a + b for a, b in zip(lens, ctx)]
+        kv.copy_(ints(c.kv_len))
+        cu.copy_(ints(offsets(lens)))
+        out.fill_(7)
+        graph.replay()
+        torch.cuda.synchronize()
+        close(out, *Q.attend_batch(c, q, offsets(lens)))
+        eager = torch.empty_like(out)
+        c.att.prompt8(batch, q, c.cache(), eager)
+        assert torch.equal(eager, out)
+    c.att.check()
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+def test_values_of_zero_beside_great_ones(dtype):
+    """A row of zeros has the scale 0, and its share of a row's weights."""
+    for dim in (64, 128, 256):
+        c = Case8(8, 2, dim, 16, dtype, torch.int8, [200, 7, 90])
+        rows = torch.arange(c.page, device="cuda") % 3 == 0
+        c.vs[:, :, rows] = 0
+        c.vs[:, :, 1] *= 64
+        q = c.q(60)
+        out = torch.empty_like(q)
+        c.att.prompt8(c.batch([0, 40, 44, 60]), q, c.cache(), out)
+        close(out, *Q.attend_batch(c, q, [0, 40, 44, 60]))
+        c.att.decode8(c.batch(), q[:3], c.cache(), out[:3])
+        close(out[:3], *Q.attend_batch(c, q[:3], [0, 1, 2, 3]))
+        c.att.check()
+
+
 def test_far_offsets_in_a_large_cache():
     """Pages whose codes start past 2^32 bytes."""
     hkv, dim, page = 2, 256, 256
