@@ -187,8 +187,8 @@ int qe_attn_read8(qe_attn_ctx *ctx, const qe_attn_batch *batch, const qe_kv_cach
  * as with a 16-bit cache, since codes are numbers of both 16-bit types; a key's
  * scale multiplies its score and a value's its probability, which is then, in
  * prompts, rounded to the context's type (fp16: to fixed steps below 2^-20 of
- * a row's greatest probability and the greatest scale), and for single tokens
- * taken as two numbers of it.  A scale that is
+ * a row's greatest probability and the greatest scale of the positions that it
+ * attends to), and for single tokens taken as two numbers of it.  A scale that is
  * not finite reaches the rows that attend to its position, and no others.  Of up to 64
  * sequences the longest are started first, in whatever order they are given. */
 int qe_attn_prompt8(qe_attn_ctx *ctx, const qe_attn_batch *batch, const qe_kv_cache8 *cache, const void *q, int64_t q_stride, void *out,

@@ -5,7 +5,7 @@
 // wave loads its part of the next tile's codes while this one is worked on, turns them to 16 bits when its work is done,
 // and writes them to the other of two buffers, so that a code is turned once for all rows of a workgroup.  With heads of 256
 // the registers are full: there the codes wait in a few KB of LDS, by direct loads.  A key's scale multiplies its scores and a
-// value's its probabilities (in fp16 in units of theirs: Units), from one register: lane n of 16 has the scale of the n-th
+// value's its probabilities (in fp16 in units of theirs: RowUnits), from one register: lane n of 16 has the scale of the n-th
 // of the 16 keys in the lane's registers.  Where tiles are few, eight waves share a tile's rows, four for the even steps and four for
 // the odd ones (HALVES, qe_attn_prompt8_halves), and join their sums in LDS.
 #include "qe_attn_stage8.h"
@@ -89,7 +89,7 @@ __global__ __launch_bounds__(64 * WAVES * HALVES, 2) void k_attn_prompt8(const Q
         page = page_of<BN, WAVES>(a, table, (t0 + HALVES) * BN, len, wave);
     }
     Rows<BF, DH> w;
-    Units units;
+    RowUnits<BF> units;
     {
         const int row = wave_row + (tid & 31), h = tid >> 5 & 1;
         const bool there = row < n_rows;
@@ -132,24 +132,36 @@ __global__ __launch_bounds__(64 * WAVES * HALVES, 2) void k_attn_prompt8(const Q
 #pragma unroll
             for (int b = 0; b < KB; ++b) scaled(s.s[b], s_lds[0][b * 32 + at]);
             const bool cut = k0 + BN > wave_clear;
-            const int limit = w.place - k0 - 4 * (lane >> 5);
-            if (cut) s.mask(limit);
+            // The last key that the row attends to, counted from the lane's first; made anew in each branch, since of one number the
+            // compiler makes all comparisons in every step (637 us for 614 at 8000 tokens).
+            auto limit = [&] {
+                int x = w.place - k0 - 4 * (lane >> 5);
+                asm volatile("" : "+v"(x));
+                return x;
+            };
+            if (cut) s.mask(limit());
             w.raise(s.top() * a.scale_log2);
-            if constexpr (!BF) w.times(units.raise(s_lds[1][lane & (BN - 1)]));
-            Probs<KB> p;
-            w.weigh(a.scale_log2, s);
+            if constexpr (!BF) {
+                unsigned top = 0;
+                if (cut) {
+                    const int last = limit();
 #pragma unroll
-            for (int b = 0; b < KB; ++b) scaled(s.s[b], BF ? s_lds[1][b * 32 + at] : s_lds[1][b * 32 + at] * units.inverse);
-            if (cut) { // a scale that is not finite reaches the rows that attend to its position
-                int again = limit;
-                asm volatile("" : "+v"(again)); // else the compiler makes these comparisons in every step: 637 us for 614 at 8000 tokens
-                s.clear(again);
+                    for (int b = 0; b < KB; ++b) top = max(top, greatest_seen(size_bits(s_lds[1][b * 32 + at]), b, last));
+                    const auto halves = __builtin_amdgcn_permlane32_swap(top, top, false, false);
+                    top = max(halves[0], halves[1]);
+                } else {
+                    top = greatest(size_bits(s_lds[1][lane & (BN - 1)]));
+                }
+                units.raise(top, w);
             }
+            Probs<KB> p;
+            w.weigh(a.scale_log2, BF ? 0.f : units.log2, s);
+#pragma unroll
+            for (int b = 0; b < KB; ++b) scaled(s.s[b], s_lds[1][b * 32 + at]);
+            if (cut) s.clear(limit()); // a scale that is not finite reaches the rows that attend to its position
             s.template pack<BF>(p);
             if (few || (cut && k0 == 0)) // (in all cut tiles it would cost 4 to 8 % of 1000 tokens, for few rows of many keys 13 %)
-#pragma unroll
-                for (int b = 0; b < KB; ++b)
-                    sum_rounded<BF>(w.l, s, p, b, inverse_of<BF>(BF ? s_lds[1][b * 32 + at] : s_lds[1][b * 32 + at] * units.inverse));
+                sum_rounded(w.l, s, p, s_lds[1] + at, units);
             w.values(v_lds, 0, p);
             schedule<3, KB * DH / 16, 2>();
         }
@@ -163,7 +175,7 @@ __global__ __launch_bounds__(64 * WAVES * HALVES, 2) void k_attn_prompt8(const Q
         work(t + half, k_a[half], v_a[half], s_a[half], k_b[half], v_b[half], s_b[half]);
         if (t + HALVES < hi) work(t + HALVES + half, k_b[half], v_b[half], s_b[half], k_a[half], v_a[half], s_a[half]);
     }
-    if constexpr (!BF) w.times(units.unit);
+    if constexpr (!BF) w.times(units.unit());
     if constexpr (HALVES == 2) { // the second half's sums, through the tiles' LDS
         constexpr int LOT = 64 * WAVES * 16, LOTS = HALVES * BN * DH / 2 / LOT; // floats of 32 columns; these that an array has room for
         static_assert(LOTS >= 1 && 4 * LOTS * 32 >= DH, "room for all columns");

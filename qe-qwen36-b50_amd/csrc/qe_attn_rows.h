@@ -175,16 +175,16 @@ struct Rows {
             }
         l += sum[0] + sum[1];
     }
-    // O counts other units: Units::raise
+    // the sums count other units: RowUnits
     __device__ __forceinline__ void times(float f) {
-        if (f != 1.f)
 #pragma unroll
-            for (int d = 0; d < DH / 32; ++d) o[d] *= f;
+        for (int d = 0; d < DH / 32; ++d) o[d] *= f;
+        l *= f;
     }
-    // the scores become probabilities, not rounded yet
+    // the scores become probabilities, not rounded yet; in units of 2^unit
     template <int KB>
-    __device__ __forceinline__ void weigh(float scale, Scores<KB> &x) {
-        const float base = exponent_base<BF, LAG>(m);
+    __device__ __forceinline__ void weigh(float scale, float unit, Scores<KB> &x) {
+        const float base = exponent_base<BF, LAG>(m) - unit;
         float sum[2] = {0, 0};
 #pragma unroll
         for (int b = 0; b < KB; ++b)

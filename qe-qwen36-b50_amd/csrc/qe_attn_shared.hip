@@ -106,7 +106,7 @@ __device__ __forceinline__ void shared_prefix(const QeSharedArgs &y, int tile, i
     };
     load(lo, k_a, v_a);
     Rows<BF, DH> w;
-    Units units;
+    RowUnits<BF> units;
     {
         const short *q = (const short *)a.q + (size_t)seq * a.q_stride + (size_t)head * DH + (tid >> 5 & 1) * 8;
 #pragma unroll
@@ -147,15 +147,12 @@ __device__ __forceinline__ void shared_prefix(const QeSharedArgs &y, int tile, i
             w.raise(s.top() * a.scale_log2);
             Probs<KB> p;
             if constexpr (CODES) {
-                if constexpr (!BF) w.times(units.raise(s_lds[1][lane & (BN - 1)]));
-                w.weigh(a.scale_log2, s);
+                if constexpr (!BF) units.raise(greatest(size_bits(s_lds[1][lane & (BN - 1)])), w);
+                w.weigh(a.scale_log2, BF ? 0.f : units.log2, s);
 #pragma unroll
-                for (int b = 0; b < KB; ++b) scaled(s.s[b], BF ? s_lds[1][b * 32 + at] : s_lds[1][b * 32 + at] * units.inverse);
+                for (int b = 0; b < KB; ++b) scaled(s.s[b], s_lds[1][b * 32 + at]);
                 s.template pack<BF>(p);
-                if (few)
-#pragma unroll
-                    for (int b = 0; b < KB; ++b)
-                        sum_rounded<BF>(w.l, s, p, b, inverse_of<BF>(BF ? s_lds[1][b * 32 + at] : s_lds[1][b * 32 + at] * units.inverse));
+                if (few) sum_rounded(w.l, s, p, s_lds[1] + at, units);
             } else {
                 w.exponentials(a.scale_log2, s, p);
             }
@@ -172,7 +169,7 @@ __device__ __forceinline__ void shared_prefix(const QeSharedArgs &y, int tile, i
         work(t, k_a, v_a, s_a, k_b, v_b, s_b);
         if (t + 1 < hi) work(t + 1, k_b, v_b, s_b, k_a, v_a, s_a);
     }
-    if constexpr (CODES && !BF) w.times(units.unit);
+    if constexpr (CODES && !BF) w.times(units.unit());
     bad = __syncthreads_or(bad);
     if (bad && tid == 0) report(a.err, QE_BAD_PAGE);
     const float sum = w.l + __shfl_xor(w.l, 32);

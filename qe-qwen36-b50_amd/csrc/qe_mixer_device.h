@@ -213,6 +213,23 @@ template <int I>
 __device__ __forceinline__ float of_lane(float x) {
     return __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(x), 0x150 + I, 0xf, 0xf, true));
 }
+// A scale's bits without sign, in the order of their sizes; none of one that is not finite, which reaches the rows that attend to it
+// without this.
+__device__ __forceinline__ unsigned size_bits(float scale) {
+    const unsigned x = __float_as_uint(scale) & 0x7fffffffu;
+    return x >= 0x7f800000u ? 0 : x;
+}
+// The greatest over all lanes.
+__device__ __forceinline__ unsigned greatest(unsigned top) {
+    top = max(top, (unsigned)__builtin_amdgcn_update_dpp(0, (int)top, 0xb1, 0xf, 0xf, true));
+    top = max(top, (unsigned)__builtin_amdgcn_update_dpp(0, (int)top, 0x4e, 0xf, 0xf, true));
+    top = max(top, (unsigned)__builtin_amdgcn_update_dpp(0, (int)top, 0x141, 0xf, 0xf, true));
+    top = max(top, (unsigned)__builtin_amdgcn_update_dpp(0, (int)top, 0x140, 0xf, 0xf, true));
+    const auto a = __builtin_amdgcn_permlane16_swap(top, top, false, false);
+    top = max(a[0], a[1]);
+    const auto b = __builtin_amdgcn_permlane32_swap(top, top, false, false);
+    return __builtin_amdgcn_readfirstlane(max(b[0], b[1]));
+}
 // The value scales of an 8-bit cache as fp16 probabilities can take them: a probability times a scale has no bounded range, but
 // times scale / unit it has, where unit is a power of two that is above all scales so far.  The sums with V count units; they are
 // brought to a new one where a tile has a greater scale.  (bf16 has the range of 32 bits and needs none.)
@@ -220,17 +237,7 @@ struct Units {
     float unit = 0, inverse = 0;
     // `scale`, over all lanes: a tile's; those of fewer lanes are in others, too.  What sums so far are to be multiplied by.
     __device__ __forceinline__ float raise(float scale) {
-        // (one that is not finite reaches the rows that attend to it without this; positive numbers' bits are in their order)
-        unsigned top = __float_as_uint(scale) & 0x7fffffffu;
-        if (top >= 0x7f800000u) top = 0;
-        top = max(top, (unsigned)__builtin_amdgcn_update_dpp(0, (int)top, 0xb1, 0xf, 0xf, true));
-        top = max(top, (unsigned)__builtin_amdgcn_update_dpp(0, (int)top, 0x4e, 0xf, 0xf, true));
-        top = max(top, (unsigned)__builtin_amdgcn_update_dpp(0, (int)top, 0x141, 0xf, 0xf, true));
-        top = max(top, (unsigned)__builtin_amdgcn_update_dpp(0, (int)top, 0x140, 0xf, 0xf, true));
-        const auto a = __builtin_amdgcn_permlane16_swap(top, top, false, false);
-        top = max(a[0], a[1]);
-        const auto b = __builtin_amdgcn_permlane32_swap(top, top, false, false);
-        const unsigned bits = __builtin_amdgcn_readfirstlane(max(b[0], b[1]));
+        const unsigned bits = greatest(size_bits(scale));
         if (__uint_as_float(bits) <= unit) return 1.f;
         // two to four times the greatest, so that it seldom changes; within 2^-100 .. 2^100
         unsigned e = (bits >> 23) + 2;
