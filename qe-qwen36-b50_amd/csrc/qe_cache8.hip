@@ -25,9 +25,22 @@ __device__ __forceinline__ void load8(const IN *p, float *x) {
     }
 }
 
-// 8 values times inv to codes
+// x / s as 32 bits have it, for s in [1, 2) and its reciprocal to nearest: next to a border between two codes the product with a
+// reciprocal would give the other one.  One correction by the remainder, which fmaf has exactly, makes the quotient one of the two floats next to
+// x / s; a second rounds it to nearest (P. Markstein, Computation of elementary functions on the IBM RISC System/6000, 1990).
+__device__ __forceinline__ float over(float x, float s, float inv) {
+    float q = x * inv;
+    q = fmaf(fmaf(-q, s, x), inv, q);
+    return fmaf(fmaf(-q, s, x), inv, q);
+}
+// 8 values over their row's scale to codes
 template <int CT>
-__device__ __forceinline__ uint2 codes8(const float *x, float inv) {
+__device__ __forceinline__ uint2 codes8(const float *x, float scale) {
+    // both by a power of two that brings the scale to [1, 2), so that no remainder is too small for 32 bits
+    const float up = __uint_as_float((254u << 23) - (__float_as_uint(scale) & 0x7f800000u)), s = scale * up, inv = 1.f / s;
+    float y[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) y[i] = over(x[i] * up, s, inv);
     unsigned w[2];
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
@@ -35,12 +48,12 @@ __device__ __forceinline__ uint2 codes8(const float *x, float inv) {
             // added to 1.5 2^23, a number's last bits are its nearest integer
             unsigned b[4];
 #pragma unroll
-            for (int i = 0; i < 4; ++i) b[i] = __float_as_uint(fmaf(x[4 * h + i], inv, 12582912.f));
+            for (int i = 0; i < 4; ++i) b[i] = __float_as_uint(y[4 * h + i] + 12582912.f);
             w[h] = __builtin_amdgcn_perm(__builtin_amdgcn_perm(b[3], b[2], 0x0c0c0400), __builtin_amdgcn_perm(b[1], b[0], 0x0c0c0400), 0x05040100);
         } else {
             int v = 0;
-            v = __builtin_amdgcn_cvt_pk_fp8_f32(x[4 * h] * inv, x[4 * h + 1] * inv, v, false);
-            v = __builtin_amdgcn_cvt_pk_fp8_f32(x[4 * h + 2] * inv, x[4 * h + 3] * inv, v, true);
+            v = __builtin_amdgcn_cvt_pk_fp8_f32(y[4 * h], y[4 * h + 1], v, false);
+            v = __builtin_amdgcn_cvt_pk_fp8_f32(y[4 * h + 2], y[4 * h + 3], v, true);
             w[h] = (unsigned)v;
         }
     }
@@ -150,14 +163,15 @@ __global__ __launch_bounds__(256) void k_append8(const QeAppend8Args x) {
 #pragma unroll
             for (int i = 0; i < 16; ++i) top = max(top, __float_as_uint(u[i]) & 0x7fffffffu);
             top = max_over<PER>(top);
-            float scale = __uint_as_float(top) / (CT == QE_I8 ? 127.f : 448.f), inv = __builtin_amdgcn_rcpf(scale);
-            if (top < 0x0d800000u) scale = 0, inv = 0; // below 2^-100
+            float scale = __uint_as_float(top) / (CT == QE_I8 ? 127.f : 448.f);
             uint2 lo = make_uint2(0, 0), hi = lo;
-            if (top >= 0x7f800000u) {
+            if (top < 0x0d800000u) { // below 2^-100
+                scale = 0;
+            } else if (top >= 0x7f800000u) {
                 scale = NAN;
             } else {
-                lo = codes8<CT>(u, inv);
-                hi = codes8<CT>(u + 8, inv);
+                lo = codes8<CT>(u, scale);
+                hi = codes8<CT>(u + 8, scale);
             }
             uint8_t *dst = (uint8_t *)(m.kind == 1 ? a.kc : a.vc) + row * DH;
             *(uint2 *)(dst + m.e0) = lo;
