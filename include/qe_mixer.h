@@ -212,7 +212,8 @@ typedef struct {
     int n_groups;          /* 1 .. 65535 */
     const int32_t *seqs;   /* device [n_groups + 1] */
     const int32_t *prefix; /* device [n_groups] */
-    int max_prefix;        /* the greatest prefix as far as the host knows, for choosing splits; 0 = the longest length */
+    int max_prefix;        /* the greatest prefix as far as the host knows, for choosing splits, as batch->max_len is: their
+                              difference is taken for the longest part that a sequence has to itself; 0 = not known */
 } qe_attn_shared;
 
 /* qe_attn_decode and qe_attn_decode8 of such sequences: a group's shared keys and

@@ -269,7 +269,9 @@ __global__ __launch_bounds__(256, 2) void k_shared(const QeSharedArgs y) {
             if (!AHEAD || sizeof k_a / 2 >= 64 * DH) return (float *)buffer(w, 0) + h * DH;
             return (float *)buffer(w, h >> 3) + (h & 7) * DH;
         };
-        shared_own<BF, DH, CT, AHEAD>(y, at / a.splits, at % a.splits, buffer(wave, 0), buffer(wave, 1), row, ml);
+        // all sequences' first splits, then their second ones: those that have no keys end the launch
+        const int items = (y.seq1 - y.seq0) * a.kv_heads;
+        shared_own<BF, DH, CT, AHEAD>(y, at % items, at / items, buffer(wave, 0), buffer(wave, 1), row, ml);
     }
 }
 

@@ -151,6 +151,12 @@ QE_MIX_HD int qe_attn_tile_splits(int n, int steps, int splits) {
 // (32 sequences of 16 / 2 heads of 256 with up to 1500 of their own: 31.8 us a call, 33.4 with 512, 37.9 with 1024; 50 of 8 / 1 with up to
 // 1000: 25.9, 27.0, 26.4.  At least eight steps: 64 of 32 / 8 heads of 128 with up to 1000 46.9 for 42.2, but 40 of 24 / 8 of 64 with up to
 // 1500 26.7 for 29.1.)
+// That is planned for max_own, the longest own part as far as the hints tell: the difference of the longest length and the longest prefix, or,
+// where not both are stated, 0 (not known: eight steps a workgroup).  It may be wrong, for a sequence behind a shorter prefix or of no group
+// may have far more of its own: there are workgroups for up to max_len positions, of at least as many steps, as long as these are 1024 in
+// all, and those that a sequence has no use for end at once.  They come last in the launch.  (One of 30,000 positions beside eight that have ten each
+// behind 30,000, 16 / 2 heads of 256: 37 us a call, 440 with workgroups for max_own alone; four of 2000 beside ten behind 16,000: 30, 43.  32
+// behind 8000 without a hint: 30, 47, and 31 with hints either way; with 2048 workgroups 31.5, and 44 where those without keys come among the others.)
 // Each leaves partial results, psplits + splits for a row of n_seqs * q_heads, which have room for QE_ATTN_SHARED_ROWS.  At
 // most 2^15 rows are in a launch (qe_attn_shared_seqs), so that each has room for two.
 #define QE_ATTN_SHARED_ROWS 65536
@@ -159,9 +165,14 @@ QE_MIX_HD int qe_attn_shared_seqs(int n_seqs, int q_heads) {
     const int most = QE_ATTN_SHARED_ROWS / 2 / q_heads;
     return n_seqs < most ? n_seqs : most;
 }
-QE_MIX_HD void qe_attn_shared_plan(int n_seqs, int q_heads, int kv_heads, int64_t max_prefix, int64_t max_own, int *psplits, int *steps, int *splits) {
+QE_MIX_HD void qe_attn_shared_plan(int n_seqs, int q_heads, int kv_heads, int64_t max_prefix, int64_t max_own, int *psplits, int *steps, int *splits,
+                                    int64_t max_len = 0) {
     const int64_t rows = (int64_t)n_seqs * q_heads, room = QE_ATTN_SHARED_ROWS / rows;
-    qe_attn_decode_cut(n_seqs, kv_heads, 768, 12, max_own, steps, splits);
+    *steps = 8, *splits = 1;
+    if (max_own > 0) qe_attn_decode_cut(n_seqs, kv_heads, 768, 12, max_own, steps, splits);
+    const int64_t longest = (max_len + (int64_t)QE_ATTN_TILE * *steps - 1) / ((int64_t)QE_ATTN_TILE * *steps), most_wgs = 1024 / ((int64_t)n_seqs * kv_heads);
+    const int64_t more = longest < most_wgs ? longest : most_wgs;
+    if (more > *splits) *splits = (int)more;
     if (*splits > (room + 1) / 2) *splits = (int)((room + 1) / 2);
     const int64_t tiles = ((int64_t)n_seqs * (q_heads / kv_heads) + QE_ATTN_SHARED_BM - 1) / QE_ATTN_SHARED_BM * kv_heads;
     const int64_t most = (max_prefix + 63) / 64, fill = (256 + tiles - 1) / tiles;
