@@ -264,11 +264,8 @@ __global__ __launch_bounds__(256, 2) void k_shared(const QeSharedArgs y) {
             if (!AHEAD) return (uint8_t *)(w < 2 ? w == 0 ? k_a : v_a : w == 2 ? k_b : v_b);
             return (uint8_t *)(second ? w < 2 ? k_b : v_b : w < 2 ? k_a : v_a) + (w & 1) * (sizeof k_a / 2);
         };
-        // and for its results: sixteen heads' in one, or eight in each
-        auto row = [&](int w, int h) {
-            if (!AHEAD || sizeof k_a / 2 >= 64 * DH) return (float *)buffer(w, 0) + h * DH;
-            return (float *)buffer(w, h >> 3) + (h & 7) * DH;
-        };
+        static_assert(!AHEAD || sizeof k_a / 2 >= 64 * DH, "room in one of two for sixteen heads' results");
+        auto row = [&](int w, int h) { return (float *)buffer(w, 0) + h * DH; };
         // all sequences' first splits, then their second ones: those that have no keys end the launch
         const int items = (y.seq1 - y.seq0) * a.kv_heads;
         shared_own<BF, DH, CT, AHEAD>(y, at % items, at / items, buffer(wave, 0), buffer(wave, 1), row, ml);
