@@ -66,8 +66,9 @@ typedef struct {
 
 typedef struct qe_attn_ctx qe_attn_ctx;
 
-/* Create a context on `device`: scratch of a fixed size (35 to 135 MB)
- * for the partial results of calls that split a sequence's length. */
+/* Create a context on `device`: scratch of a fixed size (35, 68 or 135 MB with
+ * heads of 64, 128 or 256) for the partial results of calls that split a
+ * sequence's length; half of it is for prompts over an 8-bit cache alone. */
 int qe_attn_create(int device, const qe_attn_desc *desc, qe_attn_ctx **out);
 int qe_attn_destroy(qe_attn_ctx *ctx);
 

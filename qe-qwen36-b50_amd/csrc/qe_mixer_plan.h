@@ -119,7 +119,11 @@ QE_MIX_HD bool qe_attn_prompt8_halves(int64_t tiles, int bn, int64_t max_len) {
 // of 128, int8: 600 tokens after 20,000 337 us with 1.5 times, 307 with twice and with three times, 599 without; 50, 700 and 20
 // after 5000, 0 and 19,000 of 24 / 8 heads of 64 107, 87 and 88, 406 without).  Where tiles fill half of the places and none has 40
 // steps the join costs as much as it saves (4 x 400 after 2000 103 us without, 122 with; 1500 tokens 53 and 65).
-#define QE_ATTN_PROMPT8_ROWS 131072 /* of partial results */
+// Partial results are of whole tiles, and there is room for 131,072 rows of them, twice what the other calls need: a long tile among short
+// ones is cut into as many splits as there are for all.  (int8; with 65,536 rows: 256 and 800 after 4500 and 0 67 -> 135 us, 100 and 400
+// after 30,000 and 1000 of 16 / 2 heads of 256 120 -> 222, 300 and 900 after 20,000 and 0 207 -> 552, 1500 after 10,000 of 24 / 8 of 64 205 -> 298,
+// but 600 after 20,000 288 -> 285, 300 after 8000 81 -> 74, 800 after 30,000 of 16 / 2 of 256 463 -> 451; 98,304 are between or worse.)
+#define QE_ATTN_PROMPT8_ROWS 131072
 QE_MIX_HD void qe_attn_prompt8_plan(int64_t tiles, int bm, int bn, int64_t max_len, int *steps, int *splits) {
     const int64_t longest = (max_len + bn - 1) / bn, places = bm == 256 ? 256 : 512, room = QE_ATTN_PROMPT8_ROWS / (tiles * bm);
     int64_t per = (longest * tiles + 2 * places - 1) / (2 * places);
