@@ -104,6 +104,8 @@ hipError_t qe_launch_append(const QeAppendArgs &a, int in_type, int type, hipStr
 // 37 us, 5.5 TB/s, and 5 for the join; 24 sequences of 38 to 8,095 keys, eight heads of 128, fp16, 339 MB: 70 us,
 // 4.8 TB/s.  Short ones by latency: 700 keys take 10 us (length and page, keys and values, the exchange through
 // memory, the join), where a launch that does nothing takes 2.
+// With heads of 64 at most five workgroups are on a CU: with six, which 80 registers allow, the longest of ragged sequences start later beside more of the
+// others (24 of 38 to 8,095 keys, 24 / 8 heads, 40.2 -> 44.2 us; 40 of up to 9000, 12 heads, 97 -> 107; equal ones 1 to 3 % faster).
 // ---------------------------------------------------------------------------
 template <int DH>
 __device__ __forceinline__ int v_swizzle(int row) { // of the 16-byte chunk index
@@ -111,7 +113,7 @@ __device__ __forceinline__ int v_swizzle(int row) { // of the 16-byte chunk inde
 }
 
 template <bool BF, int DH, bool ONCE>
-__global__ __launch_bounds__(256, 2) void k_attn_decode(const QeAttnArgs a) {
+__global__ __attribute__((amdgpu_flat_work_group_size(256, 256), amdgpu_waves_per_eu(2, DH == 64 ? 5 : 8))) void k_attn_decode(const QeAttnArgs a) {
     constexpr int CH = DH / 8;       // 16-byte chunks of a row
     constexpr int ROWS = 64 / CH;    // rows of one direct load
     constexpr int KS = DH / 32, DB = DH / 16;
