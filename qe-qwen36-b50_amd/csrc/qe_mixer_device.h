@@ -119,11 +119,11 @@ struct QeToken {
     long row;     // of key-value head 0 among all rows of the cache; -1 where place is below 0
     bool in_call; // of a sequence, as far as is known
 };
-// All sequences' offsets are looked at, for the report: those that are wrong may hold no token.
+// All sequences' offsets are looked at, for the report: those that are wrong may hold no token.  (Workgroups of 256 threads.)
 template <typename ARGS>
 __device__ __forceinline__ void report_offsets(const ARGS &a) {
-    if (a.cu)
-        for (int64_t i = (int64_t)blockIdx.x * blockDim.x + threadIdx.x; i < a.n_seqs; i += (int64_t)gridDim.x * blockDim.x)
+    if (a.cu && (int64_t)blockIdx.x * 256 < a.n_seqs)
+        for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < a.n_seqs; i += (int64_t)gridDim.x * 256)
             if (qe_bad_offsets(a.cu[i], a.cu[i + 1], a.n_tokens)) report(a.err, QE_BAD_LENGTH);
 }
 // Token t's, by every wave for itself, through the scalar cache, with no barrier.  False: it has none; `teller` reports why.
