@@ -26,8 +26,9 @@ __global__ __launch_bounds__(64 * WAVES * HALVES, 2) void k_attn_prompt8(const Q
     __shared__ float s_a[HALVES][2][BN], s_b[HALVES][2][BN];
     const int tid = threadIdx.x, thread_wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int half = HALVES == 1 ? 0 : thread_wave / WAVES, wave = thread_wave - half * WAVES;
-    const int split = blockIdx.x % a.splits, kvh = blockIdx.x / a.splits % a.kv_heads;
-    const int rank = blockIdx.x / a.splits / a.kv_heads; // of the workgroup's tile, in the order in which they are begun
+    const int beside = x.spread ? 1 : a.splits; // splits of a tile that are begun one after the other
+    const int split = blockIdx.x % beside + blockIdx.y, kvh = blockIdx.x / beside % a.kv_heads;
+    const int rank = blockIdx.x / beside / a.kv_heads; // of the workgroup's tile, in the order in which they are begun
     // workgroup i looks at sequence i's offsets, for the report: where they fall, a sequence may have no tile below
     const int mine = blockIdx.x < (unsigned)a.n_seqs ? blockIdx.x : a.n_seqs - 1;
     const int mine0 = scalar_load(a.cu + mine), mine1 = scalar_load(a.cu + mine + 1);
@@ -260,7 +261,7 @@ template <bool BF, int DH, int CT, int WAVES, int HALVES>
 static hipError_t launch_waves8(const QeAttn8Args &x, hipStream_t st) {
     constexpr int BM = 32 * WAVES, BN = Stage<CT, BF, DH, WAVES>::BN;
     const unsigned items = (unsigned)(x.a.tiles * x.a.kv_heads);
-    k_attn_prompt8<BF, DH, CT, WAVES, HALVES><<<dim3(items * x.a.splits), dim3(64 * WAVES * HALVES), 0, st>>>(x);
+    k_attn_prompt8<BF, DH, CT, WAVES, HALVES><<<x.spread ? dim3(items, x.a.splits) : dim3(items * x.a.splits), dim3(64 * WAVES * HALVES), 0, st>>>(x);
     // few tiles: fewer rows a workgroup
     if (x.a.splits > 1 && items >= 128) k_attn_prompt8_join<BF, DH, BM, BN, 32><<<dim3(items * (BM / 32)), dim3(256), 0, st>>>(x.a);
     else if (x.a.splits > 1) k_attn_prompt8_join<BF, DH, BM, BN, 4><<<dim3(items * (BM / 4)), dim3(256), 0, st>>>(x.a);

@@ -63,6 +63,7 @@ struct QeRead8Args {
 struct QeAttn8Args {
     QeAttnArgs a;
     const float *ks, *vs; // scales
+    bool spread;          // prompts: all tiles' first splits before their second ones (qe_attn_prompt8_blind)
 };
 
 // Sequences that share beginnings: `x` with kc, vc and, of an 8-bit cache, scales; x.a.splits and x.a.steps of their own

@@ -395,10 +395,17 @@ int qe_attn_prompt8(qe_attn_ctx *c, const qe_attn_batch *b, const qe_kv_cache8 *
     if ((rc = plan_prompt(c, b, where, &x.a, &bm, &max_len)) != QE_OK) return rc;
     const int64_t items = (int64_t)x.a.tiles * x.a.kv_heads;
     const int bn = c->d.head_dim == 256 ? 32 : 64;
-    qe_attn_prompt8_plan(items, bm, bn, max_len, &x.a.steps, &x.a.splits);
+    x.spread = !b->max_len;
+    bool halves;
+    if (x.spread) {
+        halves = qe_attn_prompt8_blind(items, bm, bn, b->n_tokens, max_len, &x.a.steps, &x.a.splits);
+    } else {
+        halves = qe_attn_prompt8_halves(items, bn, max_len);
+        qe_attn_prompt8_plan(items, bm, bn, max_len, &x.a.steps, &x.a.splits);
+    }
     OnDevice on(c->device);
     HIP_TRY(on.e);
-    HIP_TRY(qe_launch_attn_prompt8(x, c->d.head_dim, c->d.type, kv->type, bm, qe_attn_prompt8_halves(items, bn, max_len), (hipStream_t)stream));
+    HIP_TRY(qe_launch_attn_prompt8(x, c->d.head_dim, c->d.type, kv->type, bm, halves, (hipStream_t)stream));
     return QE_OK;
 }
 

@@ -135,6 +135,25 @@ QE_MIX_HD void qe_attn_prompt8_plan(int64_t tiles, int bm, int bn, int64_t max_l
     *steps = (int)per;
     *splits = (int)s;
 }
+// The same where the host says nothing of the lengths, and a table may have room for far more than any sequence has: planned as if the
+// call's tokens were all that there is, with splits (of at least 40 steps where tiles alone fill the places) for tiles that turn out to have more
+// steps, as long as these are 1024 workgroups.  All tiles' first splits are begun before the second ones, which may all have none.  (Tables of
+// 262,144 positions, int8, 32 / 8 heads of 128, us a call with lengths stated, without, and without as if all were as long as the table: 900
+// tokens 28, 30, 56; 1000 of 16 / 2 heads of 256 44, 43, 104; 200, 333 and 967 after 0, 1700 and 0 51, 54, 70; 300 after 1000 29, 32, 59;
+// 600 after 20,000 285, 325, 796; 256 and 800 after 4500 and 0 67, 85, 138; 30 after 10,000 of 16 / 2 of 256 34, 33, 85.)
+// Whether a workgroup has eight waves.
+QE_MIX_HD bool qe_attn_prompt8_blind(int64_t tiles, int bm, int bn, int64_t n_tokens, int64_t max_len, int *steps, int *splits) {
+    const int64_t likely = n_tokens < max_len ? n_tokens : max_len;
+    const bool halves = qe_attn_prompt8_halves(tiles, bn, likely);
+    qe_attn_prompt8_plan(tiles, bm, bn, likely, steps, splits);
+    if ((halves || 2 * tiles > (bm == 256 ? 256 : 512)) && *steps < 40) *steps = 40;
+    const int64_t longest = (max_len + bn - 1) / bn, room = QE_ATTN_PROMPT8_ROWS / (tiles * bm), most = 1024 / tiles;
+    int64_t s = (longest + *steps - 1) / *steps;
+    if (s > room) s = room;
+    if (s > most) s = most;
+    if (s > *splits) *splits = (int)s;
+    return halves;
+}
 // Steps of `bn` keys of the tile of rows from row0 on, up to the place of its last row.  (The sequence's rows are tokens begin ..
 // end - 1 times `group`, and its last position is the last token's.)
 QE_MIX_HD int qe_attn_tile_steps(int len, int begin, int end, int row0, int group, int bm, int bn) {
