@@ -460,7 +460,11 @@ static int decode_shared(qe_attn_ctx *c, const qe_attn_batch *b, const qe_attn_s
     if (kv8) y.x.ks = kv8->k_scale, y.x.vs = kv8->v_scale;
     y.seqs = sh->seqs; y.prefix = sh->prefix; y.n_groups = sh->n_groups;
     const int64_t most = (int64_t)b->max_pages * c->d.page;
-    const int64_t max_len = b->max_len && b->max_len < most ? b->max_len : most, max_prefix = sh->max_prefix && sh->max_prefix < max_len ? sh->max_prefix : max_len;
+    const int64_t max_len = b->max_len && b->max_len < most ? b->max_len : most;
+    // A prefix that is not stated is planned as 16,384 positions, or as many as there are: a table may have room for far more (32 behind 8000, 16 / 2
+    // heads of 256 in bf16, a table of 262,144: 31.5 us a call, 38.3 as if all were shared, 33.9 with 4096, 31.2 stated; one of 30,000 alone beside
+    // eight behind 30,000 36, 36, 55).
+    const int64_t prefix = sh->max_prefix ? sh->max_prefix : 16384, max_prefix = prefix < max_len ? prefix : max_len;
     // a launch's sequences, and their groups as far as they reach into it
     const int n = qe_attn_shared_seqs(b->n_seqs, y.x.a.q_heads);
     y.x.a.tiles = qe_attn_max_tiles(n, sh->n_groups, y.x.a.group, QE_ATTN_SHARED_BM);

@@ -24,3 +24,18 @@ def test_own_parts_of_all_lengths(heads, groups, own, prefix, before, behind, ca
         g.c.att.check()
         close(out, want, off)
         assert torch.equal(out, again)
+
+
+@pytest.mark.parametrize("cache", CACHES)
+def test_wide_tables(cache):
+    """Room for far more positions than there are, without a hint: prefixes on either side of what is assumed."""
+    for groups, own, prefix in (([3, 2], [400, 2, 0, 33, 1], [700, 5]), ([2], [10, 300], [20000])):
+        g = Grouped((8, 2, 128, 64), torch.float16, cache, groups, own, prefix, behind=0)
+        n = len(own)
+        table = torch.full((n, 262144 // 64), 1 << 30, dtype=torch.int32, device="cuda")
+        table[:, : g.c.table.shape[1]] = g.c.table
+        q = g.c.q(n)
+        out = torch.full_like(q, 7.0)
+        g.run(q, out, table=table)
+        g.c.att.check()
+        close(out, *g.expect(q))

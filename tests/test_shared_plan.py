@@ -37,7 +37,7 @@ def plan(tmp_path_factory):
         p, steps, splits = (ctypes.c_int() for _ in range(3))
         own = max(1, max_len - max_prefix) if max_len and max_prefix else 0
         max_len = max_len or table
-        lib.shared_plan(n, q, kv, min(max_prefix, max_len) or max_len, own, *(ctypes.byref(x) for x in (p, steps, splits)), max_len, groups, dim)
+        lib.shared_plan(n, q, kv, min(max_prefix or 16384, max_len), own, *(ctypes.byref(x) for x in (p, steps, splits)), max_len, groups, dim)
         return p.value, steps.value, splits.value
 
     lib.of = of
