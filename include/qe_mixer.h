@@ -187,7 +187,7 @@ int qe_attn_read8(qe_attn_ctx *ctx, const qe_attn_batch *batch, const qe_kv_cach
 /* qe_attn_prompt and qe_attn_decode over an 8-bit cache.  Products are as exact
  * as with a 16-bit cache, since codes are numbers of both 16-bit types; a key's
  * scale multiplies its score and a value's its probability, which is then, in
- * prompts, rounded to the context's type (fp16: to fixed steps below 2^-20 of
+ * prompts, rounded to the context's type (fp16: to fixed steps below 2^-19 of
  * a row's greatest probability and the greatest scale of the positions that it
  * attends to), and for single tokens taken as two numbers of it.  A scale that is
  * not finite reaches the rows that attend to its position, and no others.  Of up to 64
@@ -220,7 +220,8 @@ typedef struct {
 /* qe_attn_decode and qe_attn_decode8 of such sequences: a group's shared keys and
  * values are read once for all of its queries.  The results are those of the
  * plain calls on tables whose first entries are the shared pages, but for
- * rounding (fp16: probabilities below 2^-21 of a row's greatest to fixed steps).
+ * rounding (fp16: probabilities below 2^-21 of a row's greatest to fixed steps;
+ * over an 8-bit cache those of the shared positions are rounded as in prompts).
  * A bad page among the shared ones makes zeros of all of its
  * group's outputs. */
 int qe_attn_decode_shared(qe_attn_ctx *ctx, const qe_attn_batch *batch, const qe_attn_shared *shared, const qe_kv_cache *cache, const void *q,

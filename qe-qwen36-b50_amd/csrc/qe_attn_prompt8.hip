@@ -12,8 +12,9 @@
 
 //
 // Bound by the matrix cores and by the vector instructions beside them, which turn codes, apply scales and make exponentials: 8192
-// tokens of 16 / 2 heads of 256, e4m3, take 557 us of a pass, 980 TFLOP/s (16-bit tiles, which come by direct loads: 489); 8000 of 32 / 8 of 128
-// 614 us a call, 850 TFLOP/s.  Packed prompts of 200, 333 and 967 tokens after 0, 1700 and 0 take 54: the longest tiles' 32 steps, on a GPU half
+// tokens of 16 / 2 heads of 256, e4m3, take 545 to 575 us a pass, 960 to 1010 TFLOP/s (16-bit tiles, which come by direct loads: 480 to 515); 8000 of
+// 32 / 8 of 128 590 to 635 us, 820 to 880 TFLOP/s.  (Cards and runs differ by so much; figures that are set against each other, here and below, are of one
+// run.)  Packed prompts of 200, 333 and 967 tokens after 0, 1700 and 0 take 54: the longest tiles' 32 steps, on a GPU half
 // full.  Eight waves and 256 rows for heads of 128: 8000 tokens 613 us for 635, but 5000 of 14 / 2 185 for 158.
 template <bool BF, int DH, int CT, int WAVES, int HALVES>
 __global__ __launch_bounds__(64 * WAVES * HALVES, 2) void k_attn_prompt8(const QeAttn8Args x) {

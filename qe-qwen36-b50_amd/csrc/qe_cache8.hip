@@ -8,8 +8,8 @@
 //   y = x / sqrt(mean(x^2) + eps) w, rotated;  scale = max |y| / 127 or / 448;  codes = y / scale, to nearest.
 // The greatest is found among the bits without sign, where what is not finite is greater than all else.
 //
-// Bound by memory: 8000 tokens of 32 + 2 x 8 heads of 128, fp16 to e4m3, are 213 MB and take 40 us, 5.3 TB/s; 2000 tokens of 16 + 2 x 2
-// heads of 256 with norms, bf16 to 16 bits, 41 MB, 12 us.  Eight single tokens take 4.9 us, a launch and one round trip each for length, page and
+// Bound by memory: 8000 tokens of 32 + 2 x 8 heads of 128, fp16 to e4m3, are 181 MB and take 39 to 40 us, 4.5 to 4.7 TB/s (a large copy reaches
+// 5.0); 2000 tokens of 16 + 2 x 2 heads of 256 with norms, bf16 to 16 bits, 41 MB, 12 us.  Eight single tokens take 4.9 us, a launch and one round trip each for length, page and
 // data.  A thread for each item, up to 512 a token, is slower than turns of 256 (42 us for 8000 tokens).
 // ---------------------------------------------------------------------------
 template <typename IN>
@@ -25,6 +25,8 @@ __device__ __forceinline__ void load8(const IN *p, float *x) {
     }
 }
 
+// (Six instructions an element cost 1 to 2 % of a call whose tokens come from memory, 7 % of one of 5000 tokens of heads of 64 in the caches; the
+// compiler's division 4 and 20 %.)
 // x / s as 32 bits have it, for s in [1, 2) and its reciprocal to nearest: next to a border between two codes the product with a
 // reciprocal would give the other one.  One correction by the remainder, which fmaf has exactly, makes the quotient one of the two floats next to
 // x / s; a second rounds it to nearest (P. Markstein, Computation of elementary functions on the IBM RISC System/6000, 1990).

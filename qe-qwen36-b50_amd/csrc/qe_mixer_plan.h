@@ -116,8 +116,8 @@ QE_MIX_HD bool qe_attn_prompt8_halves(int64_t tiles, int bn, int64_t max_len) {
 // are not: `steps` steps a workgroup, at most `splits` for a tile and key-value head, as many as there is scratch for.
 // Workgroups that a tile has no use for end at once, and one that has all of a tile's keys writes its rows itself.  At
 // least eight steps, and as many as let twice the places of the GPU hold all tiles if each were as long as the longest (32 / 8 heads
-// of 128, int8: 600 tokens after 20,000 337 us with 1.5 times, 307 with twice and with three times, 599 without; 50, 700 and 20
-// after 5000, 0 and 19,000 of 24 / 8 heads of 64 107, 87 and 88, 406 without).  Where tiles fill half of the places and none has 40
+// of 128, int8: 600 tokens after 20,000 326 us with 1.5 times, 290 with twice and with three times, 545 without; 50, 700 and 20
+// after 5000, 0 and 19,000 of 24 / 8 heads of 64 93, 84 and 84, 377 without).  Where tiles fill half of the places and none has 40
 // steps the join costs as much as it saves (4 x 400 after 2000 103 us without, 122 with; 1500 tokens 53 and 65).
 // Partial results are of whole tiles, and there is room for 131,072 rows of them, twice what the other calls need: a long tile among short
 // ones is cut into as many splits as there are for all.  (int8; with 65,536 rows: 256 and 800 after 4500 and 0 67 -> 135 us, 100 and 400
