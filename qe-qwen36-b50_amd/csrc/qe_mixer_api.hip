@@ -470,7 +470,7 @@ static int decode_shared(qe_attn_ctx *c, const qe_attn_batch *b, const qe_attn_s
     y.x.a.tiles = qe_attn_max_tiles(n, sh->n_groups, y.x.a.group, QE_ATTN_SHARED_BM);
     // the longest part of a sequence's own, as far as the hints tell: see qe_attn_shared_plan
     const int64_t max_own = !b->max_len || !sh->max_prefix ? 0 : max_len > max_prefix ? max_len - max_prefix : 1;
-    qe_attn_shared_plan(n, y.x.a.q_heads, y.x.a.kv_heads, max_prefix, max_own, &y.psplits, &y.x.a.steps, &y.x.a.splits, max_len, sh->n_groups, c->d.head_dim);
+    qe_attn_shared_plan(n, y.x.a.q_heads, y.x.a.kv_heads, max_prefix, max_own, &y.psplits, &y.x.a.steps, &y.x.a.splits, max_len);
     if (!qe_fits_launch((int64_t)y.x.a.tiles * (y.x.a.kv_heads * y.psplits + 7) + (int64_t)n * y.x.a.q_heads * y.x.a.splits, 256))
         return qe_fail(QE_ERR_ARG, "%s: %d sequences of %d groups are more threads than a launch has", where, b->n_seqs, sh->n_groups);
     OnDevice on(c->device);

@@ -168,12 +168,11 @@ QE_MIX_HD int qe_attn_tile_splits(int n, int steps, int splits) {
 // A call of single tokens whose sequences share beginnings: `psplits` workgroups for every 128 rows of a group's queries and
 // key-value head over the shared keys, and `splits` of `steps` steps for a sequence's own (qe_attn_decode_cut).
 // A split of the shared keys costs its partial results, and saves the others time: P splits take about a prefix / P + b rows
-// P, which is least where P^2 is a / b times prefix / rows.  With a / b = 40, at most one workgroup a CU, and at least 64 keys,
-// 32 sequences of 16 heads of 256 behind 8000 take 34 us a call (36 with 60, 39 with 100), 8 behind 16,000 30 (29, 29).
-// Each group has tiles of its own, with few rows if it is small: of several groups as many workgroups as the GPU holds at once, two a CU or, with
-// heads of 64, three (16 / 2 heads of 256: 32 groups of two behind 2000 33 us a call, 39 if their tiles are counted as one group's; 8 of
-// three behind 500 and 12,000 34, 37 and, with one a CU, 53; 32 / 8 of 128: 100 of two behind 1000 114, 121; 24 / 8 of 64: 16 of two
-// behind 6000 42, 49 and, with two a CU, 53, but 12 / 12 of 64: 30 of two behind 1000 33, 37 and 29).
+// P, which is least where P^2 is a / b times prefix / rows.  With a / b = 40, at least 64 keys, and at most one workgroup a CU if all
+// sequences are one group's, 32 sequences of 16 heads of 256 behind 8000 take 34 us a call (36 with 60, 39 with 100), 8 behind 16,000 30 (29, 29).
+// Each group has tiles of its own, so that several have more workgroups than that.  Counting them, with as many workgroups as the GPU holds at
+// once, is right where groups are alike (32 of two behind 2000, 16 / 2 heads of 256, 33 us for 40; of 32 / 8 of 128 56 for 64) and far off where one
+// is large and others share little (8 sequences behind 20,000 beside 50 of their own 201 us for 62; 32 behind 8000 beside 32, 32 / 8 of 128, 122 for 44).
 // A sequence's own positions: at least twelve steps a workgroup, or as few as make 768 workgroups if all are as long as the longest.
 // (32 sequences of 16 / 2 heads of 256 with up to 1500 of their own: 31.8 us a call, 33.4 with 512, 37.9 with 1024; 50 of 8 / 1 with up to
 // 1000: 25.9, 27.0, 26.4.  At least eight steps: 64 of 32 / 8 heads of 128 with up to 1000 46.9 for 42.2, but 40 of 24 / 8 of 64 with up to
@@ -193,7 +192,7 @@ QE_MIX_HD int qe_attn_shared_seqs(int n_seqs, int q_heads) {
     return n_seqs < most ? n_seqs : most;
 }
 QE_MIX_HD void qe_attn_shared_plan(int n_seqs, int q_heads, int kv_heads, int64_t max_prefix, int64_t max_own, int *psplits, int *steps, int *splits,
-                                    int64_t max_len = 0, int n_groups = 1, int head_dim = 256) {
+                                    int64_t max_len = 0) {
     const int64_t rows = (int64_t)n_seqs * q_heads, room = QE_ATTN_SHARED_ROWS / rows;
     *steps = 8, *splits = 1;
     if (max_own > 0) qe_attn_decode_cut(n_seqs, kv_heads, 768, 12, max_own, steps, splits);
@@ -201,8 +200,8 @@ QE_MIX_HD void qe_attn_shared_plan(int n_seqs, int q_heads, int kv_heads, int64_
     const int64_t more = longest < most_wgs ? longest : most_wgs;
     if (more > *splits) *splits = (int)more;
     if (*splits > (room + 1) / 2) *splits = (int)((room + 1) / 2);
-    const int64_t tiles = (((int64_t)n_seqs * (q_heads / kv_heads) + QE_ATTN_SHARED_BM - 1) / QE_ATTN_SHARED_BM + n_groups - 1) * kv_heads;
-    const int64_t most = (max_prefix + 63) / 64, places = n_groups == 1 ? 256 : head_dim == 64 ? 768 : 512, fill = (places + tiles - 1) / tiles;
+    const int64_t tiles = ((int64_t)n_seqs * (q_heads / kv_heads) + QE_ATTN_SHARED_BM - 1) / QE_ATTN_SHARED_BM * kv_heads;
+    const int64_t most = (max_prefix + 63) / 64, fill = (256 + tiles - 1) / tiles;
     int64_t s = 1;
     while (s * s * rows < 40 * max_prefix && s < most && s < fill) ++s;
     if (s > room - *splits) s = room - *splits;

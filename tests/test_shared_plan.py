@@ -12,8 +12,8 @@ SHIM = """
 #include "qe_mixer_plan.h"
 extern "C" {
 int shared_seqs(int n, int h) { return qe_attn_shared_seqs(n, h); }
-void shared_plan(int n, int q, int kv, long prefix, long own, int *p, int *steps, int *splits, long len, int groups, int dim) {
-    qe_attn_shared_plan(n, q, kv, prefix, own, p, steps, splits, len, groups, dim);
+void shared_plan(int n, int q, int kv, long prefix, long own, int *p, int *steps, int *splits, long len) {
+    qe_attn_shared_plan(n, q, kv, prefix, own, p, steps, splits, len);
 }
 int shared_rows() { return QE_ATTN_SHARED_ROWS; }
 int decode_steps(int len, int steps, int splits) { return qe_attn_decode_steps(len, steps, splits); }
@@ -29,15 +29,15 @@ def plan(tmp_path_factory):
     subprocess.run(["g++", "-shared", "-fPIC", "-std=c++17", "-Wall", "-Wno-unused-function", "-I", os.path.join(PKG, "csrc"),
                     str(d / "shim.cpp"), "-o", str(d / "shim.so")], check=True)
     lib = ctypes.CDLL(str(d / "shim.so"))
-    lib.shared_plan.argtypes = [ctypes.c_int] * 3 + [ctypes.c_long] * 2 + [ctypes.c_void_p] * 3 + [ctypes.c_long, ctypes.c_int, ctypes.c_int]
+    lib.shared_plan.argtypes = [ctypes.c_int] * 3 + [ctypes.c_long] * 2 + [ctypes.c_void_p] * 3 + [ctypes.c_long]
 
-    def of(n, q, kv, max_len, max_prefix, table=None, groups=1, dim=256):
+    def of(n, q, kv, max_len, max_prefix, table=None):
         """As a call with these hints is planned, 0: not stated, whose table has room for `table` positions.  -> prefix splits, steps,
         splits"""
         p, steps, splits = (ctypes.c_int() for _ in range(3))
         own = max(1, max_len - max_prefix) if max_len and max_prefix else 0
         max_len = max_len or table
-        lib.shared_plan(n, q, kv, min(max_prefix or 16384, max_len), own, *(ctypes.byref(x) for x in (p, steps, splits)), max_len, groups, dim)
+        lib.shared_plan(n, q, kv, min(max_prefix or 16384, max_len), own, *(ctypes.byref(x) for x in (p, steps, splits)), max_len)
         return p.value, steps.value, splits.value
 
     lib.of = of
@@ -76,22 +76,10 @@ def test_partial_results_fit_and_cover(plan):
         n = plan.shared_seqs(seqs, heads * group)
         max_len = int(np.exp(rng.uniform(0, np.log(1 << 30))))
         max_prefix = int(rng.choice([0, 1, max_len // 2, max_len]))
-        p, steps, splits = plan.of(n, heads * group, heads, int(rng.choice([0, max_len])), max_prefix, max_len, int(rng.choice([1, 7, 900])), int(rng.choice([64, 256])))
+        p, steps, splits = plan.of(n, heads * group, heads, int(rng.choice([0, max_len])), max_prefix, max_len)
         assert p >= 1 and splits >= 1 and steps >= 2 and n * heads * group * (p + splits) <= plan.shared_rows()
         assert n * heads * splits <= max(2048 + n * heads, 1024)
         for own in (1, 31, 33, max_len):
             mine = plan.decode_steps(own, steps, splits)
             active = plan.decode_active(own, mine)
             assert active <= splits and (active - 1) * mine < -(-own // 32) <= active * mine
-
-
-def test_prefix_workgroups_of_many_groups(plan):
-    """Each group has tiles of its own: together they are about what the GPU holds at once, or one for each tile and head."""
-    for n, q, kv, groups, dim, places in ((64, 16, 2, 32, 256, 512), (64, 32, 8, 32, 128, 512), (32, 24, 8, 16, 64, 768), (60, 12, 12, 30, 64, 768), (24, 16, 2, 8, 256, 512)):
-        p, _, _ = plan.of(n, q, kv, 9000, 8000, groups=groups, dim=dim)
-        tiles = -(-(n * (q // kv)) // 128) + groups - 1  # no fewer than the groups have
-        assert places <= p * tiles * kv < places + tiles * kv or p == 1, (p, tiles * kv)
-    # one group is planned as it was: at most one workgroup a CU
-    for n, q, kv, prefix in ((32, 16, 2, 8000), (8, 16, 2, 16000), (2, 16, 2, 16000)):
-        p, _, _ = plan.of(n, q, kv, prefix + 1000, prefix)
-        assert (p - 1) * -(-(n * (q // kv)) // 128) * kv < 256
