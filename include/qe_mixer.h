@@ -213,8 +213,9 @@ typedef struct {
     int n_groups;          /* 1 .. 65535 */
     const int32_t *seqs;   /* device [n_groups + 1] */
     const int32_t *prefix; /* device [n_groups] */
-    int max_prefix;        /* the greatest prefix as far as the host knows, for choosing splits, as batch->max_len is: their
-                              difference is taken for the longest part that a sequence has to itself; 0 = not known */
+    int max_prefix;        /* the greatest prefix as far as the host knows, for choosing splits (results do not depend on it but
+                              for rounding): its difference from batch->max_len is what sequences are expected to have to
+                              themselves, and some may have more; 0 = not known */
 } qe_attn_shared;
 
 /* qe_attn_decode and qe_attn_decode8 of such sequences: a group's shared keys and

@@ -223,7 +223,7 @@ class Shared:
     """Groups of a batch's sequences that share their beginnings: int32 seqs [groups + 1], group g's first sequence and one
     behind its last, and prefix [groups], how many positions it shares (in the pages of its first sequence).  Both may be
     updated in place between calls.  max_prefix: the greatest as far as is known, for choosing splits (its difference from the batch's
-    max_len is taken for the longest part that a sequence has to itself)."""
+    max_len is what sequences are expected to have to themselves)."""
 
     def __init__(self, seqs, prefix, max_prefix=0):
         n, device = prefix.shape[0], prefix.get_device()
