@@ -113,7 +113,9 @@ __device__ __forceinline__ unsigned greatest_seen(unsigned top, int b, int limit
 
 // The sum of the probabilities as they are rounded, in place of as they were: x are they times their values' scales s, p is x rounded.
 // A row's weights then sum to 1, and where one probability is nearly all, its rounding is in both and none of it in the result; a row
-// of one key is its value.  (Over many rows with many keys it changes little.)  Scales far below the greatest, whose products may be
+// of one key is its value: weights w with roundings e of u at most leave a result o the sum of e w (v - o), in place of e w v.  That is u (sum w |v| +
+// |o|) at most, more than u sum w |v| where little of a row's weight is on its values and the rest on zeros, and as a rule less.  (Over many
+// rows with many keys it changes little.)  Scales far below the greatest, whose products may be
 // too small for the type, are left out: in fp16 those below 2^-6 of the row's unit.
 template <bool BF, int I = 0, int KB>
 __device__ __forceinline__ void sum_rounded(float &l, const Scores<KB> &x, const Probs<KB> &p, int b, float inverse, float most) {
